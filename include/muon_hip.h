@@ -60,7 +60,9 @@ extern "C" {
 #define MUON_HIP_K_BX_UPDATE 10 /* the a.X + B.X launch that carries the parameter update in its epilogue */
 #define MUON_HIP_K_SMALL_CHAIN 11 /* normalisation, iterations and update of matrices that one workgroup each holds */
 #define MUON_HIP_K_FLOW_CHAIN 12  /* the iterations and the update of many small matrices in one launch */
-#define MUON_HIP_K_COUNT 13
+#define MUON_HIP_K_PRODUCT 13     /* a muon_hip_product_run with its packing and joining launches */
+#define MUON_HIP_K_ACT_GRAD 14
+#define MUON_HIP_K_COUNT 15
 
 /* GEMM kernel variants; MUON_HIP_CFG_AUTO picks per kernel, shape and number of tiles.  All feed LDS with direct
  * global->LDS loads (global_load_lds_dwordx4), software pipelined behind the MFMAs. */
@@ -318,6 +320,63 @@ int muon_hip_grad_norms_static(const void* const* g_ptrs, const long* numel, con
                                long chunks, int dtype, double norm_type, float* norms, void* stream);
 int muon_hip_clip_scale(const void* const* g_ptrs, const long* numel, const long* chunk_start, int n, long chunks,
                         int dtype, const float* total_f32, int norm_dtype, double max_norm, void* stream);
+
+/* ---- products of layers -------------------------------------------------------------------
+ * The layers whose weights the step above trains, forward and backward: y = x Wt with what a layer does to it in the epilogue.  No
+ * counterpart in the reference, which leaves them to torch.
+ *
+ * An operand is a matrix of any non-negative strides (in elements): element (i, l) of a[s] is a[s][i * a_row[s] + l * a_col[s]], l the
+ * reduction index.  It is read as it lies where one of its strides is 1, the other one and the pointer are whole 16-byte pieces and a tile
+ * of it spans less than 2 GiB; anything else is packed into the workspace first, and so are the factors of a gated pair with row stride 1.
+ * Results are row-major m x n matrices.  Sums are fp32 (bf16 operands: products are exact), everything of the epilogue too, results are
+ * rounded once.
+ *
+ *   LINEAR  out[0] = act(a[0] b[0]^T + bias[0]) + residual; aux[0], where not null: act'(.), what the incoming gradient is multiplied by
+ *   GATED   g = a[0] b[0]^T + bias[0], u = a[0] b[1]^T + bias[1]:  out[0] = act(g) u; aux, where not null: aux[0] = act(g),
+ *           aux[1] = u act'(g), the factors of the gradients of u and of g
+ *   SUM     out[0] = a[0] b[0]^T + a[1] b[1]^T
+ *   EACH    out[0] = a[0] b[0]^T, out[1] = a[1] b[0]^T
+ * bias (n contiguous elements each), residual (strides res_row, res_col) and aux may be null; SUM and EACH take none of them and
+ * MUON_HIP_ACT_NONE.  All tensors share `dtype`.  m, n and k may be 0; a sum over nothing is 0.  Outputs may not overlap inputs, but for a
+ * residual that is out[0] itself. */
+#define MUON_HIP_PRODUCT_LINEAR 0
+#define MUON_HIP_PRODUCT_GATED 1
+#define MUON_HIP_PRODUCT_SUM 2
+#define MUON_HIP_PRODUCT_EACH 3
+#define MUON_HIP_ACT_NONE 0
+#define MUON_HIP_ACT_RELU 1
+#define MUON_HIP_ACT_SIGMOID 2
+#define MUON_HIP_ACT_SILU 3
+#define MUON_HIP_ACT_GELU 4      /* z Phi(z) */
+#define MUON_HIP_ACT_GELU_TANH 5 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define MUON_HIP_ACT_COUNT 6
+typedef struct {
+    int kind, dtype, activation;
+    int m, n, k;
+    const void* a[2];
+    long a_row[2], a_col[2];
+    const void* b[2];
+    long b_row[2], b_col[2];
+    const void* bias[2];
+    const void* residual;
+    long res_row, res_col;
+    void* out[2];
+    void* aux[2];
+} muon_hip_product;
+/* Bytes of workspace (256-byte aligned) that the product needs on the current device, 0 where none; negative: refused, as the call itself
+ * would be.  Depends on sizes, strides and the alignment of the pointers. */
+long muon_hip_product_workspace(const muon_hip_product* p);
+int muon_hip_product_run(const muon_hip_product* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What stands between the incoming gradient and the products of a backward pass, over row-major m x n matrices:
+ *   dz0 = dy * d0 and, with two factors, dz1 = dy * d1, rows `pitch` >= n elements apart (what lies between stays as it was);
+ *   db0, db1: the sums of dz0 and dz1 over the rows, before they are rounded (fp32, in a fixed order).
+ * `factors` is 2, 1, or 0 for dz0 = dy.  Results may be null where they are not wanted: dz0 and dz1 both or none, each of the sums by
+ * itself; dz1 and db1 come with the second factor alone.  For sums, `partials` holds muon_hip_act_grad_partials(m, n) floats for each
+ * factor (for one, where there is none). */
+long muon_hip_act_grad_partials(int m, int n);
+int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d1, void* dz0, void* dz1, long pitch, void* db0, void* db1,
+                      int dtype, int m, int n, float* partials, void* stream);
 
 /* Shape of the current device as the launchers see it, read from the runtime once per device: compute units
  * (a round of 256x256 tiles is one per compute unit) and XCDs (compute units / 32 on gfx950, whole XCDs per

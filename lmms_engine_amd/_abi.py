@@ -22,7 +22,7 @@ CFG_AUTO, CFG_128_PIPE, CFG_256_PIPE, CFG_256_PINGPONG, CFG_128_PINGPONG, CFG_25
 GEMM_CONFIGS = list(range(4))
 K_MOMENTUM, K_NORMALIZE, K_SYRK, K_SYMPOLY, K_BX, K_UPDATE, K_ADAMW, K_ADAMW_MULTI, K_GRAD_NORM, K_CLIP_SCALE = range(10)
 KERNEL_NAMES = ["momentum_norm", "normalize", "syrk", "sympoly", "bx_axpy", "apply_update", "adamw", "adamw_multi",
-                "grad_norm", "clip_scale", "bx_axpy_update", "small_chain", "flow_chain"]
+                "grad_norm", "clip_scale", "bx_axpy_update", "small_chain", "flow_chain", "product", "act_grad"]
 MULTI_CHUNK = 16384  # MUON_HIP_MULTI_CHUNK
 STATIC_MAX_CHUNKS = 1 << 20  # MUON_HIP_STATIC_MAX_CHUNKS
 PPX_COUNTER_BYTES = 576  # MUON_HIP_PPX_COUNTER_BYTES
@@ -47,6 +47,19 @@ class FlowTile(ctypes.Structure):
     """muon_hip_flow_tile"""
 
     _fields_ = [(f, c_int) for f in ("group", "bucket", "matrix", "iteration", "product", "tile", "before")]
+
+
+PRODUCT_LINEAR, PRODUCT_GATED, PRODUCT_SUM, PRODUCT_EACH = range(4)
+ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}  # MUON_HIP_ACT_*
+
+
+class Product(ctypes.Structure):
+    """muon_hip_product"""
+
+    _fields_ = [("kind", c_int), ("dtype", c_int), ("activation", c_int), ("m", c_int), ("n", c_int), ("k", c_int),
+                ("a", c_void_p * 2), ("a_row", c_long * 2), ("a_col", c_long * 2), ("b", c_void_p * 2), ("b_row", c_long * 2),
+                ("b_col", c_long * 2), ("bias", c_void_p * 2), ("residual", c_void_p), ("res_row", c_long), ("res_col", c_long),
+                ("out", c_void_p * 2), ("aux", c_void_p * 2)]
 
 
 # name -> (restype, argtypes); mirrors include/muon_hip.h one to one
@@ -95,6 +108,10 @@ SIGNATURES = {
     "muon_hip_total_norm": (c_int, [c_void_p, c_int, c_int, c_double, c_void_p, c_void_p, c_void_p]),
     "muon_hip_clip_scale": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_long, c_int, c_void_p, c_int, c_double,
                                     c_void_p]),
+    "muon_hip_product_workspace": (c_long, [c_void_p]),
+    "muon_hip_product_run": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "muon_hip_act_grad_partials": (c_long, [c_int, c_int]),
+    "muon_hip_act_grad": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_long] + [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 2),
     "muon_hip_device_shape": (c_int, [POINTER(c_int), POINTER(c_int)]),
     "muon_hip_timing_reserve": (c_int, [c_long]),
     "muon_hip_timing_untimed": (c_long, []),

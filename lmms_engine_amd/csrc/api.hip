@@ -15,6 +15,7 @@
 #include "elementwise.h"
 #include "gemm_nt.h"
 #include "multi_tensor.h"
+#include "product.h"
 #include "small_chain.h"
 
 namespace {
@@ -1059,6 +1060,100 @@ int muon_hip_clip_scale(const void* const* g_ptrs, const long* numel, const long
     const MultiTensorList l{g_ptrs, numel, chunk_start, n, chunks};
     hipError_t e = launch_clip_scale_multi(l, dtype, total_f32, norm_dtype, max_norm, s);
     return e == hipSuccess ? 0 : hip_fail(e, "clip_scale launch");
+}
+
+namespace {
+// Checks a product and restates it for its launcher.  An empty result needs nothing else to be right; a sum over nothing needs no operands.
+int check_product(const muon_hip_product* p, ProductArgs& g) {
+    if (!p) return fail(MUON_HIP_EINVAL, "null product");
+    if (p->kind < 0 || p->kind >= PRODUCT_KINDS) return fail(MUON_HIP_EINVAL, "unknown kind of product %d", p->kind);
+    if (!dtype_ok(p->dtype)) return fail(MUON_HIP_EINVAL, "unknown dtype %d", p->dtype);
+    if (p->activation < 0 || p->activation >= ACT_COUNT) return fail(MUON_HIP_EINVAL, "unknown activation %d", p->activation);
+    if (p->m < 0 || p->n < 0 || p->k < 0) return fail(MUON_HIP_EINVAL, "sizes must not be negative");
+    const bool gated = p->kind == PRODUCT_GATED, layer = gated || p->kind == PRODUCT_LINEAR;
+    const int na = layer ? 1 : 2, nb = gated || p->kind == PRODUCT_SUM ? 2 : 1, nout = p->kind == PRODUCT_EACH ? 2 : 1;
+    if (!layer && (p->bias[0] || p->bias[1] || p->residual || p->aux[0] || p->aux[1] || p->activation != ACT_NONE))
+        return fail(MUON_HIP_EINVAL, "sums of products take no bias, residual, activation or second result");
+    if (gated && p->residual) return fail(MUON_HIP_EINVAL, "a gated product takes no residual");
+    if (gated ? !p->aux[0] != !p->aux[1] : p->aux[1] != nullptr) return fail(MUON_HIP_EINVAL, "a gated product has two second results or none, others have one");
+    if (!gated && p->bias[1]) return fail(MUON_HIP_EINVAL, "only a gated product has two biases");
+    if (p->res_row < 0 || p->res_col < 0) return fail(MUON_HIP_EINVAL, "strides must not be negative");
+    for (int i = 0; i < 2; ++i) {
+        if ((i < na && (p->a_row[i] < 0 || p->a_col[i] < 0)) || (i < nb && (p->b_row[i] < 0 || p->b_col[i] < 0)))
+            return fail(MUON_HIP_EINVAL, "strides must not be negative");
+        if (p->m == 0 || p->n == 0) continue;
+        if (i < nout && !p->out[i]) return fail(MUON_HIP_EINVAL, "null result");
+        if (p->k > 0 && ((i < na && !p->a[i]) || (i < nb && !p->b[i]))) return fail(MUON_HIP_EINVAL, "null operand");
+    }
+    g = ProductArgs{};
+    g.kind = p->kind;
+    g.dtype = p->dtype;
+    g.act = p->activation;
+    g.m = p->m;
+    g.n = p->n;
+    g.k = p->k;
+    for (int i = 0; i < 2; ++i) {
+        if (i < na) g.a.base[i] = p->a[i], g.a.row[i] = p->a_row[i], g.a.col[i] = p->a_col[i];
+        if (i < nb) g.b.base[i] = p->b[i], g.b.row[i] = p->b_row[i], g.b.col[i] = p->b_col[i];
+        if (i < nout) g.out[i] = p->out[i];
+        g.bias[i] = p->bias[i];
+        g.aux[i] = p->aux[i];
+    }
+    g.residual = p->residual;
+    g.res_row = p->res_row;
+    g.res_col = p->res_col;
+    return 0;
+}
+}  // namespace
+
+long muon_hip_product_workspace(const muon_hip_product* p) {
+    ProductArgs g;
+    if (int rc = check_product(p, g)) return rc;
+    MachineShape ms;
+    if (hipError_t e = machine_shape(ms); e != hipSuccess) return hip_fail(e, "device attributes"), (long)MUON_HIP_EINVAL;
+    const long bytes = product_workspace(g, ms.cus);
+    if (bytes < 0) return fail(MUON_HIP_ESHAPE, "%d x %d x %d: a tile of an operand spans 2 GiB, or the tiles exceed one launch", p->m, p->n, p->k);
+    return bytes;
+}
+
+int muon_hip_product_run(const muon_hip_product* p, void* workspace, size_t workspace_bytes, void* stream) {
+    ProductArgs g;
+    if (int rc = check_product(p, g)) return rc;
+    if (p->m == 0 || p->n == 0) return 0;
+    MachineShape ms;
+    if (hipError_t e = machine_shape(ms); e != hipSuccess) return hip_fail(e, "device attributes");
+    const long bytes = product_workspace(g, ms.cus);
+    if (bytes < 0) return fail(MUON_HIP_ESHAPE, "%d x %d x %d: a tile of an operand spans 2 GiB, or the tiles exceed one launch", p->m, p->n, p->k);
+    if (bytes > 0) {
+        if (int rc = check_ws(workspace)) return rc;
+        if ((size_t)bytes > workspace_bytes) return fail(MUON_HIP_EINVAL, "the workspace has %zu bytes, the product needs %ld", workspace_bytes, bytes);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_PRODUCT, s);
+    hipError_t e = launch_product(g, workspace, ms.cus, ms.xcd_shift, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "product launch");
+}
+
+long muon_hip_act_grad_partials(int m, int n) { return m <= 0 || n <= 0 ? 0 : act_grad_partials(m, n); }
+
+int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d1, void* dz0, void* dz1, long pitch, void* db0, void* db1,
+                      int dtype, int m, int n, float* partials, void* stream) {
+    if (!dtype_ok(dtype) || m < 0 || n < 0) return fail(MUON_HIP_EINVAL, "bad dtype or size");
+    if (factors < 0 || factors > 2) return fail(MUON_HIP_EINVAL, "%d factors: none, one or two are wanted", factors);
+    if ((dz0 || dz1) && pitch < n) return fail(MUON_HIP_EINVAL, "rows of %d elements do not fit %ld apart", n, pitch);
+    if (n == 0) return 0;
+    if (factors < 2 && (dz1 || db1)) return fail(MUON_HIP_EINVAL, "a second result needs a second factor");
+    if (m > 0) {
+        if (!dy || (factors > 0 && !d0) || (factors > 1 && !d1)) return fail(MUON_HIP_EINVAL, "null gradient or factor");
+        if (factors > 1 && !dz0 != !dz1) return fail(MUON_HIP_EINVAL, "one of the two products alone");
+        if ((db0 || db1) && !partials) return fail(MUON_HIP_EINVAL, "sums need memory for their parts");
+    }
+    if (((long)m + 63) / 64 * (((long)n + 255) / 256) > 0x7fffffffL) return fail(MUON_HIP_ESHAPE, "%d x %d values exceed one launch", m, n);
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_ACT_GRAD, s);
+    const ActGradArgs a{dtype, m, n, factors, dy, {d0, d1}, {dz0, dz1}, pitch, {db0, db1}, partials};
+    hipError_t e = launch_act_grad(a, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "act_grad launch");
 }
 
 int muon_hip_device_shape(int* compute_units, int* xcds) {

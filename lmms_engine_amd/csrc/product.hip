@@ -1,0 +1,786 @@
+// Products of layers on gfx950: out[i][j] = sum_l a[i][l] b[j][l] with the layer's own arithmetic in the epilogue.
+//
+//   LINEAR  out = act(a b^T + bias) + residual, and act'(.) for the backward pass where it is asked for
+//   GATED   g = a b0^T + bias0, u = a b1^T + bias1, out = act(g) u, and act(g), u act'(g) for the backward pass: both products in one
+//           kernel, a tile holds the same columns of g and u
+//   SUM     out = a0 b0^T + a1 b1^T (the gradient of a gated pair's input): one reduction that runs over both products
+//   EACH    out0 = a0 b0^T, out1 = a1 b0^T (the gradients of its weights): the tiles of both in one launch
+//
+// Operands may lie with the reduction index contiguous (rows of x and W in a forward pass) or with the other index contiguous (W in the
+// gradient of the input, x and dz in that of the weight): the kernel reads both as they lie, so nothing is transposed in memory.  Anything
+// else is packed into rows of whole 16-byte pieces first.
+//
+// bf16 operands are multiplied by v_mfma_f32_16x16x32_bf16, fp32 ones by v_mfma_f32_16x16x4_f32 (full single precision); sums, biases,
+// activations and residuals are fp32, and results are rounded once.
+#include <atomic>
+#include <type_traits>
+
+#include "common.h"
+#include "gemm_nt.h"
+#include "product.h"
+
+namespace {
+
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+// s_waitcnt with only vmcnt set: vmcnt is split over bits [3:0] and [15:14] (N < 64)
+#define WAIT_VM(N) __builtin_amdgcn_s_waitcnt(0x0F70 | ((N) & 15) | (((N) >> 4) << 14))
+
+constexpr int ROWB = 128;  // bytes of a k-tile per row of an operand: 64 bf16 or 32 fp32 values
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<bf16_t> {
+    static constexpr int BK = 64, PIECE = 8;  // reduction steps of a k-tile, values in 16 bytes
+    typedef bf16x8 frag;
+};
+template <>
+struct Elem<float> {
+    static constexpr int BK = 32, PIECE = 4;
+    typedef f32x4 frag;
+};
+
+struct KernelArgs {
+    const void* a[2];
+    const void* b[2];
+    long pitch_a, pitch_b;  // elements between rows (reduction index contiguous) or between reduction steps (the other one contiguous)
+    int m, n, k;
+    int nk, segments;       // k-tiles of one product, products that are summed
+    int splits, per_split;  // parts of the k-tiles, k-tiles of each
+    int tiles_m, tiles_n, outs;
+    int act;
+    const void* bias[2];
+    const void* residual;
+    long res_row, res_col;
+    void* out[2];
+    void* aux[2];
+    float* partial;  // [split][out or factor][m][n], null: one part
+    int vec;         // rows of out, aux and partial are whole 16-byte pieces
+    int vec_res;
+    int xcd_shift;
+};
+
+// ---- activations -----------------------------------------------------------------------------
+// act(z) and act'(z).  The factor of a gated pair's gradient and the activation itself come out of one evaluation.
+struct ActPair {
+    float a, d;
+};
+__device__ __forceinline__ float sigmoid_of(float z) { return 1.0f / (1.0f + expf(-z)); }
+__device__ __forceinline__ ActPair activate(int act, float z) {
+    switch (act) {
+        case ACT_RELU: return ActPair{z <= 0.f ? 0.f : z, z <= 0.f ? 0.f : 1.f};  // (NaN stays NaN)
+        case ACT_SIGMOID: {
+            const float s = sigmoid_of(z);
+            return ActPair{s, s * (1.f - s)};
+        }
+        case ACT_SILU: {
+            const float s = sigmoid_of(z);
+            return ActPair{z * s, s * (1.f + z * (1.f - s))};
+        }
+        case ACT_GELU: {  // z Phi(z), Phi = erfc(-z / sqrt 2) / 2: no cancellation at the lower end
+            const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
+            return ActPair{z * phi, phi + z * 0.3989422804014327f * expf(-0.5f * z * z)};
+        }
+        case ACT_GELU_TANH: {  // (1 + tanh y) / 2 = sigmoid(2 y), y = c (z + 0.044715 z^3)
+            const float c2 = 2.f * 0.7978845608028654f, q = 0.044715f * z * z;
+            const float s = sigmoid_of(c2 * z * (1.f + q)), w = s * (1.f - s);
+            return ActPair{z * s, s + (w == 0.f ? 0.f : z * w * (c2 * (1.f + 3.f * q)))};
+        }
+        default: return ActPair{z, 1.f};
+    }
+}
+
+// ---- eight values of a row ----------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, long step, bool whole, int count, float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (whole) {
+            const bf16x8 w = *(const bf16x8*)p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = bf2f(w[e]);
+            return;
+        }
+    } else {
+        if (whole) {
+            const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = lo[e], v[e + 4] = hi[e];
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < count ? (float)p[e * step] : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool whole, int count, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        if (whole) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+            *(u32x4*)p = w;
+            return;
+        }
+    } else {
+        if (whole) {
+            *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
+            *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < count) p[e] = (T)v[e];
+}
+
+// The layer's arithmetic on eight sums of row i, columns j .. j + 7 (of both factors of a gated pair), and their way to memory.
+template <typename T, bool GATED>
+__device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int j, float (&v)[8], float (&u)[8]) {
+    const int count = g.n - j < 8 ? g.n - j : 8;
+    const bool whole = g.vec && count == 8;
+    const long at = i * g.n + j;
+    if constexpr (GATED) {
+        if (g.bias[0]) {
+            float b[8];
+            load8((const T*)g.bias[0] + j, 1, false, count, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b[e];
+        }
+        if (g.bias[1]) {
+            float b[8];
+            load8((const T*)g.bias[1] + j, 1, false, count, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] += b[e];
+        }
+        float h[8], s[8], t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const ActPair p = activate(g.act, v[e]);
+            h[e] = p.a * u[e];
+            s[e] = p.a;
+            t[e] = p.d * u[e];
+        }
+        store8((T*)g.out[0] + at, whole, count, h);
+        if (g.aux[0]) {
+            // Rounded once each to the tensors' type, like the activations that any layer keeps: the backward pass multiplies them by the
+            // incoming gradient and nothing else, one rounding less than from g and u themselves.
+            store8((T*)g.aux[0] + at, whole, count, s);
+            store8((T*)g.aux[1] + at, whole, count, t);
+        }
+    } else {
+        if (g.bias[0]) {
+            float b[8];
+            load8((const T*)g.bias[0] + j, 1, false, count, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b[e];
+        }
+        if (g.act != ACT_NONE) {
+            float d[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const ActPair p = activate(g.act, v[e]);
+                v[e] = p.a;
+                d[e] = p.d;
+            }
+            if (g.aux[0]) store8((T*)g.aux[0] + at, whole, count, d);
+        }
+        if (g.residual) {
+            float r[8];
+            load8((const T*)g.residual + i * g.res_row + j * g.res_col, g.res_col, g.vec_res && count == 8, count, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        store8((T*)g.out[z] + at, whole, count, v);
+    }
+}
+
+// ---- operand tiles in LDS -------------------------------------------------------------------------
+// A k-tile of an operand of R rows takes R * 128 bytes, in one of two orders:
+//   rows   row r holds its 8 pieces of 16 bytes; piece c lies at place c ^ swizzle(r)
+//   steps  reduction step k holds R values; 16-byte piece c lies at place c ^ swizzle(k)
+// The loads write LDS in lane order, so the exchange happens on the side of memory: a lane fetches the piece whose place is its own.
+//
+// Fragments: lane l takes row l % 16 of a fragment and the reduction steps of group l / 16.  The rows of the right operand are dealt to
+// its fragments so that a lane ends up with eight neighbouring columns of the result: row i of fragment j is row
+// (j / 2) * 32 + (i / 4) * 8 + (j % 2) * 4 + i % 4 of the wave's columns, and the four sums that a lane holds of fragment j are
+// columns (j / 2) * 32 + (l / 16) * 8 + (j % 2) * 4 + 0..3.  Results then leave as 16-byte pieces without a trip through LDS.
+//
+// The swizzles: reads are served 16 lanes (16-byte reads) or 32 lanes (8-byte transposing reads) at a time, and the lanes that are served
+// together are to touch different banks.  For 16-byte reads of rows the left operand's (r >> 1) & 7 does that for every order of lanes, and
+// the right operand's is the same function of the fragment's row number.  Transposing reads: eight steps, four pieces of 8 bytes each.  The
+// right operand's pieces are 16 bytes apart, which costs it two turns instead of one.
+template <bool RIGHT>
+__device__ __forceinline__ int swizzle_rows(int r) {
+    return RIGHT ? ((r >> 1) & 1) | ((r >> 3) & 3) << 1 : (r >> 1) & 7;
+}
+template <typename T, int R, bool RIGHT>
+__device__ __forceinline__ int swizzle_steps(int k) {
+    if constexpr (sizeof(T) == 2) {
+        if (RIGHT) return R >= 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+        return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : (((k >> 1) & 1) | ((k >> 3) & 1) << 1) << 1;
+    } else {
+        return RIGHT ? ((k >> 2) & 1) << 3 | ((k >> 3) & 1) : ((k >> 2) & 3) << 2;
+    }
+}
+
+// Where lane l finds its part of step group `h` (one of two halves of a k-tile) of fragment f, in bytes.
+// `first`: first row of the wave's part of the operand.
+template <typename T, int R, bool STEPS, bool RIGHT>
+__device__ __forceinline__ typename Elem<T>::frag read_fragment(const unsigned char* tile, int first, int f, int h, int lane) {
+    const int i = lane & 15, grp = lane >> 4;
+    if constexpr (!STEPS) {
+        const int r = first + (RIGHT ? (f >> 1) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3) : f * 16 + i);
+        return *(const typename Elem<T>::frag*)(tile + r * ROWB + (((h * 4 + grp) ^ swizzle_rows<RIGHT>(r)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+        // lane i of a group of 16 addresses piece i (step i / 4, rows of quarter i % 4) and receives row i of steps 0 to 3
+        s16x4 part[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int k = h * 32 + grp * 8 + p * 4 + (i >> 2);
+            const int r = first + (RIGHT ? (f >> 1) * 32 + (i & 3) * 8 + (f & 1) * 4 : f * 16 + (i & 3) * 4);
+            const unsigned char* q = tile + k * (R * 2) + (((r >> 3) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 4) * 2;
+            part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_void_ptr)q);
+        }
+        const s16x8 w = {part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
+        return __builtin_bit_cast(bf16x8, w);
+    } else {
+        f32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = h * 16 + grp * 4 + e;
+            const int r = first + (RIGHT ? (f >> 1) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3) : f * 16 + i);
+            w[e] = *(const float*)(tile + k * (R * 4) + (((r >> 2) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 3) * 4);
+        }
+        return w;
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma_step(const bf16x8& a, const bf16x8& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_step(const f32x4& a, const f32x4& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+__device__ __forceinline__ u32x4 uniform_rsrc(const char* base, unsigned bytes) {
+    const unsigned long long v = (unsigned long long)base;
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((unsigned)v);
+    r[1] = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32) & 0xffffu);
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = 0x00027000;
+    return r;
+}
+// 16 bytes per lane from base + offset into LDS, 1 KB from `lds_byte` in lane order; what lies past the buffer's end is not read.
+__device__ __forceinline__ void load_lds(const u32x4& rsrc, unsigned offset, unsigned lds_byte) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_byte), "v"(offset), "s"(rsrc) : "memory");
+}
+
+// One operand's way into LDS: which pieces a lane fetches, and what of memory may be read.
+template <typename T, int R, int NW, bool STEPS, bool RIGHT, bool GATED>
+struct Feed {
+    static constexpr int LOADS = R / 8 / NW;  // wave instructions of 1 KB
+    static constexpr int BK = Elem<T>::BK, PIECE = Elem<T>::PIECE, PIECES = R / PIECE;
+    static_assert(R % (8 * NW) == 0, "whole instructions");
+    static_assert(!GATED || (!STEPS && RIGHT), "the factors of a gated pair are interleaved by rows");
+    unsigned off[LOADS];
+    int rows;   // of this operand from the tile's first row
+    int wave;
+
+    __device__ __forceinline__ void init(int rows_left, long pitch, int wave_, int lane) {
+        rows = rows_left;
+        wave = wave_;
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int at = wave * LOADS + n;
+            if constexpr (!STEPS) {
+                const int r = at * 8 + (lane >> 3), c = (lane & 7) ^ swizzle_rows<RIGHT>(r);
+                const int src = GATED ? (r >> 6) * 32 + (r & 31) : r;
+                off[n] = (unsigned)(src * pitch * (long)sizeof(T)) + c * 16;
+            } else {
+                const int idx = at * 64 + lane, k = idx / PIECES, c = (idx % PIECES) ^ swizzle_steps<T, R, RIGHT>(k);
+                off[n] = (unsigned)(k * pitch * (long)sizeof(T)) + c * 16;
+            }
+        }
+    }
+    // Bytes that may be read from reduction step k0 of the tile's first row on: whole pieces, so that none is cut in the middle.
+    __device__ __forceinline__ unsigned bytes(long pitch, int k, int k0) const {
+        constexpr int S = sizeof(T);
+        if constexpr (!STEPS) {
+            const int used = GATED ? R / 2 : R, r = rows < used ? rows : used;
+            return (unsigned)((r - 1) * pitch * S + ((long)(k - k0) * S + 15) / 16 * 16);
+        } else {
+            const int steps = k - k0 < BK ? k - k0 : BK, c = rows < R ? rows : R;
+            return (unsigned)((steps - 1) * pitch * S + ((long)c * S + 15) / 16 * 16);
+        }
+    }
+    __device__ __forceinline__ void issue(const char* base0, const char* base1, long pitch, int k, int k0, unsigned lds) const {
+        const long skip = STEPS ? (long)k0 * pitch * (long)sizeof(T) : (long)k0 * (long)sizeof(T);
+        const unsigned nb = bytes(pitch, k, k0);
+        const u32x4 r0 = uniform_rsrc(base0 + skip, nb);
+        u32x4 r1 = r0;
+        if constexpr (GATED) r1 = uniform_rsrc(base1 + skip, nb);
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int at = wave * LOADS + n;
+            if (GATED && (at & 4)) load_lds(r1, off[n], lds + at * 1024);
+            else load_lds(r0, off[n], lds + at * 1024);
+        }
+    }
+    // Zeros in place of what the last k-tile holds past the end of the reduction.
+    static __device__ __forceinline__ void clear_tail(unsigned char* tile, int left, int tid) {
+        for (int idx = tid; idx < R * 8; idx += NW * 64) {
+            int keep;  // values of this piece that belong to the reduction
+            if constexpr (!STEPS) {
+                const int r = idx >> 3, c = (idx & 7) ^ swizzle_rows<RIGHT>(r);
+                keep = left - c * PIECE;
+            } else {
+                keep = idx / PIECES < left ? PIECE : 0;
+            }
+            if (keep >= PIECE) continue;
+            T* p = (T*)(tile + idx * 16);
+#pragma unroll
+            for (int e = 0; e < PIECE; ++e)
+                if (e >= keep) p[e] = (T)0.f;
+        }
+    }
+};
+
+// ---- the tile kernel ---------------------------------------------------------------------------
+template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
+__global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs g) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NW = WGM * WGN, BK = Elem<T>::BK;
+    constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
+    constexpr int A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB;
+    constexpr int TN = GATED ? BN / 2 : BN;  // columns of the result
+    static_assert(!GATED || WTN == 64, "a wave holds 32 columns of each factor");
+    typedef Feed<T, BM, NW, ASTEPS, false, false> FeedA;
+    typedef Feed<T, BN, NW, BSTEPS, true, GATED> FeedB;
+    constexpr int NLD = FeedA::LOADS + FeedB::LOADS;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    // tile of this workgroup: groups of rows of tiles, column by column inside, so that an XCD's tiles share panels
+    const int tiles = g.tiles_m * g.tiles_n;
+    int t = xcd_remap(blockIdx.x, gridDim.x, g.xcd_shift);
+    const int split = t / (tiles * g.outs);
+    t -= split * tiles * g.outs;
+    const int z = t / tiles;
+    t -= z * tiles;
+    constexpr int GM = 4;
+    const int group = t / (GM * g.tiles_n), row0 = group * GM, gm = g.tiles_m - row0 < GM ? g.tiles_m - row0 : GM;
+    t -= group * GM * g.tiles_n;
+    const int ti = row0 + t % gm, tj = t / gm;
+    const long m0 = (long)ti * BM, n0 = (long)tj * TN;
+
+    FeedA fa;
+    FeedB fb;
+    fa.init((int)(g.m - m0), g.pitch_a, wave, lane);
+    fb.init((int)(g.n - n0), g.pitch_b, wave, lane);
+    const long skip_a = (ASTEPS ? m0 : m0 * g.pitch_a) * (long)sizeof(T), skip_b = (BSTEPS ? n0 : n0 * g.pitch_b) * (long)sizeof(T);
+    const unsigned lds = (unsigned)(uintptr_t)(lds_void_ptr)smem;
+
+    const int first = split * g.per_split, all = g.nk * g.segments;
+    const int last = first + g.per_split < all ? first + g.per_split : all;
+    auto place = [&](int kt, int& seg) {  // reduction step that k-tile kt starts with
+        seg = kt >= g.nk ? 1 : 0;
+        return (kt - seg * g.nk) * BK;
+    };
+    auto issue = [&](int kt) {
+        int seg;
+        const int k0 = place(kt, seg);
+        const unsigned st = lds + ((kt - first) & 1) * STAGE;
+        const char* pa = (const char*)g.a[g.outs > 1 ? z : seg];
+        fa.issue(pa + skip_a, nullptr, g.pitch_a, g.k, k0, st);
+        const char* pb0 = (const char*)g.b[GATED ? 0 : seg];
+        const char* pb1 = (const char*)g.b[1];
+        fb.issue(pb0 + skip_b, pb1 + skip_b, g.pitch_b, g.k, k0, st + A_BYTES);
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (first < last) issue(first);
+    for (int kt = first; kt < last; ++kt) {
+        if (kt + 1 < last) {
+            issue(kt + 1);
+            WAIT_VM(NLD);
+        } else {
+            WAIT_VM(0);
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        unsigned char* tile = smem + ((kt - first) & 1) * STAGE;
+        int seg;
+        const int left = g.k - place(kt, seg);
+        if (left < BK) {
+            FeedA::clear_tail(tile, left, tid);
+            FeedB::clear_tail(tile + A_BYTES, left, tid);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            typename Elem<T>::frag va[FM], vb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) va[i] = read_fragment<T, BM, ASTEPS, false>(tile, wm * WTM, i, h, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) vb[j] = read_fragment<T, BN, BSTEPS, true>(tile + A_BYTES, wn * WTN, j, h, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    // One row of fragments after the other, in a loop that is not unrolled: the first is finished, the others move up.  (Unrolled, the
+    // activations of all of them are more code than the instruction cache holds.)
+    const int quad = lane >> 4;
+#pragma unroll 1
+    for (int i = 0; i < FM; ++i) {
+        const long row = m0 + wm * WTM + i * 16 + (lane & 15);
+#pragma unroll
+        for (int jp = 0; jp < FN / 2; jp += GATED ? 2 : 1) {
+            const long col = n0 + (GATED ? wn * 32 : wn * WTN + jp * 32) + quad * 8;
+            if (row >= g.m || col >= g.n) continue;
+            float v[8], u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = acc[0][2 * jp + (e >> 2)][e & 3];
+                u[e] = GATED ? acc[0][(2 * jp + 2 + (e >> 2)) % FN][e & 3] : 0.f;
+            }
+            if (g.partial) {
+                const int parts = GATED ? 2 : g.outs, count = g.n - col < 8 ? (int)(g.n - col) : 8;
+                float* p = g.partial + (((long)split * parts + z) * g.m + row) * g.n + col;
+                store8(p, g.vec && count == 8, count, v);
+                if (GATED) store8(p + (long)g.m * g.n, g.vec && count == 8, count, u);
+            } else {
+                finish8<T, GATED>(g, z, row, (int)col, v, u);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r + 1 < FM; ++r)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[r][j] = acc[r + 1][j];
+    }
+}
+
+// The parts of a reduction that several workgroups took, added in their order, and the layer's arithmetic.  Without any part (k = 0)
+// the sums are zero.
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(256) product_join_kernel(const KernelArgs g) {
+    const long pieces = (g.n + 7) / 8, all = pieces * g.m * g.outs;
+    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < all; at += (long)gridDim.x * 256) {
+        const int j = (int)(at % pieces) * 8;
+        const long r = at / pieces;
+        const int z = (int)(r / g.m);
+        const long i = r - (long)z * g.m;
+        const int count = g.n - j < 8 ? g.n - j : 8, parts = GATED ? 2 : g.outs;
+        float v[8] = {}, u[8] = {};
+        for (int s = 0; s < g.splits; ++s) {
+            const float* p = g.partial + (((long)s * parts + z) * g.m + i) * g.n + j;
+            float w[8];
+            load8(p, 1, g.vec && count == 8, count, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += w[e];
+            if (GATED) {
+                load8(p + (long)g.m * g.n, 1, g.vec && count == 8, count, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[e] += w[e];
+            }
+        }
+        finish8<T, GATED>(g, z, i, j, v, u);
+    }
+}
+
+// ---- packing ------------------------------------------------------------------------------------
+// rows x cols values from any strides into rows `pitch` apart (whole 16-byte pieces; what lies past cols is left as it is: the products
+// clear it).  64 x 64 values go through LDS, read along the nearer stride.
+template <typename T>
+__global__ void __launch_bounds__(256) product_pack_kernel(const T* src, long row, long col, int rows, int cols, T* dst, long pitch, int along) {
+    __shared__ T tile[64][65];
+    const unsigned across = (unsigned)((cols + 63L) / 64);
+    const long r0 = (long)(blockIdx.x / across) * 64, c0 = (long)(blockIdx.x % across) * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int s = y; s < 64; s += 4) {
+        const int r = along ? x : s, c = along ? s : x;
+        if (r0 + r < rows && c0 + c < cols) tile[r][c] = src[(r0 + r) * row + (c0 + c) * col];
+    }
+    __syncthreads();
+    for (int s = y; s < 64; s += 4)
+        if (r0 + s < rows && c0 + x < cols) dst[(r0 + s) * pitch + c0 + x] = tile[s][x];
+}
+
+// ---- activation gradients and sums over rows ----------------------------------------------------------
+// A workgroup takes 256 columns (32 threads, eight columns each) of GRAD_ROWS rows; eight rows at a time.
+constexpr int GRAD_ROWS = 64;
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int vec, int chunks) {
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int blocks = (g.n + 255) / 256;
+    const int chunk = blockIdx.x / blocks;
+    const int j = (blockIdx.x - chunk * blocks) * 256 + tx * 8;
+    const int count = g.n - j < 8 ? g.n - j : 8;
+    const bool whole = vec && count == 8;
+    float sum[PAIR ? 2 : 1][8] = {};
+    if (j < g.n) {
+        const long r0 = (long)chunk * GRAD_ROWS;
+#pragma unroll 2
+        for (int s = ty; s < GRAD_ROWS; s += 8) {
+            const long i = r0 + s;
+            if (i >= g.m) break;
+            float dy[8];
+            load8((const T*)g.dy + i * g.n + j, 1, whole, count, dy);
+#pragma unroll
+            for (int f = 0; f < (PAIR ? 2 : 1); ++f) {
+                float v[8];
+                if (g.factors > f) {
+                    load8((const T*)g.d[f] + i * g.n + j, 1, whole, count, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= dy[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = dy[e];
+                }
+                if (g.dz[f]) store8((T*)g.dz[f] + i * g.pitch + j, whole, count, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[f][e] += v[e];
+            }
+        }
+    }
+    if (!g.partials) return;
+    __shared__ float part[8][32][9];
+#pragma unroll
+    for (int f = 0; f < (PAIR ? 2 : 1); ++f) {
+        if (!g.db[f]) continue;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[ty][tx][e] = sum[f][e];
+        __syncthreads();
+        const int c = threadIdx.x, col = (blockIdx.x - chunk * blocks) * 256 + c;
+        if (col < g.n) {
+            float v = 0.f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) v += part[y][c >> 3][c & 7];
+            g.partials[((long)f * chunks + chunk) * g.n + col] = v;
+        }
+    }
+}
+// Four rows of threads take the parts in turn; their sums are added in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256) row_sum_kernel(const float* partials, int chunks, int n, T* out0, T* out1) {
+    __shared__ float part[4][64];
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, f = blockIdx.y;
+    T* out = f ? out1 : out0;
+    if (!out) return;
+    const int j = blockIdx.x * 64 + x;
+    float v = 0.f;
+    if (j < n)
+        for (int c = y; c < chunks; c += 4) v += partials[((long)f * chunks + c) * n + j];
+    part[y][x] = v;
+    __syncthreads();
+    if (y == 0 && j < n) out[j] = (T)((part[0][x] + part[1][x]) + (part[2][x] + part[3][x]));
+}
+
+// ---- host side ----------------------------------------------------------------------------------------
+inline long up(long v, long m) { return (v + m - 1) / m * m; }
+inline int elem_size(int dtype) { return dtype == MUON_HIP_BF16 ? 2 : 4; }
+
+enum { LIE_ROWS = 0, LIE_STEPS = 1, LIE_PACKED = 2 };
+struct Plan {
+    int lie_a, lie_b;
+    long pitch_a, pitch_b;        // elements
+    long pack_a, pack_b;          // bytes of one packed matrix
+    int count_a, count_b;         // matrices of each operand
+    int tile, splits, per_split, nk, segments, outs;
+    long partial_bytes, bytes;
+};
+
+// How an operand is read: as it lies where 16-byte pieces of its rows (or of its reduction steps) are aligned and 32 bits span a tile of it.
+int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool steps_ok, long& pitch) {
+    const long piece = 16 / size;
+    auto fits = [&](long p, long lines) { return p % piece == 0 && p <= (0x7fff0000L / size) / lines; };
+    bool by_rows = true, by_steps = steps_ok;
+    for (int i = 0; i < count; ++i) {
+        if (((uintptr_t)o.base[i]) & 15) by_rows = by_steps = false;
+        // (one row, or one step, has no stride that matters)
+        if (!(o.col[i] == 1 || k == 1) || !(rows == 1 || (fits(o.row[i], 256) && o.row[i] == o.row[0]))) by_rows = false;
+        if (!(o.row[i] == 1 || rows == 1) || !(k == 1 || (fits(o.col[i], 64) && o.col[i] == o.col[0]))) by_steps = false;
+    }
+    if (k > 0x7fff0000L / size) by_rows = false;
+    if (by_rows) {
+        pitch = rows == 1 ? 0 : o.row[0];
+        return LIE_ROWS;
+    }
+    if (by_steps) {
+        pitch = k == 1 ? 0 : o.col[0];
+        return LIE_STEPS;
+    }
+    pitch = up(k, piece);
+    return LIE_PACKED;
+}
+
+bool make_plan(const ProductArgs& p, int cus, Plan& l) {
+    const int size = elem_size(p.dtype), bk = ROWB / size;
+    const bool gated = p.kind == PRODUCT_GATED;
+    l = Plan{};
+    l.count_a = p.kind == PRODUCT_SUM || p.kind == PRODUCT_EACH ? 2 : 1;
+    l.count_b = gated || p.kind == PRODUCT_SUM ? 2 : 1;
+    l.segments = p.kind == PRODUCT_SUM ? 2 : 1;
+    l.outs = p.kind == PRODUCT_EACH ? 2 : 1;
+    if (p.m == 0 || p.n == 0) return true;
+    if (p.k == 0) return true;
+    l.lie_a = lie_of(p.a, l.count_a, p.m, p.k, size, true, l.pitch_a);
+    l.lie_b = lie_of(p.b, l.count_b, p.n, p.k, size, !gated, l.pitch_b);
+    for (const long pitch : {l.lie_a == LIE_PACKED ? l.pitch_a : 0, l.lie_b == LIE_PACKED ? l.pitch_b : 0})
+        if (pitch > (0x7fff0000L / size) / 256) return false;
+    l.pack_a = l.lie_a == LIE_PACKED ? up(p.m * l.pitch_a * size, 256) : 0;
+    l.pack_b = l.lie_b == LIE_PACKED ? up(p.n * l.pitch_b * size, 256) : 0;
+    l.nk = (int)((p.k + (long)bk - 1) / bk);
+    auto tiles_of = [&](int t) { return up(p.m, t) / t * (up(p.n, gated ? t / 2 : t) / (gated ? t / 2 : t)) * l.outs; };
+    l.tile = tiles_of(256) >= cus ? 256 : tiles_of(128) >= cus ? 128 : 64;
+    const long tiles = tiles_of(l.tile), all = (long)l.nk * l.segments;
+    for (const long rows : {l.pack_a ? p.m : 0, l.pack_b ? p.n : 0})
+        if (up(p.k, 64) / 64 * (up(rows, 64) / 64) > 0x7fffffffL) return false;
+    if (all > 0x3fffffffL || tiles > 0x3fffffffL) return false;
+    long splits = 1;
+    if (tiles < cus) splits = cus / tiles;
+    if (splits > all / 4) splits = all / 4;
+    if (splits > 32) splits = 32;
+    if (splits < 1) splits = 1;
+    l.per_split = (int)((all + splits - 1) / splits);
+    l.splits = (int)((all + l.per_split - 1) / l.per_split);
+    if (tiles * l.splits > 0x7fffffffL) return false;
+    if (l.splits > 1) l.partial_bytes = (long)l.splits * (gated ? 2 : l.outs) * p.m * p.n * 4;
+    l.bytes = l.pack_a * l.count_a + l.pack_b * l.count_b + l.partial_bytes;
+    return true;
+}
+
+template <typename T, int BM, int BN, int WGM, int WGN, bool AS, bool BS, bool GATED>
+hipError_t launch_tiles(const KernelArgs& g, hipStream_t stream) {
+    constexpr int smem = 2 * (BM + BN) * ROWB;
+    static std::atomic<unsigned long long> configured{0};
+    const auto kern = product_kernel<T, BM, BN, WGM, WGN, AS, BS, GATED>;
+    if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
+    const long grid = (long)g.tiles_m * g.tiles_n * g.outs * g.splits;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(WGM * WGN * 64), smem, stream, g);
+    return hipGetLastError();
+}
+template <typename T, bool AS, bool BS, bool GATED>
+hipError_t launch_tile(int tile, const KernelArgs& g, hipStream_t s) {
+    if (tile == 256) return launch_tiles<T, 256, 256, 2, 4, AS, BS, GATED>(g, s);
+    if (tile == 128) return launch_tiles<T, 128, 128, 2, 2, AS, BS, GATED>(g, s);
+    return launch_tiles<T, 64, 64, 4, 1, AS, BS, GATED>(g, s);
+}
+
+template <typename T>
+hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int xcd_shift, hipStream_t s) {
+    constexpr int S = sizeof(T), BK = Elem<T>::BK;
+    const bool gated = p.kind == PRODUCT_GATED;
+    KernelArgs g{};
+    char* ws = (char*)workspace;
+    auto pack = [&](const ProductOperand& o, int lie, int count, int rows, long pitch, long bytes, const void** at) {
+        for (int i = 0; i < count; ++i) {
+            at[i] = o.base[i];
+            if (lie != LIE_PACKED) continue;
+            const int along = o.row[i] < o.col[i];
+            const dim3 grid((unsigned)(up(p.k, 64) / 64 * (up(rows, 64) / 64)));
+            hipLaunchKernelGGL(product_pack_kernel<T>, grid, dim3(256), 0, s, (const T*)o.base[i], o.row[i], o.col[i], rows, p.k, (T*)ws, pitch, along);
+            if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            at[i] = ws;
+            ws += bytes;
+        }
+        return hipSuccess;
+    };
+    g.m = p.m;
+    g.n = p.n;
+    g.k = p.k;
+    g.outs = l.outs;
+    g.act = p.act;
+    for (int i = 0; i < 2; ++i) {
+        g.bias[i] = p.bias[i];
+        g.out[i] = p.out[i];
+        g.aux[i] = p.aux[i];
+    }
+    g.residual = p.residual;
+    g.res_row = p.res_row;
+    g.res_col = p.res_col;
+    auto aligned = [](const void* q) { return (((uintptr_t)q) & 15) == 0; };
+    g.vec = p.n % 8 == 0 && aligned(p.out[0]) && aligned(p.out[1]) && aligned(p.aux[0]) && aligned(p.aux[1]);
+    g.vec_res = p.residual && p.n % 8 == 0 && p.res_col == 1 && p.res_row % (16 / S) == 0 && aligned(p.residual);
+    g.xcd_shift = xcd_shift;
+    if (p.k > 0) {
+        if (hipError_t e = pack(p.a, l.lie_a, l.count_a, p.m, l.pitch_a, l.pack_a, g.a); e != hipSuccess) return e;
+        if (hipError_t e = pack(p.b, l.lie_b, l.count_b, p.n, l.pitch_b, l.pack_b, g.b); e != hipSuccess) return e;
+        g.pitch_a = l.pitch_a;
+        g.pitch_b = l.pitch_b;
+        g.nk = l.nk;
+        g.segments = l.segments;
+        g.splits = l.splits;
+        g.per_split = l.per_split;
+        const int tn = gated ? l.tile / 2 : l.tile;
+        g.tiles_m = (int)(up(p.m, l.tile) / l.tile);
+        g.tiles_n = (int)(up(p.n, tn) / tn);
+        g.partial = l.splits > 1 ? (float*)ws : nullptr;
+        const bool as = l.lie_a == LIE_STEPS, bs = l.lie_b == LIE_STEPS;
+        hipError_t e;
+        if (gated) e = as ? launch_tile<T, true, false, true>(l.tile, g, s) : launch_tile<T, false, false, true>(l.tile, g, s);
+        else if (as) e = bs ? launch_tile<T, true, true, false>(l.tile, g, s) : launch_tile<T, true, false, false>(l.tile, g, s);
+        else e = bs ? launch_tile<T, false, true, false>(l.tile, g, s) : launch_tile<T, false, false, false>(l.tile, g, s);
+        if (e != hipSuccess || l.splits == 1) return e;
+    }
+    const long work = up(p.n, 8) / 8 * p.m * l.outs;
+    const unsigned grid = (unsigned)(up(work, 256) / 256 < 65536 ? up(work, 256) / 256 : 65536);
+    if (gated) hipLaunchKernelGGL((product_join_kernel<T, true>), dim3(grid), dim3(256), 0, s, g);
+    else hipLaunchKernelGGL((product_join_kernel<T, false>), dim3(grid), dim3(256), 0, s, g);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+long product_workspace(const ProductArgs& p, int cus) {
+    Plan l;
+    return make_plan(p, cus, l) ? l.bytes : -1;
+}
+
+hipError_t launch_product(const ProductArgs& p, void* workspace, int cus, int xcd_shift, hipStream_t stream) {
+    Plan l;
+    if (!make_plan(p, cus, l)) return hipErrorInvalidValue;
+    if (p.m == 0 || p.n == 0) return hipSuccess;
+    return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, xcd_shift, stream) : run_product<float>(p, l, workspace, xcd_shift, stream);
+}
+
+long act_grad_partials(long m, long n) { return up(m, GRAD_ROWS) / GRAD_ROWS * n; }
+
+hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t stream) {
+    const bool pair = a.factors > 1;
+    const long chunks = up(a.m, GRAD_ROWS) / GRAD_ROWS, blocks = up(a.n, 256) / 256 * chunks;
+    auto aligned = [](const void* q) { return (((uintptr_t)q) & 15) == 0; };
+    const int vec = a.n % 8 == 0 && a.pitch % 8 == 0 && aligned(a.dy) && aligned(a.d[0]) && aligned(a.d[1]) && aligned(a.dz[0]) && aligned(a.dz[1]);
+    const bool bf = a.dtype == MUON_HIP_BF16;
+    if (blocks > 0) {
+        if (bf && pair) hipLaunchKernelGGL((act_grad_kernel<bf16_t, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
+        else if (bf) hipLaunchKernelGGL((act_grad_kernel<bf16_t, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
+        else if (pair) hipLaunchKernelGGL((act_grad_kernel<float, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
+        else hipLaunchKernelGGL((act_grad_kernel<float, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    if ((!a.db[0] && !a.db[1]) || a.n == 0) return hipSuccess;
+    const dim3 grid((unsigned)(up(a.n, 64) / 64), pair ? 2 : 1);
+    if (bf) hipLaunchKernelGGL(row_sum_kernel<bf16_t>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (bf16_t*)a.db[0], (bf16_t*)a.db[1]);
+    else hipLaunchKernelGGL(row_sum_kernel<float>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (float*)a.db[0], (float*)a.db[1]);
+    return hipGetLastError();
+}

@@ -1,0 +1,391 @@
+"""linear and gated_linear against their formulas in 64 bits: results and every gradient, at the sizes, layouts and values where tiles,
+reductions and masks can go wrong.  Bounds: tests/layer_reference.py."""
+import itertools
+
+import pytest
+import torch
+
+import lmms_engine_amd as E
+from lmms_engine_amd import _abi, layers
+from lmms_engine_amd.clip_grad import clip_grad_norm_
+from tests import layer_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F = torch.bfloat16, torch.float32
+
+
+def rnd(gen, *shape, scale=1.0, dtype=BF):
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(dtype)
+
+
+def gen_of(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def run_linear(x, w, b, r, name, dy):
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    for t in leaves:
+        t.requires_grad_(True)
+    y = E.linear(x, w, b, activation=name, residual=r)
+    grads = iter(torch.autograd.grad(y, leaves, dy))
+    got = {"y": y, "dx": next(grads), "dw": next(grads)}
+    if b is not None:
+        got["db"] = next(grads)
+    if r is not None:
+        got["dr"] = next(grads)
+    with torch.no_grad():  # the call that keeps nothing gives the same bits
+        assert torch.equal(E.linear(x, w, b, activation=name, residual=r).view(torch.uint8), y.detach().view(torch.uint8))
+    return got
+
+
+def run_gated(x, wg, wu, bg, bu, name, dh):
+    leaves = [t for t in (x, wg, wu, bg, bu) if t is not None]
+    for t in leaves:
+        t.requires_grad_(True)
+    y = E.gated_linear(x, wg, wu, bg, bu, activation=name)
+    names = ["dx", "dw0", "dw1"] + (["db0"] if bg is not None else []) + (["db1"] if bu is not None else [])
+    got = {"y": y, **dict(zip(names, torch.autograd.grad(y, leaves, dh)))}
+    with torch.no_grad():
+        assert torch.equal(E.gated_linear(x, wg, wu, bg, bu, activation=name).view(torch.uint8), y.detach().view(torch.uint8))
+    return got
+
+
+def compare(got, want):
+    for name, value in got.items():
+        R.check(name, value.reshape(want[name][0].shape), *want[name])
+
+
+# tokens, inner, outer: single values and rows, the edges of pieces, fragments, tiles and k-tiles, long reductions over few results
+SIZES = [(1, 1, 1), (1, 64, 8), (3, 8, 5), (2, 7, 64), (16, 64, 64), (17, 251, 33), (64, 128, 64), (65, 130, 129), (130, 72, 264), (33, 1000, 77),
+         (257, 96, 520), (1, 4096, 512), (5, 2049, 130), (2000, 24, 40), (700, 200, 1000)]
+ACTS = list(layers.ACTIVATIONS)
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=["x".join(map(str, s)) for s in SIZES])
+def test_linear(dtype, i, size):
+    t, k, n = size
+    g = gen_of(i)
+    name, bias, residual = ACTS[i % 6], i % 2 == 0, i % 3 != 0
+    x, w = rnd(g, t, k, dtype=dtype), rnd(g, n, k, scale=k ** -0.5, dtype=dtype)
+    b = rnd(g, n, dtype=dtype) if bias else None
+    r = rnd(g, t, n, dtype=dtype) if residual else None
+    dy = rnd(g, t, n, dtype=dtype)
+    compare(run_linear(x, w, b, r, name, dy), R.linear(x, w, b, r, name, dy, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=["x".join(map(str, s)) for s in SIZES])
+def test_gated_linear(dtype, i, size):
+    t, k, n = size
+    g = gen_of(100 + i)
+    name = ACTS[(i + 3) % 6]
+    x = rnd(g, t, k, dtype=dtype)
+    wg, wu = (rnd(g, n, k, scale=k ** -0.5, dtype=dtype) for _ in range(2))
+    bg, bu = (rnd(g, n, dtype=dtype) if i % 4 in wanted else None for wanted in ((1, 3), (2, 3)))
+    dh = rnd(g, t, n, dtype=dtype)
+    compare(run_gated(x, wg, wu, bg, bu, name, dh), R.gated(x, wg, wu, bg, bu, name, dh, dtype))
+
+
+# Results of many tiles: every tile size, also for gradients, whole and ragged in every direction.
+LARGE = [(2060, 200, 2056), (4100, 136, 4200), (136, 4100, 4200), (4100, 4200, 72), (4352, 320, 4096), (1024, 1024, 1024), (4099, 100, 4103)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("i,size", list(enumerate(LARGE)), ids=["x".join(map(str, s)) for s in LARGE])
+def test_many_tiles(dtype, i, size):
+    t, k, n = size
+    g = gen_of(200 + i)
+    x, w, w2, b = rnd(g, t, k, dtype=dtype), *(rnd(g, n, k, scale=k ** -0.5, dtype=dtype) for _ in range(2)), rnd(g, n, dtype=dtype)
+    r, dy = rnd(g, t, n, dtype=dtype), rnd(g, t, n, dtype=dtype)
+    name = ("gelu", "none")[i % 2]
+    compare(run_linear(x, w, b, r, name, dy), R.linear(x, w, b, r, name, dy, dtype))
+    compare(run_gated(x, w, w2, None, b, "silu", dy), R.gated(x, w, w2, None, b, "silu", dy, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("name", ACTS)
+def test_activations_from_end_to_end(dtype, name):
+    """Every activation over its whole range, subnormal and huge arguments included: z = x * 1 is the argument itself."""
+    v = torch.cat([torch.linspace(-30, 30, 1501), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-39, 88.8, -88.8, 200.0, -200.0, 1e4, -1e4, 1e18, -1e18])])
+    x = v.to(dtype).to(DEV)[:, None]
+    one = torch.ones(1, 1, dtype=dtype, device=DEV)
+    dy = torch.ones_like(x)
+    compare(run_linear(x, one, None, None, name, dy), R.linear(x, one, None, None, name, dy, dtype))
+    compare(run_gated(x, one, one.detach().clone(), None, None, name, dy), R.gated(x, one, one, None, None, name, dy, dtype))
+
+
+@pytest.mark.parametrize("size", [(0, 8, 4), (5, 0, 7), (4, 8, 0), (0, 0, 0), (0, 5, 3)], ids=str)
+def test_empty_sizes(size):
+    t, k, n = size
+    g = gen_of(7)
+    x, w, b, r, dy = rnd(g, t, k), rnd(g, n, k), rnd(g, n), rnd(g, t, n), rnd(g, t, n)
+    compare(run_linear(x, w, b, r, "silu", dy), R.linear(x, w, b, r, "silu", dy, BF))
+    compare(run_gated(x, w, w.detach().clone(), b, b.detach().clone(), "gelu", dy), R.gated(x, w, w, b, b, "gelu", dy, BF))
+
+
+def layouts(g, rows, cols, dtype):
+    """The same kind of matrix in the layouts that callers have; what lies around it is NaN."""
+    def inside(shape, cut):
+        buf = torch.full(shape, float("nan"), dtype=dtype, device=DEV)
+        view = cut(buf)
+        view.copy_(rnd(g, *view.shape, dtype=dtype))
+        return view
+
+    yield "transposed", inside((cols, rows), lambda b: b.t())
+    yield "wide rows", inside((rows, cols + 16), lambda b: b[:, 8:8 + cols])
+    yield "odd offset", inside((rows, cols + 3), lambda b: b[:, 1:1 + cols])
+    yield "transposed of wide rows", inside((cols, rows + 24), lambda b: b[:, 16:16 + rows].t())
+    yield "every other", inside((rows, 2 * cols), lambda b: b[:, ::2])
+    yield "aligned rows of odd length", inside((rows, -(-cols // 8) * 8 + 8), lambda b: b[:, :cols])
+    yield "one row for all", rnd(g, 1, cols, dtype=dtype).expand(rows, cols)
+    yield "one value per row", rnd(g, rows, 1, dtype=dtype).expand(rows, cols)
+
+
+LAYOUTS = ["transposed", "wide rows", "odd offset", "transposed of wide rows", "every other", "aligned rows of odd length", "one row for all",
+           "one value per row"]
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("size", [(72, 136, 200), (45, 99, 70)], ids=str)
+@pytest.mark.parametrize("which", ["x", "w", "r", "dy"])
+def test_layouts(which, size, dtype):
+    t, k, n = size
+    shape = dict(x=(t, k), w=(n, k), r=(t, n), dy=(t, n))[which]
+    for i, (name, view) in enumerate(layouts(gen_of(3), *shape, dtype)):
+        assert name == LAYOUTS[i]
+        g = gen_of(50 + i)
+        v = dict(x=rnd(g, t, k, dtype=dtype), w=rnd(g, n, k, scale=k ** -0.5, dtype=dtype), r=rnd(g, t, n, dtype=dtype), dy=rnd(g, t, n, dtype=dtype))
+        v[which] = view.detach()
+        for act in ("none", "silu"):
+            compare(run_linear(v["x"].detach(), v["w"].detach(), None, v["r"].detach(), act, v["dy"]), R.linear(v["x"], v["w"], None, v["r"], act, v["dy"], dtype))
+        if which == "r":
+            continue
+        other = rnd(g, n, k, scale=k ** -0.5, dtype=dtype)
+        for wg, wu in ((v["w"], other), (other, v["w"])):
+            compare(run_gated(v["x"].detach(), wg.detach(), wu.detach(), None, None, "silu", v["dy"]),
+                    R.gated(v["x"], wg, wu, None, None, "silu", v["dy"], dtype))
+
+
+def test_leading_dimensions():
+    g = gen_of(9)
+    x, w, r = rnd(g, 3, 5, 40), rnd(g, 24, 40, scale=0.2), rnd(g, 3, 5, 24)
+    y = E.linear(x, w, residual=r)
+    assert y.shape == (3, 5, 24) and torch.equal(y.view(15, 24), E.linear(x.view(15, 40), w, residual=r.view(15, 24)))
+    t = x.transpose(0, 1)
+    assert torch.equal(E.linear(t, w), E.linear(t.contiguous(), w))
+    one = E.linear(x[0, 0], w)
+    assert one.shape == (24,) and torch.equal(one, E.linear(x, w)[0, 0])
+    assert E.gated_linear(x[1, 2], w, w).shape == (24,)
+    x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(E.linear(x.transpose(0, 1), w).float().sum(), x)
+    assert dx.shape == x.shape
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    """A NaN or an infinity of x or W reaches the results that contain it and no other; so do gradients."""
+    g = gen_of(11)
+    t, k, n = 140, 200, 150
+    x, w, dy = rnd(g, t, k), rnd(g, n, k, scale=0.1), rnd(g, t, n)
+    clean = E.linear(x, w)
+    x[7, 3], x[131, 199], w[149, 0] = float("nan"), float("inf"), float("-inf")
+    y = E.linear(x, w)
+    want = x.double() @ w.double().t()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    keep = torch.isfinite(want)
+    assert torch.equal(y[keep], clean[keep])
+    dy[3, 5] = float("nan")
+    dx, dw = torch.autograd.grad(E.linear(x.requires_grad_(True), w.requires_grad_(True)), (x, w), dy)
+    assert torch.isnan(dx[3]).all() and torch.isfinite(dx[4, 1:]).all()
+    assert torch.isnan(dw[5]).all() and torch.isfinite(dw[6, :3]).all() and torch.isnan(dw[6, 3]) and not torch.isfinite(dw[6, 199])
+
+
+def test_each_gradient_alone():
+    """What is not asked for is not computed, and what is asked for does not depend on what else is."""
+    g = gen_of(13)
+    t, k, n = 50, 72, 88
+    make = dict(x=rnd(g, t, k), wg=rnd(g, n, k, scale=0.2), wu=rnd(g, n, k, scale=0.2), bg=rnd(g, n), bu=rnd(g, n))
+    dh = rnd(g, t, n)
+
+    def grads(names):
+        v = {m: a.clone().requires_grad_(m in names) for m, a in make.items()}
+        y = E.gated_linear(v["x"], v["wg"], v["wu"], v["bg"], v["bu"])
+        return dict(zip(names, torch.autograd.grad(y, [v[m] for m in names], dh)))
+
+    whole = grads(list(make))
+    for some in itertools.chain(itertools.combinations(make, 1), itertools.combinations(make, 2)):
+        for m, a in grads(list(some)).items():
+            assert torch.equal(a, whole[m]), (some, m)
+    lin = dict(x=make["x"], w=make["wg"], b=make["bg"], r=rnd(g, t, n))
+
+    def lgrads(names, act):
+        v = {m: a.clone().requires_grad_(m in names) for m, a in lin.items()}
+        return dict(zip(names, torch.autograd.grad(E.linear(v["x"], v["w"], v["b"], activation=act, residual=v["r"]), [v[m] for m in names], dh)))
+
+    for act in ("none", "gelu"):
+        whole = lgrads(list(lin), act)
+        for some in itertools.combinations(lin, 1):
+            for m, a in lgrads(list(some), act).items():
+                assert torch.equal(a, whole[m]), (act, m)
+
+
+def test_gradients_against_differences():
+    """The gradients of a scalar against central differences of the function itself, in fp32: a step of 2^-6 along a random direction.
+    The differences are off by the third derivative (a sixth of the step squared times it) and by the rounding of two sums."""
+    g = gen_of(17)
+    t, k, n = 12, 40, 24
+    for name in ("sigmoid", "silu", "gelu", "gelu_tanh"):
+        v = [rnd(g, t, k, dtype=F), rnd(g, n, k, scale=0.15, dtype=F), rnd(g, n, k, scale=0.15, dtype=F), rnd(g, n, dtype=F), rnd(g, n, dtype=F)]
+        c = rnd(g, t, n, dtype=F).double()
+        for f in (lambda a: E.gated_linear(*a, activation=name), lambda a: E.linear(a[0], a[1], a[3], activation=name)):
+            leaves = [a.clone().requires_grad_(True) for a in v]
+            grads = torch.autograd.grad(f(leaves), leaves, c.float(), allow_unused=True)
+            for i, gi in enumerate(grads):
+                if gi is None:
+                    continue
+                d = rnd(g, *v[i].shape, dtype=F)
+                d /= d.norm()
+                h = 2.0 ** -6
+                with torch.no_grad():
+                    up, down = (f([a + s * h * d if j == i else a for j, a in enumerate(v)]).double() for s in (1, -1))
+                slope = ((up - down) * c).sum().item() / (2 * h)
+                told = (gi.double() * d.double()).sum().item()
+                # |x| <= 6, |w| <= 1: a direction of norm 1 moves z by at most 7, third derivatives of the factors stay below 2 * 7^3 * max(1, |u|)
+                room = (h * h / 6 * 2 * 7 ** 3 * 8 * c.abs().mean().item() + 2 ** -22 * 8 * c.abs().sum().item() / h)
+                assert abs(slope - told) <= room, (name, i, slope, told, room)
+
+
+def test_rows_behind_the_result_are_left_alone():
+    """Results at the end of a tile that reaches past them: what lies around them in memory stays as it was."""
+    g = gen_of(19)
+    for (t, k, n), kind in itertools.product([(5, 64, 24), (70, 64, 72), (130, 520, 9)], (_abi.PRODUCT_LINEAR, _abi.PRODUCT_GATED, _abi.PRODUCT_EACH)):
+        x, x2, w, w2 = rnd(g, t, k), rnd(g, t, k), rnd(g, n, k), rnd(g, n, k)
+        bufs = [torch.full((t * n + 4096,), 7.0, dtype=BF, device=DEV) for _ in range(2)]
+        out = [b[2048:2048 + t * n].view(t, n) for b in bufs]
+        a = layers._operands(x, x2) if kind == _abi.PRODUCT_EACH else layers._operands(x)
+        layers._run(kind, x, t, n, k, a, layers._operands(w, w2), out, act=0)
+        for o, b, left in zip(out, bufs, (x, x2)):
+            assert (b[:2048] == 7).all() and (b[2048 + t * n:] == 7).all()
+            if kind == _abi.PRODUCT_EACH:
+                assert torch.equal(o, E.linear(left, w))
+        if kind != _abi.PRODUCT_EACH:
+            assert (bufs[1] == 7).all()
+            assert torch.equal(out[0], E.linear(x, w) if kind == _abi.PRODUCT_LINEAR else E.gated_linear(x, w, w2, activation="none"))
+
+
+def test_results_past_four_gib():
+    """Rows whose elements are more than 2^32 bytes from the first."""
+    t, k, n = 2 ** 17 + 3, 64, 20000
+    g = gen_of(23)
+    x, w = rnd(g, t, k), rnd(g, n, k, scale=0.1)
+    y = E.linear(x, w)
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 40), slice(t // 2, t // 2 + 40), slice(t - 40, t)):
+        want = R.linear(x[rows], w, None, None, "none", torch.zeros(40, n, device=DEV), BF)
+        R.check("y", y[rows], *want["y"])
+    # and as an operand: the gradient of x reads all of it
+    dx = E.linear(y, w.t())
+    rows = slice(t - 40, t)
+    R.check("dx", dx[rows], *R.linear(y[rows], w.t(), None, None, "none", torch.zeros(40, k, device=DEV), BF)["y"])
+
+
+def block(x, p):
+    """A feed-forward block with its residual."""
+    return E.linear(E.gated_linear(x, p["gate"], p["up"]), p["down"], residual=x)
+
+
+def block_by_torch(x, p):
+    v = torch.nn.functional
+    return x + v.linear(v.silu(v.linear(x, p["gate"])) * v.linear(x, p["up"]), p["down"])
+
+
+def test_a_block_is_trained_by_the_step():
+    """The operators as a training loop uses them: forward, loss gradient, backward into .grad, clipping, Muon step.  The gradients are those of
+    the block in 64 bits; what the step makes of them is what it makes of the same gradients without the operators."""
+    g = gen_of(29)
+    d, inter, t = 128, 320, 200
+    init = {"gate": rnd(g, inter, d, scale=d ** -0.5), "up": rnd(g, inter, d, scale=d ** -0.5), "down": rnd(g, d, inter, scale=inter ** -0.5)}
+    mine = {m: torch.nn.Parameter(a.clone()) for m, a in init.items()}
+    twin = {m: torch.nn.Parameter(a.clone()) for m, a in init.items()}
+    opts = [E.Muon([dict(params=list(p.values()), use_muon=True, lr=0.02, rms_scale=False)]) for p in (mine, twin)]
+    for step in range(3):
+        x, dy = rnd(g, 4, t // 4, d), rnd(g, 4, t // 4, d, scale=1e-2)
+        y = block(x, mine)
+        y.backward(dy)
+        wide = {m: a.detach().double().requires_grad_(True) for m, a in mine.items()}
+        grads = torch.autograd.grad(block_by_torch(x.double(), wide), list(wide.values()), dy.double())
+        for (m, p), want, (_, q) in zip(mine.items(), grads, twin.items()):
+            # h, its factors and two gradients are rounded to bf16 on the way (each 2^-8 of its own size at most, so less of a sum's norm)
+            err = ((p.grad.double() - want).norm() / want.norm()).item()
+            assert err <= 5 * 2.0 ** -8, (step, m, err)
+            q.grad = p.grad.clone()
+        for params, opt in zip((mine, twin), opts):
+            clip_grad_norm_(params.values(), 1.0)
+            opt.step()
+            opt.zero_grad(set_to_none=True)
+        for m in mine:
+            assert torch.equal(mine[m], twin[m])
+            assert not torch.equal(mine[m], init[m])
+
+
+def test_forward_and_backward_in_a_graph():
+    """Recorded once, replayed with other inputs in the same memory, with eager calls and synchronizations between."""
+    g = gen_of(31)
+    t, k, n = 96, 256, 200
+    x, dy = rnd(g, t, k).requires_grad_(True), rnd(g, t, n)
+    w = [rnd(g, n, k, scale=0.1).requires_grad_(True) for _ in range(2)]
+    b = rnd(g, n).requires_grad_(True)
+
+    def both():
+        h = E.gated_linear(x, w[0], w[1], b, None)
+        y = E.linear(x, w[0], b, activation="gelu", residual=h)
+        return [y, *torch.autograd.grad(y, [x, *w, b], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for r in range(4):
+        with torch.no_grad():
+            x.copy_(rnd(g, t, k))
+            dy.copy_(rnd(g, t, n))
+            b.copy_(rnd(g, n))
+        graph.replay()
+        torch.cuda.synchronize()
+        now = [a.detach().clone() for a in held]
+        for a, e in zip(now, both()):
+            assert torch.equal(a, e.detach()), r
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: each gives what it gives alone."""
+    g = gen_of(37)
+    x, w = rnd(g, 48, 4096), rnd(g, 520, 4096, scale=0.02)
+    x2, w2 = rnd(g, 40, 4096), rnd(g, 520, 4096, scale=0.02)
+    want, want2 = E.linear(x, w, activation="silu"), E.gated_linear(x2, w, w2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (s1, s2):
+        s.wait_stream(torch.cuda.current_stream())
+    got, got2 = [], []
+    for _ in range(8):
+        with torch.cuda.stream(s1):
+            got.append(E.linear(x, w, activation="silu"))
+        with torch.cuda.stream(s2):
+            got2.append(E.gated_linear(x2, w, w2))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) for a in got) and all(torch.equal(a, want2) for a in got2)
+
+
+def test_the_same_call_gives_the_same_bits():
+    g = gen_of(41)
+    x, w, dy = rnd(g, 300, 2000), rnd(g, 264, 2000, scale=0.02), rnd(g, 300, 264)
+    first = run_linear(x, w, None, None, "silu", dy)
+    for _ in range(3):
+        for m, a in run_linear(x, w, None, None, "silu", dy).items():
+            assert torch.equal(a, first[m]), m

@@ -1,0 +1,128 @@
+"""What linear, gated_linear and the entry points behind them refuse, before anything is launched: no GPU needed."""
+import ctypes
+
+import pytest
+import torch
+
+import lmms_engine_amd as E
+from lmms_engine_amd import _abi, layers
+
+
+def test_cpu_tensors_and_wrong_arguments_are_refused():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    with pytest.raises(_abi.MuonHipError, match="no CPU path"):
+        E.linear(x, w)
+    with pytest.raises(_abi.MuonHipError, match="no CPU path"):
+        E.gated_linear(x, w, w)
+    with pytest.raises(ValueError, match="activation is one of none, relu"):
+        E.linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="activation is one of"):
+        E.gated_linear(x, w, w, activation=None)
+    with pytest.raises(TypeError):
+        E.linear(x, w, None, "silu")  # the activation is named
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on a GPU: what is checked behind that, without one."""
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+def gpu(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu)
+
+
+@pytest.mark.parametrize("make,error,match", [
+    (lambda: E.linear(gpu(2, 8), gpu(4, 9)), ValueError, "do not fit"),
+    (lambda: E.linear(gpu(2, 8), gpu(8)), ValueError, "do not fit"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8).sum()), ValueError, "do not fit"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8).view(1, 4, 8)), ValueError, "do not fit"),
+    (lambda: E.linear(gpu(2, 8).sum(), gpu(4, 8)), ValueError, "dimension"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8), gpu(1)), ValueError, "bias has shape"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8), gpu(1, 4)), ValueError, "bias has shape"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8), residual=gpu(4)), ValueError, "residual has shape"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8), residual=gpu(1, 4)), ValueError, "residual has shape"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8, dtype=torch.float32)), TypeError, "share one type"),
+    (lambda: E.linear(gpu(2, 8), gpu(4, 8), gpu(4, dtype=torch.float32)), TypeError, "share one type"),
+    (lambda: E.linear(gpu(2, 8, dtype=torch.float16), gpu(4, 8, dtype=torch.float16)), TypeError, "float32 and bfloat16"),
+    (lambda: E.linear(gpu(2, 8, dtype=torch.int32), gpu(4, 8, dtype=torch.int32)), TypeError, "float32 and bfloat16"),
+    (lambda: E.gated_linear(gpu(2, 8), gpu(4, 8), gpu(5, 8)), ValueError, "do not fit"),
+    (lambda: E.gated_linear(gpu(2, 8), gpu(4, 8), gpu(4, 8), None, gpu(5)), ValueError, "bias has shape"),
+    (lambda: E.gated_linear(gpu(2, 8), gpu(4, 8), torch.zeros(4, 8, dtype=torch.bfloat16)), _abi.MuonHipError, "no CPU path"),
+])
+def test_shapes_and_types_are_refused(make, error, match):
+    with pytest.raises(error, match=match):
+        make()
+
+
+def valid(kind=0):
+    p = _abi.Product(kind=kind, dtype=_abi.BF16, m=16, n=16, k=16)
+    one = 1 << 20  # never read: every call below is refused
+    for f in ("a", "b"):
+        getattr(p, f)[:] = (one, one)
+        getattr(p, f + "_row")[:] = (16, 16)
+        getattr(p, f + "_col")[:] = (1, 1)
+    p.out[:] = (one, one)
+    return p
+
+
+@pytest.mark.parametrize("kind,change,match", [
+    (9, {}, "kind"),
+    (-1, {}, "kind"),
+    (0, dict(dtype=7), "dtype"),
+    (0, dict(activation=6), "activation"),
+    (0, dict(activation=-1), "activation"),
+    (0, dict(m=-1), "negative"),
+    (0, dict(k=-3), "negative"),
+    (0, dict(a_row=(-16, 16)), "negative"),
+    (2, dict(b_col=(1, -1)), "negative"),
+    (0, dict(a=(None, None)), "null operand"),
+    (1, dict(b=(1 << 20, None)), "null operand"),
+    (2, dict(a=(1 << 20, None)), "null operand"),
+    (3, dict(out=(1 << 20, None)), "null result"),
+    (0, dict(aux=(None, 1 << 20)), "second results"),
+    (1, dict(aux=(1 << 20, None)), "second results"),
+    (1, dict(residual=1 << 20), "residual"),
+    (0, dict(bias=(None, 1 << 20)), "two biases"),
+    (2, dict(bias=(1 << 20, None)), "sums of products"),
+    (3, dict(activation=3), "sums of products"),
+    (2, dict(residual=1 << 20), "sums of products"),
+])
+def test_products_are_checked_before_any_launch(kind, change, match):
+    lib, p = _abi.lib(), valid(kind)
+    for name, v in change.items():
+        if isinstance(v, tuple):
+            getattr(p, name)[:] = v
+        else:
+            setattr(p, name, v)
+    at = ctypes.addressof(p)
+    assert lib.muon_hip_product_run(at, None, 0, None) == -1
+    assert match in lib.muon_hip_last_error().decode()
+    assert lib.muon_hip_product_workspace(at) == -1
+
+
+def test_null_products_and_empty_results():
+    lib = _abi.lib()
+    assert lib.muon_hip_product_run(None, None, 0, None) == -1
+    p = _abi.Product(kind=0, dtype=_abi.F32, m=0, n=5, k=3)
+    assert lib.muon_hip_product_run(ctypes.addressof(p), None, 0, None) == 0  # nothing to write, nothing to read
+
+
+def test_activation_gradients_are_checked_before_any_launch():
+    lib, one = _abi.lib(), 1 << 20
+    run = lib.muon_hip_act_grad
+    assert run(one, 1, one, None, one, None, 8, None, None, 5, 4, 8, None, None) == -1  # dtype
+    assert run(one, 1, one, None, one, None, 7, None, None, 1, 4, 8, None, None) == -1  # rows that overlap
+    assert run(one, 1, one, None, one, one, 8, None, None, 1, 4, 8, None, None) == -1  # a second result of one factor
+    assert run(one, 2, None, one, one, one, 8, None, None, 1, 4, 8, None, None) == -1  # a second factor alone
+    assert run(one, 2, one, one, one, None, 8, None, None, 1, 4, 8, None, None) == -1  # one product of two
+    assert run(one, 3, one, one, one, one, 8, None, None, 1, 4, 8, None, None) == -1
+    assert run(None, 1, one, None, one, None, 8, None, None, 1, 4, 8, None, None) == -1
+    assert run(one, 1, one, None, one, None, 8, one, None, 1, 4, 8, None, None) == -1  # sums without room for their parts
+    assert lib.muon_hip_act_grad_partials(0, 5) == 0 and lib.muon_hip_act_grad_partials(65, 3) == 6
+
+
+def test_activation_names_are_those_of_the_header():
+    assert layers.ACTIVATIONS == ("none", "relu", "sigmoid", "silu", "gelu", "gelu_tanh")
