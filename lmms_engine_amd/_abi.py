@@ -162,6 +162,27 @@ def scan():
     return _scan
 
 
+_layers = None
+
+
+def layers():
+    """The native form of linear and gated_linear (csrc/layers.cpp)."""
+    global _layers
+    if _layers is None:
+        lib()  # a library that is missing is reported as such
+        try:
+            from . import _layers as module
+        except ImportError as e:
+            raise MuonHipError(f"the module lmms_engine_amd._layers cannot be loaded ({e}): build it with `python -m lmms_engine_amd.build`") from e
+        of = getattr(module, "torch_version", "of another kind")
+        if of != torch.__version__:  # as for _scan
+            raise MuonHipError(f"lmms_engine_amd._layers was built for torch {of}, this is {torch.__version__}: "
+                               "build it again with `python -m lmms_engine_amd.build`")
+        module.set_error(MuonHipError)
+        _layers = module
+    return _layers
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = lib().muon_hip_last_error().decode()

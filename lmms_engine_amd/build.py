@@ -21,6 +21,8 @@ PROBE_SOURCES = ["probe.hip"]
 # Reads lists of torch tensors for the optimizer step (host code; a Python module, since it handles Python objects).  Its name says
 # which Python it is for, and it carries the version of the torch whose headers it was compiled with (checked when it is loaded).
 SCAN_LIB = os.path.join(HERE, "_scan" + sysconfig.get_config_var("EXT_SUFFIX"))
+# linear and gated_linear between torch and the library: host code too, under the same conditions, linked against the library beside it.
+LAYERS_LIB = os.path.join(HERE, "_layers" + sysconfig.get_config_var("EXT_SUFFIX"))
 # Packed-fp32 VALU forms stay off for every device function.
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -59,23 +61,35 @@ def _compile_and_link(sources, lib, hipcc, verbose):
     return lib
 
 
-def _build_scan(verbose):
+def _build_module(source, out, define, flags, verbose):
+    """A Python module from one host source, with the headers of the torch that is installed."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DSCAN_TORCH_VERSION="{torch.__version__}"', *[f"-isystem{p}" for p in include_paths()], f"-isystem{sysconfig.get_paths()['include']}", os.path.join(CSRC, "scan.cpp"), "-o", SCAN_LIB,
-           *[f"-L{p}" for p in library_paths()], "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+           f'-D{define}="{torch.__version__}"', *[f"-isystem{p}" for p in include_paths()], f"-isystem{sysconfig.get_paths()['include']}", os.path.join(CSRC, source), "-o", out,
+           *[f"-L{p}" for p in library_paths()], *flags, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on scan.cpp:\n{r.stdout}")
+        raise RuntimeError(f"g++ failed on {source}:\n{r.stdout}")
+
+
+def _build_scan(verbose):
+    _build_module("scan.cpp", SCAN_LIB, "SCAN_TORCH_VERSION", [], verbose)
+
+
+def _build_layers(hipcc, verbose):
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc)))
+    flags = ["-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-isystem{os.path.join(rocm, 'include')}", f"-L{HERE}", "-l:" + os.path.basename(LIB),
+             "-Wl,-rpath,$ORIGIN", "-lc10_hip"]
+    _build_module("layers.cpp", LAYERS_LIB, "LAYERS_TORCH_VERSION", flags, verbose)
 
 
 def built() -> bool:
     """Whether everything that the package loads is there."""
-    return os.path.exists(LIB) and os.path.exists(SCAN_LIB)
+    return all(os.path.exists(p) for p in (LIB, SCAN_LIB, LAYERS_LIB))
 
 
 def build_library(verbose: bool = False) -> str:
@@ -84,7 +98,9 @@ def build_library(verbose: bool = False) -> str:
         raise RuntimeError("hipcc not found; cannot build libmuon_hip.so")
     _build_scan(verbose)
     _compile_and_link(PROBE_SOURCES, PROBE_LIB, hipcc, verbose)
-    return _compile_and_link(SOURCES, LIB, hipcc, verbose)
+    lib = _compile_and_link(SOURCES, LIB, hipcc, verbose)
+    _build_layers(hipcc, verbose)
+    return lib
 
 
 if __name__ == "__main__":

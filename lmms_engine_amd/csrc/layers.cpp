@@ -1,0 +1,381 @@
+// linear and gated_linear as differentiable functions of torch tensors: what stands between a call and the launches of libmuon_hip, forward
+// and backward, in native code.  The same in Python (ctypes and torch.autograd.Function) costs 25 us for a call and 200 for a training step,
+// more than the kernels of a layer of 500 tokens.
+//
+// Each function takes calls in which nothing needs a decision: plain tensors of one type on one GPU, of shapes that fit.  For anything else
+// it returns None before it has done anything, and the caller says what is wrong.
+#define PY_SSIZE_T_CLEAN
+#include <ATen/DeviceGuard.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/muon_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+PyObject* error_type = nullptr;  // MuonHipError
+
+[[noreturn]] void raise(const char* what, long code) {
+    const std::string text = std::string(what) + " failed (code " + std::to_string(code) + "): " + muon_hip_last_error();
+    python_error e;
+    {
+        pybind11::gil_scoped_acquire gil;
+        PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, text.c_str());
+        e.persist();
+    }
+    throw e;
+}
+
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? MUON_HIP_F32 : MUON_HIP_BF16; }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream(); }
+
+// ---- products -----------------------------------------------------------------------------------
+
+// One or two matrices as an operand; turned: the reduction runs down their columns.
+void operand(const void** at, long* row, long* col, const Tensor& t0, const Tensor& t1, bool turned) {
+    const Tensor* t[2] = {&t0, &t1};
+    for (int i = 0; i < 2; ++i) {
+        at[i] = t[i]->data_ptr();
+        row[i] = t[i]->stride(turned ? 1 : 0);
+        col[i] = t[i]->stride(turned ? 0 : 1);
+    }
+}
+struct Product : muon_hip_product {
+    Product(int kind_, const Tensor& like, int64_t m_, int64_t n_, int64_t k_) : muon_hip_product{} {
+        kind = kind_;
+        dtype = dtype_of(like);
+        m = (int)m_;
+        n = (int)n_;
+        k = (int)k_;
+    }
+    void left(const Tensor& t0, const Tensor& t1, bool turned = false) { operand(a, a_row, a_col, t0, t1, turned); }
+    void right(const Tensor& t0, const Tensor& t1, bool turned = false) { operand(b, b_row, b_col, t0, t1, turned); }
+    void run(const Tensor& like) {
+        const long need = muon_hip_product_workspace(this);
+        if (need < 0) raise("product", need);
+        Tensor ws;
+        if (need > 0) ws = at::empty({need}, like.options().dtype(at::kByte));
+        if (const int rc = muon_hip_product_run(this, need > 0 ? ws.data_ptr() : nullptr, (size_t)need, stream_of(like))) raise("product", rc);
+    }
+};
+
+// t without its history, its values where its pointer says
+Tensor bare(const Tensor& t) {
+    if (!t.defined()) return t;
+    const Tensor d = t.detach();
+    return d.is_neg() ? d.resolve_neg() : d;
+}
+Tensor dense(const Tensor& t) { return t.defined() ? bare(t).contiguous() : t; }
+int64_t rows_of(const Tensor& t) {
+    int64_t m = 1;
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) m *= t.size(d);
+    return m;
+}
+// t as a matrix of the rows of its last dimension: a view where there is one
+Tensor matrix(const Tensor& t) {
+    const Tensor b = bare(t);
+    return b.dim() == 2 ? b : b.reshape({rows_of(b), b.size(-1)});
+}
+Tensor result(const Tensor& x, int64_t n) {
+    auto shape = x.sizes().vec();
+    shape.back() = n;
+    return at::empty(shape, x.options());
+}
+const void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Results of a forward pass, and the factors of the backward pass where they are kept.
+struct Forward {
+    Tensor out, aux[2];
+};
+Forward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, int act, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x2 = matrix(x), w2 = bare(w), b1 = dense(b), r2 = r.defined() ? matrix(r) : r;
+    const int64_t m = x2.size(0), n = w2.size(0);
+    Forward f;
+    f.out = result(x, n);
+    if (keep && act != MUON_HIP_ACT_NONE) f.aux[0] = at::empty({m, n}, x2.options());
+    Product p(MUON_HIP_PRODUCT_LINEAR, x, m, n, x2.size(1));
+    p.activation = act;
+    p.left(x2, x2);
+    p.right(w2, w2);
+    p.bias[0] = pointer(b1);
+    if (r2.defined()) {
+        p.residual = r2.data_ptr();
+        p.res_row = r2.stride(0);
+        p.res_col = r2.stride(1);
+    }
+    p.out[0] = f.out.data_ptr();
+    p.aux[0] = (void*)pointer(f.aux[0]);
+    p.run(x);
+    return f;
+}
+Forward gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu, int act, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x2 = matrix(x), g2 = bare(wg), u2 = bare(wu), b0 = dense(bg), b1 = dense(bu);
+    const int64_t m = x2.size(0), n = g2.size(0);
+    Forward f;
+    f.out = result(x, n);
+    Product p(MUON_HIP_PRODUCT_GATED, x, m, n, x2.size(1));
+    p.activation = act;
+    p.left(x2, x2);
+    p.right(g2, u2);
+    p.bias[0] = pointer(b0);
+    p.bias[1] = pointer(b1);
+    p.out[0] = f.out.data_ptr();
+    for (int i = 0; keep && i < 2; ++i) {
+        f.aux[i] = at::empty({m, n}, x2.options());
+        p.aux[i] = f.aux[i].data_ptr();
+    }
+    p.run(x);
+    return f;
+}
+
+// dz = dy * d for up to two factors and their sums over the rows.  Without a factor dz is dy itself, where its rows are whole 16-byte pieces.
+struct Incoming {
+    Tensor dz[2], db[2];
+};
+Incoming act_grad(const Tensor& dy_, int factors, const Tensor& d0, const Tensor& d1, bool want_dz, bool want_db0, bool want_db1, int64_t m, int64_t n) {
+    const Tensor dy = dense(dy_).view({m, n});
+    const int64_t pitch = (n + 7) / 8 * 8;
+    const bool make = want_dz && (factors > 0 || pitch != n || ((uintptr_t)dy.data_ptr() & 15) != 0);
+    const bool want_db[2] = {want_db0, want_db1};
+    Incoming g;
+    for (int i = 0; i < (factors > 1 ? 2 : 1); ++i) {
+        g.dz[i] = make ? at::empty({m, pitch}, dy.options()).narrow(1, 0, n) : dy;
+        if (want_db[i]) g.db[i] = at::empty({n}, dy.options());
+    }
+    if (make || want_db0 || want_db1) {
+        Tensor parts;
+        if (want_db0 || want_db1)
+            parts = at::empty({muon_hip_act_grad_partials((int)m, (int)n) * (factors > 1 ? 2 : 1)}, dy.options().dtype(at::kFloat));
+        const int rc = muon_hip_act_grad(dy.data_ptr(), factors, pointer(d0), pointer(d1), make ? g.dz[0].data_ptr() : nullptr,
+                                         make && factors > 1 ? g.dz[1].data_ptr() : nullptr, pitch, (void*)pointer(g.db[0]), (void*)pointer(g.db[1]),
+                                         dtype_of(dy), (int)m, (int)n, (float*)pointer(parts), stream_of(dy));
+        if (rc) raise("act_grad", rc);
+    }
+    return g;
+}
+
+// What a backward pass gives has no history of its own: to differentiate it once more raises.
+void close_history(variable_list& grads, int count, const variable_list& inputs) {
+    if (!at::GradMode::is_enabled()) return;
+    bool any = false;
+    for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
+    if (!any) return;
+    for (int i = 0; i < count; ++i) {
+        Tensor& g = grads[i];
+        if (!g.defined()) continue;
+        torch::autograd::DelayedError fn("linear and gated_linear can be differentiated once: their backward pass has none of its own", 1);
+        Tensor v = g.detach();
+        v.set_requires_grad(true);
+        g = fn.apply(variable_list{v})[0];
+    }
+}
+
+// Tensors that a call may lack travel as optionals, and a context numbers the tensors that there are: `has` holds a bit for each of the two.
+typedef std::optional<Tensor> Maybe;
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
+void note(AutogradContext* ctx, const Maybe& a, const Maybe& b) { ctx->saved_data["has"] = (int64_t)(a.has_value() + 2 * b.has_value()); }
+// Whether the optional tensors behind `first` others need a gradient.
+struct Wanted {
+    bool a, b;
+    Wanted(AutogradContext* ctx, int first) {
+        const int64_t has = ctx->saved_data["has"].toInt();
+        a = (has & 1) && ctx->needs_input_grad(first);
+        b = (has & 2) && ctx->needs_input_grad(first + (has & 1));
+    }
+};
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act) {
+        const bool keep = x.requires_grad() || w.requires_grad() || (b && b->requires_grad());
+        Forward f = linear_forward(x, w, given(b), given(r), (int)act, keep);
+        ctx->save_for_backward({x, w, f.aux[0]});
+        note(ctx, b, r);
+        return f.out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &d = saved[2], &dy = incoming[0];
+        const Wanted more(ctx, 2);
+        const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = more.a;
+        variable_list grads(5);
+        {
+            const at::AutoGradMode off(false);
+            const c10::DeviceGuard guard(x.device());
+            if (want_x || want_w || want_b) {
+                const Tensor x2 = matrix(x), w2 = bare(w);
+                const int64_t m = x2.size(0), k = x2.size(1), n = w2.size(0);
+                Incoming g = act_grad(dy, d.defined() ? 1 : 0, d, Tensor(), want_x || want_w, want_b, false, m, n);
+                grads[2] = g.db[0];
+                if (want_x) {
+                    grads[0] = at::empty(x.sizes(), x.options());
+                    Product p(MUON_HIP_PRODUCT_LINEAR, x, m, k, n);
+                    p.left(g.dz[0], g.dz[0]);
+                    p.right(w2, w2, true);
+                    p.out[0] = grads[0].data_ptr();
+                    p.run(x);
+                }
+                if (want_w) {
+                    grads[1] = at::empty({n, k}, x.options());
+                    Product p(MUON_HIP_PRODUCT_LINEAR, x, n, k, m);
+                    p.left(g.dz[0], g.dz[0], true);
+                    p.right(x2, x2, true);
+                    p.out[0] = grads[1].data_ptr();
+                    p.run(x);
+                }
+            }
+            if (more.b) grads[3] = dy;
+        }
+        close_history(grads, 3, {x, w, d, dy});  // (the residual's is the incoming one, history and all)
+        return grads;
+    }
+};
+
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg, const Maybe& bu, int64_t act) {
+        Forward f = gated_forward(x, wg, wu, given(bg), given(bu), (int)act, true);
+        note(ctx, bg, bu);
+        ctx->save_for_backward({x, wg, wu, f.aux[0], f.aux[1]});
+        return f.out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &s = saved[3], &t = saved[4], &dh = incoming[0];
+        const bool want_x = ctx->needs_input_grad(0), want_wg = ctx->needs_input_grad(1), want_wu = ctx->needs_input_grad(2);
+        const Wanted more(ctx, 3);
+        variable_list grads(6);
+        {
+            const at::AutoGradMode off(false);
+            const c10::DeviceGuard guard(x.device());
+            const Tensor x2 = matrix(x), g2 = bare(wg), u2 = bare(wu);
+            const int64_t m = x2.size(0), k = x2.size(1), n = g2.size(0);
+            Incoming g = act_grad(dh, 2, t, s, want_x || want_wg || want_wu, more.a, more.b, m, n);
+            grads[3] = g.db[0];
+            grads[4] = g.db[1];
+            if (want_x) {
+                grads[0] = at::empty(x.sizes(), x.options());
+                Product p(MUON_HIP_PRODUCT_SUM, x, m, k, n);
+                p.left(g.dz[0], g.dz[1]);
+                p.right(g2, u2, true);
+                p.out[0] = grads[0].data_ptr();
+                p.run(x);
+            }
+            if (want_wg || want_wu) {
+                const bool both = want_wg && want_wu;
+                Product p(both ? MUON_HIP_PRODUCT_EACH : MUON_HIP_PRODUCT_LINEAR, x, n, k, m);
+                if (want_wg) grads[1] = at::empty({n, k}, x.options());
+                if (want_wu) grads[2] = at::empty({n, k}, x.options());
+                const int first = want_wg ? 0 : 1;
+                p.left(g.dz[first], g.dz[1], true);
+                p.right(x2, x2, true);
+                p.out[0] = grads[1 + first].data_ptr();
+                p.out[1] = both ? grads[2].data_ptr() : nullptr;
+                p.run(x);
+            }
+        }
+        close_history(grads, 5, {x, wg, wu, s, t, dh});
+        return grads;
+    }
+};
+
+// ---- calls ------------------------------------------------------------------------------------
+
+// A plain tensor on a GPU, of x's type and device.
+bool plain(PyObject* o, const Tensor* x) {
+    if (!THPVariable_CheckExact(o)) return false;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->is_python_dispatch()) return false;
+    if (x) return t.scalar_type() == x->scalar_type() && t.device() == x->device();
+    return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+// The tensors of a call, None as an undefined one; false where something has to be decided.
+bool unpack(PyObject* const* args, int count, int needed, Tensor* out) {
+    if (!plain(args[0], nullptr)) return false;
+    out[0] = THPVariable_Unpack(args[0]);
+    for (int i = 1; i < count; ++i) {
+        if (i >= needed && args[i] == Py_None) continue;
+        if (!plain(args[i], &out[0])) return false;
+        out[i] = THPVariable_Unpack(args[i]);
+    }
+    return true;
+}
+// Whether x, weight and bias fit, and their sizes are ones that the entry points take.
+bool fits(const Tensor& x, const Tensor& w, const Tensor& b) {
+    constexpr int64_t most = 0x7fffffff;
+    return x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) <= most && w.size(1) <= most && rows_of(x) <= most &&
+           (!b.defined() || (b.dim() == 1 && b.size(0) == w.size(0)));
+}
+bool differentiated(const Tensor* t, int count) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (int i = 0; i < count; ++i)
+        if (t[i].defined() && t[i].requires_grad()) return true;
+    return false;
+}
+
+// linear(x, weight, bias or None, residual or None, activation code)
+PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    Tensor t[4];
+    if (count != 5 || !unpack(args, 4, 2, t) || !fits(t[0], t[1], t[2])) Py_RETURN_NONE;
+    if (t[3].defined()) {
+        bool same = t[3].dim() == t[0].dim() && t[3].size(-1) == t[1].size(0);
+        for (int64_t d = 0; same && d + 1 < t[0].dim(); ++d) same = t[3].size(d) == t[0].size(d);
+        if (!same) Py_RETURN_NONE;
+    }
+    const long act = PyLong_AsLong(args[4]);
+    if (act == -1 && PyErr_Occurred()) return nullptr;
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (differentiated(t, 4)) out = Linear::apply(t[0], t[1], maybe(t[2]), maybe(t[3]), (int64_t)act);
+        else out = linear_forward(t[0], t[1], t[2], t[3], (int)act, false).out;
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+// gated_linear(x, weight_gate, weight_up, bias_gate or None, bias_up or None, activation code)
+PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    Tensor t[5];
+    if (count != 6 || !unpack(args, 5, 3, t) || !fits(t[0], t[1], t[3]) || !fits(t[0], t[2], t[4]) || t[1].size(0) != t[2].size(0)) Py_RETURN_NONE;
+    const long act = PyLong_AsLong(args[5]);
+    if (act == -1 && PyErr_Occurred()) return nullptr;
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (differentiated(t, 5)) out = GatedLinear::apply(t[0], t[1], t[2], maybe(t[3]), maybe(t[4]), (int64_t)act);
+        else out = gated_forward(t[0], t[1], t[2], t[3], t[4], (int)act, false).out;
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+// set_error(type): what a refusal of the library is raised as
+PyObject* set_error(PyObject*, PyObject* type) {
+    Py_INCREF(type);
+    Py_XDECREF(error_type);
+    error_type = type;
+    Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {{"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
+                         {"gated_linear", (PyCFunction)(void (*)(void))gated_linear, METH_FASTCALL, nullptr},
+                         {"set_error", set_error, METH_O, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_layers", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__layers() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", LAYERS_TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
+}

@@ -1,5 +1,6 @@
 """linear and gated_linear against their formulas in 64 bits: results and every gradient, at the sizes, layouts and values where tiles,
 reductions and masks can go wrong.  Bounds: tests/layer_reference.py."""
+import ctypes
 import itertools
 
 import pytest
@@ -256,6 +257,21 @@ def test_gradients_against_differences():
                 assert abs(slope - told) <= room, (name, i, slope, told, room)
 
 
+def product(kind, x, m, n, k, a, b, out):
+    """One muon_hip_product_run on row-major operands."""
+    lib = _abi.lib()
+    p = _abi.Product(kind=kind, dtype=_abi.dtype_code(x.dtype), m=m, n=n, k=k)
+    for field, pair in (("a", a), ("b", b)):
+        getattr(p, field)[:] = [t.data_ptr() for t in pair]
+        getattr(p, field + "_row")[:] = [t.stride(0) for t in pair]
+        getattr(p, field + "_col")[:] = [t.stride(1) for t in pair]
+    p.out[:] = [t.data_ptr() for t in out]
+    need = lib.muon_hip_product_workspace(ctypes.addressof(p))
+    assert need >= 0
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+    _abi.check(lib.muon_hip_product_run(ctypes.addressof(p), ws.data_ptr(), need, _abi.stream_ptr(x.device)), "product")
+
+
 def test_rows_behind_the_result_are_left_alone():
     """Results at the end of a tile that reaches past them: what lies around them in memory stays as it was."""
     g = gen_of(19)
@@ -263,8 +279,7 @@ def test_rows_behind_the_result_are_left_alone():
         x, x2, w, w2 = rnd(g, t, k), rnd(g, t, k), rnd(g, n, k), rnd(g, n, k)
         bufs = [torch.full((t * n + 4096,), 7.0, dtype=BF, device=DEV) for _ in range(2)]
         out = [b[2048:2048 + t * n].view(t, n) for b in bufs]
-        a = layers._operands(x, x2) if kind == _abi.PRODUCT_EACH else layers._operands(x)
-        layers._run(kind, x, t, n, k, a, layers._operands(w, w2), out, act=0)
+        product(kind, x, t, n, k, (x, x2), (w, w2), out)
         for o, b, left in zip(out, bufs, (x, x2)):
             assert (b[:2048] == 7).all() and (b[2048 + t * n:] == 7).all()
             if kind == _abi.PRODUCT_EACH:
@@ -389,3 +404,49 @@ def test_the_same_call_gives_the_same_bits():
     for _ in range(3):
         for m, a in run_linear(x, w, None, None, "silu", dy).items():
             assert torch.equal(a, first[m]), m
+
+
+def test_a_second_derivative_raises():
+    """The backward pass has none of its own; the residual's, which is the incoming gradient itself, has."""
+    g = gen_of(43)
+    x, w, r = rnd(g, 8, 16).requires_grad_(True), rnd(g, 24, 16).requires_grad_(True), rnd(g, 8, 24).requires_grad_(True)
+    for y in (E.linear(x, w, activation="silu"), E.gated_linear(x, w, w)):
+        (dx,) = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            dx.float().sum().backward()
+    (dr,) = torch.autograd.grad(E.linear(x, w, residual=r).float().square().sum(), r, create_graph=True)
+    dr.float().sum().backward()
+
+
+def test_what_the_entry_points_refuse_is_raised_as_the_packages_error():
+    """A row that packs into more than a tile may span, forward; the same in a backward pass, which runs on a thread of its own."""
+    long = torch.zeros(1, 5_000_001, dtype=BF, device=DEV)
+    with pytest.raises(_abi.MuonHipError, match="2 GiB"):
+        E.linear(long[:, 1:], torch.zeros(3, 5_000_000, dtype=BF, device=DEV))
+
+
+def test_tensors_of_other_kinds_are_refused():
+    class Mine(torch.Tensor):
+        pass
+
+    x, w = torch.zeros(4, 8, dtype=BF, device=DEV), torch.zeros(5, 8, dtype=BF, device=DEV)
+    with pytest.raises(NotImplementedError, match="Mine"):
+        E.linear(x.as_subclass(Mine), w)
+    with pytest.raises(NotImplementedError, match="sparse"):
+        E.linear(x.to_sparse(), w)
+    with pytest.raises(TypeError, match="no tensor"):
+        E.gated_linear(x, w, [1.0])
+    with pytest.raises(TypeError, match="share one type"):
+        E.linear(x, w.float())
+    with pytest.raises(ValueError, match="do not fit"):
+        E.linear(x, w[:, :7])
+
+
+def test_values_behind_a_lazy_negation():
+    """The imaginary part of a conjugate: the memory holds the values with the other sign."""
+    z = torch.view_as_complex(torch.randn(6, 9, 2, device=DEV, generator=gen_of(47))).conj()
+    assert z.imag.is_neg()
+    w = torch.eye(9, device=DEV)
+    assert torch.equal(E.linear(z.imag, w), z.imag.resolve_neg())
+    assert torch.equal(E.linear(torch.zeros(6, 9, device=DEV), w, residual=z.imag), z.imag.resolve_neg())
+    assert torch.equal(E.linear(w, z.imag), z.imag.resolve_neg().t())
