@@ -226,37 +226,55 @@ __device__ __forceinline__ int swizzle_steps(int k) {
     }
 }
 
-// Where lane l finds its part of step group `h` (one of two halves of a k-tile) of fragment f, in bytes.
-// `first`: first row of the wave's part of the operand.
-template <typename T, int R, bool STEPS, bool RIGHT>
-__device__ __forceinline__ typename Elem<T>::frag read_fragment(const unsigned char* tile, int first, int f, int h, int lane) {
-    const int i = lane & 15, grp = lane >> 4;
-    if constexpr (!STEPS) {
-        const int r = first + (RIGHT ? (f >> 1) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3) : f * 16 + i);
-        return *(const typename Elem<T>::frag*)(tile + r * ROWB + (((h * 4 + grp) ^ swizzle_rows<RIGHT>(r)) << 4));
-    } else if constexpr (sizeof(T) == 2) {
-        // lane i of a group of 16 addresses piece i (step i / 4, rows of quarter i % 4) and receives row i of steps 0 to 3
-        s16x4 part[2];
+// Where a lane finds its parts of the F fragments of its wave, whose rows start at `first`: as few addresses as the swizzle allows, everything
+// else is a constant that fits a read's offset (a k-tile half h, and the stages of an operand, which lie one behind the other).
+template <typename T, int R, bool STEPS, bool RIGHT, int F>
+struct Reader {
+    static constexpr bool HALF = sizeof(T) == 2;
+    static constexpr int N = !STEPS ? 2 : HALF ? (RIGHT ? F / 2 : F) : (RIGHT || F < 4 ? F : 4);
+    unsigned at[N];
+    __device__ __forceinline__ void init(unsigned base, int first, int lane) {
+        const int i = lane & 15, grp = lane >> 4;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int k = h * 32 + grp * 8 + p * 4 + (i >> 2);
-            const int r = first + (RIGHT ? (f >> 1) * 32 + (i & 3) * 8 + (f & 1) * 4 : f * 16 + (i & 3) * 4);
-            const unsigned char* q = tile + k * (R * 2) + (((r >> 3) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 4) * 2;
-            part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_void_ptr)q);
+        for (int n = 0; n < N; ++n) {
+            if constexpr (!STEPS) {  // n: half of the k-tile
+                const int r = first + (RIGHT ? (i >> 2) * 8 + (i & 3) : i);
+                at[n] = base + r * ROWB + (((n * 4 + grp) ^ swizzle_rows<RIGHT>(r)) << 4);
+            } else if constexpr (HALF) {
+                // lane i of a group of 16 addresses piece i (step i / 4, rows of quarter i % 4) and receives row i of steps 0 to 3
+                const int k = grp * 8 + (i >> 2), r = first + (RIGHT ? n * 32 + (i & 3) * 8 : n * 16 + (i & 3) * 4);
+                at[n] = base + k * (R * 2) + (((r >> 3) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 4) * 2;
+            } else {
+                const int k = grp * 4, r = first + (RIGHT ? (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3) : n * 16 + i);
+                at[n] = base + k * (R * 4) + (((r >> 2) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 3) * 4;
+            }
         }
-        const s16x8 w = {part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
-        return __builtin_bit_cast(bf16x8, w);
-    } else {
-        f32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int k = h * 16 + grp * 4 + e;
-            const int r = first + (RIGHT ? (f >> 1) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3) : f * 16 + i);
-            w[e] = *(const float*)(tile + k * (R * 4) + (((r >> 2) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 3) * 4);
-        }
-        return w;
     }
-}
+    __device__ __forceinline__ void move(int bytes) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) at[n] += bytes;
+    }
+    __device__ __forceinline__ typename Elem<T>::frag read(const unsigned char* smem, int stage, int f, int h) const {
+        const int st = stage * (R * ROWB);
+        if constexpr (!STEPS) {
+            return *(const typename Elem<T>::frag*)(smem + at[h] + st + (RIGHT ? (f >> 1) * 32 + (f & 1) * 4 : f * 16) * ROWB);
+        } else if constexpr (HALF) {
+            s16x4 part[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const unsigned char* q = smem + at[RIGHT ? f >> 1 : f] + st + (h * 32 + p * 4) * (R * 2) + (RIGHT ? (f & 1) * 8 : 0);
+                part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_void_ptr)q);
+            }
+            const s16x8 w = {part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
+            return __builtin_bit_cast(bf16x8, w);
+        } else {
+            f32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = *(const float*)(smem + at[f % N] + st + (h * 16 + e) * (R * 4) + f / N * 256);
+            return w;
+        }
+    }
+};
 
 __device__ __forceinline__ f32x4 mfma_step(const bf16x8& a, const bf16x8& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -289,42 +307,50 @@ struct Feed {
     static_assert(R % (8 * NW) == 0, "whole instructions");
     static_assert(!GATED || (!STEPS && RIGHT), "the factors of a gated pair are interleaved by rows");
     unsigned off[LOADS];
-    int rows;   // of this operand from the tile's first row
+    const char *base0, *base1;  // the tile's first row at reduction step 0, of each product (of each factor, GATED)
+    unsigned step_bytes;        // STEPS: from one reduction step to the next
+    unsigned span;              // bytes that may be read from there on: of all steps (rows), of one step
     int wave;
 
-    __device__ __forceinline__ void init(int rows_left, long pitch, int wave_, int lane) {
-        rows = rows_left;
+    __device__ __forceinline__ void init(const void* m0, const void* m1, long row0, int rows, long pitch, int k, int wave_, int lane) {
+        constexpr int S = sizeof(T);
         wave = wave_;
+        const long skip = (STEPS ? row0 : row0 * pitch) * S;
+        base0 = (const char*)m0 + skip;
+        base1 = (const char*)m1 + skip;
+        const int used = GATED ? R / 2 : R, r = rows < used ? rows : used;
+        // whole pieces, so that none is cut in the middle
+        span = STEPS ? (unsigned)(r * S + 15) / 16 * 16 : (unsigned)((r - 1) * pitch * S + ((long)k * S + 15) / 16 * 16);
+        step_bytes = (unsigned)(pitch * S);
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
             const int at = wave * LOADS + n;
             if constexpr (!STEPS) {
-                const int r = at * 8 + (lane >> 3), c = (lane & 7) ^ swizzle_rows<RIGHT>(r);
-                const int src = GATED ? (r >> 6) * 32 + (r & 31) : r;
-                off[n] = (unsigned)(src * pitch * (long)sizeof(T)) + c * 16;
+                const int line = at * 8 + (lane >> 3), c = (lane & 7) ^ swizzle_rows<RIGHT>(line);
+                const int src = GATED ? (line >> 6) * 32 + (line & 31) : line;
+                off[n] = src * step_bytes + c * 16;
             } else {
-                const int idx = at * 64 + lane, k = idx / PIECES, c = (idx % PIECES) ^ swizzle_steps<T, R, RIGHT>(k);
-                off[n] = (unsigned)(k * pitch * (long)sizeof(T)) + c * 16;
+                const int idx = at * 64 + lane, step = idx / PIECES, c = (idx % PIECES) ^ swizzle_steps<T, R, RIGHT>(step);
+                off[n] = step * step_bytes + c * 16;
             }
         }
     }
-    // Bytes that may be read from reduction step k0 of the tile's first row on: whole pieces, so that none is cut in the middle.
-    __device__ __forceinline__ unsigned bytes(long pitch, int k, int k0) const {
-        constexpr int S = sizeof(T);
-        if constexpr (!STEPS) {
-            const int used = GATED ? R / 2 : R, r = rows < used ? rows : used;
-            return (unsigned)((r - 1) * pitch * S + ((long)(k - k0) * S + 15) / 16 * 16);
+    // Reduction steps k0 .. k0 + BK - 1 of product `seg`, of which `left` are there.
+    __device__ __forceinline__ void issue(int seg, int k0, int left, unsigned lds) const {
+        const char* base = seg ? base1 : base0;
+        long skip;
+        unsigned bytes;
+        if constexpr (STEPS) {
+            skip = (long)k0 * step_bytes;
+            bytes = ((left < BK ? left : BK) - 1) * step_bytes + span;
         } else {
-            const int steps = k - k0 < BK ? k - k0 : BK, c = rows < R ? rows : R;
-            return (unsigned)((steps - 1) * pitch * S + ((long)c * S + 15) / 16 * 16);
+            skip = (long)k0 * (long)sizeof(T);
+            bytes = span - (unsigned)skip;
         }
-    }
-    __device__ __forceinline__ void issue(const char* base0, const char* base1, long pitch, int k, int k0, unsigned lds) const {
-        const long skip = STEPS ? (long)k0 * pitch * (long)sizeof(T) : (long)k0 * (long)sizeof(T);
-        const unsigned nb = bytes(pitch, k, k0);
-        const u32x4 r0 = uniform_rsrc(base0 + skip, nb);
+        if (left <= 0) bytes = 0;  // a k-tile that there is none of: nothing is read
+        const u32x4 r0 = uniform_rsrc((GATED ? base0 : base) + skip, bytes);
         u32x4 r1 = r0;
-        if constexpr (GATED) r1 = uniform_rsrc(base1 + skip, nb);
+        if constexpr (GATED) r1 = uniform_rsrc(base1 + skip, bytes);
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
             const int at = wave * LOADS + n;
@@ -332,17 +358,15 @@ struct Feed {
             else load_lds(r0, off[n], lds + at * 1024);
         }
     }
-    // Zeros in place of what the last k-tile holds past the end of the reduction.
-    static __device__ __forceinline__ void clear_tail(unsigned char* tile, int left, int tid) {
-        for (int idx = tid; idx < R * 8; idx += NW * 64) {
-            int keep;  // values of this piece that belong to the reduction
-            if constexpr (!STEPS) {
-                const int r = idx >> 3, c = (idx & 7) ^ swizzle_rows<RIGHT>(r);
-                keep = left - c * PIECE;
-            } else {
-                keep = idx / PIECES < left ? PIECE : 0;
-            }
-            if (keep >= PIECE) continue;
+    // Zeros in place of what this lane has fetched past the end of the reduction: the last k-tile of a product that is not whole.
+    __device__ __forceinline__ void clear_tail(unsigned char* tile, int left, int lane) const {
+        asm volatile("" : "+v"(lane));  // (what depends on it is not worth registers across the loop over k-tiles)
+#pragma unroll 1
+        for (int n = 0; n < LOADS; ++n) {
+            const int idx = (wave * LOADS + n) * 64 + lane;
+            int keep;  // values of the piece that belong to the reduction
+            if constexpr (!STEPS) keep = left - ((lane & 7) ^ swizzle_rows<RIGHT>(idx >> 3)) * PIECE;
+            else keep = idx / PIECES < left ? PIECE : 0;
             T* p = (T*)(tile + idx * 16);
 #pragma unroll
             for (int e = 0; e < PIECE; ++e)
@@ -351,110 +375,87 @@ struct Feed {
     }
 };
 
-// ---- the tile kernel ---------------------------------------------------------------------------
-template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
-__global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs g) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int NW = WGM * WGN, BK = Elem<T>::BK;
-    constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
-    constexpr int A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB;
-    constexpr int TN = GATED ? BN / 2 : BN;  // columns of the result
-    static_assert(!GATED || WTN == 64, "a wave holds 32 columns of each factor");
-    typedef Feed<T, BM, NW, ASTEPS, false, false> FeedA;
-    typedef Feed<T, BN, NW, BSTEPS, true, GATED> FeedB;
-    constexpr int NLD = FeedA::LOADS + FeedB::LOADS;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WGN, wn = wave % WGN;
-    // tile of this workgroup: groups of rows of tiles, column by column inside, so that an XCD's tiles share panels
+// ---- tiles ----------------------------------------------------------------------------------------
+// Which tile of which result over which k-tiles a workgroup computes: groups of four rows of tiles, column by column inside, so that the
+// tiles of an XCD share panels.
+struct Tile {
+    int split, z, first, last;
+    long m0, n0;
+};
+template <int BM, int TN>
+__device__ __forceinline__ Tile tile_of(const KernelArgs& g) {
+    constexpr int GM = 4;
+    Tile r;
     const int tiles = g.tiles_m * g.tiles_n;
     int t = xcd_remap(blockIdx.x, gridDim.x, g.xcd_shift);
-    const int split = t / (tiles * g.outs);
-    t -= split * tiles * g.outs;
-    const int z = t / tiles;
-    t -= z * tiles;
-    constexpr int GM = 4;
+    r.split = t / (tiles * g.outs);
+    t -= r.split * tiles * g.outs;
+    r.z = t / tiles;
+    t -= r.z * tiles;
     const int group = t / (GM * g.tiles_n), row0 = group * GM, gm = g.tiles_m - row0 < GM ? g.tiles_m - row0 : GM;
     t -= group * GM * g.tiles_n;
-    const int ti = row0 + t % gm, tj = t / gm;
-    const long m0 = (long)ti * BM, n0 = (long)tj * TN;
+    r.m0 = (long)(row0 + t % gm) * BM;
+    r.n0 = (long)(t / gm) * TN;
+    const int all = g.nk * g.segments;
+    r.first = r.split * g.per_split;
+    r.last = r.first + g.per_split < all ? r.first + g.per_split : all;
+    return r;
+}
 
+// Both operands of a tile: what a wave fetches of a k-tile.
+template <typename T, int BM, int BN, int NW, bool ASTEPS, bool BSTEPS, bool GATED>
+struct Panels {
+    static constexpr int BK = Elem<T>::BK;
+    typedef Feed<T, BM, NW, ASTEPS, false, false> FeedA;
+    typedef Feed<T, BN, NW, BSTEPS, true, GATED> FeedB;
+    static constexpr int LOADS = FeedA::LOADS + FeedB::LOADS;
     FeedA fa;
     FeedB fb;
-    fa.init((int)(g.m - m0), g.pitch_a, wave, lane);
-    fb.init((int)(g.n - n0), g.pitch_b, wave, lane);
-    const long skip_a = (ASTEPS ? m0 : m0 * g.pitch_a) * (long)sizeof(T), skip_b = (BSTEPS ? n0 : n0 * g.pitch_b) * (long)sizeof(T);
-    const unsigned lds = (unsigned)(uintptr_t)(lds_void_ptr)smem;
-
-    const int first = split * g.per_split, all = g.nk * g.segments;
-    const int last = first + g.per_split < all ? first + g.per_split : all;
-    auto place = [&](int kt, int& seg) {  // reduction step that k-tile kt starts with
-        seg = kt >= g.nk ? 1 : 0;
-        return (kt - seg * g.nk) * BK;
-    };
-    auto issue = [&](int kt) {
-        int seg;
-        const int k0 = place(kt, seg);
-        const unsigned st = lds + ((kt - first) & 1) * STAGE;
-        const char* pa = (const char*)g.a[g.outs > 1 ? z : seg];
-        fa.issue(pa + skip_a, nullptr, g.pitch_a, g.k, k0, st);
-        const char* pb0 = (const char*)g.b[GATED ? 0 : seg];
-        const char* pb1 = (const char*)g.b[1];
-        fb.issue(pb0 + skip_b, pb1 + skip_b, g.pitch_b, g.k, k0, st + A_BYTES);
-    };
-
-    f32x4 acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (first < last) issue(first);
-    for (int kt = first; kt < last; ++kt) {
-        if (kt + 1 < last) {
-            issue(kt + 1);
-            WAIT_VM(NLD);
-        } else {
-            WAIT_VM(0);
-        }
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        unsigned char* tile = smem + ((kt - first) & 1) * STAGE;
-        int seg;
-        const int left = g.k - place(kt, seg);
-        if (left < BK) {
-            FeedA::clear_tail(tile, left, tid);
-            FeedB::clear_tail(tile + A_BYTES, left, tid);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            typename Elem<T>::frag va[FM], vb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) va[i] = read_fragment<T, BM, ASTEPS, false>(tile, wm * WTM, i, h, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) vb[j] = read_fragment<T, BN, BSTEPS, true>(tile + A_BYTES, wn * WTN, j, h, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+    int nk, k, wave, lane;
+    __device__ __forceinline__ Panels(const KernelArgs& g, const Tile& t, int wave_, int lane_) : nk(g.nk), k(g.k), wave(wave_), lane(lane_) {
+        const bool each = g.outs > 1;
+        fa.init(each && t.z ? g.a[1] : g.a[0], each && !t.z ? g.a[0] : g.a[1], t.m0, (int)(g.m - t.m0), g.pitch_a, k, wave, lane);
+        fb.init(g.b[0], g.b[1], t.n0, (int)(g.n - t.n0), g.pitch_b, k, wave, lane);
     }
+    // Loads of k-tile kt, LOADS of a wave for each operand; past the last one of the workgroup they read nothing.
+    __device__ __forceinline__ void issue_a(int kt, int last, unsigned lds) const {
+        const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * BK;
+        fa.issue(seg, k0, kt < last ? k - k0 : 0, lds);
+    }
+    __device__ __forceinline__ void issue_b(int kt, int last, unsigned lds) const {
+        const int seg = kt >= nk ? 1 : 0, k0 = (kt - seg * nk) * BK;
+        fb.issue(seg, k0, kt < last ? k - k0 : 0, lds);
+    }
+    // What this wave has fetched of k-tile kt has landed: nothing of it lies past the end of the reduction any more.
+    __device__ __forceinline__ void landed(int kt, unsigned char* tile_a, unsigned char* tile_b) const {
+        const int left = k - (kt - (kt >= nk ? nk : 0)) * BK;
+        if (left < BK) {
+            fa.clear_tail(tile_a, left, lane);
+            fb.clear_tail(tile_b, left, lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+};
 
-    // One row of fragments after the other, in a loop that is not unrolled: the first is finished, the others move up.  (Unrolled, the
-    // activations of all of them are more code than the instruction cache holds.)
+// A barrier that waits for no load.
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+#define WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+
+// The sums of a wave's part of a tile on their way to memory: one row of fragments after the other, in a loop that is not unrolled; the
+// first is finished, the others move up.  (Unrolled, the activations of all of them are more code than the instruction cache holds.)
+template <typename T, bool GATED, int FM, int FN>
+__device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, f32x4 (&acc)[FM][FN], int row0, int col0, int lane) {
     const int quad = lane >> 4;
 #pragma unroll 1
     for (int i = 0; i < FM; ++i) {
-        const long row = m0 + wm * WTM + i * 16 + (lane & 15);
+        const long row = t.m0 + row0 + i * 16 + (lane & 15);
 #pragma unroll
         for (int jp = 0; jp < FN / 2; jp += GATED ? 2 : 1) {
-            const long col = n0 + (GATED ? wn * 32 : wn * WTN + jp * 32) + quad * 8;
+            const long col = t.n0 + col0 + jp * 32 + quad * 8;
             if (row >= g.m || col >= g.n) continue;
             float v[8], u[8];
 #pragma unroll
@@ -464,11 +465,11 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
             }
             if (g.partial) {
                 const int parts = GATED ? 2 : g.outs, count = g.n - col < 8 ? (int)(g.n - col) : 8;
-                float* p = g.partial + (((long)split * parts + z) * g.m + row) * g.n + col;
+                float* p = g.partial + (((long)t.split * parts + t.z) * g.m + row) * g.n + col;
                 store8(p, g.vec && count == 8, count, v);
                 if (GATED) store8(p + (long)g.m * g.n, g.vec && count == 8, count, u);
             } else {
-                finish8<T, GATED>(g, z, row, (int)col, v, u);
+                finish8<T, GATED>(g, t.z, row, (int)col, v, u);
             }
         }
 #pragma unroll
@@ -476,6 +477,164 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[r][j] = acc[r + 1][j];
     }
+}
+
+// ---- small tiles: two stages, one workgroup's loads behind its own products -----------------------------
+template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
+__global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs g) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int NW = WGM * WGN;
+    constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
+    static_assert(!GATED || WTN == 64, "a wave holds 32 columns of each factor");
+    typedef Panels<T, BM, BN, NW, ASTEPS, BSTEPS, GATED> P;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const Tile t = tile_of<BM, GATED ? BN / 2 : BN>(g);
+    const P panels(g, t, wave, lane);
+    const unsigned lds = (unsigned)(uintptr_t)(lds_void_ptr)smem;
+    Reader<T, BM, ASTEPS, false, FM> ra;
+    Reader<T, BN, BSTEPS, true, FN> rb;
+    ra.init(0, wm * WTM, lane);
+    rb.init(2 * BM * ROWB, wn * WTN, lane);  // (behind the two stages of the left operand)
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto stage_a = [](int s) { return s * (BM * ROWB); };
+    auto stage_b = [](int s) { return 2 * BM * ROWB + s * (BN * ROWB); };
+    auto issue = [&](int kt, int s) {
+        panels.issue_a(kt, t.last, lds + stage_a(s));
+        panels.issue_b(kt, t.last, lds + stage_b(s));
+    };
+    if (t.first < t.last) issue(t.first, 0);
+    for (int kt = t.first; kt < t.last; ++kt) {
+        const int stage = (kt - t.first) & 1;
+        if (kt + 1 < t.last) {
+            issue(kt + 1, stage ^ 1);
+            WAIT_VM(P::LOADS);
+        } else {
+            WAIT_VM(0);
+        }
+        panels.landed(kt, smem + stage_a(stage), smem + stage_b(stage));
+        barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            typename Elem<T>::frag va[FM], vb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, stage, i, h);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, stage, j, h);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+        }
+        WAIT_LDS();
+        barrier();
+    }
+    finish_tile<T, GATED>(g, t, acc, wm * WTM, GATED ? wn * 32 : wn * WTN, lane);
+}
+
+// ---- 256x256 tiles: eight waves in two groups that alternate between memory and products -------------------
+// Wave w and wave w + 4 share a SIMD.  Each runs  { M(t, h): read the fragments of half h of k-tile t, issue loads;  barrier;  C(t, h): the
+// half's products;  barrier }  and waves 4 to 7 enter one barrier later than waves 0 to 3, so that at any time one wave of a SIMD issues
+// nothing but matrix instructions from registers while the other reads LDS and issues loads.
+//
+// LDS holds three k-tiles of the left operand and two of the right one, all 160 KB: M(t, 0) reads the right operand's fragments of both
+// halves, so that its stage is free half a k-tile earlier and a third one would buy nothing.
+// Phases between barriers: group 0 runs M(t, 0) in phase 4t, C(t, 0) in 4t + 1, M(t, 1) in 4t + 2, C(t, 1) in 4t + 3, group 1 each of them
+// one phase later.  The left operand's stage of k-tile t is last read in phase 4t + 3; k-tile t + 3 is issued into it in M(t + 1, 0), phases
+// 4t + 4 and 4t + 5.  The right operand's is last read in phase 4t + 1; k-tile t + 2 is issued into it in M(t, 1), phases 4t + 2 and 4t + 3.  At
+// the end of M(t, 1) each wave waits for its own loads of k-tile t + 1, the last of which are one k-tile old: the two groups issued after
+// them stay in flight.  k-tile t + 1 is first read in phase 4t + 4.
+template <typename T, bool ASTEPS, bool BSTEPS, bool GATED>
+__global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int BM = 256, BN = 256, NW = 8, WGN = 4;
+    constexpr int WTM = 128, WTN = 64, FM = 8, FN = 4;
+    constexpr int UNIT = 256 * ROWB, A_AT = 2 * UNIT;  // a stage of an operand; the left one's lie behind the right one's
+    typedef Panels<T, BM, BN, NW, ASTEPS, BSTEPS, GATED> P;
+    typedef typename Elem<T>::frag frag;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave >> 2, wm = wave / WGN, wn = wave % WGN;
+    const Tile t = tile_of<BM, GATED ? BN / 2 : BN>(g);
+    const P panels(g, t, wave, lane);
+    const unsigned lds = (unsigned)(uintptr_t)(lds_void_ptr)smem;
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    Reader<T, BM, ASTEPS, false, FM> ra;
+    Reader<T, BN, BSTEPS, true, FN> rb;
+    ra.init(A_AT, wm * WTM, lane);
+    rb.init(0, wn * WTN, lane);
+    auto multiply = [&](const frag (&va)[FM], const frag (&vb)[FN]) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int ii = 0; ii < FM; ++ii) {
+                const int i = (j & 1) ? FM - 1 - ii : ii;
+                acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+            }
+    };
+    auto fence = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (t.first < t.last) {
+        auto slot_a = [](int s) { return A_AT + s * UNIT; };
+        auto slot_b = [](int s) { return s * UNIT; };
+        for (int n = 0; n < 2; ++n) {
+            panels.issue_a(t.first + n, t.last, lds + slot_a(n));
+            panels.issue_b(t.first + n, t.last, lds + slot_b(n));
+        }
+        WAIT_VM(P::LOADS);
+        panels.landed(t.first, smem + slot_a(0), smem + slot_b(0));
+        barrier();
+        if (grp) barrier();
+        int sa = 0, sb = 0;  // stages of k-tile kt
+#pragma unroll 1
+        for (int kt = t.first; kt < t.last; ++kt) {
+            const int sa1 = sa == 2 ? 0 : sa + 1, sa2 = sa1 == 2 ? 0 : sa1 + 1;
+            frag va[FM], vb[2][FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) vb[h][j] = rb.read(smem, 0, j, h);
+            panels.issue_a(kt + 2, t.last, lds + slot_a(sa2));
+            WAIT_LDS();
+            fence();
+            multiply(va, vb[0]);
+            fence();
+#pragma unroll
+            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, 1);
+            panels.issue_b(kt + 2, t.last, lds + slot_b(sb));
+            ra.move((sa1 - sa) * UNIT);
+            rb.move(sb ? -UNIT : UNIT);
+            sa = sa1;
+            sb ^= 1;
+            WAIT_LDS();
+            WAIT_VM(P::LOADS);
+            if (kt + 1 < t.last) panels.landed(kt + 1, smem + slot_a(sa), smem + slot_b(sb));
+            fence();
+            multiply(va, vb[1]);
+            fence();
+        }
+        if (!grp) barrier();
+        WAIT_VM(0);  // (the loads of no k-tile have to end before the workgroup's LDS is another's)
+    }
+    finish_tile<T, GATED>(g, t, acc, wm * WTM, GATED ? wn * 32 : wn * WTN, lane);
 }
 
 // The parts of a reduction that several workgroups took, added in their order, and the layer's arithmetic.  Without any part (k = 0)
@@ -680,8 +839,17 @@ hipError_t launch_tiles(const KernelArgs& g, hipStream_t stream) {
     return hipGetLastError();
 }
 template <typename T, bool AS, bool BS, bool GATED>
+hipError_t launch_pp(const KernelArgs& g, hipStream_t stream) {
+    constexpr int smem = 5 * 256 * ROWB;
+    static std::atomic<unsigned long long> configured{0};
+    const auto kern = product_pp_kernel<T, AS, BS, GATED>;
+    if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)g.tiles_m * g.tiles_n * g.outs * g.splits)), dim3(512), smem, stream, g);
+    return hipGetLastError();
+}
+template <typename T, bool AS, bool BS, bool GATED>
 hipError_t launch_tile(int tile, const KernelArgs& g, hipStream_t s) {
-    if (tile == 256) return launch_tiles<T, 256, 256, 2, 4, AS, BS, GATED>(g, s);
+    if (tile == 256) return launch_pp<T, AS, BS, GATED>(g, s);
     if (tile == 128) return launch_tiles<T, 128, 128, 2, 2, AS, BS, GATED>(g, s);
     return launch_tiles<T, 64, 64, 4, 1, AS, BS, GATED>(g, s);
 }
