@@ -13,6 +13,7 @@
 // bf16 operands are multiplied by v_mfma_f32_16x16x32_bf16, fp32 ones by v_mfma_f32_16x16x4_f32 (full single precision); sums, biases,
 // activations and residuals are fp32, and results are rounded once.
 #include <atomic>
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -65,28 +66,49 @@ struct KernelArgs {
 
 // ---- activations -----------------------------------------------------------------------------
 // act(z) and act'(z).  The factor of a gated pair's gradient and the activation itself come out of one evaluation.
+//
+// Results of bf16 tensors are rounded to 8 bits, so theirs take the hardware's exponential and reciprocal (one step of fp32 each), and the
+// complementary error function by the rational approximation 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most: 8192 x
+// 4096 x 4096 with silu take 196 us (178 without), with the full functions 217.  fp32 tensors get those.
 struct ActPair {
     float a, d;
 };
-__device__ __forceinline__ float sigmoid_of(float z) { return 1.0f / (1.0f + expf(-z)); }
+template <bool FAST>
+__device__ __forceinline__ float exp_of(float z) {
+    return FAST ? __builtin_amdgcn_exp2f(1.4426950408889634f * z) : expf(z);
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_of(float z) {
+    const float e = 1.0f + exp_of<FAST>(-z);
+    return FAST ? __builtin_amdgcn_rcpf(e) : 1.0f / e;
+}
+template <bool FAST>
 __device__ __forceinline__ ActPair activate(int act, float z) {
     switch (act) {
         case ACT_RELU: return ActPair{z <= 0.f ? 0.f : z, z <= 0.f ? 0.f : 1.f};  // (NaN stays NaN)
         case ACT_SIGMOID: {
-            const float s = sigmoid_of(z);
+            const float s = sigmoid_of<FAST>(z);
             return ActPair{s, s * (1.f - s)};
         }
         case ACT_SILU: {
-            const float s = sigmoid_of(z);
+            const float s = sigmoid_of<FAST>(z);
             return ActPair{z * s, s * (1.f + z * (1.f - s))};
         }
-        case ACT_GELU: {  // z Phi(z), Phi = erfc(-z / sqrt 2) / 2: no cancellation at the lower end
-            const float phi = 0.5f * erfcf(-0.70710678118654752f * z);
-            return ActPair{z * phi, phi + z * 0.3989422804014327f * expf(-0.5f * z * z)};
+        case ACT_GELU: {  // z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2: no cancellation at the lower end
+            const float gauss = exp_of<FAST>(-0.5f * z * z);
+            float phi;
+            if constexpr (FAST) {
+                const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
+                const float lower = 0.5f * gauss * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+                phi = z < 0.f ? lower : 1.f - lower;
+            } else {
+                phi = 0.5f * erfcf(-0.70710678118654752f * z);
+            }
+            return ActPair{z * phi, phi + z * 0.3989422804014327f * gauss};
         }
         case ACT_GELU_TANH: {  // (1 + tanh y) / 2 = sigmoid(2 y), y = c (z + 0.044715 z^3)
             const float c2 = 2.f * 0.7978845608028654f, q = 0.044715f * z * z;
-            const float s = sigmoid_of(c2 * z * (1.f + q)), w = s * (1.f - s);
+            const float s = sigmoid_of<FAST>(c2 * z * (1.f + q)), w = s * (1.f - s);
             return ActPair{z * s, s + (w == 0.f ? 0.f : z * w * (c2 * (1.f + 3.f * q)))};
         }
         default: return ActPair{z, 1.f};
@@ -158,7 +180,7 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
         float h[8], s[8], t[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const ActPair p = activate(g.act, v[e]);
+            const ActPair p = activate<sizeof(T) == 2>(g.act, v[e]);
             h[e] = p.a * u[e];
             s[e] = p.a;
             t[e] = p.d * u[e];
@@ -181,7 +203,7 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
             float d[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const ActPair p = activate(g.act, v[e]);
+                const ActPair p = activate<sizeof(T) == 2>(g.act, v[e]);
                 v[e] = p.a;
                 d[e] = p.d;
             }
@@ -195,6 +217,19 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
         }
         store8((T*)g.out[z] + at, whole, count, v);
     }
+}
+
+// Eight sums on their way: to the parts of a split reduction, or through the layer's arithmetic.
+template <typename T, bool GATED>
+__device__ __forceinline__ void emit8(const KernelArgs& g, int split, int z, long i, int j, float (&v)[8], float (&u)[8]) {
+    if (!g.partial) {
+        finish8<T, GATED>(g, z, i, j, v, u);
+        return;
+    }
+    const int parts = GATED ? 2 : g.outs, count = g.n - j < 8 ? g.n - j : 8;
+    float* p = g.partial + (((long)split * parts + z) * g.m + i) * g.n + j;
+    store8(p, g.vec && count == 8, count, v);
+    if (GATED) store8(p + (long)g.m * g.n, g.vec && count == 8, count, u);
 }
 
 // ---- operand tiles in LDS -------------------------------------------------------------------------
@@ -376,15 +411,16 @@ struct Feed {
 };
 
 // ---- tiles ----------------------------------------------------------------------------------------
-// Which tile of which result over which k-tiles a workgroup computes: groups of four rows of tiles, column by column inside, so that the
-// tiles of an XCD share panels.
+// Which tile of which result over which k-tiles a workgroup computes.
 struct Tile {
     int split, z, first, last;
     long m0, n0;
 };
 template <int BM, int TN>
 __device__ __forceinline__ Tile tile_of(const KernelArgs& g) {
-    constexpr int GM = 4;
+    // 4 x 8 tiles make one XCD's run of 32, and four of them above each other a block of 16 x 8: what all XCDs work on at a time is as
+    // square as can be.
+    constexpr int HIGH = 16, WIDE = 8, GM = 4;
     Tile r;
     const int tiles = g.tiles_m * g.tiles_n;
     int t = xcd_remap(blockIdx.x, gridDim.x, g.xcd_shift);
@@ -392,10 +428,14 @@ __device__ __forceinline__ Tile tile_of(const KernelArgs& g) {
     t -= r.split * tiles * g.outs;
     r.z = t / tiles;
     t -= r.z * tiles;
-    const int group = t / (GM * g.tiles_n), row0 = group * GM, gm = g.tiles_m - row0 < GM ? g.tiles_m - row0 : GM;
-    t -= group * GM * g.tiles_n;
-    r.m0 = (long)(row0 + t % gm) * BM;
-    r.n0 = (long)(t / gm) * TN;
+    const int band = t / (HIGH * g.tiles_n), high = g.tiles_m - band * HIGH < HIGH ? g.tiles_m - band * HIGH : HIGH;
+    t -= band * HIGH * g.tiles_n;
+    const int block = t / (high * WIDE), wide = g.tiles_n - block * WIDE < WIDE ? g.tiles_n - block * WIDE : WIDE;
+    t -= block * high * WIDE;
+    const int group = t / (GM * wide), gm = high - group * GM < GM ? high - group * GM : GM;
+    t -= group * GM * wide;
+    r.m0 = (long)(band * HIGH + group * GM + t % gm) * BM;
+    r.n0 = (long)(block * WIDE + t / gm) * TN;
     const int all = g.nk * g.segments;
     r.first = r.split * g.per_split;
     r.last = r.first + g.per_split < all ? r.first + g.per_split : all;
@@ -445,14 +485,31 @@ __device__ __forceinline__ void barrier() {
 }
 #define WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
 
-// The sums of a wave's part of a tile on their way to memory: one row of fragments after the other, in a loop that is not unrolled; the
-// first is finished, the others move up.  (Unrolled, the activations of all of them are more code than the instruction cache holds.)
+// Row i of the fragments, for an i that is no constant but the same in every lane.
+template <int I = 0, int FM, int FN>
+__device__ __forceinline__ void pick_row(const f32x4 (&acc)[FM][FN], int i, f32x4 (&row)[FN]) {
+    if constexpr (I + 1 < FM) {
+        if (i != I) {
+            pick_row<I + 1>(acc, i, row);
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        row[j] = acc[I][j];
+        asm volatile("; row %1" : "+v"(row[j]) : "n"(I));  // (merged, the copies would become a look-up in memory)
+    }
+}
+// The sums of a wave's part of a tile on their way to memory: one row of fragments after the other, in a loop that is not unrolled (the
+// activations of all of them are more code than the instruction cache holds).
 template <typename T, bool GATED, int FM, int FN>
-__device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, f32x4 (&acc)[FM][FN], int row0, int col0, int lane) {
+__device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, const f32x4 (&acc)[FM][FN], int row0, int col0, int lane) {
     const int quad = lane >> 4;
 #pragma unroll 1
     for (int i = 0; i < FM; ++i) {
         const long row = t.m0 + row0 + i * 16 + (lane & 15);
+        f32x4 sums[FN];
+        pick_row(acc, i, sums);
 #pragma unroll
         for (int jp = 0; jp < FN / 2; jp += GATED ? 2 : 1) {
             const long col = t.n0 + col0 + jp * 32 + quad * 8;
@@ -460,33 +517,26 @@ __device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, 
             float v[8], u[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = acc[0][2 * jp + (e >> 2)][e & 3];
-                u[e] = GATED ? acc[0][(2 * jp + 2 + (e >> 2)) % FN][e & 3] : 0.f;
+                v[e] = sums[2 * jp + (e >> 2)][e & 3];
+                u[e] = GATED ? sums[(2 * jp + 2 + (e >> 2)) % FN][e & 3] : 0.f;
             }
-            if (g.partial) {
-                const int parts = GATED ? 2 : g.outs, count = g.n - col < 8 ? (int)(g.n - col) : 8;
-                float* p = g.partial + (((long)t.split * parts + t.z) * g.m + row) * g.n + col;
-                store8(p, g.vec && count == 8, count, v);
-                if (GATED) store8(p + (long)g.m * g.n, g.vec && count == 8, count, u);
-            } else {
-                finish8<T, GATED>(g, t.z, row, (int)col, v, u);
-            }
+            emit8<T, GATED>(g, t.split, t.z, row, (int)col, v, u);
         }
-#pragma unroll
-        for (int r = 0; r + 1 < FM; ++r)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[r][j] = acc[r + 1][j];
     }
 }
 
-// ---- small tiles: two stages, one workgroup's loads behind its own products -----------------------------
-template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
+// ---- small tiles -----------------------------------------------------------------------------------
+// S stages: a wave waits for its own loads of k-tile t, crosses the one barrier of the k-tile (behind which every wave has read all of k-tile
+// t - 1), issues the loads of k-tile t + S - 1 into the stage that is free now, and multiplies.
+template <typename T, int BM, int BN, int WGM, int WGN, int S, bool ASTEPS, bool BSTEPS, bool GATED>
 __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs g) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int NW = WGM * WGN;
     constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
+    constexpr int UNIT_A = BM * ROWB, UNIT_B = BN * ROWB, B_AT = S * UNIT_A;
     static_assert(!GATED || WTN == 64, "a wave holds 32 columns of each factor");
     typedef Panels<T, BM, BN, NW, ASTEPS, BSTEPS, GATED> P;
+    typedef typename Elem<T>::frag frag;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WGN, wn = wave % WGN;
@@ -496,7 +546,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
     Reader<T, BM, ASTEPS, false, FM> ra;
     Reader<T, BN, BSTEPS, true, FN> rb;
     ra.init(0, wm * WTM, lane);
-    rb.init(2 * BM * ROWB, wn * WTN, lane);  // (behind the two stages of the left operand)
+    rb.init(B_AT, wn * WTN, lane);
 
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -504,37 +554,39 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    auto stage_a = [](int s) { return s * (BM * ROWB); };
-    auto stage_b = [](int s) { return 2 * BM * ROWB + s * (BN * ROWB); };
     auto issue = [&](int kt, int s) {
-        panels.issue_a(kt, t.last, lds + stage_a(s));
-        panels.issue_b(kt, t.last, lds + stage_b(s));
+        panels.issue_a(kt, t.last, lds + s * UNIT_A);
+        panels.issue_b(kt, t.last, lds + B_AT + s * UNIT_B);
     };
-    if (t.first < t.last) issue(t.first, 0);
-    for (int kt = t.first; kt < t.last; ++kt) {
-        const int stage = (kt - t.first) & 1;
-        if (kt + 1 < t.last) {
-            issue(kt + 1, stage ^ 1);
-            WAIT_VM(P::LOADS);
-        } else {
-            WAIT_VM(0);
+    if (t.first < t.last) {
+#pragma unroll
+        for (int n = 0; n < S - 1; ++n) issue(t.first + n, n);
+        int s = 0;  // stage of k-tile kt
+#pragma unroll 1
+        for (int kt = t.first; kt < t.last; ++kt) {
+            WAIT_VM((S - 2) * P::LOADS);
+            panels.landed(kt, smem + s * UNIT_A, smem + B_AT + s * UNIT_B);
+            barrier();
+            issue(kt + S - 1, s == 0 ? S - 1 : s - 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                frag va[FM], vb[FN];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, h);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, 0, j, h);
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+            }
+            const int s1 = s + 1 == S ? 0 : s + 1;
+            ra.move((s1 - s) * UNIT_A);
+            rb.move((s1 - s) * UNIT_B);
+            s = s1;
+            WAIT_LDS();
         }
-        panels.landed(kt, smem + stage_a(stage), smem + stage_b(stage));
-        barrier();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            typename Elem<T>::frag va[FM], vb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, stage, i, h);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, stage, j, h);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
-        }
-        WAIT_LDS();
-        barrier();
+        WAIT_VM(0);  // (the loads of no k-tile have to end before the workgroup's LDS is another's)
     }
     finish_tile<T, GATED>(g, t, acc, wm * WTM, GATED ? wn * 32 : wn * WTN, lane);
 }
@@ -551,12 +603,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 // 4t + 4 and 4t + 5.  The right operand's is last read in phase 4t + 1; k-tile t + 2 is issued into it in M(t, 1), phases 4t + 2 and 4t + 3.  At
 // the end of M(t, 1) each wave waits for its own loads of k-tile t + 1, the last of which are one k-tile old: the two groups issued after
 // them stay in flight.  k-tile t + 1 is first read in phase 4t + 4.
-template <typename T, bool ASTEPS, bool BSTEPS, bool GATED>
-__global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) {
+template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
+__global__ void __launch_bounds__(512, BM == 128 ? 4 : 2) product_pp_kernel(const KernelArgs g) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int BM = 256, BN = 256, NW = 8, WGN = 4;
-    constexpr int WTM = 128, WTN = 64, FM = 8, FN = 4;
-    constexpr int UNIT = 256 * ROWB, A_AT = 2 * UNIT;  // a stage of an operand; the left one's lie behind the right one's
+    constexpr int NW = WGM * WGN;
+    constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
+    constexpr int UNIT_A = BM * ROWB, UNIT_B = BN * ROWB, A_AT = 2 * UNIT_B;  // stages; the left operand's lie behind the right one's
+    static_assert(NW == 8 && WTN == 64, "two groups of four waves; a wave of a gated pair holds 32 columns of each factor");
     typedef Panels<T, BM, BN, NW, ASTEPS, BSTEPS, GATED> P;
     typedef typename Elem<T>::frag frag;
 
@@ -591,8 +644,8 @@ __global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) 
         __builtin_amdgcn_sched_barrier(0);
     };
     if (t.first < t.last) {
-        auto slot_a = [](int s) { return A_AT + s * UNIT; };
-        auto slot_b = [](int s) { return s * UNIT; };
+        auto slot_a = [](int s) { return A_AT + s * UNIT_A; };
+        auto slot_b = [](int s) { return s * UNIT_B; };
         for (int n = 0; n < 2; ++n) {
             panels.issue_a(t.first + n, t.last, lds + slot_a(n));
             panels.issue_b(t.first + n, t.last, lds + slot_b(n));
@@ -620,8 +673,8 @@ __global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) 
 #pragma unroll
             for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, 1);
             panels.issue_b(kt + 2, t.last, lds + slot_b(sb));
-            ra.move((sa1 - sa) * UNIT);
-            rb.move(sb ? -UNIT : UNIT);
+            ra.move((sa1 - sa) * UNIT_A);
+            rb.move(sb ? -UNIT_B : UNIT_B);
             sa = sa1;
             sb ^= 1;
             WAIT_LDS();
@@ -635,6 +688,98 @@ __global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) 
         WAIT_VM(0);  // (the loads of no k-tile have to end before the workgroup's LDS is another's)
     }
     finish_tile<T, GATED>(g, t, acc, wm * WTM, GATED ? wn * 32 : wn * WTN, lane);
+}
+
+// ---- few rows: the right operand is read once, straight into registers ---------------------------------------
+// For a few rows on the left (tokens that are being answered) the product is a walk over the weight.  A workgroup takes 16 rows of it (of both
+// factors of a gated pair), its eight waves an eighth of the reduction each: a wave's load is 16 rows x 64 bytes, a fragment as the matrix
+// instruction takes it, and the fragments of x come out of the caches the same way.  The next STEPS of them are on their way while the last
+// are multiplied.  The waves' sums meet in LDS.  Rows may start at any element: the hardware reads vectors from any address.
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(512) product_rows_kernel(const KernelArgs g) {
+    typedef typename Elem<T>::frag frag;
+    typedef frag __attribute__((aligned(sizeof(T)))) frag_any;
+    constexpr int W = GATED ? 2 : 1, NW = 8, PIECE = Elem<T>::PIECE, STEP = 4 * PIECE;  // reduction steps of a fragment
+    constexpr int STEPS = GATED ? 4 : 6;
+    __shared__ __align__(16) float part[NW][W][16][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, grp = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int row = n0 + i < g.n ? n0 + i : g.n - 1;  // (rows past the end are the last one again: what they give is not wanted)
+    const T* wp[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) wp[w] = (const T*)g.b[w] + row * g.pitch_b + grp * PIECE;
+    const T* xp = (const T*)g.a[0] + (i < g.m ? i : g.m - 1) * g.pitch_a + grp * PIECE;
+
+    f32x4 acc[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) acc[w] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // this wave's part of the reduction, in whole fragments; the last one of all may be cut
+    const int all = g.k / STEP, mine = (all + NW - 1) / NW;
+    int s = wave * mine;
+    const int end = s + mine < all ? s + mine : all;
+    frag vw[2][STEPS][W], vx[2][STEPS];
+    auto load = [&](int b, int s, int count) {
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+            if (c >= count) break;
+#pragma unroll
+            for (int w = 0; w < W; ++w) vw[b][c][w] = *(const frag_any*)(wp[w] + (long)(s + c) * STEP);
+            vx[b][c] = *(const frag_any*)(xp + (long)(s + c) * STEP);
+        }
+    };
+    auto multiply = [&](int b, int count) {
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+            if (c >= count) break;
+#pragma unroll
+            for (int w = 0; w < W; ++w) acc[w] = mfma_step(vw[b][c][w], vx[b][c], acc[w]);
+        }
+    };
+    const int batches = s < end ? (end - s) / STEPS : 0;
+    if (batches > 0) load(0, s, STEPS);
+    for (int n = 0; n < batches; n += 2) {
+        if (n + 1 < batches) load(1, s + STEPS, STEPS);
+        multiply(0, STEPS);
+        s += STEPS;
+        if (n + 1 >= batches) break;
+        if (n + 2 < batches) load(0, s + STEPS, STEPS);
+        multiply(1, STEPS);
+        s += STEPS;
+    }
+    if (s < end) {
+        load(0, s, end - s);
+        multiply(0, end - s);
+    }
+    if (wave == NW - 1 && all * STEP < g.k) {  // what is left of the reduction, value by value
+        const int k0 = all * STEP + grp * PIECE;
+        frag tw[W], tx;
+#pragma unroll
+        for (int e = 0; e < PIECE; ++e) {
+            const bool there = k0 + e < g.k;
+#pragma unroll
+            for (int w = 0; w < W; ++w) tw[w][e] = there ? wp[w][(long)all * STEP + e] : (T)0.f;
+            tx[e] = there ? xp[(long)all * STEP + e] : (T)0.f;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) acc[w] = mfma_step(tw[w], tx, acc[w]);
+    }
+    // a lane holds rows n0 + 4 grp .. + 3 of the weight against row i of x
+#pragma unroll
+    for (int w = 0; w < W; ++w) *(f32x4*)&part[wave][w][i][grp * 4] = acc[w];
+    __syncthreads();
+    const int half = (tid & 1) * 8, j = n0 + half, token = tid >> 1;
+    if (token >= g.m || j >= g.n) return;  // (g.m <= 16)
+    float v[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = u[e] = 0.f;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) {
+            v[e] += part[q][0][token][half + e];
+            if (GATED) u[e] += part[q][W - 1][token][half + e];
+        }
+    }
+    finish8<T, GATED>(g, 0, token, j, v, u);
 }
 
 // The parts of a reduction that several workgroups took, added in their order, and the layer's arithmetic.  Without any part (k = 0)
@@ -764,9 +909,21 @@ struct Plan {
     long pitch_a, pitch_b;        // elements
     long pack_a, pack_b;          // bytes of one packed matrix
     int count_a, count_b;         // matrices of each operand
-    int tile, splits, per_split, nk, segments, outs;
+    int tile, splits, per_split, nk, segments, outs;  // tile 0: the kernel of few rows
     long partial_bytes, bytes;
 };
+
+// What a way of computing a product of bf16 (fp32) matrices takes, in microseconds, as measured on 256 compute units: `start`, and for every
+// workgroup of a compute unit `each` and its k-tiles, which take `alone` while it has the compute unit for itself and `busy` where there are
+// more.  256-tiles reach 1.5 PFLOP/s where they fill the machine, 128-tiles 1.0; over few or short products the smaller ones win because they
+// start and end sooner.
+struct Cost {
+    float start, each, alone, busy;
+};
+constexpr Cost kCost[2][3] = {{{4.5f, 0.5f, 0.72f, 0.50f}, {5.f, 1.f, 2.2f, 1.88f}, {0.f, 0.f, 0.f, 0.f}},   // fp32: tiles of 64 and 128 (no 256)
+                              {{2.5f, 0.5f, 0.30f, 0.22f}, {3.f, 1.f, 0.66f, 0.52f}, {3.f, 3.f, 1.15f, 1.35f}}};  // bf16: 64, 128, 256
+constexpr float kJoinStart = 4.f, kJoinBytes = 5.5e6f;  // of a split reduction: its launch, and bytes in a microsecond
+constexpr int kTile[3] = {64, 128, 256};
 
 // How an operand is read: as it lies where 16-byte pieces of its rows (or of its reduction steps) are aligned and 32 bits span a tile of it.
 int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool steps_ok, long& pitch) {
@@ -792,6 +949,22 @@ int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool s
     return LIE_PACKED;
 }
 
+// Few rows against rows of a weight, wherever they start: one launch, where tiles that leave most of the machine idle would have to share the
+// reduction and be joined (1 x 4096 x 4096: 9 us against 14).  From 9 rows on the fragments of x are as much to fetch as the weight and the
+// tiles, which keep theirs in LDS, are faster (16 x 4096 x 12288: 24 us against 30).
+constexpr int kFewRows = 8;
+bool few_rows(const ProductArgs& p, Plan& l) {
+    if (p.m > kFewRows || (p.kind != PRODUCT_LINEAR && p.kind != PRODUCT_GATED)) return false;
+    if (p.k > 16384 && p.n < 1024) return false;  // long rows on few compute units
+    if (p.k > 1 && (p.a.col[0] != 1 || p.b.col[0] != 1)) return false;
+    if (p.kind == PRODUCT_GATED && ((p.k > 1 && p.b.col[1] != 1) || p.b.row[1] != p.b.row[0])) return false;
+    l.tile = 0;
+    l.pitch_a = p.a.row[0];
+    l.pitch_b = p.b.row[0];
+    l.segments = l.outs = l.splits = 1;
+    return true;
+}
+
 bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     const int size = elem_size(p.dtype), bk = ROWB / size;
     const bool gated = p.kind == PRODUCT_GATED;
@@ -802,6 +975,7 @@ bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     l.outs = p.kind == PRODUCT_EACH ? 2 : 1;
     if (p.m == 0 || p.n == 0) return true;
     if (p.k == 0) return true;
+    if (few_rows(p, l)) return true;
     l.lie_a = lie_of(p.a, l.count_a, p.m, p.k, size, true, l.pitch_a);
     l.lie_b = lie_of(p.b, l.count_b, p.n, p.k, size, !gated, l.pitch_b);
     for (const long pitch : {l.lie_a == LIE_PACKED ? l.pitch_a : 0, l.lie_b == LIE_PACKED ? l.pitch_b : 0})
@@ -810,53 +984,77 @@ bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     l.pack_b = l.lie_b == LIE_PACKED ? up(p.n * l.pitch_b * size, 256) : 0;
     l.nk = (int)((p.k + (long)bk - 1) / bk);
     auto tiles_of = [&](int t) { return up(p.m, t) / t * (up(p.n, gated ? t / 2 : t) / (gated ? t / 2 : t)) * l.outs; };
-    l.tile = tiles_of(256) >= cus ? 256 : tiles_of(128) >= cus ? 128 : 64;
-    const long tiles = tiles_of(l.tile), all = (long)l.nk * l.segments;
-    for (const long rows : {l.pack_a ? p.m : 0, l.pack_b ? p.n : 0})
-        if (up(p.k, 64) / 64 * (up(rows, 64) / 64) > 0x7fffffffL) return false;
-    if (all > 0x3fffffffL || tiles > 0x3fffffffL) return false;
-    long splits = 1;
-    if (tiles < cus) splits = cus / tiles;
-    if (splits > all / 4) splits = all / 4;
-    if (splits > 32) splits = 32;
-    if (splits < 1) splits = 1;
-    l.per_split = (int)((all + splits - 1) / splits);
-    l.splits = (int)((all + l.per_split - 1) / l.per_split);
+    const long all = (long)l.nk * l.segments;
+    if (all > 0x3fffffffL) return false;
+    const bool bf = p.dtype == MUON_HIP_BF16;
+    float best = 1e30f;
+    long tiles = 0;
+    for (int c = 0; c < (bf ? 3 : 2); ++c) {
+        const long here = tiles_of(kTile[c]);
+        const Cost& q = kCost[bf][c];
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (want > 1 && (want > all / 4 || here * want > 8L * cus)) break;
+            const long per = (all + want - 1) / want, parts = (all + per - 1) / per;
+            const long load = (here * parts + cus - 1) / cus;
+            float t = q.start + q.each * load + (float)per * (load <= 1 ? q.alone : std::max(q.alone, q.busy * load));
+            if (parts > 1) t += kJoinStart + (float)p.m * p.n * (gated ? 2 : l.outs) * 8.f * parts / kJoinBytes;
+            if (t < best) {
+                best = t;
+                tiles = here;
+                l.tile = kTile[c];
+                l.per_split = (int)per;
+                l.splits = (int)parts;
+            }
+        }
+    }
+    if (tiles > 0x3fffffffL) return false;
     if (tiles * l.splits > 0x7fffffffL) return false;
     if (l.splits > 1) l.partial_bytes = (long)l.splits * (gated ? 2 : l.outs) * p.m * p.n * 4;
     l.bytes = l.pack_a * l.count_a + l.pack_b * l.count_b + l.partial_bytes;
     return true;
 }
 
-template <typename T, int BM, int BN, int WGM, int WGN, bool AS, bool BS, bool GATED>
+template <typename T, int BM, int BN, int WGM, int WGN, int S, bool AS, bool BS, bool GATED>
 hipError_t launch_tiles(const KernelArgs& g, hipStream_t stream) {
-    constexpr int smem = 2 * (BM + BN) * ROWB;
+    constexpr int smem = S * (BM + BN) * ROWB;
     static std::atomic<unsigned long long> configured{0};
-    const auto kern = product_kernel<T, BM, BN, WGM, WGN, AS, BS, GATED>;
+    const auto kern = product_kernel<T, BM, BN, WGM, WGN, S, AS, BS, GATED>;
     if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
     const long grid = (long)g.tiles_m * g.tiles_n * g.outs * g.splits;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(WGM * WGN * 64), smem, stream, g);
     return hipGetLastError();
 }
-template <typename T, bool AS, bool BS, bool GATED>
+template <typename T, int BM, int BN, int WGM, int WGN, bool AS, bool BS, bool GATED>
 hipError_t launch_pp(const KernelArgs& g, hipStream_t stream) {
-    constexpr int smem = 5 * 256 * ROWB;
+    constexpr int smem = (3 * BM + 2 * BN) * ROWB;
     static std::atomic<unsigned long long> configured{0};
-    const auto kern = product_pp_kernel<T, AS, BS, GATED>;
+    const auto kern = product_pp_kernel<T, BM, BN, WGM, WGN, AS, BS, GATED>;
     if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)((long)g.tiles_m * g.tiles_n * g.outs * g.splits)), dim3(512), smem, stream, g);
     return hipGetLastError();
 }
 template <typename T, bool AS, bool BS, bool GATED>
-hipError_t launch_tile(int tile, const KernelArgs& g, hipStream_t s) {
-    if (tile == 256) return launch_pp<T, AS, BS, GATED>(g, s);
-    if (tile == 128) return launch_tiles<T, 128, 128, 2, 2, AS, BS, GATED>(g, s);
-    return launch_tiles<T, 64, 64, 4, 1, AS, BS, GATED>(g, s);
+hipError_t launch_tile(int tile, const KernelArgs& g, int cus, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (tile == 256) return launch_pp<T, 256, 256, 2, 4, AS, BS, GATED>(g, s);
+    }
+    if (tile == 128) {
+        // Where every compute unit has at most one of them, eight waves and four stages (4096 x 4096 x 1024: 48 us against 55); otherwise two
+        // workgroups of four waves share one.
+        if (sizeof(T) == 2 && (long)g.tiles_m * g.tiles_n * g.outs * g.splits <= cus) return launch_tiles<T, 128, 128, 4, 2, 4, AS, BS, GATED>(g, s);
+        return launch_tiles<T, 128, 128, 2, 2, 2, AS, BS, GATED>(g, s);
+    }
+    return launch_tiles<T, 64, 64, 4, 1, 3, AS, BS, GATED>(g, s);
+}
+template <typename T, bool GATED>
+hipError_t launch_rows(const KernelArgs& g, hipStream_t s) {
+    hipLaunchKernelGGL((product_rows_kernel<T, GATED>), dim3((unsigned)(up(g.n, 16) / 16)), dim3(512), 0, s, g);
+    return hipGetLastError();
 }
 
 template <typename T>
-hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int xcd_shift, hipStream_t s) {
-    constexpr int S = sizeof(T), BK = Elem<T>::BK;
+hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int cus, int xcd_shift, hipStream_t s) {
+    constexpr int S = sizeof(T);
     const bool gated = p.kind == PRODUCT_GATED;
     KernelArgs g{};
     char* ws = (char*)workspace;
@@ -900,14 +1098,17 @@ hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int
         g.splits = l.splits;
         g.per_split = l.per_split;
         const int tn = gated ? l.tile / 2 : l.tile;
-        g.tiles_m = (int)(up(p.m, l.tile) / l.tile);
-        g.tiles_n = (int)(up(p.n, tn) / tn);
+        if (l.tile) {
+            g.tiles_m = (int)(up(p.m, l.tile) / l.tile);
+            g.tiles_n = (int)(up(p.n, tn) / tn);
+        }
         g.partial = l.splits > 1 ? (float*)ws : nullptr;
         const bool as = l.lie_a == LIE_STEPS, bs = l.lie_b == LIE_STEPS;
         hipError_t e;
-        if (gated) e = as ? launch_tile<T, true, false, true>(l.tile, g, s) : launch_tile<T, false, false, true>(l.tile, g, s);
-        else if (as) e = bs ? launch_tile<T, true, true, false>(l.tile, g, s) : launch_tile<T, true, false, false>(l.tile, g, s);
-        else e = bs ? launch_tile<T, false, true, false>(l.tile, g, s) : launch_tile<T, false, false, false>(l.tile, g, s);
+        if (l.tile == 0) e = gated ? launch_rows<T, true>(g, s) : launch_rows<T, false>(g, s);
+        else if (gated) e = as ? launch_tile<T, true, false, true>(l.tile, g, cus, s) : launch_tile<T, false, false, true>(l.tile, g, cus, s);
+        else if (as) e = bs ? launch_tile<T, true, true, false>(l.tile, g, cus, s) : launch_tile<T, true, false, false>(l.tile, g, cus, s);
+        else e = bs ? launch_tile<T, false, true, false>(l.tile, g, cus, s) : launch_tile<T, false, false, false>(l.tile, g, cus, s);
         if (e != hipSuccess || l.splits == 1) return e;
     }
     const long work = up(p.n, 8) / 8 * p.m * l.outs;
@@ -928,7 +1129,7 @@ hipError_t launch_product(const ProductArgs& p, void* workspace, int cus, int xc
     Plan l;
     if (!make_plan(p, cus, l)) return hipErrorInvalidValue;
     if (p.m == 0 || p.n == 0) return hipSuccess;
-    return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, xcd_shift, stream) : run_product<float>(p, l, workspace, xcd_shift, stream);
+    return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, cus, xcd_shift, stream) : run_product<float>(p, l, workspace, cus, xcd_shift, stream);
 }
 
 long act_grad_partials(long m, long n) { return up(m, GRAD_ROWS) / GRAD_ROWS * n; }

@@ -420,7 +420,7 @@ def test_a_second_derivative_raises():
 
 def test_what_the_entry_points_refuse_is_raised_as_the_packages_error():
     """A row that packs into more than a tile may span, forward; the same in a backward pass, which runs on a thread of its own."""
-    long = torch.zeros(1, 5_000_001, dtype=BF, device=DEV)
+    long = torch.zeros(41, 5_000_001, dtype=BF, device=DEV)
     with pytest.raises(_abi.MuonHipError, match="2 GiB"):
         E.linear(long[:, 1:], torch.zeros(3, 5_000_000, dtype=BF, device=DEV))
 
