@@ -327,7 +327,7 @@ int muon_hip_clip_scale(const void* const* g_ptrs, const long* numel, const long
  *
  * An operand is a matrix of any non-negative strides (in elements): element (i, l) of a[s] is a[s][i * a_row[s] + l * a_col[s]], l the
  * reduction index.  It is read as it lies where one of its strides is 1, the other one and the pointer are whole 16-byte pieces and a tile
- * of it spans less than 2 GiB; anything else is packed into the workspace first, and so are the factors of a gated pair with row stride 1.
+ * of it spans less than 2 GiB; anything else is copied into the workspace first, and so are the factors of a gated pair with row stride 1.
  * Results are row-major m x n matrices.  Sums are fp32 (bf16 operands: products are exact), everything of the epilogue too, results are
  * rounded once.
  *
@@ -336,6 +336,8 @@ int muon_hip_clip_scale(const void* const* g_ptrs, const long* numel, const long
  *           aux[1] = u act'(g), the factors of the gradients of u and of g
  *   SUM     out[0] = a[0] b[0]^T + a[1] b[1]^T
  *   EACH    out[0] = a[0] b[0]^T, out[1] = a[1] b[0]^T
+ * aux holds muon_hip_product_aux_bytes() bytes each, in a form that muon_hip_act_grad reads: the values to 24 bits of which 8 are the
+ * exponent's and one the sign for bf16 tensors, fp32 for fp32 ones.
  * bias (n contiguous elements each), residual (strides res_row, res_col) and aux may be null; SUM and EACH take none of them and
  * MUON_HIP_ACT_NONE.  All tensors share `dtype`.  m, n and k may be 0; a sum over nothing is 0.  Outputs may not overlap inputs, but for a
  * residual that is out[0] itself. */
@@ -367,8 +369,10 @@ typedef struct {
  * would be.  Depends on sizes, strides and the alignment of the pointers. */
 long muon_hip_product_workspace(const muon_hip_product* p);
 int muon_hip_product_run(const muon_hip_product* p, void* workspace, size_t workspace_bytes, void* stream);
+long muon_hip_product_aux_bytes(int dtype, int m, int n);
 
-/* What stands between the incoming gradient and the products of a backward pass, over row-major m x n matrices:
+/* What stands between the incoming gradient and the products of a backward pass, over a row-major m x n gradient and factors that a product
+ * has left as aux:
  *   dz0 = dy * d0 and, with two factors, dz1 = dy * d1, rows `pitch` >= n elements apart (what lies between stays as it was);
  *   db0, db1: the sums of dz0 and dz1 over the rows, before they are rounded (fp32, in a fixed order).
  * `factors` is 2, 1, or 0 for dz0 = dy.  Results may be null where they are not wanted: dz0 and dz1 both or none, each of the sums by

@@ -110,6 +110,7 @@ SIGNATURES = {
                                     c_void_p]),
     "muon_hip_product_workspace": (c_long, [c_void_p]),
     "muon_hip_product_run": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "muon_hip_product_aux_bytes": (c_long, [c_int, c_int, c_int]),
     "muon_hip_act_grad_partials": (c_long, [c_int, c_int]),
     "muon_hip_act_grad": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_long] + [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 2),
     "muon_hip_device_shape": (c_int, [POINTER(c_int), POINTER(c_int)]),

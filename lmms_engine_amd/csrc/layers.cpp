@@ -90,6 +90,11 @@ Tensor result(const Tensor& x, int64_t n) {
 }
 const void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Memory for a factor that the backward pass multiplies by, in the form that the library keeps it in.
+Tensor factor(const Tensor& like, int64_t m, int64_t n) {
+    return at::empty({muon_hip_product_aux_bytes(dtype_of(like), (int)m, (int)n)}, like.options().dtype(at::kByte));
+}
+
 // Results of a forward pass, and the factors of the backward pass where they are kept.
 struct Forward {
     Tensor out, aux[2];
@@ -100,7 +105,7 @@ Forward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, const 
     const int64_t m = x2.size(0), n = w2.size(0);
     Forward f;
     f.out = result(x, n);
-    if (keep && act != MUON_HIP_ACT_NONE) f.aux[0] = at::empty({m, n}, x2.options());
+    if (keep && act != MUON_HIP_ACT_NONE) f.aux[0] = factor(x, m, n);
     Product p(MUON_HIP_PRODUCT_LINEAR, x, m, n, x2.size(1));
     p.activation = act;
     p.left(x2, x2);
@@ -130,7 +135,7 @@ Forward gated_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const
     p.bias[1] = pointer(b1);
     p.out[0] = f.out.data_ptr();
     for (int i = 0; keep && i < 2; ++i) {
-        f.aux[i] = at::empty({m, n}, x2.options());
+        f.aux[i] = factor(x, m, n);
         p.aux[i] = f.aux[i].data_ptr();
     }
     p.run(x);

@@ -59,8 +59,6 @@ struct KernelArgs {
     void* out[2];
     void* aux[2];
     float* partial;  // [split][out or factor][m][n], null: one part
-    int vec;         // rows of out, aux and partial are whole 16-byte pieces
-    int vec_res;
     int xcd_shift;
 };
 
@@ -116,67 +114,113 @@ __device__ __forceinline__ ActPair activate(int act, float z) {
 }
 
 // ---- eight values of a row ----------------------------------------------------------------------
+// Read and written whole where there are eight, at any address (common.h), and one by one at the end of a row.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef u32x2 __attribute__((aligned(1))) u32x2_any;
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long step, bool whole, int count, float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        if (whole) {
-            const bf16x8 w = *(const bf16x8*)p;
+__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
+    if (count >= 8) {
+        if constexpr (sizeof(T) == 2) {
+            const bf16x8 w = *(const bf16x8_any*)p;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = bf2f(w[e]);
-            return;
-        }
-    } else {
-        if (whole) {
-            const f32x4 lo = *(const f32x4*)p, hi = *(const f32x4*)(p + 4);
+        } else {
+            const f32x4 lo = *(const f32x4_any*)p, hi = *(const f32x4_any*)(p + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = lo[e], v[e + 4] = hi[e];
-            return;
         }
+        return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < count ? (float)p[e * step] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = e < count ? (float)p[e] : 0.f;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, bool whole, int count, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        if (whole) {
+__device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
+    if (count >= 8) {
+        if constexpr (sizeof(T) == 2) {
             u32x4 w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
-            *(u32x4*)p = w;
-            return;
+            *(u32x4_any*)p = w;
+        } else {
+            *(f32x4_any*)p = f32x4{v[0], v[1], v[2], v[3]};
+            *(f32x4_any*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
         }
-    } else {
-        if (whole) {
-            *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
-            *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-            return;
-        }
+        return;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (e < count) p[e] = (T)v[e];
 }
 
+// Factors that are kept for the backward pass of bf16 tensors: the upper 24 bits of each, in a plane of the upper 16 and one of the other 8.
+// Cut off, they are off by 2^-16; rounded to bf16 like any activation they are off by 2^-8, as much as the rounding of dy * d behind them, and
+// gradients then were 1.7 times as far from the formula's as results that are rounded once (2.9e-3 against 1.7e-3 in the 2-norm; so it is 2.4e-3).
+// The third byte costs 2 % of a gated training step over 8192 x 4096 x 12288 and half as much memory again; fp32 tensors keep all 32 bits.
+template <typename T>
+__device__ __forceinline__ void keep8(void* base, long all, long at, int count, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        store8((float*)base + at, count, v);
+    } else {
+        uint16_t* high = (uint16_t*)base + at;
+        uint8_t* low = (uint8_t*)base + 2 * all + at;
+        uint32_t b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = __builtin_bit_cast(uint32_t, v[e]);
+        if (count >= 8) {
+            u32x4 h;
+            u32x2 l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = __builtin_amdgcn_perm(b[2 * e + 1], b[2 * e], 0x07060302);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                l[e] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * e + 3], b[4 * e + 2], 0x0c0c0501), __builtin_amdgcn_perm(b[4 * e + 1], b[4 * e], 0x0c0c0501),
+                                             0x05040100);
+            *(u32x4_any*)high = h;
+            *(u32x2_any*)low = l;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < count) high[e] = (uint16_t)(b[e] >> 16), low[e] = (uint8_t)(b[e] >> 8);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void kept8(const void* base, long all, long at, int count, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        load8((const float*)base + at, count, v);
+    } else {
+        const uint16_t* high = (const uint16_t*)base + at;
+        const uint8_t* low = (const uint8_t*)base + 2 * all + at;
+        if (count >= 8) {
+            const u32x4 h = *(const u32x4_any*)high;
+            const u32x2 l = *(const u32x2_any*)low;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t top = e & 1 ? h[e >> 1] & 0xffff0000u : h[e >> 1] << 16;
+                v[e] = __builtin_bit_cast(float, top | ((l[e >> 2] >> (8 * (e & 3))) & 0xffu) << 8);
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < count ? __builtin_bit_cast(float, (uint32_t)high[e] << 16 | (uint32_t)low[e] << 8) : 0.f;
+    }
+}
+
 // The layer's arithmetic on eight sums of row i, columns j .. j + 7 (of both factors of a gated pair), and their way to memory.
 template <typename T, bool GATED>
 __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int j, float (&v)[8], float (&u)[8]) {
     const int count = g.n - j < 8 ? g.n - j : 8;
-    const bool whole = g.vec && count == 8;
-    const long at = i * g.n + j;
+    const long at = i * g.n + j, all = (long)g.m * g.n;
+    auto add = [&](float (&x)[8], const void* base, long off) {
+        float b[8];
+        load8((const T*)base + off, count, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += b[e];
+    };
+    if (g.bias[0]) add(v, g.bias[0], j);
     if constexpr (GATED) {
-        if (g.bias[0]) {
-            float b[8];
-            load8((const T*)g.bias[0] + j, 1, false, count, b);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += b[e];
-        }
-        if (g.bias[1]) {
-            float b[8];
-            load8((const T*)g.bias[1] + j, 1, false, count, b);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] += b[e];
-        }
+        if (g.bias[1]) add(u, g.bias[1], j);
         float h[8], s[8], t[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -185,20 +229,12 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
             s[e] = p.a;
             t[e] = p.d * u[e];
         }
-        store8((T*)g.out[0] + at, whole, count, h);
+        store8((T*)g.out[0] + at, count, h);
         if (g.aux[0]) {
-            // Rounded once each to the tensors' type, like the activations that any layer keeps: the backward pass multiplies them by the
-            // incoming gradient and nothing else, one rounding less than from g and u themselves.
-            store8((T*)g.aux[0] + at, whole, count, s);
-            store8((T*)g.aux[1] + at, whole, count, t);
+            keep8<T>(g.aux[0], all, at, count, s);
+            keep8<T>(g.aux[1], all, at, count, t);
         }
     } else {
-        if (g.bias[0]) {
-            float b[8];
-            load8((const T*)g.bias[0] + j, 1, false, count, b);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += b[e];
-        }
         if (g.act != ACT_NONE) {
             float d[8];
 #pragma unroll
@@ -207,15 +243,19 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
                 v[e] = p.a;
                 d[e] = p.d;
             }
-            if (g.aux[0]) store8((T*)g.aux[0] + at, whole, count, d);
+            if (g.aux[0]) keep8<T>(g.aux[0], all, at, count, d);
         }
         if (g.residual) {
-            float r[8];
-            load8((const T*)g.residual + i * g.res_row + j * g.res_col, g.res_col, g.vec_res && count == 8, count, r);
+            const T* r = (const T*)g.residual + i * g.res_row + j * g.res_col;
+            if (g.res_col == 1) {
+                add(v, r, 0);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += r[e];
+                for (int e = 0; e < 8; ++e)
+                    if (e < count) v[e] += (float)r[e * g.res_col];
+            }
         }
-        store8((T*)g.out[z] + at, whole, count, v);
+        store8((T*)g.out[z] + at, count, v);
     }
 }
 
@@ -228,8 +268,8 @@ __device__ __forceinline__ void emit8(const KernelArgs& g, int split, int z, lon
     }
     const int parts = GATED ? 2 : g.outs, count = g.n - j < 8 ? g.n - j : 8;
     float* p = g.partial + (((long)split * parts + z) * g.m + i) * g.n + j;
-    store8(p, g.vec && count == 8, count, v);
-    if (GATED) store8(p + (long)g.m * g.n, g.vec && count == 8, count, u);
+    store8(p, count, v);
+    if (GATED) store8(p + (long)g.m * g.n, count, u);
 }
 
 // ---- operand tiles in LDS -------------------------------------------------------------------------
@@ -238,50 +278,38 @@ __device__ __forceinline__ void emit8(const KernelArgs& g, int split, int z, lon
 //   steps  reduction step k holds R values; 16-byte piece c lies at place c ^ swizzle(k)
 // The loads write LDS in lane order, so the exchange happens on the side of memory: a lane fetches the piece whose place is its own.
 //
-// Fragments: lane l takes row l % 16 of a fragment and the reduction steps of group l / 16.  The rows of the right operand are dealt to
-// its fragments so that a lane ends up with eight neighbouring columns of the result: row i of fragment j is row
-// (j / 2) * 32 + (i / 4) * 8 + (j % 2) * 4 + i % 4 of the wave's columns, and the four sums that a lane holds of fragment j are
-// columns (j / 2) * 32 + (l / 16) * 8 + (j % 2) * 4 + 0..3.  Results then leave as 16-byte pieces without a trip through LDS.
+// Fragments: lane l takes row l % 16 of a fragment and the reduction steps of group l / 16, and holds four neighbouring columns of the result.
 //
 // The swizzles: reads are served 16 lanes (16-byte reads) or 32 lanes (8-byte transposing reads) at a time, and the lanes that are served
-// together are to touch different banks.  For 16-byte reads of rows the left operand's (r >> 1) & 7 does that for every order of lanes, and
-// the right operand's is the same function of the fragment's row number.  Transposing reads: eight steps, four pieces of 8 bytes each.  The
-// right operand's pieces are 16 bytes apart, which costs it two turns instead of one.
-template <bool RIGHT>
-__device__ __forceinline__ int swizzle_rows(int r) {
-    return RIGHT ? ((r >> 1) & 1) | ((r >> 3) & 3) << 1 : (r >> 1) & 7;
-}
-template <typename T, int R, bool RIGHT>
+// together are to touch different banks: sixteen rows of one step group, and the 32-byte pieces of eight reduction steps.
+__device__ __forceinline__ int swizzle_rows(int r) { return (r >> 1) & 7; }
+template <typename T, int R>
 __device__ __forceinline__ int swizzle_steps(int k) {
-    if constexpr (sizeof(T) == 2) {
-        if (RIGHT) return R >= 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
-        return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : (((k >> 1) & 1) | ((k >> 3) & 1) << 1) << 1;
-    } else {
-        return RIGHT ? ((k >> 2) & 1) << 3 | ((k >> 3) & 1) : ((k >> 2) & 3) << 2;
-    }
+    if constexpr (sizeof(T) == 2) return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) << 1 : (((k >> 1) & 1) | ((k >> 3) & 1) << 1) << 1;
+    else return ((k >> 2) & 3) << 2;
 }
 
 // Where a lane finds its parts of the F fragments of its wave, whose rows start at `first`: as few addresses as the swizzle allows, everything
 // else is a constant that fits a read's offset (a k-tile half h, and the stages of an operand, which lie one behind the other).
-template <typename T, int R, bool STEPS, bool RIGHT, int F>
+template <typename T, int R, bool STEPS, int F>
 struct Reader {
     static constexpr bool HALF = sizeof(T) == 2;
-    static constexpr int N = !STEPS ? 2 : HALF ? (RIGHT ? F / 2 : F) : (RIGHT || F < 4 ? F : 4);
+    static constexpr int N = !STEPS ? 2 : HALF || F < 4 ? F : 4;
     unsigned at[N];
     __device__ __forceinline__ void init(unsigned base, int first, int lane) {
         const int i = lane & 15, grp = lane >> 4;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             if constexpr (!STEPS) {  // n: half of the k-tile
-                const int r = first + (RIGHT ? (i >> 2) * 8 + (i & 3) : i);
-                at[n] = base + r * ROWB + (((n * 4 + grp) ^ swizzle_rows<RIGHT>(r)) << 4);
+                const int r = first + i;
+                at[n] = base + r * ROWB + (((n * 4 + grp) ^ swizzle_rows(r)) << 4);
             } else if constexpr (HALF) {
                 // lane i of a group of 16 addresses piece i (step i / 4, rows of quarter i % 4) and receives row i of steps 0 to 3
-                const int k = grp * 8 + (i >> 2), r = first + (RIGHT ? n * 32 + (i & 3) * 8 : n * 16 + (i & 3) * 4);
-                at[n] = base + k * (R * 2) + (((r >> 3) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 4) * 2;
+                const int k = grp * 8 + (i >> 2), r = first + n * 16 + (i & 3) * 4;
+                at[n] = base + k * (R * 2) + (((r >> 3) ^ swizzle_steps<T, R>(k)) << 4) + (r & 4) * 2;
             } else {
-                const int k = grp * 4, r = first + (RIGHT ? (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3) : n * 16 + i);
-                at[n] = base + k * (R * 4) + (((r >> 2) ^ swizzle_steps<T, R, RIGHT>(k)) << 4) + (r & 3) * 4;
+                const int k = grp * 4, r = first + n * 16 + i;
+                at[n] = base + k * (R * 4) + (((r >> 2) ^ swizzle_steps<T, R>(k)) << 4) + (r & 3) * 4;
             }
         }
     }
@@ -289,15 +317,14 @@ struct Reader {
 #pragma unroll
         for (int n = 0; n < N; ++n) at[n] += bytes;
     }
-    __device__ __forceinline__ typename Elem<T>::frag read(const unsigned char* smem, int stage, int f, int h) const {
-        const int st = stage * (R * ROWB);
+    __device__ __forceinline__ typename Elem<T>::frag read(const unsigned char* smem, int f, int h) const {
         if constexpr (!STEPS) {
-            return *(const typename Elem<T>::frag*)(smem + at[h] + st + (RIGHT ? (f >> 1) * 32 + (f & 1) * 4 : f * 16) * ROWB);
+            return *(const typename Elem<T>::frag*)(smem + at[h] + f * 16 * ROWB);
         } else if constexpr (HALF) {
             s16x4 part[2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                const unsigned char* q = smem + at[RIGHT ? f >> 1 : f] + st + (h * 32 + p * 4) * (R * 2) + (RIGHT ? (f & 1) * 8 : 0);
+                const unsigned char* q = smem + at[f] + (h * 32 + p * 4) * (R * 2);
                 part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_void_ptr)q);
             }
             const s16x8 w = {part[0][0], part[0][1], part[0][2], part[0][3], part[1][0], part[1][1], part[1][2], part[1][3]};
@@ -305,11 +332,24 @@ struct Reader {
         } else {
             f32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = *(const float*)(smem + at[f % N] + st + (h * 16 + e) * (R * 4) + f / N * 256);
+            for (int e = 0; e < 4; ++e) w[e] = *(const float*)(smem + at[f % N] + (h * 16 + e) * (R * 4) + f / N * 256);
             return w;
         }
     }
 };
+
+// Two fragments side by side, of which a lane holds four columns each (4 q .. 4 q + 3 of its 16, q the lane's sixteenth): afterwards it holds
+// eight neighbouring columns, 16 (q % 2) + 8 (q / 2) .. + 7 of their 32, so that results leave in 16-byte pieces without a trip through LDS.
+__device__ __forceinline__ void pair_columns(f32x4& lo, f32x4& hi) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float a = lo[r], b = hi[r];  // (a cast of a vector's element is one of its first element)
+        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+        const unsigned c = s[0], d = s[1];
+        lo[r] = __builtin_bit_cast(float, c);
+        hi[r] = __builtin_bit_cast(float, d);
+    }
+}
 
 __device__ __forceinline__ f32x4 mfma_step(const bf16x8& a, const bf16x8& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -335,12 +375,12 @@ __device__ __forceinline__ void load_lds(const u32x4& rsrc, unsigned offset, uns
 }
 
 // One operand's way into LDS: which pieces a lane fetches, and what of memory may be read.
-template <typename T, int R, int NW, bool STEPS, bool RIGHT, bool GATED>
+template <typename T, int R, int NW, bool STEPS, bool GATED>
 struct Feed {
     static constexpr int LOADS = R / 8 / NW;  // wave instructions of 1 KB
     static constexpr int BK = Elem<T>::BK, PIECE = Elem<T>::PIECE, PIECES = R / PIECE;
     static_assert(R % (8 * NW) == 0, "whole instructions");
-    static_assert(!GATED || (!STEPS && RIGHT), "the factors of a gated pair are interleaved by rows");
+    static_assert(!GATED || !STEPS, "the factors of a gated pair are interleaved by rows");
     unsigned off[LOADS];
     const char *base0, *base1;  // the tile's first row at reduction step 0, of each product (of each factor, GATED)
     unsigned step_bytes;        // STEPS: from one reduction step to the next
@@ -361,11 +401,11 @@ struct Feed {
         for (int n = 0; n < LOADS; ++n) {
             const int at = wave * LOADS + n;
             if constexpr (!STEPS) {
-                const int line = at * 8 + (lane >> 3), c = (lane & 7) ^ swizzle_rows<RIGHT>(line);
+                const int line = at * 8 + (lane >> 3), c = (lane & 7) ^ swizzle_rows(line);
                 const int src = GATED ? (line >> 6) * 32 + (line & 31) : line;
                 off[n] = src * step_bytes + c * 16;
             } else {
-                const int idx = at * 64 + lane, step = idx / PIECES, c = (idx % PIECES) ^ swizzle_steps<T, R, RIGHT>(step);
+                const int idx = at * 64 + lane, step = idx / PIECES, c = (idx % PIECES) ^ swizzle_steps<T, R>(step);
                 off[n] = step * step_bytes + c * 16;
             }
         }
@@ -400,7 +440,7 @@ struct Feed {
         for (int n = 0; n < LOADS; ++n) {
             const int idx = (wave * LOADS + n) * 64 + lane;
             int keep;  // values of the piece that belong to the reduction
-            if constexpr (!STEPS) keep = left - ((lane & 7) ^ swizzle_rows<RIGHT>(idx >> 3)) * PIECE;
+            if constexpr (!STEPS) keep = left - ((lane & 7) ^ swizzle_rows(idx >> 3)) * PIECE;
             else keep = idx / PIECES < left ? PIECE : 0;
             T* p = (T*)(tile + idx * 16);
 #pragma unroll
@@ -446,8 +486,8 @@ __device__ __forceinline__ Tile tile_of(const KernelArgs& g) {
 template <typename T, int BM, int BN, int NW, bool ASTEPS, bool BSTEPS, bool GATED>
 struct Panels {
     static constexpr int BK = Elem<T>::BK;
-    typedef Feed<T, BM, NW, ASTEPS, false, false> FeedA;
-    typedef Feed<T, BN, NW, BSTEPS, true, GATED> FeedB;
+    typedef Feed<T, BM, NW, ASTEPS, false> FeedA;
+    typedef Feed<T, BN, NW, BSTEPS, GATED> FeedB;
     static constexpr int LOADS = FeedA::LOADS + FeedB::LOADS;
     FeedA fa;
     FeedB fb;
@@ -511,8 +551,10 @@ __device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, 
         f32x4 sums[FN];
         pick_row(acc, i, sums);
 #pragma unroll
+        for (int j = 0; j < FN; j += 2) pair_columns(sums[j], sums[j + 1]);
+#pragma unroll
         for (int jp = 0; jp < FN / 2; jp += GATED ? 2 : 1) {
-            const long col = t.n0 + col0 + jp * 32 + quad * 8;
+            const long col = t.n0 + col0 + jp * 32 + (quad & 1) * 16 + (quad >> 1) * 8;
             if (row >= g.m || col >= g.n) continue;
             float v[8], u[8];
 #pragma unroll
@@ -543,8 +585,8 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
     const Tile t = tile_of<BM, GATED ? BN / 2 : BN>(g);
     const P panels(g, t, wave, lane);
     const unsigned lds = (unsigned)(uintptr_t)(lds_void_ptr)smem;
-    Reader<T, BM, ASTEPS, false, FM> ra;
-    Reader<T, BN, BSTEPS, true, FN> rb;
+    Reader<T, BM, ASTEPS, FM> ra;
+    Reader<T, BN, BSTEPS, FN> rb;
     ra.init(0, wm * WTM, lane);
     rb.init(B_AT, wn * WTN, lane);
 
@@ -572,9 +614,9 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
             for (int h = 0; h < 2; ++h) {
                 frag va[FM], vb[FN];
 #pragma unroll
-                for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, h);
+                for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, i, h);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, 0, j, h);
+                for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, j, h);
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -625,8 +667,8 @@ __global__ void __launch_bounds__(512, BM == 128 ? 4 : 2) product_pp_kernel(cons
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    Reader<T, BM, ASTEPS, false, FM> ra;
-    Reader<T, BN, BSTEPS, true, FN> rb;
+    Reader<T, BM, ASTEPS, FM> ra;
+    Reader<T, BN, BSTEPS, FN> rb;
     ra.init(A_AT, wm * WTM, lane);
     rb.init(0, wn * WTN, lane);
     auto multiply = [&](const frag (&va)[FM], const frag (&vb)[FN]) {
@@ -660,18 +702,18 @@ __global__ void __launch_bounds__(512, BM == 128 ? 4 : 2) product_pp_kernel(cons
             const int sa1 = sa == 2 ? 0 : sa + 1, sa2 = sa1 == 2 ? 0 : sa1 + 1;
             frag va[FM], vb[2][FN];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, 0);
+            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, i, 0);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) vb[h][j] = rb.read(smem, 0, j, h);
+                for (int j = 0; j < FN; ++j) vb[h][j] = rb.read(smem, j, h);
             panels.issue_a(kt + 2, t.last, lds + slot_a(sa2));
             WAIT_LDS();
             fence();
             multiply(va, vb[0]);
             fence();
 #pragma unroll
-            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, 0, i, 1);
+            for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, i, 1);
             panels.issue_b(kt + 2, t.last, lds + slot_b(sb));
             ra.move((sa1 - sa) * UNIT_A);
             rb.move(sb ? -UNIT_B : UNIT_B);
@@ -797,11 +839,11 @@ __global__ void __launch_bounds__(256) product_join_kernel(const KernelArgs g) {
         for (int s = 0; s < g.splits; ++s) {
             const float* p = g.partial + (((long)s * parts + z) * g.m + i) * g.n + j;
             float w[8];
-            load8(p, 1, g.vec && count == 8, count, w);
+            load8(p, count, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += w[e];
             if (GATED) {
-                load8(p + (long)g.m * g.n, 1, g.vec && count == 8, count, w);
+                load8(p + (long)g.m * g.n, count, w);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) u[e] += w[e];
             }
@@ -811,10 +853,43 @@ __global__ void __launch_bounds__(256) product_join_kernel(const KernelArgs g) {
 }
 
 // ---- packing ------------------------------------------------------------------------------------
-// rows x cols values from any strides into rows `pitch` apart (whole 16-byte pieces; what lies past cols is left as it is: the products
-// clear it).  64 x 64 values go through LDS, read along the nearer stride.
+// Operands whose lines are no whole 16-byte pieces, copied to lines `pitch` values apart (what lies past a line's end is left as it is: the
+// products clear it).  A line is a row or a reduction step, whichever is contiguous; a thread copies a piece, the matrices of a product one
+// after the other.
+struct PackJob {
+    const void* src;
+    void* dst;
+    long stride, pitch;  // between lines
+    long first;          // piece of the launch that the job starts with
+    int lines, length;
+};
+struct PackList {
+    int n;
+    long pieces;
+    PackJob job[4];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) product_pack_kernel(const T* src, long row, long col, int rows, int cols, T* dst, long pitch, int along) {
+__global__ void __launch_bounds__(256) product_pack_kernel(const PackList l) {
+    constexpr int PIECE = 16 / sizeof(T);
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= l.pieces) return;
+    int n = 0;
+    while (n + 1 < l.n && at >= l.job[n + 1].first) ++n;
+    const PackJob& j = l.job[n];
+    const long each = (j.length + PIECE - 1) / PIECE, line = (at - j.first) / each;
+    const int c = (int)((at - j.first) - line * each) * PIECE;
+    const T* src = (const T*)j.src + line * j.stride + c;
+    T* dst = (T*)j.dst + line * j.pitch + c;
+    if (c + PIECE <= j.length) {
+        if constexpr (sizeof(T) == 2) *(bf16x8*)dst = *(const bf16x8_any*)src;
+        else *(f32x4*)dst = *(const f32x4_any*)src;
+    } else {
+        for (int e = 0; c + e < j.length; ++e) dst[e] = src[e];
+    }
+}
+// rows x cols values of any strides into rows `pitch` apart: 64 x 64 of them go through LDS, read along the nearer stride.
+template <typename T>
+__global__ void __launch_bounds__(256) product_gather_kernel(const T* src, long row, long col, int rows, int cols, T* dst, long pitch, int along) {
     __shared__ T tile[64][65];
     const unsigned across = (unsigned)((cols + 63L) / 64);
     const long r0 = (long)(blockIdx.x / across) * 64, c0 = (long)(blockIdx.x % across) * 64;
@@ -829,37 +904,36 @@ __global__ void __launch_bounds__(256) product_pack_kernel(const T* src, long ro
 }
 
 // ---- activation gradients and sums over rows ----------------------------------------------------------
-// A workgroup takes 256 columns (32 threads, eight columns each) of GRAD_ROWS rows; eight rows at a time.
-constexpr int GRAD_ROWS = 64;
+// A workgroup takes 256 columns (32 threads, eight columns each) of `rows` rows, eight at a time.
 template <typename T, bool PAIR>
-__global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int vec, int chunks) {
+__global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int chunks, int rows) {
+    constexpr int F = PAIR ? 2 : 1;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int blocks = (g.n + 255) / 256;
-    const int chunk = blockIdx.x / blocks;
-    const int j = (blockIdx.x - chunk * blocks) * 256 + tx * 8;
+    const int chunk = blockIdx.x / blocks, j0 = (blockIdx.x - chunk * blocks) * 256, j = j0 + tx * 8;
     const int count = g.n - j < 8 ? g.n - j : 8;
-    const bool whole = vec && count == 8;
-    float sum[PAIR ? 2 : 1][8] = {};
+    const long all = (long)g.m * g.n;
+    float sum[F][8] = {};
     if (j < g.n) {
-        const long r0 = (long)chunk * GRAD_ROWS;
+        const long r0 = (long)chunk * rows;
 #pragma unroll 2
-        for (int s = ty; s < GRAD_ROWS; s += 8) {
+        for (int s = ty; s < rows; s += 8) {
             const long i = r0 + s;
             if (i >= g.m) break;
             float dy[8];
-            load8((const T*)g.dy + i * g.n + j, 1, whole, count, dy);
+            load8((const T*)g.dy + i * g.n + j, count, dy);
 #pragma unroll
-            for (int f = 0; f < (PAIR ? 2 : 1); ++f) {
+            for (int f = 0; f < F; ++f) {
                 float v[8];
                 if (g.factors > f) {
-                    load8((const T*)g.d[f] + i * g.n + j, 1, whole, count, v);
+                    kept8<T>(g.d[f], all, i * g.n + j, count, v);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] *= dy[e];
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = dy[e];
                 }
-                if (g.dz[f]) store8((T*)g.dz[f] + i * g.pitch + j, whole, count, v);
+                if (g.dz[f]) store8((T*)g.dz[f] + i * g.pitch + j, count, v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[f][e] += v[e];
             }
@@ -868,42 +942,48 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int 
     if (!g.partials) return;
     __shared__ float part[8][32][9];
 #pragma unroll
-    for (int f = 0; f < (PAIR ? 2 : 1); ++f) {
+    for (int f = 0; f < F; ++f) {
         if (!g.db[f]) continue;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 8; ++e) part[ty][tx][e] = sum[f][e];
         __syncthreads();
-        const int c = threadIdx.x, col = (blockIdx.x - chunk * blocks) * 256 + c;
-        if (col < g.n) {
+        const int c = threadIdx.x;
+        if (j0 + c < g.n) {
             float v = 0.f;
 #pragma unroll
             for (int y = 0; y < 8; ++y) v += part[y][c >> 3][c & 7];
-            g.partials[((long)f * chunks + chunk) * g.n + col] = v;
+            g.partials[((long)f * chunks + chunk) * g.n + j0 + c] = v;
         }
     }
 }
-// Four rows of threads take the parts in turn; their sums are added in a fixed order.
+// Sixteen rows of threads take the parts in turn; their sums are added in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) row_sum_kernel(const float* partials, int chunks, int n, T* out0, T* out1) {
-    __shared__ float part[4][64];
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, f = blockIdx.y;
+    __shared__ float part[16][16];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, f = blockIdx.y, j = blockIdx.x * 16 + x;
     T* out = f ? out1 : out0;
     if (!out) return;
-    const int j = blockIdx.x * 64 + x;
     float v = 0.f;
-    if (j < n)
-        for (int c = y; c < chunks; c += 4) v += partials[((long)f * chunks + c) * n + j];
+    if (j < n) {
+#pragma unroll 4
+        for (int c = y; c < chunks; c += 16) v += partials[((long)f * chunks + c) * n + j];
+    }
     part[y][x] = v;
     __syncthreads();
-    if (y == 0 && j < n) out[j] = (T)((part[0][x] + part[1][x]) + (part[2][x] + part[3][x]));
+    if (y > 0 || j >= n) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += part[r][x];
+    out[j] = (T)v;
 }
 
 // ---- host side ----------------------------------------------------------------------------------------
 inline long up(long v, long m) { return (v + m - 1) / m * m; }
 inline int elem_size(int dtype) { return dtype == MUON_HIP_BF16 ? 2 : 4; }
 
-enum { LIE_ROWS = 0, LIE_STEPS = 1, LIE_PACKED = 2 };
+// How an operand is read: rows or reduction steps as they lie, or copies of them, or rows put together from any strides.
+enum { LIE_ROWS, LIE_STEPS, LIE_PACKED_ROWS, LIE_PACKED_STEPS, LIE_GATHERED };
+inline bool by_steps(int lie) { return lie == LIE_STEPS || lie == LIE_PACKED_STEPS; }
 struct Plan {
     int lie_a, lie_b;
     long pitch_a, pitch_b;        // elements
@@ -925,28 +1005,34 @@ constexpr Cost kCost[2][3] = {{{4.5f, 0.5f, 0.72f, 0.50f}, {5.f, 1.f, 2.2f, 1.88
 constexpr float kJoinStart = 4.f, kJoinBytes = 5.5e6f;  // of a split reduction: its launch, and bytes in a microsecond
 constexpr int kTile[3] = {64, 128, 256};
 
-// How an operand is read: as it lies where 16-byte pieces of its rows (or of its reduction steps) are aligned and 32 bits span a tile of it.
+// Lines may lie where 16-byte pieces of them are aligned and 32 bits span a tile's: 256 rows, or the 64 reduction steps of a k-tile.
 int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool steps_ok, long& pitch) {
     const long piece = 16 / size;
     auto fits = [&](long p, long lines) { return p % piece == 0 && p <= (0x7fff0000L / size) / lines; };
-    bool by_rows = true, by_steps = steps_ok;
+    bool rows_lie = k <= 0x7fff0000L / size, steps_lie = steps_ok, rows_run = true, steps_run = steps_ok;
     for (int i = 0; i < count; ++i) {
-        if (((uintptr_t)o.base[i]) & 15) by_rows = by_steps = false;
+        const bool aligned = (((uintptr_t)o.base[i]) & 15) == 0;
         // (one row, or one step, has no stride that matters)
-        if (!(o.col[i] == 1 || k == 1) || !(rows == 1 || (fits(o.row[i], 256) && o.row[i] == o.row[0]))) by_rows = false;
-        if (!(o.row[i] == 1 || rows == 1) || !(k == 1 || (fits(o.col[i], 64) && o.col[i] == o.col[0]))) by_steps = false;
+        rows_run = rows_run && (o.col[i] == 1 || k == 1);
+        steps_run = steps_run && (o.row[i] == 1 || rows == 1);
+        rows_lie = rows_lie && aligned && (rows == 1 || (fits(o.row[i], 256) && o.row[i] == o.row[0]));
+        steps_lie = steps_lie && aligned && (k == 1 || (fits(o.col[i], 64) && o.col[i] == o.col[0]));
     }
-    if (k > 0x7fff0000L / size) by_rows = false;
-    if (by_rows) {
+    if (rows_lie && rows_run) {
         pitch = rows == 1 ? 0 : o.row[0];
         return LIE_ROWS;
     }
-    if (by_steps) {
+    if (steps_lie && steps_run) {
         pitch = k == 1 ? 0 : o.col[0];
         return LIE_STEPS;
     }
-    pitch = up(k, piece);
-    return LIE_PACKED;
+    const long row_pitch = up(k, piece), step_pitch = up(rows, piece);
+    if (steps_run && (!rows_run || !fits(row_pitch, 256)) && fits(step_pitch, 64)) {
+        pitch = step_pitch;
+        return LIE_PACKED_STEPS;
+    }
+    pitch = row_pitch;
+    return rows_run ? LIE_PACKED_ROWS : LIE_GATHERED;
 }
 
 // Few rows against rows of a weight, wherever they start: one launch, where tiles that leave most of the machine idle would have to share the
@@ -978,10 +1064,15 @@ bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     if (few_rows(p, l)) return true;
     l.lie_a = lie_of(p.a, l.count_a, p.m, p.k, size, true, l.pitch_a);
     l.lie_b = lie_of(p.b, l.count_b, p.n, p.k, size, !gated, l.pitch_b);
-    for (const long pitch : {l.lie_a == LIE_PACKED ? l.pitch_a : 0, l.lie_b == LIE_PACKED ? l.pitch_b : 0})
-        if (pitch > (0x7fff0000L / size) / 256) return false;
-    l.pack_a = l.lie_a == LIE_PACKED ? up(p.m * l.pitch_a * size, 256) : 0;
-    l.pack_b = l.lie_b == LIE_PACKED ? up(p.n * l.pitch_b * size, 256) : 0;
+    auto pack_bytes = [&](int lie, long pitch, long rows) {
+        if (lie == LIE_ROWS || lie == LIE_STEPS) return 0L;
+        if (lie != LIE_PACKED_STEPS && pitch > (0x7fff0000L / size) / 256) return -1L;
+        if (up(p.k, 64) / 64 * (up(rows, 64) / 64) > 0x7fffffffL / 32) return -1L;  // (workgroups of the copies)
+        return up((lie == LIE_PACKED_STEPS ? p.k : rows) * pitch * size, 256);
+    };
+    l.pack_a = pack_bytes(l.lie_a, l.pitch_a, p.m);
+    l.pack_b = pack_bytes(l.lie_b, l.pitch_b, p.n);
+    if (l.pack_a < 0 || l.pack_b < 0) return false;
     l.nk = (int)((p.k + (long)bk - 1) / bk);
     auto tiles_of = [&](int t) { return up(p.m, t) / t * (up(p.n, gated ? t / 2 : t) / (gated ? t / 2 : t)) * l.outs; };
     const long all = (long)l.nk * l.segments;
@@ -1058,14 +1149,22 @@ hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int
     const bool gated = p.kind == PRODUCT_GATED;
     KernelArgs g{};
     char* ws = (char*)workspace;
+    PackList copies{};
     auto pack = [&](const ProductOperand& o, int lie, int count, int rows, long pitch, long bytes, const void** at) {
         for (int i = 0; i < count; ++i) {
             at[i] = o.base[i];
-            if (lie != LIE_PACKED) continue;
-            const int along = o.row[i] < o.col[i];
-            const dim3 grid((unsigned)(up(p.k, 64) / 64 * (up(rows, 64) / 64)));
-            hipLaunchKernelGGL(product_pack_kernel<T>, grid, dim3(256), 0, s, (const T*)o.base[i], o.row[i], o.col[i], rows, p.k, (T*)ws, pitch, along);
-            if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            if (bytes == 0) continue;
+            if (lie == LIE_GATHERED) {
+                const dim3 grid((unsigned)(up(p.k, 64) / 64 * (up(rows, 64) / 64)));
+                hipLaunchKernelGGL(product_gather_kernel<T>, grid, dim3(256), 0, s, (const T*)o.base[i], o.row[i], o.col[i], rows, p.k, (T*)ws, pitch,
+                                   (int)(o.row[i] < o.col[i]));
+                if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+            } else {
+                const bool steps = lie == LIE_PACKED_STEPS;
+                PackJob& j = copies.job[copies.n++];
+                j = PackJob{o.base[i], ws, steps ? o.col[i] : o.row[i], pitch, copies.pieces, steps ? p.k : rows, steps ? rows : p.k};
+                copies.pieces += j.lines * (up(j.length, 16 / S) / (16 / S));
+            }
             at[i] = ws;
             ws += bytes;
         }
@@ -1084,13 +1183,14 @@ hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int
     g.residual = p.residual;
     g.res_row = p.res_row;
     g.res_col = p.res_col;
-    auto aligned = [](const void* q) { return (((uintptr_t)q) & 15) == 0; };
-    g.vec = p.n % 8 == 0 && aligned(p.out[0]) && aligned(p.out[1]) && aligned(p.aux[0]) && aligned(p.aux[1]);
-    g.vec_res = p.residual && p.n % 8 == 0 && p.res_col == 1 && p.res_row % (16 / S) == 0 && aligned(p.residual);
     g.xcd_shift = xcd_shift;
     if (p.k > 0) {
         if (hipError_t e = pack(p.a, l.lie_a, l.count_a, p.m, l.pitch_a, l.pack_a, g.a); e != hipSuccess) return e;
         if (hipError_t e = pack(p.b, l.lie_b, l.count_b, p.n, l.pitch_b, l.pack_b, g.b); e != hipSuccess) return e;
+        if (copies.n > 0) {
+            hipLaunchKernelGGL(product_pack_kernel<T>, dim3((unsigned)(up(copies.pieces, 256) / 256)), dim3(256), 0, s, copies);
+            if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        }
         g.pitch_a = l.pitch_a;
         g.pitch_b = l.pitch_b;
         g.nk = l.nk;
@@ -1103,7 +1203,7 @@ hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int
             g.tiles_n = (int)(up(p.n, tn) / tn);
         }
         g.partial = l.splits > 1 ? (float*)ws : nullptr;
-        const bool as = l.lie_a == LIE_STEPS, bs = l.lie_b == LIE_STEPS;
+        const bool as = by_steps(l.lie_a), bs = by_steps(l.lie_b);
         hipError_t e;
         if (l.tile == 0) e = gated ? launch_rows<T, true>(g, s) : launch_rows<T, false>(g, s);
         else if (gated) e = as ? launch_tile<T, true, false, true>(l.tile, g, cus, s) : launch_tile<T, false, false, true>(l.tile, g, cus, s);
@@ -1132,23 +1232,30 @@ hipError_t launch_product(const ProductArgs& p, void* workspace, int cus, int xc
     return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, cus, xcd_shift, stream) : run_product<float>(p, l, workspace, cus, xcd_shift, stream);
 }
 
-long act_grad_partials(long m, long n) { return up(m, GRAD_ROWS) / GRAD_ROWS * n; }
+// Rows of a workgroup: as many as leave the machine enough of them, so that small gradients are not a loop and large ones have few parts.
+static long act_grad_rows(long m, long n) {
+    long rows = 64;
+    while (rows > 8 && up(m, rows) / rows * (up(n, 256) / 256) < 1024) rows /= 2;
+    return rows;
+}
+long act_grad_partials(long m, long n) {
+    const long rows = act_grad_rows(m, n);
+    return up(m, rows) / rows * n;
+}
 
 hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t stream) {
     const bool pair = a.factors > 1;
-    const long chunks = up(a.m, GRAD_ROWS) / GRAD_ROWS, blocks = up(a.n, 256) / 256 * chunks;
-    auto aligned = [](const void* q) { return (((uintptr_t)q) & 15) == 0; };
-    const int vec = a.n % 8 == 0 && a.pitch % 8 == 0 && aligned(a.dy) && aligned(a.d[0]) && aligned(a.d[1]) && aligned(a.dz[0]) && aligned(a.dz[1]);
+    const long rows = act_grad_rows(a.m, a.n), chunks = up(a.m, rows) / rows, blocks = up(a.n, 256) / 256 * chunks;
     const bool bf = a.dtype == MUON_HIP_BF16;
     if (blocks > 0) {
-        if (bf && pair) hipLaunchKernelGGL((act_grad_kernel<bf16_t, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
-        else if (bf) hipLaunchKernelGGL((act_grad_kernel<bf16_t, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
-        else if (pair) hipLaunchKernelGGL((act_grad_kernel<float, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
-        else hipLaunchKernelGGL((act_grad_kernel<float, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, vec, (int)chunks);
+        void (*kern)(const ActGradArgs, int, int);
+        if (bf) kern = pair ? act_grad_kernel<bf16_t, true> : act_grad_kernel<bf16_t, false>;
+        else kern = pair ? act_grad_kernel<float, true> : act_grad_kernel<float, false>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream, a, (int)chunks, (int)rows);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     if ((!a.db[0] && !a.db[1]) || a.n == 0) return hipSuccess;
-    const dim3 grid((unsigned)(up(a.n, 64) / 64), pair ? 2 : 1);
+    const dim3 grid((unsigned)(up(a.n, 16) / 16), pair ? 2 : 1);
     if (bf) hipLaunchKernelGGL(row_sum_kernel<bf16_t>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (bf16_t*)a.db[0], (bf16_t*)a.db[1]);
     else hipLaunchKernelGGL(row_sum_kernel<float>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (float*)a.db[0], (float*)a.db[1]);
     return hipGetLastError();

@@ -10,8 +10,9 @@ products of float32 tensors keep single precision.  Operands are read as they li
 16-byte pieces go through packed copies.  There is no counterpart in the reference, which leaves its layers to torch, and, as everywhere in
 this package, no CPU path.
 
-Both functions can be differentiated once by every tensor argument.  What the backward pass needs is kept in the tensors' type: the
-inputs, and for every result the factors that the incoming gradient is multiplied by (nothing of the kind without an activation).
+Both functions can be differentiated once by every tensor argument.  For the backward pass they keep the inputs, and for every result the
+factors that the incoming gradient is multiplied by: one with an activation, two of a gated pair, none otherwise, in 24 bits for bfloat16
+tensors (three bytes a value) and in 32 for float32.
 """
 from __future__ import annotations
 

@@ -3,13 +3,17 @@
 A rounding to a type is off by at most u = eps / 2 of the value.  The kernels add products of exact operands in fp32, in some order: the sum
 is off by at most terms * 2^-24 of the sum of magnitudes (+ 4 for bias, join and residual).  An activation is evaluated in fp32 within 2^-20 of
 max(1, |z|) (a handful of operations and math functions of a few steps each) and carries an error of z on with a slope of at most 1.2; so does
-its derivative, whose slope is at most 1.2 too and which is at most 1.2 itself.  What is kept for the backward pass is rounded once more, and so
-is its product with the incoming gradient."""
+its derivative, whose slope is at most 1.2 too and which is at most 1.2 itself.  What is kept for the backward pass is cut off behind 16 bits of
+the significand (2^-15 at most, bf16 tensors) or kept whole, and its product with the incoming gradient is rounded."""
 import math
 
 import torch
 
 F32 = 2.0 ** -24
+
+
+def cut(dtype):
+    return 2.0 ** -15 if dtype == torch.bfloat16 else 0.0
 
 
 def unit(dtype):
@@ -61,7 +65,7 @@ def linear(x, w, b, r, name, dy, dtype):
     y = a if r is None else a + r
     out = {"y": (y, ea + (u + 2 * F32) * (y.abs() + ea))}
     dz = dy * d
-    kept = 0.0 if name == "none" else u
+    kept = 0.0 if name == "none" else cut(dtype)
     edz = dy.abs() * (ed + kept * (d.abs() + ed))          # of the unrounded product
     made = edz + (0.0 if name == "none" else u + F32) * (dz.abs() + edz)  # of the rounded one
     mag = dz.abs() + made
@@ -88,9 +92,9 @@ def gated(x, wg, wu, bg, bu, name, dh, dtype):
     et = ed * v.abs() + d.abs() * ev + ed * ev + 2 * F32 * (d * v).abs()
     dzs = []
     for factor, ef in ((d * v, et), (a, ea)):  # of g, of u
-        kept = ef + u * (factor.abs() + ef)
+        kept = ef + cut(dtype) * (factor.abs() + ef)
         dz = dh * factor
-        edz = dh.abs() * kept
+        edz = dh.abs() * kept + F32 * (dz.abs() + dh.abs() * kept)
         dzs.append((dz, edz, edz + (u + F32) * (dz.abs() + edz)))
     dx = sum(dz @ w for (dz, _, _), w in zip(dzs, (wg, wu)))
     edx = sum(m @ w.abs() + (2 * w.size(0) + 4) * F32 * ((dz.abs() + m) @ w.abs()) for (dz, _, m), w in zip(dzs, (wg, wu)))

@@ -121,7 +121,13 @@ def test_activation_gradients_are_checked_before_any_launch():
     assert run(one, 3, one, one, one, one, 8, None, None, 1, 4, 8, None, None) == -1
     assert run(None, 1, one, None, one, None, 8, None, None, 1, 4, 8, None, None) == -1
     assert run(one, 1, one, None, one, None, 8, one, None, 1, 4, 8, None, None) == -1  # sums without room for their parts
-    assert lib.muon_hip_act_grad_partials(0, 5) == 0 and lib.muon_hip_act_grad_partials(65, 3) == 6
+    assert lib.muon_hip_act_grad_partials(0, 5) == 0
+    for m, n in ((1, 1), (65, 3), (5000, 4096), (100000, 20000)):
+        floats = lib.muon_hip_act_grad_partials(m, n)
+        assert floats > 0 and floats % n == 0 and floats * 4 <= 4 * n + m * n  # a part is a row of sums, at most one for eight rows
+    assert lib.muon_hip_product_aux_bytes(_abi.BF16, 5, 7) == 105 and lib.muon_hip_product_aux_bytes(_abi.F32, 5, 7) == 140
+    assert lib.muon_hip_product_aux_bytes(_abi.BF16, 1 << 30, 1 << 20) == 3 << 50
+    assert lib.muon_hip_product_aux_bytes(9, 5, 7) < 0
 
 
 def test_activation_names_are_those_of_the_header():
