@@ -1005,9 +1005,9 @@ constexpr Cost kCost[2][3] = {{{4.5f, 0.5f, 0.72f, 0.50f}, {5.f, 1.f, 2.2f, 1.88
 constexpr float kJoinStart = 4.f, kJoinBytes = 5.5e6f;  // of a split reduction: its launch, and bytes in a microsecond
 constexpr int kTile[3] = {64, 128, 256};
 
-// Lines may lie where 16-byte pieces of them are aligned and 32 bits span a tile's: 256 rows, or the 64 reduction steps of a k-tile.
+// Lines may lie where 16-byte pieces of them are aligned and 31 bits span a tile's: 256 rows, or the 64 reduction steps of a k-tile.
 int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool steps_ok, long& pitch) {
-    const long piece = 16 / size;
+    const long piece = 16 / size, lines = rows < 256 ? rows : 256;
     auto fits = [&](long p, long lines) { return p % piece == 0 && p <= (0x7fff0000L / size) / lines; };
     bool rows_lie = k <= 0x7fff0000L / size, steps_lie = steps_ok, rows_run = true, steps_run = steps_ok;
     for (int i = 0; i < count; ++i) {
@@ -1015,7 +1015,7 @@ int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool s
         // (one row, or one step, has no stride that matters)
         rows_run = rows_run && (o.col[i] == 1 || k == 1);
         steps_run = steps_run && (o.row[i] == 1 || rows == 1);
-        rows_lie = rows_lie && aligned && (rows == 1 || (fits(o.row[i], 256) && o.row[i] == o.row[0]));
+        rows_lie = rows_lie && aligned && (rows == 1 || (fits(o.row[i], lines) && o.row[i] == o.row[0]));
         steps_lie = steps_lie && aligned && (k == 1 || (fits(o.col[i], 64) && o.col[i] == o.col[0]));
     }
     if (rows_lie && rows_run) {
@@ -1027,7 +1027,7 @@ int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool s
         return LIE_STEPS;
     }
     const long row_pitch = up(k, piece), step_pitch = up(rows, piece);
-    if (steps_run && (!rows_run || !fits(row_pitch, 256)) && fits(step_pitch, 64)) {
+    if (steps_run && (!rows_run || !fits(row_pitch, lines)) && fits(step_pitch, 64)) {
         pitch = step_pitch;
         return LIE_PACKED_STEPS;
     }
@@ -1066,7 +1066,7 @@ bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     l.lie_b = lie_of(p.b, l.count_b, p.n, p.k, size, !gated, l.pitch_b);
     auto pack_bytes = [&](int lie, long pitch, long rows) {
         if (lie == LIE_ROWS || lie == LIE_STEPS) return 0L;
-        if (lie != LIE_PACKED_STEPS && pitch > (0x7fff0000L / size) / 256) return -1L;
+        if (lie != LIE_PACKED_STEPS && pitch > (0x7fff0000L / size) / (rows < 256 ? rows : 256)) return -1L;
         if (up(p.k, 64) / 64 * (up(rows, 64) / 64) > 0x7fffffffL / 32) return -1L;  // (workgroups of the copies)
         return up((lie == LIE_PACKED_STEPS ? p.k : rows) * pitch * size, 256);
     };

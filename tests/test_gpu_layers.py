@@ -59,7 +59,8 @@ def compare(got, want):
 
 # tokens, inner, outer: single values and rows, the edges of pieces, fragments, tiles and k-tiles, long reductions over few results
 SIZES = [(1, 1, 1), (1, 64, 8), (3, 8, 5), (2, 7, 64), (16, 64, 64), (17, 251, 33), (64, 128, 64), (65, 130, 129), (130, 72, 264), (33, 1000, 77),
-         (257, 96, 520), (1, 4096, 512), (5, 2049, 130), (2000, 24, 40), (700, 200, 1000)]
+         (257, 96, 520), (1, 4096, 512), (5, 2049, 130), (2000, 24, 40), (700, 200, 1000), (8, 250, 35),
+         (9, 250, 35), (6, 4100, 17), (40, 9000, 24)]
 ACTS = list(layers.ACTIVATIONS)
 
 
@@ -419,10 +420,90 @@ def test_a_second_derivative_raises():
 
 
 def test_what_the_entry_points_refuse_is_raised_as_the_packages_error():
-    """A row that packs into more than a tile may span, forward; the same in a backward pass, which runs on a thread of its own."""
-    long = torch.zeros(41, 5_000_001, dtype=BF, device=DEV)
+    """Rows of which a tile spans more than 31 bits reach, forward; the same in a backward pass, which runs on a thread of its own."""
+    long = torch.zeros(41, 30_000_001, dtype=BF, device=DEV)
     with pytest.raises(_abi.MuonHipError, match="2 GiB"):
-        E.linear(long[:, 1:], torch.zeros(3, 5_000_000, dtype=BF, device=DEV))
+        E.linear(long[:, 1:], torch.zeros(3, 30_000_000, dtype=BF, device=DEV))
+    del long
+    x, w = torch.ones(300, 1, dtype=BF, device=DEV, requires_grad=True), torch.ones(4_300_000, 1, dtype=BF, device=DEV)
+    y = E.linear(x, w)
+    assert (y == 1).all()
+    with pytest.raises(_abi.MuonHipError, match="2 GiB"):
+        torch.autograd.grad(y, x, y.detach())
+
+
+def test_more_tokens_than_a_row_may_span():
+    """The reduction of a weight's gradient over millions of rows that have to be copied first.  Whole numbers: every partial sum is exact."""
+    g = gen_of(53)
+    t, k, n = 4_400_003, 9, 5
+    x = torch.randint(-1, 2, (t, k), generator=g, device=DEV).to(BF)
+    dy = torch.randint(-1, 2, (t, n), generator=g, device=DEV).to(BF)
+    w, b = torch.zeros(n, k, dtype=F, device=DEV), torch.zeros(n, dtype=F, device=DEV)
+    for dt in (F, BF):
+        xs, ws, bs = x.to(dt), w.to(dt).requires_grad_(True), b.to(dt).requires_grad_(True)
+        dw, db = torch.autograd.grad(E.linear(xs, ws, bs), (ws, bs), dy.to(dt))
+        want = dy.double().t() @ x.double()
+        assert want.abs().max() < 2 ** 24
+        assert torch.equal(dw.double(), want.to(dt).double()) and torch.equal(db.double(), dy.double().sum(0).to(dt).double())
+
+
+def test_activation_gradients_leave_the_room_between_rows():
+    """muon_hip_act_grad on rows further apart than they are long, with two factors, one or none, and with sums or results alone."""
+    lib, g = _abi.lib(), gen_of(59)
+    for dtype, (m, n) in itertools.product((BF, F), ((5, 7), (70, 264), (600, 1001))):
+        dy, one = rnd(g, m, n, dtype=dtype), torch.ones(1, 1, dtype=dtype, device=DEV)
+        kept = []
+        for _ in range(2):  # factors as a product leaves them: act'(z) of z = x * 1, here of rows of one column
+            x = rnd(g, m * n, 1, dtype=dtype)
+            aux = torch.empty(lib.muon_hip_product_aux_bytes(_abi.dtype_code(dtype), m, n), dtype=torch.uint8, device=DEV)
+            out = torch.empty_like(x)
+            p = _abi.Product(kind=0, dtype=_abi.dtype_code(dtype), activation=3, m=m * n, n=1, k=1)
+            p.a[:], p.a_row[:], p.a_col[:] = [x.data_ptr()] * 2, (1, 1), (1, 1)
+            p.b[:], p.b_row[:], p.b_col[:] = [one.data_ptr()] * 2, (1, 1), (1, 1)
+            p.out[0], p.aux[0] = out.data_ptr(), aux.data_ptr()
+            need = lib.muon_hip_product_workspace(ctypes.addressof(p))
+            ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+            _abi.check(lib.muon_hip_product_run(ctypes.addressof(p), ws.data_ptr(), need, _abi.stream_ptr(x.device)))
+            kept.append((aux, R.activation("silu", x.double().view(m, n))[1]))
+        pitch = n + 11
+        for factors, results, sums in itertools.product((0, 1, 2), (True, False), (True, False)):
+            dz = [torch.full((m, pitch), 7.0, dtype=dtype, device=DEV) for _ in range(max(1, factors))]
+            db = [torch.full((n + 3,), 7.0, dtype=dtype, device=DEV) for _ in range(max(1, factors))]
+            parts = torch.empty(lib.muon_hip_act_grad_partials(m, n) * max(1, factors), dtype=F, device=DEV)
+            ptr = lambda ts, i, on: ts[i].data_ptr() if on and i < max(1, factors) else None
+            _abi.check(lib.muon_hip_act_grad(dy.data_ptr(), factors, kept[0][0].data_ptr() if factors else None, kept[1][0].data_ptr() if factors > 1 else None,
+                                             ptr(dz, 0, results), ptr(dz, 1, results), pitch, ptr(db, 0, sums), ptr(db, 1, sums), _abi.dtype_code(dtype),
+                                             m, n, parts.data_ptr(), _abi.stream_ptr(dy.device)))
+            for i in range(max(1, factors)):
+                d = kept[i][1] if factors else torch.ones(m, n, dtype=torch.float64, device=DEV)
+                want = dy.double() * d
+                err = want.abs() * (R.cut(dtype) + 2 * R.F32) + dy.double().abs() * 2.0 ** -20 if factors else torch.zeros_like(want)
+                if results:
+                    R.check("dz", dz[i][:, :n], want, err + (R.unit(dtype) if factors else 0) * (want.abs() + err))
+                assert (dz[i][:, n if results else 0:] == 7).all() and (db[i][n if sums else 0:] == 7).all()
+                if sums:
+                    total, room = want.sum(0), err.sum(0) + (m + 4) * R.F32 * (want.abs() + err).sum(0)
+                    R.check("db", db[i][:n], total, room + R.unit(dtype) * (total.abs() + room))
+
+
+def test_two_graphs_that_share_a_pool_and_replay_in_turn():
+    g = gen_of(61)
+    x, x2, w = rnd(g, 40, 4096), rnd(g, 40, 4096), rnd(g, 264, 4096, scale=0.02)
+    E.linear(x, w, activation="silu")
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    pool = torch.cuda.graph_pool_handle()
+    for gr, v in zip(graphs, (x, x2)):
+        with torch.cuda.graph(gr, pool=pool):
+            outs.append(E.linear(v, w, activation="silu"))
+    for r in range(3):
+        for v in (x, x2):
+            v.copy_(rnd(g, 40, 4096))
+        graphs[0].replay()
+        graphs[1].replay()
+        got = [o.clone() for o in outs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, E.linear(v, w, activation="silu")) for a, v in zip(got, (x, x2))), r
 
 
 def test_tensors_of_other_kinds_are_refused():
