@@ -319,10 +319,11 @@ bool fits(const Tensor& x, const Tensor& w, const Tensor& b) {
     return x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) <= most && w.size(1) <= most && rows_of(x) <= most &&
            (!b.defined() || (b.dim() == 1 && b.size(0) == w.size(0)));
 }
+// Whether the call has a history; a tangent of forward mode counts too, so that autograd refuses it.
 bool differentiated(const Tensor* t, int count) {
-    if (!at::GradMode::is_enabled()) return false;
+    const bool backward = at::GradMode::is_enabled();
     for (int i = 0; i < count; ++i)
-        if (t[i].defined() && t[i].requires_grad()) return true;
+        if (t[i].defined() && ((backward && t[i].requires_grad()) || t[i]._fw_grad(0).defined())) return true;
     return false;
 }
 

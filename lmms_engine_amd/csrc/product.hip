@@ -744,7 +744,8 @@ __global__ void __launch_bounds__(512) product_rows_kernel(const KernelArgs g) {
     constexpr int W = GATED ? 2 : 1, NW = 8, PIECE = Elem<T>::PIECE, STEP = 4 * PIECE;  // reduction steps of a fragment
     constexpr int STEPS = GATED ? 4 : 6;
     __shared__ __align__(16) float part[NW][W][16][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, grp = lane >> 4;
+    // (Matrix instructions run whichever lanes are switched on: what decides over them has to be known to be the same in all of a wave's.)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, grp = lane >> 4;
     const int n0 = blockIdx.x * 16;
     const int row = n0 + i < g.n ? n0 + i : g.n - 1;  // (rows past the end are the last one again: what they give is not wanted)
     const T* wp[W];

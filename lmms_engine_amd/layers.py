@@ -12,7 +12,8 @@ this package, no CPU path.
 
 Both functions can be differentiated once by every tensor argument.  For the backward pass they keep the inputs, and for every result the
 factors that the incoming gradient is multiplied by: one with an activation, two of a gated pair, none otherwise, in 24 bits for bfloat16
-tensors (three bytes a value) and in 32 for float32.
+tensors (three bytes a value) and in 32 for float32.  Forward-mode differentiation, second derivatives and tensor subclasses are refused;
+autocast leaves the calls alone.
 """
 from __future__ import annotations
 

@@ -90,6 +90,20 @@ def test_gated_linear(dtype, i, size):
     compare(run_gated(x, wg, wu, bg, bu, name, dh), R.gated(x, wg, wu, bg, bu, name, dh, dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("steps", range(1, 30))
+def test_few_rows_with_every_rest(dtype, steps):
+    """Up to eight rows, whose reduction eight waves share in batches of fragments: every number of fragments that may be left for a wave."""
+    g = gen_of(300 + steps)
+    step = 32 if dtype == BF else 16
+    for k in (8 * step * steps, 8 * step * steps - 3 * step - 5):
+        x, w, w2 = rnd(g, 1 + steps % 8, k, dtype=dtype), *(rnd(g, 40, k, scale=k ** -0.5, dtype=dtype) for _ in range(2))
+        dy = torch.zeros(x.size(0), 40, dtype=dtype, device=DEV)
+        for _ in range(2):
+            R.check("linear", E.linear(x, w), *R.linear(x, w, None, None, "none", dy, dtype)["y"])
+            R.check("gated", E.gated_linear(x, w, w2), *R.gated(x, w, w2, None, None, "silu", dy, dtype)["y"])
+
+
 # Results of many tiles: every tile size, also for gradients, whole and ragged in every direction.
 LARGE = [(2060, 200, 2056), (4100, 136, 4200), (136, 4100, 4200), (4100, 4200, 72), (4352, 320, 4096), (1024, 1024, 1024), (4099, 100, 4103)]
 
@@ -417,6 +431,32 @@ def test_a_second_derivative_raises():
             dx.float().sum().backward()
     (dr,) = torch.autograd.grad(E.linear(x, w, residual=r).float().square().sum(), r, create_graph=True)
     dr.float().sum().backward()
+
+
+def test_forward_mode_is_refused():
+    """A tangent is not dropped silently."""
+    x, w = rnd(gen_of(67), 4, 16, dtype=F), rnd(gen_of(68), 8, 16, dtype=F)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: E.linear(dual, w), lambda: E.gated_linear(dual, w, w), lambda: E.linear(x, w, residual=torch.autograd.forward_ad.make_dual(rnd(gen_of(69), 4, 8, dtype=F), torch.ones(4, 8, device=DEV)))):
+            with pytest.raises(RuntimeError):
+                f()
+
+
+def test_leaves_that_are_used_twice():
+    """x as its own weight, and one weight for both factors: both contributions arrive."""
+    g = gen_of(71)
+    x = rnd(g, 24, 24, dtype=F).requires_grad_(True)
+    (got,) = torch.autograd.grad(E.linear(x, x).square().sum(), x)
+    y = x.detach().double().requires_grad_(True)
+    (want,) = torch.autograd.grad((y @ y.t()).square().sum(), y)
+    assert ((got - want).norm() / want.norm()).item() <= 64 * R.F32 * 24 ** 0.5
+    w = rnd(g, 16, 24, dtype=F, scale=0.2).requires_grad_(True)
+    (got,) = torch.autograd.grad(E.gated_linear(x.detach(), w, w, activation="sigmoid").sum(), w)
+    v = w.detach().double().requires_grad_(True)
+    z = x.detach().double() @ v.t()
+    (want,) = torch.autograd.grad((torch.sigmoid(z) * z).sum(), v)
+    assert ((got - want).norm() / want.norm()).item() <= 64 * R.F32 * 24 ** 0.5
 
 
 def test_what_the_entry_points_refuse_is_raised_as_the_packages_error():
