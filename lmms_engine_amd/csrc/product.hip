@@ -746,13 +746,13 @@ __global__ void __launch_bounds__(512, BM == 128 ? 4 : 2) product_pp_kernel(cons
 // factors of a gated pair), its eight waves an eighth of the reduction each: a wave's load is 16 rows x 64 bytes, a fragment as the matrix
 // instruction takes it, and the fragments of x come out of the caches the same way.  The next STEPS of them are on their way while the last
 // are multiplied.  The waves' sums meet in LDS.  Rows may start at any element: the hardware reads vectors from any address.  Bound by
-// memory: two factors of 12288 x 4096, 201 MB, take 38 us (5.3 TB/s).
+// memory: two factors of 12288 x 4096, 201 MB, take 40 us (5.0 TB/s), one 21.  Deeper batches in one workgroup a compute unit: 41 and 23.
 template <typename T, bool GATED>
-__global__ void __launch_bounds__(512) product_rows_kernel(const KernelArgs g) {
+__global__ void __launch_bounds__(512, 4) product_rows_kernel(const KernelArgs g) {
     typedef typename Elem<T>::frag frag;
     typedef frag __attribute__((aligned(sizeof(T)))) frag_any;
     constexpr int W = GATED ? 2 : 1, NW = 8, PIECE = Elem<T>::PIECE, STEP = 4 * PIECE;  // reduction steps of a fragment
-    constexpr int STEPS = GATED ? 4 : 6;
+    constexpr int STEPS = GATED ? 3 : 4;  // (in the registers that two workgroups of a compute unit have)
     __shared__ __align__(16) float part[NW][W][16][16];
     // (Matrix instructions run whichever lanes are switched on: what decides over them has to be known to be the same in all of a wave's.)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, grp = lane >> 4;
@@ -1049,10 +1049,11 @@ int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool s
 
 // Few rows against rows of a weight, wherever they start: one launch, where tiles that leave most of the machine idle would have to share the
 // reduction and be joined (1 x 4096 x 4096: 9 us against 14).  From 9 rows on the fragments of x are as much to fetch as the weight and the
-// tiles, which keep theirs in LDS, are faster (16 x 4096 x 12288: 24 us against 30).
-constexpr int kFewRows = 8;
+// tiles, which keep theirs in LDS, are faster (16 x 4096 x 12288: 24 us against 30; a gated pair of 8 rows: 40 against 44, of 4 rows 40 both, of
+// 4 x 4096 x 4096 18 against 16).
+constexpr int kFewRows = 8, kFewRowsGated = 4;
 bool few_rows(const ProductArgs& p, Plan& l) {
-    if (p.m > kFewRows || (p.kind != PRODUCT_LINEAR && p.kind != PRODUCT_GATED)) return false;
+    if (p.kind == PRODUCT_GATED ? p.m > kFewRowsGated : p.kind != PRODUCT_LINEAR || p.m > kFewRows) return false;
     if (p.k > 16384 && p.n < 1024) return false;  // long rows on few compute units
     if (p.k > 1 && (p.a.col[0] != 1 || p.b.col[0] != 1)) return false;
     if (p.kind == PRODUCT_GATED && ((p.k > 1 && p.b.col[1] != 1) || p.b.row[1] != p.b.row[0])) return false;
