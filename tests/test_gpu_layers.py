@@ -370,7 +370,7 @@ def test_forward_and_backward_in_a_graph():
     def both():
         h = E.gated_linear(x, w[0], w[1], b, None)
         y = E.linear(x, w[0], b, activation="gelu", residual=h)
-        return [y, *torch.autograd.grad(y, [x, *w, b], dy)]
+        return [y.detach(), *torch.autograd.grad(y, [x, *w, b], dy)]  # (no history outlives the call)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
