@@ -569,9 +569,9 @@ __device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, 
 
 // ---- small tiles -----------------------------------------------------------------------------------
 // What bounds them is the way from the caches to LDS, 11 to 12 TB/s over the machine for rows as tensors have them: 32 KB a k-tile of a
-// 128-tile take 0.68 us while it has its compute unit for itself (its matrix instructions 0.25), so it reaches 0.7 PFLOP/s where a 256-tile,
+// 128-tile take 0.63 us while it has its compute unit for itself (its matrix instructions 0.25), so it reaches 0.75 PFLOP/s where a 256-tile,
 // which needs half as much for the same work, reaches twice that.  Fragments of the next half read ahead of the products: 10 to 20 %
-// slower; two k-tiles to a barrier, a fragment's rows dealt to eight waves: nothing.
+// slower; two k-tiles to a barrier: nothing.
 // S stages: a wave waits for its own loads of k-tile t, crosses the one barrier of the k-tile (behind which every wave has read all of k-tile
 // t - 1), issues the loads of k-tile t + S - 1 into the stage that is free now, and multiplies.
 template <typename T, int BM, int BN, int WGM, int WGN, int S, bool ASTEPS, bool BSTEPS, bool GATED>
@@ -613,18 +613,43 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
             WAIT_VM((S - 2) * P::LOADS);
             panels.landed(kt, smem + s * UNIT_A, smem + B_AT + s * UNIT_B);
             barrier();
-            issue(kt + S - 1, s == 0 ? S - 1 : s - 1);
+            const int free = s == 0 ? S - 1 : s - 1;
+            if constexpr (sizeof(T) == 2) {
+                // Every fragment of the k-tile first, then the loads, whose addresses are worked out while the reads are on their way
+                // (4096 x 4096 x 1024 on 128-tiles 45 us, 49 to 53 half by half).
+                frag va[2][FM], vb[2][FN];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                frag va[FM], vb[FN];
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, i, h);
+                    for (int i = 0; i < FM; ++i) va[h][i] = ra.read(smem, i, h);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, j, h);
+                    for (int j = 0; j < FN; ++j) vb[h][j] = rb.read(smem, j, h);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                issue(kt + S - 1, free);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[h][j], va[h][i], acc[i][j]);
+            } else {
+                // Four instructions for each pair of fragments are time enough for the reads of the next (4096 x 4096 x 4096 966 us, all of
+                // them first 986).
+                issue(kt + S - 1, free);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    frag va[FM], vb[FN];
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) va[i] = ra.read(smem, i, h);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) vb[j] = rb.read(smem, j, h);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) acc[i][j] = mfma_step(vb[j], va[i], acc[i][j]);
+                }
             }
             const int s1 = s + 1 == S ? 0 : s + 1;
             ra.move((s1 - s) * UNIT_A);
@@ -1013,7 +1038,7 @@ struct Cost {
     float start, each, alone, busy;
 };
 constexpr Cost kCost[2][3] = {{{4.5f, 0.5f, 0.72f, 0.50f}, {5.f, 1.f, 2.2f, 1.88f}, {0.f, 0.f, 0.f, 0.f}},   // fp32: tiles of 64 and 128 (no 256)
-                              {{2.5f, 0.5f, 0.30f, 0.22f}, {3.f, 1.f, 0.66f, 0.52f}, {3.f, 3.f, 1.15f, 1.35f}}};  // bf16: 64, 128, 256
+                              {{2.5f, 0.5f, 0.30f, 0.22f}, {3.f, 1.f, 0.62f, 0.50f}, {3.f, 3.f, 1.15f, 1.35f}}};  // bf16: 64, 128, 256
 constexpr float kJoinStart = 4.f, kJoinBytes = 5.5e6f;  // of a split reduction: its launch, and bytes in a microsecond
 constexpr int kTile[3] = {64, 128, 256};
 
@@ -1143,7 +1168,7 @@ hipError_t launch_tile(int tile, const KernelArgs& g, int cus, hipStream_t s) {
         if (tile == 256) return launch_pp<T, 256, 256, 2, 4, AS, BS, GATED>(g, s);
     }
     if (tile == 128) {
-        // Where every compute unit has at most one of them, eight waves and four stages (4096 x 4096 x 1024: 48 us against 55); otherwise two
+        // Where every compute unit has at most one of them, eight waves and four stages (4096 x 4096 x 1024: 45 us against 52); otherwise two
         // workgroups of four waves share one.
         if (sizeof(T) == 2 && (long)g.tiles_m * g.tiles_n * g.outs * g.splits <= cus) return launch_tiles<T, 128, 128, 4, 2, 4, AS, BS, GATED>(g, s);
         return launch_tiles<T, 128, 128, 2, 2, 2, AS, BS, GATED>(g, s);
