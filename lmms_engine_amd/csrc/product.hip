@@ -66,8 +66,8 @@ struct KernelArgs {
 // act(z) and act'(z).  The factor of a gated pair's gradient and the activation itself come out of one evaluation.
 //
 // Results of bf16 tensors are rounded to 8 bits, so theirs take the hardware's exponential and reciprocal (one step of fp32 each), and the
-// complementary error function by the rational approximation 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most: 8192 x
-// 4096 x 4096 with silu take 196 us (178 without), with the full functions 217.  fp32 tensors get those.
+// complementary error function by the rational approximation 7.1.26 of Abramowitz and Stegun, off by 1.5e-7 at most: 8192 x 4096 x 4096 with
+// silu takes 202 us where it takes 191 without, with gelu 211.  fp32 tensors get the full functions.
 struct ActPair {
     float a, d;
 };
@@ -80,36 +80,53 @@ __device__ __forceinline__ float sigmoid_of(float z) {
     const float e = 1.0f + exp_of<FAST>(-z);
     return FAST ? __builtin_amdgcn_rcpf(e) : 1.0f / e;
 }
+template <bool FAST, int ACT>
+__device__ __forceinline__ ActPair activate(float z) {
+    if constexpr (ACT == ACT_RELU) {
+        return ActPair{z <= 0.f ? 0.f : z, z <= 0.f ? 0.f : 1.f};  // (NaN stays NaN)
+    } else if constexpr (ACT == ACT_SIGMOID) {
+        const float s = sigmoid_of<FAST>(z);
+        return ActPair{s, s * (1.f - s)};
+    } else if constexpr (ACT == ACT_SILU) {
+        const float s = sigmoid_of<FAST>(z);
+        return ActPair{z * s, s * (1.f + z * (1.f - s))};
+    } else if constexpr (ACT == ACT_GELU) {  // z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2: no cancellation at the lower end
+        const float gauss = exp_of<FAST>(-0.5f * z * z);
+        float phi;
+        if constexpr (FAST) {
+            const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
+            const float lower = 0.5f * gauss * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+            phi = z < 0.f ? lower : 1.f - lower;
+        } else {
+            phi = 0.5f * erfcf(-0.70710678118654752f * z);
+        }
+        return ActPair{z * phi, phi + z * 0.3989422804014327f * gauss};
+    } else if constexpr (ACT == ACT_GELU_TANH) {  // (1 + tanh y) / 2 = sigmoid(2 y), y = c (z + 0.044715 z^3)
+        const float c2 = 2.f * 0.7978845608028654f, q = 0.044715f * z * z;
+        const float s = sigmoid_of<FAST>(c2 * z * (1.f + q)), w = s * (1.f - s);
+        return ActPair{z * s, s + (w == 0.f ? 0.f : z * w * (c2 * (1.f + 3.f * q)))};
+    } else {
+        return ActPair{z, 1.f};
+    }
+}
+// Eight of them behind one decision (one for each value took the epilogue of a 256-tile 8 us, for a relu).
 template <bool FAST>
-__device__ __forceinline__ ActPair activate(int act, float z) {
+__device__ __forceinline__ void activate8(int act, const float (&z)[8], float (&a)[8], float (&d)[8]) {
+    auto all = [&](auto act_c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const ActPair p = activate<FAST, decltype(act_c)::value>(z[e]);
+            a[e] = p.a;
+            d[e] = p.d;
+        }
+    };
     switch (act) {
-        case ACT_RELU: return ActPair{z <= 0.f ? 0.f : z, z <= 0.f ? 0.f : 1.f};  // (NaN stays NaN)
-        case ACT_SIGMOID: {
-            const float s = sigmoid_of<FAST>(z);
-            return ActPair{s, s * (1.f - s)};
-        }
-        case ACT_SILU: {
-            const float s = sigmoid_of<FAST>(z);
-            return ActPair{z * s, s * (1.f + z * (1.f - s))};
-        }
-        case ACT_GELU: {  // z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2: no cancellation at the lower end
-            const float gauss = exp_of<FAST>(-0.5f * z * z);
-            float phi;
-            if constexpr (FAST) {
-                const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
-                const float lower = 0.5f * gauss * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-                phi = z < 0.f ? lower : 1.f - lower;
-            } else {
-                phi = 0.5f * erfcf(-0.70710678118654752f * z);
-            }
-            return ActPair{z * phi, phi + z * 0.3989422804014327f * gauss};
-        }
-        case ACT_GELU_TANH: {  // (1 + tanh y) / 2 = sigmoid(2 y), y = c (z + 0.044715 z^3)
-            const float c2 = 2.f * 0.7978845608028654f, q = 0.044715f * z * z;
-            const float s = sigmoid_of<FAST>(c2 * z * (1.f + q)), w = s * (1.f - s);
-            return ActPair{z * s, s + (w == 0.f ? 0.f : z * w * (c2 * (1.f + 3.f * q)))};
-        }
-        default: return ActPair{z, 1.f};
+        case ACT_RELU: return all(std::integral_constant<int, ACT_RELU>{});
+        case ACT_SIGMOID: return all(std::integral_constant<int, ACT_SIGMOID>{});
+        case ACT_SILU: return all(std::integral_constant<int, ACT_SILU>{});
+        case ACT_GELU: return all(std::integral_constant<int, ACT_GELU>{});
+        case ACT_GELU_TANH: return all(std::integral_constant<int, ACT_GELU_TANH>{});
+        default: return all(std::integral_constant<int, ACT_NONE>{});
     }
 }
 
@@ -222,12 +239,11 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
     if constexpr (GATED) {
         if (g.bias[1]) add(u, g.bias[1], j);
         float h[8], s[8], t[8];
+        activate8<sizeof(T) == 2>(g.act, v, s, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const ActPair p = activate<sizeof(T) == 2>(g.act, v[e]);
-            h[e] = p.a * u[e];
-            s[e] = p.a;
-            t[e] = p.d * u[e];
+            h[e] = s[e] * u[e];
+            t[e] *= u[e];
         }
         store8((T*)g.out[0] + at, count, h);
         if (g.aux[0]) {
@@ -236,13 +252,10 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
         }
     } else {
         if (g.act != ACT_NONE) {
-            float d[8];
+            float z8[8], d[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const ActPair p = activate<sizeof(T) == 2>(g.act, v[e]);
-                v[e] = p.a;
-                d[e] = p.d;
-            }
+            for (int e = 0; e < 8; ++e) z8[e] = v[e];
+            activate8<sizeof(T) == 2>(g.act, z8, v, d);
             if (g.aux[0]) keep8<T>(g.aux[0], all, at, count, d);
         }
         if (g.residual) {
