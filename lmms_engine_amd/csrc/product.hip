@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 // the end of M(t, 1) each wave waits for its own loads of k-tile t + 1, the last of which are one k-tile old: the two groups issued after
 // them stay in flight.  k-tile t + 1 is first read in phase 4t + 4.
 //
-// Measured, 8192 x 12288 x 4096 (rows against rows): two stages each and one k-tile of distance 1320 TFLOP/s, this 1480 to 1530, as much as the
+// Measured, 8192 x 12288 x 4096 (rows against rows): two stages each and one k-tile of distance 1320 TFLOP/s, this 1480 to 1570, as much as the
 // library's product of the same matrices (1540 to 1600); gradients, whose operands come through transposing reads, 1350 to 1430 (the
 // library 1130 to 1330).  64 KB a k-tile are 12 TB/s over the machine, what the way to LDS takes.  Loads or fragments of the right operand
 // moved into the multiplying phases cost 10 %, a higher priority for those phases does nothing.
