@@ -9,7 +9,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/muon_hip.h"
@@ -168,34 +168,54 @@ Incoming act_grad(const Tensor& dy_, int factors, const Tensor& d0, const Tensor
     return g;
 }
 
-// What a backward pass gives has no history of its own: to differentiate it once more raises.
-void close_history(variable_list& grads, int count, const variable_list& inputs) {
-    if (!at::GradMode::is_enabled()) return;
-    bool any = false;
-    for (const Tensor& t : inputs) any = any || (t.defined() && t.requires_grad());
-    if (!any) return;
-    for (int i = 0; i < count; ++i) {
-        Tensor& g = grads[i];
-        if (!g.defined()) continue;
-        torch::autograd::DelayedError fn("linear and gated_linear can be differentiated once: their backward pass has none of its own", 1);
-        Tensor v = g.detach();
-        v.set_requires_grad(true);
-        g = fn.apply(variable_list{v})[0];
+// Stands for the second derivatives that there are none of: whoever comes through here on the way to an input is told so.
+struct Once : torch::autograd::Node {
+    variable_list apply(variable_list&&) override {
+        TORCH_CHECK(false, "linear and gated_linear can be differentiated once: their backward pass has none of its own");
     }
+};
+// Gradient `g` depends on the inputs whose bits are set in `on` (positions of `edges`; those that need no gradient have no edge) and on
+// the incoming gradient.  Where one of them is differentiated, so would g be: its history leads to all of them, so that a loss that g is a
+// part of raises for each of them and loses no term, and to no other.
+void close_history(Tensor& g, unsigned on, const torch::autograd::edge_list& edges, const Tensor& dy) {
+    if (!g.defined()) return;
+    torch::autograd::edge_list next;
+    for (size_t i = 0; i < edges.size(); ++i)
+        if ((on >> i & 1) && edges[i].is_valid()) next.push_back(edges[i]);
+    if (dy.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(dy));
+    if (next.empty()) return;
+    const auto node = std::shared_ptr<Once>(new Once(), torch::autograd::deleteNode);
+    node->set_next_edges(std::move(next));
+    torch::autograd::impl::set_gradient_edge(g, {node, node->add_input_metadata(g)});
 }
+// The second derivative of an activation without a curve is zero.
+bool curved(int act) { return act != MUON_HIP_ACT_NONE && act != MUON_HIP_ACT_RELU; }
 
 // Tensors that a call may lack travel as optionals, and a context numbers the tensors that there are: `has` holds a bit for each of the two.
 typedef std::optional<Tensor> Maybe;
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
-void note(AutogradContext* ctx, const Maybe& a, const Maybe& b) { ctx->saved_data["has"] = (int64_t)(a.has_value() + 2 * b.has_value()); }
+void note(AutogradContext* ctx, const Maybe& a, const Maybe& b, int64_t act) {
+    ctx->saved_data["has"] = (int64_t)(a.has_value() + 2 * b.has_value());
+    ctx->saved_data["act"] = act;
+}
 // Whether the optional tensors behind `first` others need a gradient.
 struct Wanted {
     bool a, b;
+    int64_t has;
     Wanted(AutogradContext* ctx, int first) {
-        const int64_t has = ctx->saved_data["has"].toInt();
+        has = ctx->saved_data["has"].toInt();
         a = (has & 1) && ctx->needs_input_grad(first);
         b = (has & 2) && ctx->needs_input_grad(first + (has & 1));
+    }
+    // Where the inputs' own gradients go, one place for each that a call may have.
+    torch::autograd::edge_list edges(int first) const {
+        const auto node = torch::autograd::get_current_node();
+        torch::autograd::edge_list all(first + 2);
+        for (int i = 0; i < first; ++i) all[i] = node->next_edge(i);
+        if (has & 1) all[first] = node->next_edge(first);
+        if (has & 2) all[first + 1] = node->next_edge(first + (has & 1));
+        return all;
     }
 };
 
@@ -204,7 +224,7 @@ struct Linear : torch::autograd::Function<Linear> {
         const bool keep = x.requires_grad() || w.requires_grad() || (b && b->requires_grad());
         Forward f = linear_forward(x, w, given(b), given(r), (int)act, keep);
         ctx->save_for_backward({x, w, f.aux[0]});
-        note(ctx, b, r);
+        note(ctx, b, r, act);
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
@@ -240,7 +260,14 @@ struct Linear : torch::autograd::Function<Linear> {
             }
             if (more.b) grads[3] = dy;
         }
-        close_history(grads, 3, {x, w, d, dy});  // (the residual's is the incoming one, history and all)
+        if (at::GradMode::is_enabled()) {  // (the residual's is the incoming one, history and all)
+            enum { X = 1, W = 2, B = 4 };
+            const auto edges = more.edges(2);
+            const unsigned dz = curved((int)ctx->saved_data["act"].toInt()) ? X | W | B : 0;
+            close_history(grads[0], dz | W, edges, dy);
+            close_history(grads[1], dz | X, edges, dy);
+            close_history(grads[2], dz, edges, dy);
+        }
         return grads;
     }
 };
@@ -248,7 +275,7 @@ struct Linear : torch::autograd::Function<Linear> {
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg, const Maybe& bu, int64_t act) {
         Forward f = gated_forward(x, wg, wu, given(bg), given(bu), (int)act, true);
-        note(ctx, bg, bu);
+        note(ctx, bg, bu, act);
         ctx->save_for_backward({x, wg, wu, f.aux[0], f.aux[1]});
         return f.out;
     }
@@ -287,7 +314,17 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
                 p.run(x);
             }
         }
-        close_history(grads, 5, {x, wg, wu, s, t, dh});
+        if (at::GradMode::is_enabled()) {
+            enum { X = 1, WG = 2, WU = 4, BG = 8, BU = 16 };
+            const auto edges = more.edges(3);
+            const unsigned of_g = X | WG | BG, of_u = X | WU | BU;
+            const unsigned dg = of_u | (curved((int)ctx->saved_data["act"].toInt()) ? of_g : 0), du = of_g;
+            close_history(grads[0], dg | du | WG | WU, edges, dh);
+            close_history(grads[1], dg | X, edges, dh);
+            close_history(grads[2], du | X, edges, dh);
+            close_history(grads[3], dg, edges, dh);
+            close_history(grads[4], du, edges, dh);
+        }
         return grads;
     }
 };
