@@ -3,14 +3,17 @@
 // more than the kernels of a layer of 500 tokens.
 //
 // Each function takes calls in which nothing needs a decision: plain tensors of one type on one GPU, of shapes that fit.  For anything else
-// it returns None before it has done anything, and the caller says what is wrong.
+// it returns None before it has done anything, and the caller says what is wrong.  What a thread does is looked at here: refuse_recording.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/DeviceGuard.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/muon_hip.h"
 
@@ -31,6 +34,16 @@ PyObject* error_type = nullptr;  // MuonHipError
         e.persist();
     }
     throw e;
+}
+
+// Tools that record the torch operations of a function, to run them again on other tensors, or that run it on tensors without values, see the
+// allocation of a result and none of the launches that fill it: what they made would return memory that nothing has written.
+void refuse_recording() {
+    using c10::impl::TorchDispatchModeKey;
+    bool on = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        on = on || c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
+    TORCH_CHECK_NOT_IMPLEMENTED(!on, "linear and gated_linear cannot be recorded or run on tensors without values: their launches are no torch operations");
 }
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? MUON_HIP_F32 : MUON_HIP_BF16; }
@@ -228,6 +241,7 @@ struct Linear : torch::autograd::Function<Linear> {
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        refuse_recording();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &d = saved[2], &dy = incoming[0];
         const Wanted more(ctx, 2);
@@ -280,6 +294,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        refuse_recording();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &s = saved[3], &t = saved[4], &dh = incoming[0];
         const bool want_x = ctx->needs_input_grad(0), want_wg = ctx->needs_input_grad(1), want_wu = ctx->needs_input_grad(2);
@@ -367,6 +382,7 @@ bool differentiated(const Tensor* t, int count) {
 // linear(x, weight, bias or None, residual or None, activation code)
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
+    refuse_recording();
     Tensor t[4];
     if (count != 5 || !unpack(args, 4, 2, t) || !fits(t[0], t[1], t[2])) Py_RETURN_NONE;
     if (t[3].defined()) {
@@ -388,6 +404,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
 // gated_linear(x, weight_gate, weight_up, bias_gate or None, bias_up or None, activation code)
 PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
+    refuse_recording();
     Tensor t[5];
     if (count != 6 || !unpack(args, 5, 3, t) || !fits(t[0], t[1], t[3]) || !fits(t[0], t[2], t[4]) || t[1].size(0) != t[2].size(0)) Py_RETURN_NONE;
     const long act = PyLong_AsLong(args[5]);

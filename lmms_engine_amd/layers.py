@@ -12,8 +12,9 @@ this package, no CPU path.
 
 Both functions can be differentiated once by every tensor argument.  For the backward pass they keep the inputs, and for every result the
 factors that the incoming gradient is multiplied by: one with an activation, two of a gated pair, none otherwise, in 24 bits for bfloat16
-tensors (three bytes a value) and in 32 for float32.  Forward-mode differentiation, second derivatives and tensor subclasses are refused;
-autocast leaves the calls alone.
+tensors (three bytes a value) and in 32 for float32.  Forward-mode differentiation, second derivatives, tensor subclasses and recording
+(torch.jit.trace, make_fx, fake tensors) are refused; autocast leaves the calls alone, and modes that only watch torch operations
+(counters, selective recomputation) see none of the products.
 """
 from __future__ import annotations
 
