@@ -173,9 +173,10 @@ __device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
         if (e < count) p[e] = (T)v[e];
 }
 
-// Factors that are kept for the backward pass of bf16 tensors: the upper 24 bits of each, in a plane of the upper 16 and one of the other 8.
-// Cut off, they are off by 2^-16; rounded to bf16 like any activation they are off by 2^-8, as much as the rounding of dy * d behind them, and
-// gradients then were 1.7 times as far from the formula's as results that are rounded once (2.9e-3 against 1.7e-3 in the 2-norm; so it is 2.4e-3).
+// Factors that are kept for the backward pass of bf16 tensors: each rounded to its upper 24 bits, in a plane of the upper 16 and one of the
+// other 8.  So they are off by 2^-16 at most, to either side (cut off: 2^-15, all towards zero, which sums over rows do not even out).  Rounded
+// to bf16 like any activation they are off by 2^-8, as much as the rounding of dy * d behind them, and gradients then were 1.7 times as far
+// from the formula's as results that are rounded once (2.9e-3 against 1.7e-3 in the 2-norm; so it is 2.4e-3).
 // The third byte costs 2 % of a gated training step over 8192 x 4096 x 12288 and half as much memory again; fp32 tensors keep all 32 bits.
 template <typename T>
 __device__ __forceinline__ void keep8(void* base, long all, long at, int count, const float (&v)[8]) {
@@ -186,7 +187,7 @@ __device__ __forceinline__ void keep8(void* base, long all, long at, int count, 
         uint8_t* low = (uint8_t*)base + 2 * all + at;
         uint32_t b[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = __builtin_bit_cast(uint32_t, v[e]);
+        for (int e = 0; e < 8; ++e) b[e] = __builtin_bit_cast(uint32_t, v[e]) + 0x80;  // (a NaN stays one: its lower half is zero, as the bf16 value's that it comes from)
         if (count >= 8) {
             u32x4 h;
             u32x2 l;

@@ -34,3 +34,17 @@ def test_the_lower_tail_of_gelu_is_right_to_its_own_size(dtype):
     h = E.gated_linear(z.detach(), one, one, activation="gelu")
     off = ((h.double() - a * z.detach().double()).abs() / (a * z.detach().double()).abs()).max().item()
     assert off <= u + 2.0 ** -14, off
+
+
+def test_factors_are_rounded_to_the_bits_that_are_kept():
+    """24 bits of a factor, 16 of them its significand's: off by half a step of theirs, 2^-16 of the value, to either side.  Two rows' factors differ
+    by less than a bf16 value shows, and their difference is what is left of the bias's gradient."""
+    tiny = 2.0 ** -15
+    for part in (255 / 256, 129 / 256, 127 / 256, 3 / 256):
+        x = torch.tensor([[1.0, part * tiny], [1.0, 0.0]], dtype=BF, device=DEV)
+        w = torch.ones(8, 2, dtype=BF, device=DEV)
+        bg = torch.zeros(8, dtype=BF, device=DEV, requires_grad=True)
+        h = E.gated_linear(x, w, w, bg, None, activation="none")  # the factor of bg's gradient is x w^T: 1 + part * 2^-15 and 1, exact sums
+        (db,) = torch.autograd.grad(h, bg, torch.tensor([[1.0], [-1.0]], dtype=BF, device=DEV).expand(2, 8))
+        off = (db.double() - part * tiny).abs().max().item()
+        assert off <= 2.0 ** -16 * (1 + tiny) + 2.0 ** -9 * tiny, (part, off)
