@@ -255,7 +255,7 @@ __device__ __forceinline__ void finish8(const KernelArgs& g, int z, long i, int 
             keep8<T>(g.aux[1], all, at, count, t);
         }
     } else {
-        if (g.act != ACT_NONE) {
+        if (g.act != ACT_NONE || g.aux[0]) {
             float z8[8], d[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) z8[e] = v[e];

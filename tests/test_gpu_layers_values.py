@@ -1,6 +1,5 @@
 """Values of activations and of what is kept for the backward pass, relative to themselves."""
 import ctypes
-import itertools
 
 import pytest
 import torch
@@ -48,3 +47,25 @@ def test_factors_are_rounded_to_the_bits_that_are_kept():
         (db,) = torch.autograd.grad(h, bg, torch.tensor([[1.0], [-1.0]], dtype=BF, device=DEV).expand(2, 8))
         off = (db.double() - part * tiny).abs().max().item()
         assert off <= 2.0 ** -16 * (1 + tiny) + 2.0 ** -9 * tiny, (part, off)
+
+
+@pytest.mark.parametrize("dtype", [BF, F], ids=["bf16", "f32"])
+@pytest.mark.parametrize("size", [(3, 40, 24), (70, 64, 75), (300, 2000, 40)], ids=str)
+def test_a_product_without_an_activation_keeps_its_factor_too(size, dtype):
+    """act'(.) is 1 where there is none: whoever asks for it gets it."""
+    t, k, n = size
+    g = torch.Generator(device=DEV).manual_seed(2)
+    lib, code = _abi.lib(), _abi.dtype_code(dtype)
+    x, w, dy = (torch.randn(*s, generator=g, device=DEV).to(dtype) for s in ((t, k), (n, k), (t, n)))
+    out, dz = torch.empty(t, n, dtype=dtype, device=DEV), torch.empty(t, n, dtype=dtype, device=DEV)
+    aux = torch.zeros(lib.muon_hip_product_aux_bytes(code, t, n), dtype=torch.uint8, device=DEV)
+    p = _abi.Product(kind=_abi.PRODUCT_LINEAR, dtype=code, m=t, n=n, k=k)
+    p.a[0], p.a_row[0], p.a_col[0] = x.data_ptr(), k, 1
+    p.b[0], p.b_row[0], p.b_col[0] = w.data_ptr(), k, 1
+    p.out[0], p.aux[0] = out.data_ptr(), aux.data_ptr()
+    need = lib.muon_hip_product_workspace(ctypes.addressof(p))
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+    stream = _abi.stream_ptr(x.device)
+    _abi.check(lib.muon_hip_product_run(ctypes.addressof(p), ws.data_ptr(), need, stream))
+    _abi.check(lib.muon_hip_act_grad(dy.data_ptr(), 1, aux.data_ptr(), None, dz.data_ptr(), None, n, None, None, code, t, n, None, stream))
+    assert torch.equal(dz, dy) and torch.equal(out, E.linear(x, w))
