@@ -232,11 +232,13 @@ struct Wanted {
     }
 };
 
+// What is kept for a backward pass is what the gradients that can be asked for read, so that a frozen weight does not hold its input, and an
+// input that no gradient reads may change.  k is the kept operand's, everything else of the shapes the incoming gradient's.
 struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& b, const Maybe& r, int64_t act) {
-        const bool keep = x.requires_grad() || w.requires_grad() || (b && b->requires_grad());
-        Forward f = linear_forward(x, w, given(b), given(r), (int)act, keep);
-        ctx->save_for_backward({x, w, f.aux[0]});
+        const bool for_x = x.requires_grad(), for_w = w.requires_grad(), for_b = b && b->requires_grad();
+        Forward f = linear_forward(x, w, given(b), given(r), (int)act, for_x || for_w || for_b);
+        ctx->save_for_backward({for_w ? x : Tensor(), for_x ? w : Tensor(), f.aux[0]});
         note(ctx, b, r, act);
         return f.out;
     }
@@ -249,27 +251,28 @@ struct Linear : torch::autograd::Function<Linear> {
         variable_list grads(5);
         {
             const at::AutoGradMode off(false);
-            const c10::DeviceGuard guard(x.device());
+            const c10::DeviceGuard guard(dy.device());
             if (want_x || want_w || want_b) {
-                const Tensor x2 = matrix(x), w2 = bare(w);
-                const int64_t m = x2.size(0), k = x2.size(1), n = w2.size(0);
+                const int64_t m = rows_of(dy), n = dy.size(-1);
                 Incoming g = act_grad(dy, d.defined() ? 1 : 0, d, Tensor(), want_x || want_w, want_b, false, m, n);
                 grads[2] = g.db[0];
                 if (want_x) {
-                    grads[0] = at::empty(x.sizes(), x.options());
-                    Product p(MUON_HIP_PRODUCT_LINEAR, x, m, k, n);
+                    const Tensor w2 = bare(w);
+                    grads[0] = result(dy, w2.size(1));
+                    Product p(MUON_HIP_PRODUCT_LINEAR, dy, m, w2.size(1), n);
                     p.left(g.dz[0], g.dz[0]);
                     p.right(w2, w2, true);
                     p.out[0] = grads[0].data_ptr();
-                    p.run(x);
+                    p.run(dy);
                 }
                 if (want_w) {
-                    grads[1] = at::empty({n, k}, x.options());
-                    Product p(MUON_HIP_PRODUCT_LINEAR, x, n, k, m);
+                    const Tensor x2 = matrix(x);
+                    grads[1] = at::empty({n, x2.size(1)}, dy.options());
+                    Product p(MUON_HIP_PRODUCT_LINEAR, dy, n, x2.size(1), m);
                     p.left(g.dz[0], g.dz[0], true);
                     p.right(x2, x2, true);
                     p.out[0] = grads[1].data_ptr();
-                    p.run(x);
+                    p.run(dy);
                 }
             }
             if (more.b) grads[3] = dy;
@@ -286,11 +289,15 @@ struct Linear : torch::autograd::Function<Linear> {
     }
 };
 
+// The gate's gradients (wg, bg) read the factor t = u act'(g), those of the other projection (wu, bu) s = act(g), x's both.
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg, const Maybe& bu, int64_t act) {
+        const bool for_x = x.requires_grad(), for_wg = wg.requires_grad(), for_wu = wu.requires_grad();
+        const bool for_g = for_x || for_wg || (bg && bg->requires_grad()), for_u = for_x || for_wu || (bu && bu->requires_grad());
         Forward f = gated_forward(x, wg, wu, given(bg), given(bu), (int)act, true);
+        const Tensor none;
+        ctx->save_for_backward({for_wg || for_wu ? x : none, for_x ? wg : none, for_x ? wu : none, for_u ? f.aux[0] : none, for_g ? f.aux[1] : none});
         note(ctx, bg, bu, act);
-        ctx->save_for_backward({x, wg, wu, f.aux[0], f.aux[1]});
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
@@ -299,34 +306,38 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &s = saved[3], &t = saved[4], &dh = incoming[0];
         const bool want_x = ctx->needs_input_grad(0), want_wg = ctx->needs_input_grad(1), want_wu = ctx->needs_input_grad(2);
         const Wanted more(ctx, 3);
+        const bool want_g = want_x || want_wg || more.a, want_u = want_x || want_wu || more.b, two = want_g && want_u;
         variable_list grads(6);
-        {
+        if (want_g || want_u) {
             const at::AutoGradMode off(false);
-            const c10::DeviceGuard guard(x.device());
-            const Tensor x2 = matrix(x), g2 = bare(wg), u2 = bare(wu);
-            const int64_t m = x2.size(0), k = x2.size(1), n = g2.size(0);
-            Incoming g = act_grad(dh, 2, t, s, want_x || want_wg || want_wu, more.a, more.b, m, n);
-            grads[3] = g.db[0];
-            grads[4] = g.db[1];
+            const c10::DeviceGuard guard(dh.device());
+            const int64_t m = rows_of(dh), n = dh.size(-1);
+            Incoming g = act_grad(dh, two ? 2 : 1, want_g ? t : s, two ? s : Tensor(), want_x || want_wg || want_wu, want_g ? more.a : more.b,
+                                  two && more.b, m, n);
+            const int u = two ? 1 : 0;  // which of them is the other projection's, where it is wanted
+            if (more.a) grads[3] = g.db[0];
+            if (more.b) grads[4] = g.db[u];
             if (want_x) {
-                grads[0] = at::empty(x.sizes(), x.options());
-                Product p(MUON_HIP_PRODUCT_SUM, x, m, k, n);
+                const Tensor g2 = bare(wg), u2 = bare(wu);
+                grads[0] = result(dh, g2.size(1));
+                Product p(MUON_HIP_PRODUCT_SUM, dh, m, g2.size(1), n);
                 p.left(g.dz[0], g.dz[1]);
                 p.right(g2, u2, true);
                 p.out[0] = grads[0].data_ptr();
-                p.run(x);
+                p.run(dh);
             }
             if (want_wg || want_wu) {
+                const Tensor x2 = matrix(x);
                 const bool both = want_wg && want_wu;
-                Product p(both ? MUON_HIP_PRODUCT_EACH : MUON_HIP_PRODUCT_LINEAR, x, n, k, m);
-                if (want_wg) grads[1] = at::empty({n, k}, x.options());
-                if (want_wu) grads[2] = at::empty({n, k}, x.options());
-                const int first = want_wg ? 0 : 1;
-                p.left(g.dz[first], g.dz[1], true);
+                Product p(both ? MUON_HIP_PRODUCT_EACH : MUON_HIP_PRODUCT_LINEAR, dh, n, x2.size(1), m);
+                if (want_wg) grads[1] = at::empty({n, x2.size(1)}, dh.options());
+                if (want_wu) grads[2] = at::empty({n, x2.size(1)}, dh.options());
+                const int first = want_wg ? 0 : u;
+                p.left(g.dz[first], g.dz[both ? 1 : first], true);
                 p.right(x2, x2, true);
-                p.out[0] = grads[1 + first].data_ptr();
+                p.out[0] = grads[want_wg ? 1 : 2].data_ptr();
                 p.out[1] = both ? grads[2].data_ptr() : nullptr;
-                p.run(x);
+                p.run(dh);
             }
         }
         if (at::GradMode::is_enabled()) {

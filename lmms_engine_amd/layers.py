@@ -10,9 +10,10 @@ products of float32 tensors keep single precision.  Operands are read as they li
 16-byte pieces go through packed copies.  There is no counterpart in the reference, which leaves its layers to torch, and, as everywhere in
 this package, no CPU path.
 
-Both functions can be differentiated once by every tensor argument.  For the backward pass they keep the inputs, and for every result the
-factors that the incoming gradient is multiplied by: one with an activation, two of a gated pair, none otherwise, in 24 bits for bfloat16
-tensors (three bytes a value) and in 32 for float32.  Forward-mode differentiation, second derivatives, tensor subclasses and recording
+Both functions can be differentiated once by every tensor argument.  For the backward pass they keep x where a weight is trained, the weights
+where x has a gradient, and for every result the factors that the incoming gradient is multiplied by, of those that a trained input's
+gradient reads: one with an activation, one for each projection of a gated pair, none otherwise, in 24 bits for bfloat16 tensors (three
+bytes a value) and in 32 for float32.  Forward-mode differentiation, second derivatives, tensor subclasses and recording
 (torch.jit.trace, make_fx, fake tensors) are refused; autocast leaves the calls alone, and modes that only watch torch operations
 (counters, selective recomputation) see none of the products.
 """

@@ -95,3 +95,81 @@ def test_a_loss_whose_gradient_has_a_history_closes_every_gradient(kind):
             continue
         with pytest.raises(RuntimeError, match="differentiated once"):
             torch.autograd.grad(first.square().sum() + v[asked].square().sum(), v[asked])
+
+
+def grads_of(kind, base, trained, act, between):
+    """Gradients by `trained` of a call between whose passes `between` is done with its inputs."""
+    v = {m: a.clone().requires_grad_(m in trained) for m, a in base.items()}
+    used = {m: a * 1 if m in trained else a for m, a in v.items()}  # (a leaf that is trained cannot be changed in place)
+    y = call(kind, used, act)
+    between(used)
+    return dict(zip(trained, torch.autograd.grad(y, [v[m] for m in trained], torch.ones_like(y))))
+
+
+# what the gradient by an input reads beside what is kept of the activation
+READS = {"linear": dict(x="w", w="x", b="", r=""), "gated": dict(x=("wg", "wu"), wg="x", wu="x", bg="", bu="")}
+
+
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("kind", list(NAMES))
+def test_inputs_that_no_gradient_reads_may_change(kind, act):
+    """An input that is changed in place between the passes: the gradients that do not read it are what they were, those that do raise."""
+    base = inputs(kind)
+    for trained in itertools.chain(itertools.combinations(base, 1), itertools.combinations(base, 2)):
+        want = grads_of(kind, base, trained, act, lambda v: None)
+        for changed in base:
+            def change(v):
+                with torch.no_grad():
+                    v[changed].mul_(3).add_(1)
+
+            if any(changed in READS[kind][m] for m in trained):
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    grads_of(kind, base, trained, act, change)
+                continue
+            got = grads_of(kind, base, trained, act, change)
+            for m in trained:
+                assert torch.equal(got[m], want[m]), (trained, changed, m)
+
+
+@pytest.mark.parametrize("dtype,each", [(torch.bfloat16, 3), (torch.float32, 4)], ids=["bf16", "f32"])
+def test_what_is_kept_is_what_is_read(dtype, each):
+    """Memory between the passes, beside the result: the factors that the gradients need and no input that they do not."""
+    t, k, n = 1024, 2048, 512  # buffers of whole megabytes each
+    mb = 1 << 20
+
+    def kept(f, **shapes):
+        """Bytes that the call holds on to once the caller has let go of what it passed."""
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        v = {m: torch.zeros(*s, dtype=dtype, device=DEV) for m, s in shapes.items()}
+        y = f(v)
+        del v
+        return torch.cuda.memory_allocated() - before - y.numel() * y.element_size()
+
+    factor, size = t * n * each, torch.finfo(dtype).bits // 8
+    x, w, b = t * k * size, n * k * size, n * size
+    slack = 64 * 1024
+    shapes = dict(x=(t, k), w=(n, k), w2=(n, k), b=(n,), b2=(n,), r=(t, n))
+
+    def trained(*names, **call):
+        def f(v):
+            for m in names:
+                v[m].requires_grad_(True)
+            if "w2" in v:
+                return E.gated_linear(v["x"], v["w"], v["w2"], v["b"], v["b2"], **call)
+            return E.linear(v["x"], v["w"], v["b"], residual=v["r"], **call)
+        return f
+
+    def pick(*names):
+        return {m: shapes[m] for m in names}
+
+    lin, gated = pick("x", "w", "b", "r"), pick("x", "w", "w2", "b", "b2")
+    # (a trained leaf lives on in its own gradient's node)
+    for names, act, want in ((("x",), "none", x + w), (("w",), "none", x + w), (("b",), "none", b), (("r",), "silu", t * n * size),
+                             (("b",), "silu", b + factor), (("x",), "silu", x + w + factor)):
+        got = kept(trained(*names, activation=act), **lin)
+        assert abs(got - want) <= slack, (names, act, got / mb, want / mb)
+    for names, want in ((("b",), b + factor), (("b2",), b + factor), (("w",), w + x + factor), (("w2",), w + x + factor), (("x",), x + 2 * w + 2 * factor),
+                        (("b", "b2"), 2 * b + 2 * factor)):
+        got = kept(trained(*names), **gated)
+        assert abs(got - want) <= slack, (names, got / mb, want / mb)
