@@ -371,6 +371,23 @@ long muon_hip_product_workspace(const muon_hip_product* p);
 int muon_hip_product_run(const muon_hip_product* p, void* workspace, size_t workspace_bytes, void* stream);
 long muon_hip_product_aux_bytes(int dtype, int m, int n);
 
+/* How such a call is computed on a device of `cus` compute units.  Touches no device and reads nothing behind the pointers, of which the
+ * alignment counts.  For tests and measurements. */
+#define MUON_HIP_OPERAND_ROWS 0        /* as it lies, the reduction index contiguous */
+#define MUON_HIP_OPERAND_STEPS 1       /* as it lies, the other index contiguous */
+#define MUON_HIP_OPERAND_ROWS_COPIED 2 /* the same of a copy in the workspace */
+#define MUON_HIP_OPERAND_STEPS_COPIED 3
+#define MUON_HIP_OPERAND_GATHERED 4    /* rows put together from elements that lie apart */
+typedef struct {
+    int tile;    /* rows of a workgroup's tile, and columns (half as many of each factor of a gated pair); 0: the kernel of few rows */
+    int parts;   /* of the reduction, joined by another launch where there are more than one */
+    int a, b;    /* MUON_HIP_OPERAND_ (tile 0: ROWS, from any address) */
+    long groups; /* workgroups of the product's launch */
+    int threads; /* of each of them */
+    long copies; /* threads of the largest launch that copies operands, 0 where none is copied */
+} muon_hip_product_route;
+int muon_hip_route_product(const muon_hip_product* p, int cus, muon_hip_product_route* out);
+
 /* What stands between the incoming gradient and the products of a backward pass, over a row-major m x n gradient and factors that a product
  * has left as aux:
  *   dz0 = dy * d0 and, with two factors, dz1 = dy * d1, rows `pitch` >= n elements apart (what lies between stays as it was);

@@ -62,6 +62,16 @@ class Product(ctypes.Structure):
                 ("out", c_void_p * 2), ("aux", c_void_p * 2)]
 
 
+OPERAND_ROWS, OPERAND_STEPS, OPERAND_ROWS_COPIED, OPERAND_STEPS_COPIED, OPERAND_GATHERED = range(5)
+
+
+class ProductRoute(ctypes.Structure):
+    """muon_hip_product_route"""
+
+    _fields_ = [("tile", c_int), ("parts", c_int), ("a", c_int), ("b", c_int), ("groups", c_long), ("threads", c_int),
+                ("copies", c_long)]
+
+
 # name -> (restype, argtypes); mirrors include/muon_hip.h one to one
 SIGNATURES = {
     "muon_hip_version": (c_int, []),
@@ -111,6 +121,7 @@ SIGNATURES = {
     "muon_hip_product_workspace": (c_long, [c_void_p]),
     "muon_hip_product_run": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "muon_hip_product_aux_bytes": (c_long, [c_int, c_int, c_int]),
+    "muon_hip_route_product": (c_int, [c_void_p, c_int, c_void_p]),
     "muon_hip_act_grad_partials": (c_long, [c_int, c_int]),
     "muon_hip_act_grad": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_long] + [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 2),
     "muon_hip_device_shape": (c_int, [POINTER(c_int), POINTER(c_int)]),
@@ -237,6 +248,13 @@ def flow_tiles(shapes, steps: int, update: bool, xcds: int = 8, recorded: bool =
     out = (FlowTile * count.value)()
     check(lib().muon_hip_flow_tiles(*args, out, count.value, ctypes.byref(count)), "flow_tiles")
     return list(out)
+
+
+def product_route(p: Product, cus: int = 256) -> ProductRoute:
+    """How a product is computed on a device of `cus` compute units."""
+    out = ProductRoute()
+    check(lib().muon_hip_route_product(ctypes.addressof(p), cus, ctypes.addressof(out)), "route_product")
+    return out
 
 
 def device_shape():

@@ -1134,6 +1134,14 @@ int muon_hip_product_run(const muon_hip_product* p, void* workspace, size_t work
     return e == hipSuccess ? 0 : hip_fail(e, "product launch");
 }
 
+int muon_hip_route_product(const muon_hip_product* p, int cus, muon_hip_product_route* out) {
+    ProductArgs g;
+    if (!out || cus < 1) return fail(MUON_HIP_EINVAL, "bad device or output");
+    if (int rc = check_product(p, g)) return rc;
+    if (!plan_product(g, cus, *out)) return fail(MUON_HIP_ESHAPE, "%d x %d x %d: a tile of an operand spans 2 GiB, or the tiles exceed one launch", p->m, p->n, p->k);
+    return 0;
+}
+
 long muon_hip_product_aux_bytes(int dtype, int m, int n) {
     if (!dtype_ok(dtype) || m < 0 || n < 0) return fail(MUON_HIP_EINVAL, "bad dtype or size");
     return (long)m * n * (dtype == MUON_HIP_BF16 ? 3 : 4);
@@ -1153,7 +1161,7 @@ int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d
         if (factors > 1 && !dz0 != !dz1) return fail(MUON_HIP_EINVAL, "one of the two products alone");
         if ((db0 || db1) && !partials) return fail(MUON_HIP_EINVAL, "sums need memory for their parts");
     }
-    if (((long)m + 7) / 8 * (((long)n + 255) / 256) > 0x7fffffffL) return fail(MUON_HIP_ESHAPE, "%d x %d values exceed one launch", m, n);
+    if (!act_grad_fits(m, n)) return fail(MUON_HIP_ESHAPE, "%d x %d values exceed one launch", m, n);
     hipStream_t s = (hipStream_t)stream;
     Timed t(MUON_HIP_K_ACT_GRAD, s);
     const ActGradArgs a{dtype, m, n, factors, dy, {d0, d1}, {dz0, dz1}, pitch, {db0, db1}, partials};

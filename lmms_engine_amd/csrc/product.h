@@ -1,6 +1,7 @@
 // Host-side description of the products of layers (product.hip).
 #pragma once
 #include <hip/hip_runtime.h>
+#include "../../include/muon_hip.h"
 #include "common.h"
 
 // What becomes of the sums; the codes of include/muon_hip.h.
@@ -25,6 +26,8 @@ struct ProductArgs {
 
 // Bytes of workspace that launch_product needs on a device of `cus` compute units; negative: the sizes are out of range.
 long product_workspace(const ProductArgs& p, int cus);
+// How launch_product computes it there; false where it cannot.
+bool plan_product(const ProductArgs& p, int cus, muon_hip_product_route& out);
 hipError_t launch_product(const ProductArgs& p, void* workspace, int cus, int xcd_shift, hipStream_t stream);
 
 // dz0 = dy * d0 (and dz1 = dy * d1) with rows `pitch` elements apart, and the sums over the rows; no factor: dz0 = dy.
@@ -38,4 +41,5 @@ struct ActGradArgs {
     float* partials;  // act_grad_partials(m, n) floats for each factor
 };
 long act_grad_partials(long m, long n);
+bool act_grad_fits(long m, long n);  // whether a launch has workgroups enough
 hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t stream);

@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(512, 4) product_rows_kernel(const KernelArgs g
 // the sums are zero.
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(256) product_join_kernel(const KernelArgs g) {
-    const long pieces = (g.n + 7) / 8, all = pieces * g.m * g.outs;
+    const long pieces = (g.n + 7L) / 8, all = pieces * g.m * g.outs;
     for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < all; at += (long)gridDim.x * 256) {
         const int j = (int)(at % pieces) * 8;
         const long r = at / pieces;
@@ -963,7 +963,7 @@ template <typename T, bool PAIR>
 __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int chunks, int rows) {
     constexpr int F = PAIR ? 2 : 1;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int blocks = (g.n + 255) / 256;
+    const int blocks = (int)((g.n + 255L) / 256);
     const int chunk = blockIdx.x / blocks, j0 = (blockIdx.x - chunk * blocks) * 256, j = j0 + tx * 8;
     const int count = g.n - j < 8 ? g.n - j : 8;
     const long all = (long)g.m * g.n;
@@ -1011,32 +1011,44 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs g, int 
         }
     }
 }
-// Sixteen rows of threads take the parts in turn; their sums are added in a fixed order.
+// Sixteen rows of threads take the parts of sixteen columns in turn; their sums are added in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) row_sum_kernel(const float* partials, int chunks, int n, T* out0, T* out1) {
     __shared__ float part[16][16];
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, f = blockIdx.y, j = blockIdx.x * 16 + x;
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, f = blockIdx.y;
     T* out = f ? out1 : out0;
     if (!out) return;
-    float v = 0.f;
-    if (j < n) {
+    for (long j0 = blockIdx.x * 16L; j0 < n; j0 += gridDim.x * 16L) {
+        const long j = j0 + x;
+        float v = 0.f;
+        if (j < n) {
 #pragma unroll 4
-        for (int c = y; c < chunks; c += 16) v += partials[((long)f * chunks + c) * n + j];
-    }
-    part[y][x] = v;
-    __syncthreads();
-    if (y > 0 || j >= n) return;
+            for (int c = y; c < chunks; c += 16) v += partials[((long)f * chunks + c) * n + j];
+        }
+        part[y][x] = v;
+        __syncthreads();
+        if (y == 0 && j < n) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) v += part[r][x];
-    out[j] = (T)v;
+            for (int r = 1; r < 16; ++r) v += part[r][x];
+            out[j] = (T)v;
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------
 inline long up(long v, long m) { return (v + m - 1) / m * m; }
+constexpr long MOST_THREADS = 0xffffffffL;  // of a launch
 inline int elem_size(int dtype) { return dtype == MUON_HIP_BF16 ? 2 : 4; }
 
 // How an operand is read: rows or reduction steps as they lie, or copies of them, or rows put together from any strides.
-enum { LIE_ROWS, LIE_STEPS, LIE_PACKED_ROWS, LIE_PACKED_STEPS, LIE_GATHERED };
+enum {
+    LIE_ROWS = MUON_HIP_OPERAND_ROWS,
+    LIE_STEPS = MUON_HIP_OPERAND_STEPS,
+    LIE_PACKED_ROWS = MUON_HIP_OPERAND_ROWS_COPIED,
+    LIE_PACKED_STEPS = MUON_HIP_OPERAND_STEPS_COPIED,
+    LIE_GATHERED = MUON_HIP_OPERAND_GATHERED
+};
 inline bool by_steps(int lie) { return lie == LIE_STEPS || lie == LIE_PACKED_STEPS; }
 struct Plan {
     int lie_a, lie_b;
@@ -1044,6 +1056,9 @@ struct Plan {
     long pack_a, pack_b;          // bytes of one packed matrix
     int count_a, count_b;         // matrices of each operand
     int tile, splits, per_split, nk, segments, outs;  // tile 0: the kernel of few rows
+    long groups;                  // workgroups of the launch
+    int threads;                  // of each
+    long copies;                  // threads of the largest launch that packs
     long partial_bytes, bytes;
 };
 
@@ -1058,6 +1073,10 @@ constexpr Cost kCost[2][3] = {{{4.5f, 0.5f, 0.72f, 0.50f}, {5.f, 1.f, 2.2f, 1.88
                               {{2.5f, 0.5f, 0.30f, 0.22f}, {3.f, 1.f, 0.62f, 0.50f}, {3.f, 3.f, 1.15f, 1.35f}}};  // bf16: 64, 128, 256
 constexpr float kJoinStart = 4.f, kJoinBytes = 5.5e6f;  // of a split reduction: its launch, and bytes in a microsecond
 constexpr int kTile[3] = {64, 128, 256};
+
+// Threads of a workgroup of such a tile.  128-tiles of bf16 matrices that have a compute unit each take eight waves and four stages
+// (4096 x 4096 x 1024: 45 us against 52); otherwise two workgroups of four waves share one.
+inline int threads_of(int tile, int size, long groups, int cus) { return tile == 256 || (tile == 128 && size == 2 && groups <= cus) ? 512 : 256; }
 
 // Lines may lie where 16-byte pieces of them are aligned and 31 bits span a tile's: 256 rows, or the 64 reduction steps of a k-tile.
 int lie_of(const ProductOperand& o, int count, int rows, int k, int size, bool steps_ok, long& pitch) {
@@ -1097,12 +1116,15 @@ constexpr int kFewRows = 8, kFewRowsGated = 4;
 bool few_rows(const ProductArgs& p, Plan& l) {
     if (p.kind == PRODUCT_GATED ? p.m > kFewRowsGated : p.kind != PRODUCT_LINEAR || p.m > kFewRows) return false;
     if (p.k > 16384 && p.n < 1024) return false;  // long rows on few compute units
+    if (up(p.n, 16) / 16 * 512 > MOST_THREADS) return false;
     if (p.k > 1 && (p.a.col[0] != 1 || p.b.col[0] != 1)) return false;
     if (p.kind == PRODUCT_GATED && ((p.k > 1 && p.b.col[1] != 1) || p.b.row[1] != p.b.row[0])) return false;
     l.tile = 0;
     l.pitch_a = p.a.row[0];
     l.pitch_b = p.b.row[0];
     l.segments = l.outs = l.splits = 1;
+    l.groups = up(p.n, 16) / 16;
+    l.threads = 512;
     return true;
 }
 
@@ -1122,84 +1144,85 @@ bool make_plan(const ProductArgs& p, int cus, Plan& l) {
     auto pack_bytes = [&](int lie, long pitch, long rows) {
         if (lie == LIE_ROWS || lie == LIE_STEPS) return 0L;
         if (lie != LIE_PACKED_STEPS && pitch > (0x7fff0000L / size) / (rows < 256 ? rows : 256)) return -1L;
-        if (up(p.k, 64) / 64 * (up(rows, 64) / 64) > 0x7fffffffL / 32) return -1L;  // (workgroups of the copies)
+        if (lie == LIE_GATHERED) l.copies = std::max(l.copies, up(p.k, 64) / 64 * (up(rows, 64) / 64) * 256);
         return up((lie == LIE_PACKED_STEPS ? p.k : rows) * pitch * size, 256);
     };
     l.pack_a = pack_bytes(l.lie_a, l.pitch_a, p.m);
     l.pack_b = pack_bytes(l.lie_b, l.pitch_b, p.n);
     if (l.pack_a < 0 || l.pack_b < 0) return false;
+    auto pieces = [&](int lie, long rows, int count) {  // of lines that are copied whole, a thread each
+        const long length = lie == LIE_PACKED_STEPS ? rows : p.k, lines = lie == LIE_PACKED_STEPS ? p.k : rows;
+        return lie == LIE_PACKED_ROWS || lie == LIE_PACKED_STEPS ? up(length, 16 / size) / (16 / size) * lines * count : 0L;
+    };
+    l.copies = std::max(l.copies, up(pieces(l.lie_a, p.m, l.count_a) + pieces(l.lie_b, p.n, l.count_b), 256));
+    if (l.copies > MOST_THREADS) return false;
     l.nk = (int)((p.k + (long)bk - 1) / bk);
     auto tiles_of = [&](int t) { return up(p.m, t) / t * (up(p.n, gated ? t / 2 : t) / (gated ? t / 2 : t)) * l.outs; };
     const long all = (long)l.nk * l.segments;
     if (all > 0x3fffffffL) return false;
     const bool bf = p.dtype == MUON_HIP_BF16;
     float best = 1e30f;
-    long tiles = 0;
     for (int c = 0; c < (bf ? 3 : 2); ++c) {
         const long here = tiles_of(kTile[c]);
         const Cost& q = kCost[bf][c];
         for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
             if (want > 1 && (want > all / 4 || here * want > 8L * cus)) break;
             const long per = (all + want - 1) / want, parts = (all + per - 1) / per;
+            if (here * parts > MOST_THREADS / threads_of(kTile[c], size, here * parts, cus)) break;
             const long load = (here * parts + cus - 1) / cus;
             float t = q.start + q.each * load + (float)per * (load <= 1 ? q.alone : std::max(q.alone, q.busy * load));
             if (parts > 1) t += kJoinStart + (float)p.m * p.n * (gated ? 2 : l.outs) * 8.f * parts / kJoinBytes;
             if (t < best) {
                 best = t;
-                tiles = here;
                 l.tile = kTile[c];
                 l.per_split = (int)per;
                 l.splits = (int)parts;
+                l.groups = here * parts;
+                l.threads = threads_of(kTile[c], size, l.groups, cus);
             }
         }
     }
-    if (tiles > 0x3fffffffL) return false;
-    if (tiles * l.splits > 0x7fffffffL) return false;
+    if (l.tile == 0) return false;
     if (l.splits > 1) l.partial_bytes = (long)l.splits * (gated ? 2 : l.outs) * p.m * p.n * 4;
     l.bytes = l.pack_a * l.count_a + l.pack_b * l.count_b + l.partial_bytes;
     return true;
 }
 
 template <typename T, int BM, int BN, int WGM, int WGN, int S, bool AS, bool BS, bool GATED>
-hipError_t launch_tiles(const KernelArgs& g, hipStream_t stream) {
+hipError_t launch_tiles(const KernelArgs& g, const Plan& l, hipStream_t stream) {
     constexpr int smem = S * (BM + BN) * ROWB;
     static std::atomic<unsigned long long> configured{0};
     const auto kern = product_kernel<T, BM, BN, WGM, WGN, S, AS, BS, GATED>;
     if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
-    const long grid = (long)g.tiles_m * g.tiles_n * g.outs * g.splits;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(WGM * WGN * 64), smem, stream, g);
+    hipLaunchKernelGGL(kern, dim3((unsigned)l.groups), dim3(WGM * WGN * 64), smem, stream, g);
     return hipGetLastError();
 }
 template <typename T, int BM, int BN, int WGM, int WGN, bool AS, bool BS, bool GATED>
-hipError_t launch_pp(const KernelArgs& g, hipStream_t stream) {
+hipError_t launch_pp(const KernelArgs& g, const Plan& l, hipStream_t stream) {
     constexpr int smem = (3 * BM + 2 * BN) * ROWB;
     static std::atomic<unsigned long long> configured{0};
     const auto kern = product_pp_kernel<T, BM, BN, WGM, WGN, AS, BS, GATED>;
     if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)g.tiles_m * g.tiles_n * g.outs * g.splits)), dim3(512), smem, stream, g);
+    hipLaunchKernelGGL(kern, dim3((unsigned)l.groups), dim3(512), smem, stream, g);
     return hipGetLastError();
 }
 template <typename T, bool AS, bool BS, bool GATED>
-hipError_t launch_tile(int tile, const KernelArgs& g, int cus, hipStream_t s) {
+hipError_t launch_tile(const KernelArgs& g, const Plan& l, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (tile == 256) return launch_pp<T, 256, 256, 2, 4, AS, BS, GATED>(g, s);
+        if (l.tile == 256) return launch_pp<T, 256, 256, 2, 4, AS, BS, GATED>(g, l, s);
+        if (l.tile == 128 && l.threads == 512) return launch_tiles<T, 128, 128, 4, 2, 4, AS, BS, GATED>(g, l, s);
     }
-    if (tile == 128) {
-        // Where every compute unit has at most one of them, eight waves and four stages (4096 x 4096 x 1024: 45 us against 52); otherwise two
-        // workgroups of four waves share one.
-        if (sizeof(T) == 2 && (long)g.tiles_m * g.tiles_n * g.outs * g.splits <= cus) return launch_tiles<T, 128, 128, 4, 2, 4, AS, BS, GATED>(g, s);
-        return launch_tiles<T, 128, 128, 2, 2, 2, AS, BS, GATED>(g, s);
-    }
-    return launch_tiles<T, 64, 64, 4, 1, 3, AS, BS, GATED>(g, s);
+    if (l.tile == 128) return launch_tiles<T, 128, 128, 2, 2, 2, AS, BS, GATED>(g, l, s);
+    return launch_tiles<T, 64, 64, 4, 1, 3, AS, BS, GATED>(g, l, s);
 }
 template <typename T, bool GATED>
-hipError_t launch_rows(const KernelArgs& g, hipStream_t s) {
-    hipLaunchKernelGGL((product_rows_kernel<T, GATED>), dim3((unsigned)(up(g.n, 16) / 16)), dim3(512), 0, s, g);
+hipError_t launch_rows(const KernelArgs& g, const Plan& l, hipStream_t s) {
+    hipLaunchKernelGGL((product_rows_kernel<T, GATED>), dim3((unsigned)l.groups), dim3(l.threads), 0, s, g);
     return hipGetLastError();
 }
 
 template <typename T>
-hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int cus, int xcd_shift, hipStream_t s) {
+hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int xcd_shift, hipStream_t s) {
     constexpr int S = sizeof(T);
     const bool gated = p.kind == PRODUCT_GATED;
     KernelArgs g{};
@@ -1260,10 +1283,10 @@ hipError_t run_product(const ProductArgs& p, const Plan& l, void* workspace, int
         g.partial = l.splits > 1 ? (float*)ws : nullptr;
         const bool as = by_steps(l.lie_a), bs = by_steps(l.lie_b);
         hipError_t e;
-        if (l.tile == 0) e = gated ? launch_rows<T, true>(g, s) : launch_rows<T, false>(g, s);
-        else if (gated) e = as ? launch_tile<T, true, false, true>(l.tile, g, cus, s) : launch_tile<T, false, false, true>(l.tile, g, cus, s);
-        else if (as) e = bs ? launch_tile<T, true, true, false>(l.tile, g, cus, s) : launch_tile<T, true, false, false>(l.tile, g, cus, s);
-        else e = bs ? launch_tile<T, false, true, false>(l.tile, g, cus, s) : launch_tile<T, false, false, false>(l.tile, g, cus, s);
+        if (l.tile == 0) e = gated ? launch_rows<T, true>(g, l, s) : launch_rows<T, false>(g, l, s);
+        else if (gated) e = as ? launch_tile<T, true, false, true>(g, l, s) : launch_tile<T, false, false, true>(g, l, s);
+        else if (as) e = bs ? launch_tile<T, true, true, false>(g, l, s) : launch_tile<T, true, false, false>(g, l, s);
+        else e = bs ? launch_tile<T, false, true, false>(g, l, s) : launch_tile<T, false, false, false>(g, l, s);
         if (e != hipSuccess || l.splits == 1) return e;
     }
     const long work = up(p.n, 8) / 8 * p.m * l.outs;
@@ -1280,19 +1303,29 @@ long product_workspace(const ProductArgs& p, int cus) {
     return make_plan(p, cus, l) ? l.bytes : -1;
 }
 
+bool plan_product(const ProductArgs& p, int cus, muon_hip_product_route& out) {
+    Plan l;
+    if (!make_plan(p, cus, l)) return false;
+    out = muon_hip_product_route{l.tile, l.splits, l.lie_a, l.lie_b, l.groups, l.threads, l.copies};
+    return true;
+}
+
 hipError_t launch_product(const ProductArgs& p, void* workspace, int cus, int xcd_shift, hipStream_t stream) {
     Plan l;
     if (!make_plan(p, cus, l)) return hipErrorInvalidValue;
     if (p.m == 0 || p.n == 0) return hipSuccess;
-    return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, cus, xcd_shift, stream) : run_product<float>(p, l, workspace, cus, xcd_shift, stream);
+    return p.dtype == MUON_HIP_BF16 ? run_product<bf16_t>(p, l, workspace, xcd_shift, stream) : run_product<float>(p, l, workspace, xcd_shift, stream);
 }
 
 // Rows of a workgroup: as many as leave the machine enough of them, so that small gradients are not a loop and large ones have few parts.
+static long act_grad_groups(long m, long n, long rows) { return up(m, rows) / rows * (up(n, 256) / 256); }
 static long act_grad_rows(long m, long n) {
     long rows = 64;
-    while (rows > 8 && up(m, rows) / rows * (up(n, 256) / 256) < 1024) rows /= 2;
+    while (rows > 8 && act_grad_groups(m, n, rows) < 1024) rows /= 2;
+    while (rows < (1 << 20) && act_grad_groups(m, n, rows) > MOST_THREADS / 256) rows *= 2;  // (more than a launch has)
     return rows;
 }
+bool act_grad_fits(long m, long n) { return act_grad_groups(m, n, act_grad_rows(m, n)) <= MOST_THREADS / 256; }
 long act_grad_partials(long m, long n) {
     const long rows = act_grad_rows(m, n);
     return up(m, rows) / rows * n;
@@ -1310,7 +1343,7 @@ hipError_t launch_act_grad(const ActGradArgs& a, hipStream_t stream) {
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     if ((!a.db[0] && !a.db[1]) || a.n == 0) return hipSuccess;
-    const dim3 grid((unsigned)(up(a.n, 16) / 16), pair ? 2 : 1);
+    const dim3 grid((unsigned)std::min(up(a.n, 16) / 16, 65536L), pair ? 2 : 1);
     if (bf) hipLaunchKernelGGL(row_sum_kernel<bf16_t>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (bf16_t*)a.db[0], (bf16_t*)a.db[1]);
     else hipLaunchKernelGGL(row_sum_kernel<float>, grid, dim3(256), 0, stream, a.partials, (int)chunks, a.n, (float*)a.db[0], (float*)a.db[1]);
     return hipGetLastError();

@@ -69,3 +69,22 @@ def test_a_product_without_an_activation_keeps_its_factor_too(size, dtype):
     _abi.check(lib.muon_hip_product_run(ctypes.addressof(p), ws.data_ptr(), need, stream))
     _abi.check(lib.muon_hip_act_grad(dy.data_ptr(), 1, aux.data_ptr(), None, dz.data_ptr(), None, n, None, None, code, t, n, None, stream))
     assert torch.equal(dz, dy) and torch.equal(out, E.linear(x, w))
+
+
+def test_launches_at_the_limit_of_a_grid():
+    """Few rows against 2^27 rows of a table, for which the walk over it has more threads than a launch; sums over 2^30 rows, for which 64 rows to a
+    workgroup would be."""
+    n, k = 2 ** 27 + 24, 8
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x, w = (torch.randint(-4, 5, s, generator=g, device=DEV, dtype=torch.int8).to(BF) for s in ((3, k), (n, k)))
+    y, h = E.linear(x, w), E.gated_linear(x, w, w, activation="none")
+    for at in (slice(0, 100), slice(2 ** 26, 2 ** 26 + 100), slice(n - 100, n)):
+        want = x.double() @ w[at].double().t()  # whole numbers below 2^8, and their squares, rounded once
+        assert torch.equal(y[:, at].double(), want) and torch.equal(h[:, at], want.square().to(BF))
+    del w, y, h
+    m = 2 ** 30 + 9
+    part = torch.randint(-1, 2, (2 ** 20, 1), generator=g, device=DEV, dtype=torch.int8).float()
+    dy = torch.cat([part.repeat(2 ** 10, 1), part[:9]])
+    b = torch.zeros(1, device=DEV, requires_grad=True)
+    (db,) = torch.autograd.grad(E.linear(torch.zeros(m, 1, device=DEV), torch.zeros(1, 1, device=DEV), b), b, dy)
+    assert db.item() == part.sum().item() * 2 ** 10 + part[:9].sum().item()  # (every partial sum is a whole number below 2^24)

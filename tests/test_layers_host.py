@@ -1,5 +1,6 @@
 """What linear, gated_linear and the entry points behind them refuse, before anything is launched: no GPU needed."""
 import ctypes
+import itertools
 
 import pytest
 import torch
@@ -132,3 +133,53 @@ def test_activation_gradients_are_checked_before_any_launch():
 
 def test_activation_names_are_those_of_the_header():
     assert layers.ACTIVATIONS == ("none", "relu", "sigmoid", "silu", "gelu", "gelu_tanh")
+
+
+def product_of(kind, m, n, k, dtype=_abi.BF16, turned=(False, False), at=1 << 20):
+    """A product of contiguous matrices, turned where the reduction runs down their columns; nothing is there to be read."""
+    p = _abi.Product(kind=kind, dtype=dtype, m=m, n=n, k=k)
+    for f, lines, turn in (("a", m, turned[0]), ("b", n, turned[1])):
+        getattr(p, f)[:] = (at, at)
+        getattr(p, f + "_row")[:] = (1, 1) if turn else (k, k)
+        getattr(p, f + "_col")[:] = (lines, lines) if turn else (1, 1)
+    p.out[:] = (1 << 20, 1 << 20)
+    return p
+
+
+MOST_THREADS = 2 ** 32 - 1  # of a launch
+
+
+def test_no_launch_has_more_threads_than_a_grid_may_have():
+    """Sizes up to the largest: a product is planned within the limit, or refused before anything is launched."""
+    planned = 0
+    big = [1, 7, 16, 250, 4096, 2 ** 20 + 1, 2 ** 24, 2 ** 27 - 16, 2 ** 27, 2 ** 28 + 5, 2 ** 30, 2 ** 31 - 70, 2 ** 31 - 1]
+    for kind, dtype, m, n, k, turned, at in itertools.product(range(4), (_abi.BF16, _abi.F32), big, big, (1, 8, 33, 4096), itertools.product((False, True), repeat=2),
+                                                              (1 << 20, (1 << 20) + 4)):
+        try:
+            r = _abi.product_route(product_of(kind, m, n, k, dtype, turned, at))
+        except _abi.MuonHipError as e:
+            assert "exceed one launch" in str(e)
+            continue
+        planned += 1
+        assert 0 < r.groups * r.threads <= MOST_THREADS, (kind, dtype, m, n, k, turned, r.tile, r.parts, r.groups)
+        assert r.copies <= MOST_THREADS and (r.copies > 0) == (max(r.a, r.b) >= _abi.OPERAND_ROWS_COPIED), (kind, dtype, m, n, k, turned, r.a, r.b, r.copies)
+    assert planned > 1000
+
+
+@pytest.mark.parametrize("kind", (_abi.PRODUCT_LINEAR, _abi.PRODUCT_GATED))
+def test_a_few_rows_against_a_very_large_table(kind):
+    """Where the walk over the weight has more workgroups than a launch, tiles take the call."""
+    assert _abi.product_route(product_of(kind, 4, 2 ** 27 - 16, 64)).tile == 0
+    for n in (2 ** 27, 2 ** 28, 2 ** 30 - 64):
+        r = _abi.product_route(product_of(kind, 4, n, 64))
+        assert r.tile > 0 and r.groups * r.threads <= MOST_THREADS, n
+
+
+def test_activation_gradients_fit_a_launch():
+    lib, one = _abi.lib(), 1 << 20
+    for m, n in itertools.product((1, 9, 4096, 2 ** 24, 2 ** 30, 2 ** 31 - 1), (1, 255, 257, 4096, 2 ** 24, 2 ** 31 - 1)):
+        chunks, rest = divmod(lib.muon_hip_act_grad_partials(m, n), n)
+        assert rest == 0 and 1 <= chunks <= -(-m // 8)
+        if chunks * -(-n // 256) * 256 > MOST_THREADS:
+            assert m * n > 2 ** 50  # (a petabyte)
+            assert lib.muon_hip_act_grad(one, 1, one, None, one, None, n, None, None, 1, m, n, None, None) == -2
