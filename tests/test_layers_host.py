@@ -7,6 +7,7 @@ import torch
 
 import lmms_engine_amd as E
 from lmms_engine_amd import _abi, layers
+from tests import layer_cases as cases
 
 
 def test_cpu_tensors_and_wrong_arguments_are_refused():
@@ -183,3 +184,23 @@ def test_activation_gradients_fit_a_launch():
         if chunks * -(-n // 256) * 256 > MOST_THREADS:
             assert m * n > 2 ** 50  # (a petabyte)
             assert lib.muon_hip_act_grad(one, 1, one, None, one, None, n, None, None, 1, m, n, None, None) == -2
+
+
+def test_the_cases_run_every_kernel():
+    """EVERY_KERNEL, which a GPU test runs, takes every tile of every type in every pass, over rows and over columns, whole and split, as 256
+    compute units choose them: a rule that changes has to bring new cases."""
+    ran = set()
+    for dtype, t, k, n in cases.EVERY_KERNEL:
+        for layer, xt, wt in itertools.product(cases.LAYERS, (False, True), (False, True)):
+            for which, p in cases.products(layer, dtype, t, k, n, xt, wt).items():
+                kernel, split = cases.kernel(p)
+                parts, bk = _abi.product_route(p).parts, 64 if dtype == _abi.BF16 else 32
+                if -(-p.k // bk) // parts >= 4:
+                    ran.add((layer, which) + kernel + (split,))
+    tiles = [(_abi.BF16, 64, 256), (_abi.BF16, 128, 256), (_abi.BF16, 128, 512), (_abi.BF16, 256, 512), (_abi.F32, 64, 256), (_abi.F32, 128, 256)]
+    orders = {("linear", "forward"): [(0, 0), (0, 1), (1, 0), (1, 1)], ("gated", "forward"): [(0, 0), (1, 0)]}  # of the left and the right operand
+    for (layer, which), split, tile in itertools.product(itertools.product(cases.LAYERS, ("forward", "dx", "dw")), (False, True), tiles):
+        if layer == "linear" and split and tile == (_abi.BF16, 128, 256):
+            continue  # (more tiles than compute units: one result of so many is not split)
+        for a, b in orders.get((layer, which), [(int(which == "dw"), b) for b in (0, 1)]):
+            assert (layer, which, *tile, a, b, layer == "gated" and which == "forward", split) in ran, (layer, which, tile, a, b, split)
