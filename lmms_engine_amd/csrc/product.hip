@@ -311,7 +311,7 @@ __device__ __forceinline__ int swizzle_steps(int k) {
 template <typename T, int R, bool STEPS, int F>
 struct Reader {
     static constexpr bool HALF = sizeof(T) == 2;
-    static constexpr int N = !STEPS ? 2 : HALF || F < 4 ? F : 4;
+    static constexpr int N = STEPS ? F : 2;
     unsigned at[N];
     __device__ __forceinline__ void init(unsigned base, int first, int lane) {
         const int i = lane & 15, grp = lane >> 4;
@@ -349,7 +349,7 @@ struct Reader {
         } else {
             f32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = *(const float*)(smem + at[f % N] + (h * 16 + e) * (R * 4) + f / N * 256);
+            for (int e = 0; e < 4; ++e) w[e] = *(const float*)(smem + at[f] + (h * 16 + e) * (R * 4));
             return w;
         }
     }
@@ -696,13 +696,13 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 // library's product of the same matrices (1540 to 1600); gradients, whose operands come through transposing reads, 1350 to 1430 (the
 // library 1130 to 1330).  64 KB a k-tile are 12 TB/s over the machine, what the way to LDS takes.  Loads or fragments of the right operand
 // moved into the multiplying phases cost 10 %, a higher priority for those phases does nothing.
-template <typename T, int BM, int BN, int WGM, int WGN, bool ASTEPS, bool BSTEPS, bool GATED>
-__global__ void __launch_bounds__(512, BM == 128 ? 4 : 2) product_pp_kernel(const KernelArgs g) {
+template <typename T, bool ASTEPS, bool BSTEPS, bool GATED>
+__global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int NW = WGM * WGN;
+    constexpr int BM = 256, BN = 256, WGM = 2, WGN = 4, NW = WGM * WGN;
     constexpr int WTM = BM / WGM, WTN = BN / WGN, FM = WTM / 16, FN = WTN / 16;
     constexpr int UNIT_A = BM * ROWB, UNIT_B = BN * ROWB, A_AT = 2 * UNIT_B;  // stages; the left operand's lie behind the right one's
-    static_assert(NW == 8 && WTN == 64, "two groups of four waves; a wave of a gated pair holds 32 columns of each factor");
+    static_assert(WTN == 64, "a wave of a gated pair holds 32 columns of each factor");
     typedef Panels<T, BM, BN, NW, ASTEPS, BSTEPS, GATED> P;
     typedef typename Elem<T>::frag frag;
 
@@ -1197,11 +1197,11 @@ hipError_t launch_tiles(const KernelArgs& g, const Plan& l, hipStream_t stream) 
     hipLaunchKernelGGL(kern, dim3((unsigned)l.groups), dim3(WGM * WGN * 64), smem, stream, g);
     return hipGetLastError();
 }
-template <typename T, int BM, int BN, int WGM, int WGN, bool AS, bool BS, bool GATED>
+template <typename T, bool AS, bool BS, bool GATED>
 hipError_t launch_pp(const KernelArgs& g, const Plan& l, hipStream_t stream) {
-    constexpr int smem = (3 * BM + 2 * BN) * ROWB;
+    constexpr int smem = 5 * 256 * ROWB;
     static std::atomic<unsigned long long> configured{0};
-    const auto kern = product_pp_kernel<T, BM, BN, WGM, WGN, AS, BS, GATED>;
+    const auto kern = product_pp_kernel<T, AS, BS, GATED>;
     if (hipError_t e = allow_dynamic_lds((const void*)kern, smem, configured); e != hipSuccess) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)l.groups), dim3(512), smem, stream, g);
     return hipGetLastError();
@@ -1209,7 +1209,7 @@ hipError_t launch_pp(const KernelArgs& g, const Plan& l, hipStream_t stream) {
 template <typename T, bool AS, bool BS, bool GATED>
 hipError_t launch_tile(const KernelArgs& g, const Plan& l, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        if (l.tile == 256) return launch_pp<T, 256, 256, 2, 4, AS, BS, GATED>(g, l, s);
+        if (l.tile == 256) return launch_pp<T, AS, BS, GATED>(g, l, s);
         if (l.tile == 128 && l.threads == 512) return launch_tiles<T, 128, 128, 4, 2, 4, AS, BS, GATED>(g, l, s);
     }
     if (l.tile == 128) return launch_tiles<T, 128, 128, 2, 2, 2, AS, BS, GATED>(g, l, s);
