@@ -139,12 +139,12 @@ def test_what_is_kept_is_what_is_read(dtype, each):
 
     def kept(f, **shapes):
         """Bytes that the call holds on to once the caller has let go of what it passed."""
-        torch.cuda.synchronize()
-        before = torch.cuda.memory_allocated()
+        asked = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]  # (allocated ones count what is left of a cached block too)
+        before = asked()
         v = {m: torch.zeros(*s, dtype=dtype, device=DEV) for m, s in shapes.items()}
         y = f(v)
         del v
-        return torch.cuda.memory_allocated() - before - y.numel() * y.element_size()
+        return asked() - before - y.numel() * y.element_size()
 
     factor, size = t * n * each, torch.finfo(dtype).bits // 8
     x, w, b = t * k * size, n * k * size, n * size
