@@ -336,8 +336,8 @@ int muon_hip_clip_scale(const void* const* g_ptrs, const long* numel, const long
  *           aux[1] = u act'(g), the factors of the gradients of u and of g
  *   SUM     out[0] = a[0] b[0]^T + a[1] b[1]^T
  *   EACH    out[0] = a[0] b[0]^T, out[1] = a[1] b[0]^T
- * aux holds muon_hip_product_aux_bytes() bytes each, in a form that muon_hip_act_grad reads: the values to 24 bits of which 8 are the
- * exponent's and one the sign for bf16 tensors, fp32 for fp32 ones.
+ * aux holds muon_hip_product_aux_bytes() bytes each, in a form that muon_hip_act_grad reads: the values rounded to 24 bits, of which 8
+ * are the exponent's and one the sign, for bf16 tensors, fp32 for fp32 ones.
  * bias (n contiguous elements each), residual (strides res_row, res_col) and aux may be null; SUM and EACH take none of them and
  * MUON_HIP_ACT_NONE.  All tensors share `dtype`.  m, n and k may be 0; a sum over nothing is 0.  Outputs may not overlap inputs, but for a
  * residual that is out[0] itself. */

@@ -176,7 +176,7 @@ __device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
 // Factors that are kept for the backward pass of bf16 tensors: each rounded to its upper 24 bits, in a plane of the upper 16 and one of the
 // other 8.  So they are off by 2^-16 at most, to either side (cut off: 2^-15, all towards zero, which sums over rows do not even out).  Rounded
 // to bf16 like any activation they are off by 2^-8, as much as the rounding of dy * d behind them, and gradients then were 1.7 times as far
-// from the formula's as results that are rounded once (2.9e-3 against 1.7e-3 in the 2-norm; so it is 2.4e-3).
+// from the formula's as results that are rounded once (2.9e-3 against 1.66e-3 in the 2-norm; so it is 2.35e-3).
 // The third byte costs 2 % of a gated training step over 8192 x 4096 x 12288 and half as much memory again; fp32 tensors keep all 32 bits.
 template <typename T>
 __device__ __forceinline__ void keep8(void* base, long all, long at, int count, const float (&v)[8]) {
@@ -585,10 +585,10 @@ __device__ __forceinline__ void finish_tile(const KernelArgs& g, const Tile& t, 
 }
 
 // ---- small tiles -----------------------------------------------------------------------------------
-// What bounds them is the way from the caches to LDS, 11 to 12 TB/s over the machine for rows as tensors have them: 32 KB a k-tile of a
-// 128-tile take 0.63 us while it has its compute unit for itself (its matrix instructions 0.25), so it reaches 0.75 PFLOP/s where a 256-tile,
-// which needs half as much for the same work, reaches twice that.  Fragments of the next half read ahead of the products: 10 to 20 %
-// slower; two k-tiles to a barrier: nothing.
+// What seems to bound them (from times, no counter) is the way from the caches to LDS, 11 to 12 TB/s over the machine for rows as tensors
+// have them: 32 KB a k-tile of a 128-tile take 0.63 us while it has its compute unit for itself (its matrix instructions 0.25), so it
+// reaches 0.75 PFLOP/s where a 256-tile, which needs half as much for the same work, reaches twice that.  Fragments of the next half read
+// ahead of the products: 10 to 20 % slower; two k-tiles to a barrier: nothing.
 // S stages: a wave waits for its own loads of k-tile t, crosses the one barrier of the k-tile (behind which every wave has read all of k-tile
 // t - 1), issues the loads of k-tile t + S - 1 into the stage that is free now, and multiplies.
 template <typename T, int BM, int BN, int WGM, int WGN, int S, bool ASTEPS, bool BSTEPS, bool GATED>
@@ -692,9 +692,9 @@ __global__ void __launch_bounds__(WGM* WGN * 64) product_kernel(const KernelArgs
 // the end of M(t, 1) each wave waits for its own loads of k-tile t + 1, the last of which are one k-tile old: the two groups issued after
 // them stay in flight.  k-tile t + 1 is first read in phase 4t + 4.
 //
-// Measured, 8192 x 12288 x 4096 (rows against rows): two stages each and one k-tile of distance 1320 TFLOP/s, this 1480 to 1570, as much as the
-// library's product of the same matrices (1540 to 1600); gradients, whose operands come through transposing reads, 1350 to 1430 (the
-// library 1130 to 1330).  64 KB a k-tile are 12 TB/s over the machine, what the way to LDS takes.  Loads or fragments of the right operand
+// Measured, 8192 x 12288 x 4096 (rows against rows): two stages each and one k-tile of distance 1320 TFLOP/s, this 1450 to 1570, as much as the
+// library's product of the same matrices (1540 to 1600); gradients, whose operands come through transposing reads, 1230 to 1430 (the
+// library 1130 to 1330).  64 KB a k-tile are 12 TB/s over the machine, as in the small tiles.  Loads or fragments of the right operand
 // moved into the multiplying phases cost 10 %, a higher priority for those phases does nothing.
 template <typename T, bool ASTEPS, bool BSTEPS, bool GATED>
 __global__ void __launch_bounds__(512, 2) product_pp_kernel(const KernelArgs g) {
@@ -957,6 +957,8 @@ __global__ void __launch_bounds__(256) product_gather_kernel(const T* src, long 
 }
 
 // ---- activation gradients and sums over rows ----------------------------------------------------------
+// dz is an operand of two products, whose matrix instructions take the tensors' type, and is rounded to it (bf16: 2^-8 of each value at most);
+// the sums over rows add the values before that.
 // A workgroup takes 256 columns (32 threads, eight columns each) of `rows` rows, eight at a time.  Bound by memory: the pair of gradients of
 // 8192 x 12288 bf16 values, 12 bytes a value, takes 245 us (4.9 TB/s, the rate of a copy).
 template <typename T, bool PAIR>
