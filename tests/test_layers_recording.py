@@ -84,3 +84,21 @@ def test_modes_that_watch_see_the_same_results(name):
     chosen = both(lambda a, b: checkpoint(FUNCTIONS[name], a, b, use_reentrant=False, context_fn=lambda: create_selective_checkpoint_contexts(policy)))
     for got in (counted, recomputed, chosen):
         assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+@pytest.mark.parametrize("name", list(FUNCTIONS))
+def test_compiled_functions_break_their_graph_at_a_call(name, backend):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x, w = (torch.randn(*s, generator=g, device="cuda").requires_grad_(True) for s in ((6, 16), (8, 16)))
+
+    def f(a, b):
+        return FUNCTIONS[name](a * 2, b).relu() + 1
+
+    def both(f):
+        y = f(x, w)
+        return [y.detach(), *torch.autograd.grad(y, (x, w), torch.ones_like(y))]
+
+    for got, want in zip(both(torch.compile(f, backend=backend)), both(f)):
+        assert torch.equal(got, want)
