@@ -357,11 +357,12 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 // ---- calls ------------------------------------------------------------------------------------
 
-// A plain tensor on a GPU, of x's type and device.
+// A plain tensor on a GPU, of x's type and device, whose memory is there.
 bool plain(PyObject* o, const Tensor* x) {
     if (!THPVariable_CheckExact(o)) return false;
     const Tensor& t = THPVariable_Unpack(o);
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->is_python_dispatch()) return false;
+    if (t.has_storage() && t.numel() > 0 && !t.storage().data()) return false;
     if (x) return t.scalar_type() == x->scalar_type() && t.device() == x->device();
     return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
 }

@@ -108,4 +108,6 @@ def _refuse(*tensors) -> None:
             raise NotImplementedError(f"linear and gated_linear take plain tensors and parameters, got {type(t).__name__}")
         if t is not None and t.layout != torch.strided:
             raise NotImplementedError(f"linear and gated_linear take strided tensors, got {t.layout}")
+        if t is not None and t.numel() > 0 and t.untyped_storage().data_ptr() == 0:
+            raise ValueError(f"the memory of a tensor of shape {tuple(t.shape)} was freed")
     raise ValueError(f"rows or columns are too many for one call: {[tuple(t.shape) for t in tensors if t is not None]}")

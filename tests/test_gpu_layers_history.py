@@ -173,3 +173,15 @@ def test_what_is_kept_is_what_is_read(dtype, each):
                         (("b", "b2"), 2 * b + 2 * factor)):
         got = kept(trained(*names), **gated)
         assert abs(got - want) <= slack, (names, got / mb, want / mb)
+
+
+@pytest.mark.parametrize("which", ["x", "w", "b", "r"])
+def test_a_tensor_whose_memory_was_freed_is_refused(which):
+    """Sharded training frees a parameter's storage and keeps the tensor: it is not taken for one that was left out."""
+    v = inputs("linear")
+    v[which].untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="freed"):
+        call("linear", v, "silu")
+    if which != "r":
+        with pytest.raises(ValueError, match="freed"):
+            E.gated_linear(v["x"], v["w"], v["w"], v["b"], v["b"])
