@@ -62,7 +62,12 @@ extern "C" {
 #define MUON_HIP_K_FLOW_CHAIN 12  /* the iterations and the update of many small matrices in one launch */
 #define MUON_HIP_K_PRODUCT 13     /* a muon_hip_product_run with its packing and joining launches */
 #define MUON_HIP_K_ACT_GRAD 14
-#define MUON_HIP_K_COUNT 15
+#define MUON_HIP_K_NORM 15
+#define MUON_HIP_K_NORM_GRAD 16
+#define MUON_HIP_K_EMBEDDING 17
+#define MUON_HIP_K_EMBEDDING_GRAD 18
+#define MUON_HIP_K_DROPOUT 19
+#define MUON_HIP_K_COUNT 20
 
 /* GEMM kernel variants; MUON_HIP_CFG_AUTO picks per kernel, shape and number of tiles.  All feed LDS with direct
  * global->LDS loads (global_load_lds_dwordx4), software pipelined behind the MFMAs. */
@@ -398,6 +403,80 @@ int muon_hip_route_product(const muon_hip_product* p, int cus, muon_hip_product_
 long muon_hip_act_grad_partials(int m, int n);
 int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d1, void* dz0, void* dz1, long pitch, void* db0, void* db1,
                       int dtype, int m, int n, float* partials, void* stream);
+
+/* ---- rows of layers -----------------------------------------------------------------------
+ * What stands around the products of a layer, row by row: norms, embedding, dropout, forward and backward.  No counterpart in the
+ * reference, which leaves them to torch.  Rows of n values lie `..._row` elements apart (n at least, where there is more than one row), their
+ * values back to back; any address.  Results are row-major without gaps and may not overlap inputs (but for muon_hip_dropout).  All tensors of a call
+ * share `dtype`.  Everything is computed in fp32 and rounded once; sums have a fixed order.  Sizes may be 0.
+ *
+ * muon_hip_norm_run, of each of `rows` rows:
+ *   s = x + residual, rounded to dtype and written to `sum`, where there is a residual (null: s = x);
+ *   LAYER  y = (s - mean) * rstd * weight + bias, rstd = 1 / sqrt(mean((s - mean)^2) + eps)
+ *   RMS    y = s * rstd * weight, rstd = 1 / sqrt(mean(s^2) + eps); bias is null.
+ * weight and bias (n elements, back to back) may be null.  stats, where not null, keeps `rows` floats, rstd, and behind them with LAYER `rows`
+ * more, the means.
+ *
+ * muon_hip_norm_grad_run: with g = dy * weight and hat = (s - mean) * rstd (s * rstd),
+ *   LAYER  dx = rstd * (g - mean(g) - hat * mean(g * hat)) + ds
+ *   RMS    dx = rstd * (g - hat * mean(g * hat)) + ds
+ *   dweight = the sum of dy * hat over the rows, dbias that of dy.
+ * ds, the gradient of `sum`, may be null; dx, dweight and dbias where they are not wanted; dbias alone
+ * needs no s and no stats.  dx is the gradient of x and of the residual. */
+#define MUON_HIP_NORM_LAYER 0
+#define MUON_HIP_NORM_RMS 1
+typedef struct {
+    int kind, dtype;
+    int rows, n;
+    const void* x;
+    long x_row;
+    const void* residual;
+    long res_row;
+    const void* weight;
+    const void* bias;
+    double eps;
+    void* y;
+    void* sum;
+    float* stats;
+} muon_hip_norm;
+int muon_hip_norm_run(const muon_hip_norm* p, void* stream);
+
+typedef struct {
+    int kind, dtype;
+    int rows, n;
+    const void* dy;
+    long dy_row;
+    const void* s;
+    long s_row;
+    const void* ds;
+    long ds_row;
+    const void* weight;
+    const float* stats;
+    void* dx;
+    void* dweight;
+    void* dbias;
+} muon_hip_norm_grad;
+/* Bytes of workspace (256-byte aligned) that the call needs on the current device, 0 where none; negative: refused. */
+long muon_hip_norm_grad_workspace(const muon_hip_norm_grad* p);
+int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[t] = table[ids[t]] * scale for `tokens` ids, 64-bit integers (wide_ids) or 32-bit ones, into a table of `vocab` rows.  An id outside
+ * of it reads nothing: its row of `out` is NaN.
+ * Its gradient: dtable[v] = scale * the sum of dy[t] over the tokens whose id is v, in their order; rows without tokens are zero, and so is row `skip` (-1:
+ * none).  All of dtable is written.  Ids outside the table are left out. */
+int muon_hip_embedding(const void* ids, int wide_ids, int tokens, const void* table, long table_row, int vocab, int n, int dtype, double scale,
+                       void* out, void* stream);
+long muon_hip_embedding_grad_workspace(int tokens, int vocab, int n, int dtype);
+int muon_hip_embedding_grad(const void* ids, int wide_ids, int tokens, const void* dy, long dy_row, int vocab, int n, int dtype, double scale, int skip,
+                            void* dtable, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = residual + (x / (1 - P) where a value is kept, 0 where it is dropped), of `count` values back to back; P is p in whole 2^-32.  residual may be null; y may
+ * be x or the residual.  Value i is dropped where u < P * 2^32: u is a number of 32 bits whose upper half is half i % 8 (the lower half of a word first) of
+ * the four words of Philox4x32-10 of the counter (i / 8 mod 2^32, i / 2^35, site, 0) and the key (seed mod 2^32, seed / 2^32), and its lower half that
+ * of the counter (.., .., site, 1).  Calls with one seed and site draw the same numbers: the gradient is the call on dy.  seed_at, where not
+ * null, is a 64-bit integer in device memory that is read instead of `seed` when the kernel runs. */
+int muon_hip_dropout(const void* x, const void* residual, void* y, long count, int dtype, double p, unsigned long long seed, const void* seed_at,
+                     unsigned site, void* stream);
 
 /* Shape of the current device as the launchers see it, read from the runtime once per device: compute units
  * (a round of 256x256 tiles is one per compute unit) and XCDs (compute units / 32 on gfx950, whole XCDs per

@@ -12,6 +12,7 @@ from .muon_utils import (  # noqa: F401
     matmul_transpose_assign,
     muon_update,
 )
+from .rows import dropout, embedding, layer_norm, rms_norm  # noqa: F401
 
 __all__ = [
     "Muon",
@@ -20,10 +21,14 @@ __all__ = [
     "adam_update",
     "apply_momentum",
     "apply_scaling",
+    "dropout",
+    "embedding",
     "fast_newtonschulz",
     "gated_linear",
+    "layer_norm",
     "linear",
     "matmul_transpose",
     "matmul_transpose_assign",
     "muon_update",
+    "rms_norm",
 ]

@@ -6,8 +6,9 @@ error: there is no fallback implementation.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
-from ctypes import c_char_p, c_double, c_int, c_long, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_int, c_long, c_size_t, c_uint, c_ulonglong, c_void_p, POINTER
 
 import torch
 
@@ -22,7 +23,8 @@ CFG_AUTO, CFG_128_PIPE, CFG_256_PIPE, CFG_256_PINGPONG, CFG_128_PINGPONG, CFG_25
 GEMM_CONFIGS = list(range(4))
 K_MOMENTUM, K_NORMALIZE, K_SYRK, K_SYMPOLY, K_BX, K_UPDATE, K_ADAMW, K_ADAMW_MULTI, K_GRAD_NORM, K_CLIP_SCALE = range(10)
 KERNEL_NAMES = ["momentum_norm", "normalize", "syrk", "sympoly", "bx_axpy", "apply_update", "adamw", "adamw_multi",
-                "grad_norm", "clip_scale", "bx_axpy_update", "small_chain", "flow_chain", "product", "act_grad"]
+                "grad_norm", "clip_scale", "bx_axpy_update", "small_chain", "flow_chain", "product", "act_grad", "norm", "norm_grad", "embedding",
+                "embedding_grad", "dropout"]
 MULTI_CHUNK = 16384  # MUON_HIP_MULTI_CHUNK
 STATIC_MAX_CHUNKS = 1 << 20  # MUON_HIP_STATIC_MAX_CHUNKS
 PPX_COUNTER_BYTES = 576  # MUON_HIP_PPX_COUNTER_BYTES
@@ -70,6 +72,25 @@ class ProductRoute(ctypes.Structure):
 
     _fields_ = [("tile", c_int), ("parts", c_int), ("a", c_int), ("b", c_int), ("groups", c_long), ("threads", c_int),
                 ("copies", c_long)]
+
+
+NORM_LAYER, NORM_RMS = range(2)
+
+
+class Norm(ctypes.Structure):
+    """muon_hip_norm"""
+
+    _fields_ = [("kind", c_int), ("dtype", c_int), ("rows", c_int), ("n", c_int), ("x", c_void_p), ("x_row", c_long), ("residual", c_void_p),
+                ("res_row", c_long), ("weight", c_void_p), ("bias", c_void_p), ("eps", c_double), ("y", c_void_p), ("sum", c_void_p),
+                ("stats", c_void_p)]
+
+
+class NormGrad(ctypes.Structure):
+    """muon_hip_norm_grad"""
+
+    _fields_ = [("kind", c_int), ("dtype", c_int), ("rows", c_int), ("n", c_int), ("dy", c_void_p), ("dy_row", c_long), ("s", c_void_p),
+                ("s_row", c_long), ("ds", c_void_p), ("ds_row", c_long), ("weight", c_void_p), ("stats", c_void_p), ("dx", c_void_p),
+                ("dweight", c_void_p), ("dbias", c_void_p)]
 
 
 # name -> (restype, argtypes); mirrors include/muon_hip.h one to one
@@ -124,6 +145,14 @@ SIGNATURES = {
     "muon_hip_route_product": (c_int, [c_void_p, c_int, c_void_p]),
     "muon_hip_act_grad_partials": (c_long, [c_int, c_int]),
     "muon_hip_act_grad": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_long] + [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 2),
+    "muon_hip_norm_run": (c_int, [c_void_p] * 2),
+    "muon_hip_norm_grad_workspace": (c_long, [c_void_p]),
+    "muon_hip_norm_grad_run": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "muon_hip_embedding": (c_int, [c_void_p, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_double, c_void_p, c_void_p]),
+    "muon_hip_embedding_grad_workspace": (c_long, [c_int] * 4),
+    "muon_hip_embedding_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_double, c_int, c_void_p, c_void_p, c_size_t,
+                                        c_void_p]),
+    "muon_hip_dropout": (c_int, [c_void_p] * 3 + [c_long, c_int, c_double, c_ulonglong, c_void_p, c_uint, c_void_p]),
     "muon_hip_device_shape": (c_int, [POINTER(c_int), POINTER(c_int)]),
     "muon_hip_timing_reserve": (c_int, [c_long]),
     "muon_hip_timing_untimed": (c_long, []),
@@ -174,25 +203,39 @@ def scan():
     return _scan
 
 
+def _load(name: str):
+    """A native module of autograd functions."""
+    lib()  # a library that is missing is reported as such
+    try:
+        module = importlib.import_module("." + name, __package__)
+    except ImportError as e:
+        raise MuonHipError(f"the module lmms_engine_amd.{name} cannot be loaded ({e}): build it with `python -m lmms_engine_amd.build`") from e
+    of = getattr(module, "torch_version", "of another kind")
+    if of != torch.__version__:  # as for _scan
+        raise MuonHipError(f"lmms_engine_amd.{name} was built for torch {of}, this is {torch.__version__}: "
+                           "build it again with `python -m lmms_engine_amd.build`")
+    module.set_error(MuonHipError)
+    return module
+
+
 _layers = None
+_rows = None
 
 
 def layers():
     """The native form of linear and gated_linear (csrc/layers.cpp)."""
     global _layers
     if _layers is None:
-        lib()  # a library that is missing is reported as such
-        try:
-            from . import _layers as module
-        except ImportError as e:
-            raise MuonHipError(f"the module lmms_engine_amd._layers cannot be loaded ({e}): build it with `python -m lmms_engine_amd.build`") from e
-        of = getattr(module, "torch_version", "of another kind")
-        if of != torch.__version__:  # as for _scan
-            raise MuonHipError(f"lmms_engine_amd._layers was built for torch {of}, this is {torch.__version__}: "
-                               "build it again with `python -m lmms_engine_amd.build`")
-        module.set_error(MuonHipError)
-        _layers = module
+        _layers = _load("_layers")
     return _layers
+
+
+def rows():
+    """The native form of embedding, layer_norm, rms_norm and dropout (csrc/rows.cpp)."""
+    global _rows
+    if _rows is None:
+        _rows = _load("_rows")
+    return _rows
 
 
 def check(rc: int, what: str = "") -> None:

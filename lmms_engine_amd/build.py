@@ -14,7 +14,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmuon_hip.so")
-SOURCES = ["gemm_nt.hip", "elementwise.hip", "small_chain.hip", "multi_tensor.hip", "product.hip", "api.hip"]
+SOURCES = ["gemm_nt.hip", "elementwise.hip", "small_chain.hip", "multi_tensor.hip", "product.hip", "rows.hip", "api.hip"]
 # Measurement kernels (MFMA-only loops) for the benchmark's operand-power legs: a library of their own, no part of the product.
 PROBE_LIB = os.path.join(HERE, "libmuon_probe.so")
 PROBE_SOURCES = ["probe.hip"]
@@ -23,6 +23,8 @@ PROBE_SOURCES = ["probe.hip"]
 SCAN_LIB = os.path.join(HERE, "_scan" + sysconfig.get_config_var("EXT_SUFFIX"))
 # linear and gated_linear between torch and the library: host code too, under the same conditions, linked against the library beside it.
 LAYERS_LIB = os.path.join(HERE, "_layers" + sysconfig.get_config_var("EXT_SUFFIX"))
+# embedding, layer_norm, rms_norm and dropout, in the same way
+ROWS_LIB = os.path.join(HERE, "_rows" + sysconfig.get_config_var("EXT_SUFFIX"))
 # Packed-fp32 VALU forms stay off for every device function.
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -80,16 +82,16 @@ def _build_scan(verbose):
     _build_module("scan.cpp", SCAN_LIB, "SCAN_TORCH_VERSION", [], verbose)
 
 
-def _build_layers(hipcc, verbose):
+def _build_functions(source, out, define, hipcc, verbose):
     rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc)))
     flags = ["-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-isystem{os.path.join(rocm, 'include')}", f"-L{HERE}", "-l:" + os.path.basename(LIB),
              "-Wl,-rpath,$ORIGIN", "-lc10_hip"]
-    _build_module("layers.cpp", LAYERS_LIB, "LAYERS_TORCH_VERSION", flags, verbose)
+    _build_module(source, out, define, flags, verbose)
 
 
 def built() -> bool:
     """Whether everything that the package loads is there."""
-    return all(os.path.exists(p) for p in (LIB, SCAN_LIB, LAYERS_LIB))
+    return all(os.path.exists(p) for p in (LIB, SCAN_LIB, LAYERS_LIB, ROWS_LIB))
 
 
 def build_library(verbose: bool = False) -> str:
@@ -99,7 +101,8 @@ def build_library(verbose: bool = False) -> str:
     _build_scan(verbose)
     _compile_and_link(PROBE_SOURCES, PROBE_LIB, hipcc, verbose)
     lib = _compile_and_link(SOURCES, LIB, hipcc, verbose)
-    _build_layers(hipcc, verbose)
+    _build_functions("layers.cpp", LAYERS_LIB, "LAYERS_TORCH_VERSION", hipcc, verbose)
+    _build_functions("rows.cpp", ROWS_LIB, "ROWS_TORCH_VERSION", hipcc, verbose)
     return lib
 
 

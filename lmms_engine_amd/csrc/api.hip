@@ -1,5 +1,6 @@
 // C ABI of libmuon_hip.so (declared in include/muon_hip.h): argument checks, workspace
 // partitioning, the grouped launch sequence of one Muon step, and per-kernel event timing.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <algorithm>
@@ -16,6 +17,7 @@
 #include "gemm_nt.h"
 #include "multi_tensor.h"
 #include "product.h"
+#include "rows.h"
 #include "small_chain.h"
 
 namespace {
@@ -1167,6 +1169,130 @@ int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d
     const ActGradArgs a{dtype, m, n, factors, dy, {d0, d1}, {dz0, dz1}, pitch, {db0, db1}, partials};
     hipError_t e = launch_act_grad(a, s);
     return e == hipSuccess ? 0 : hip_fail(e, "act_grad launch");
+}
+
+// ---- rows of layers ---------------------------------------------------------------------------
+namespace {
+constexpr int kMostColumns = 0x7fffffff - (1 << 20);  // indexes step beyond a row by less than that
+
+int check_sizes(int dtype, int rows, int n) {
+    if (!dtype_ok(dtype) || rows < 0 || n < 0) return fail(MUON_HIP_EINVAL, "bad dtype or size");
+    if (n > kMostColumns) return fail(MUON_HIP_ESHAPE, "rows of %d values: %d are the most", n, kMostColumns);
+    return 0;
+}
+bool rows_overlap(const void* p, long row, int rows, int n) { return p && rows > 1 && row < n; }
+
+int check_norm_grad(const muon_hip_norm_grad* p) {
+    if (!p) return fail(MUON_HIP_EINVAL, "null norm");
+    if (p->kind != MUON_HIP_NORM_LAYER && p->kind != MUON_HIP_NORM_RMS) return fail(MUON_HIP_EINVAL, "kind %d of norm", p->kind);
+    if (int rc = check_sizes(p->dtype, p->rows, p->n)) return rc;
+    if (p->rows == 0 || p->n == 0) return 0;
+    if (!p->dy || ((p->dx || p->dweight) && (!p->s || !p->stats))) return fail(MUON_HIP_EINVAL, "null gradient, input or statistics");
+    if (rows_overlap(p->dy, p->dy_row, p->rows, p->n) || rows_overlap(p->s, p->s_row, p->rows, p->n) || rows_overlap(p->ds, p->ds_row, p->rows, p->n))
+        return fail(MUON_HIP_EINVAL, "rows of %d values that overlap", p->n);
+    return 0;
+}
+long norm_grad_bytes(const muon_hip_norm_grad* p, int cus) {
+    return (p->dweight != nullptr) + (p->dbias != nullptr) == 0 ? 0 : ((p->dweight != nullptr) + (p->dbias != nullptr)) * norm_grad_groups(*p, cus) * p->n * 4;
+}
+
+int check_embedding(const void* ids, int tokens, const void* rows, long pitch, int count, int vocab, int n, int dtype, double scale) {
+    if (int rc = check_sizes(dtype, tokens, n)) return rc;
+    if (vocab < 0 || vocab == 0x7fffffff) return fail(MUON_HIP_EINVAL, "a table of %d rows", vocab);
+    if (tokens > 0 && n > 0 && (!ids || (!rows && count > 0))) return fail(MUON_HIP_EINVAL, "null ids or rows");
+    if (rows_overlap(rows, pitch, count, n)) return fail(MUON_HIP_EINVAL, "rows of %d values that overlap", n);
+    return 0;
+}
+}  // namespace
+
+int muon_hip_norm_run(const muon_hip_norm* p, void* stream) {
+    if (!p) return fail(MUON_HIP_EINVAL, "null norm");
+    if (p->kind != MUON_HIP_NORM_LAYER && p->kind != MUON_HIP_NORM_RMS) return fail(MUON_HIP_EINVAL, "kind %d of norm", p->kind);
+    if (int rc = check_sizes(p->dtype, p->rows, p->n)) return rc;
+    if (p->kind == MUON_HIP_NORM_RMS && p->bias) return fail(MUON_HIP_EINVAL, "an RMS norm has no bias");
+    if (!(p->eps >= 0)) return fail(MUON_HIP_EINVAL, "eps is %g", p->eps);
+    if (p->rows == 0 || p->n == 0) return 0;
+    if (!p->x || !p->y) return fail(MUON_HIP_EINVAL, "null input or result");
+    if (!p->residual != !p->sum) return fail(MUON_HIP_EINVAL, "a residual and the sum with it come together");
+    if (rows_overlap(p->x, p->x_row, p->rows, p->n) || rows_overlap(p->residual, p->res_row, p->rows, p->n))
+        return fail(MUON_HIP_EINVAL, "rows of %d values that overlap", p->n);
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_NORM, s);
+    hipError_t e = launch_norm(*p, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "norm launch");
+}
+
+long muon_hip_norm_grad_workspace(const muon_hip_norm_grad* p) {
+    if (int rc = check_norm_grad(p)) return rc;
+    MachineShape ms;
+    if (hipError_t e = machine_shape(ms); e != hipSuccess) return hip_fail(e, "device attributes"), (long)MUON_HIP_EINVAL;
+    return norm_grad_bytes(p, ms.cus);
+}
+
+int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_norm_grad(p)) return rc;
+    if (p->n == 0 || (p->rows == 0 && !p->dweight && !p->dbias)) return 0;
+    MachineShape ms;
+    if (hipError_t e = machine_shape(ms); e != hipSuccess) return hip_fail(e, "device attributes");
+    const long bytes = norm_grad_bytes(p, ms.cus);
+    if (bytes > 0) {
+        if (int rc = check_ws(workspace)) return rc;
+        if ((size_t)bytes > workspace_bytes) return fail(MUON_HIP_EINVAL, "the workspace has %zu bytes, the sums need %ld", workspace_bytes, bytes);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_NORM_GRAD, s);
+    hipError_t e = launch_norm_grad(*p, (float*)workspace, ms.cus, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "norm_grad launch");
+}
+
+int muon_hip_embedding(const void* ids, int wide_ids, int tokens, const void* table, long table_row, int vocab, int n, int dtype, double scale,
+                       void* out, void* stream) {
+    if (int rc = check_embedding(ids, tokens, table, table_row, vocab, vocab, n, dtype, scale)) return rc;
+    if (tokens == 0 || n == 0) return 0;
+    if (!out) return fail(MUON_HIP_EINVAL, "null result");
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_EMBEDDING, s);
+    hipError_t e = launch_embedding(EmbeddingArgs{ids, wide_ids, tokens, vocab, n, dtype, (float)scale, table, table_row, out, -1}, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "embedding launch");
+}
+
+long muon_hip_embedding_grad_workspace(int tokens, int vocab, int n, int dtype) {
+    if (int rc = check_sizes(dtype, tokens, n)) return rc;
+    if (vocab < 0 || vocab == 0x7fffffff) return fail(MUON_HIP_EINVAL, "a table of %d rows", vocab);
+    return embedding_grad_workspace(tokens, vocab, n, dtype);
+}
+
+int muon_hip_embedding_grad(const void* ids, int wide_ids, int tokens, const void* dy, long dy_row, int vocab, int n, int dtype, double scale, int skip,
+                            void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_embedding(ids, tokens, dy, dy_row, tokens, vocab, n, dtype, scale)) return rc;
+    if (skip < -1 || skip >= vocab) return fail(MUON_HIP_EINVAL, "row %d of a table of %d is to be left out", skip, vocab);
+    if (vocab == 0 || n == 0) return 0;
+    if (!dtable) return fail(MUON_HIP_EINVAL, "null result");
+    const long bytes = embedding_grad_workspace(tokens, vocab, n, dtype);
+    if (bytes > 0) {
+        if (int rc = check_ws(workspace)) return rc;
+        if ((size_t)bytes > workspace_bytes) return fail(MUON_HIP_EINVAL, "the workspace has %zu bytes, the gradient needs %ld", workspace_bytes, bytes);
+    }
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_EMBEDDING_GRAD, s);
+    hipError_t e = launch_embedding_grad(EmbeddingArgs{ids, wide_ids, tokens, vocab, n, dtype, (float)scale, dy, dy_row, dtable, skip}, workspace, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "embedding_grad launch");
+}
+
+int muon_hip_dropout(const void* x, const void* residual, void* y, long count, int dtype, double p, unsigned long long seed, const void* seed_at,
+                     unsigned site, void* stream) {
+    if (!dtype_ok(dtype) || count < 0) return fail(MUON_HIP_EINVAL, "bad dtype or size");
+    if (!(p >= 0 && p <= 1)) return fail(MUON_HIP_EINVAL, "p is %g: a share from 0 to 1 is wanted", p);
+    if (count == 0) return 0;
+    if (!x || !y) return fail(MUON_HIP_EINVAL, "null input or result");
+    const unsigned long long limit = (unsigned long long)nearbyint(p * 0x1p32);
+    const double kept = 0x1p32 - (double)limit;
+    hipStream_t s = (hipStream_t)stream;
+    Timed t(MUON_HIP_K_DROPOUT, s);
+    const DropoutArgs a{x, residual, y, count, dtype, (unsigned)(limit >> 16), (unsigned)(limit & 0xffff), kept > 0 ? (float)(0x1p32 / kept) : 0.f,
+                        seed, (const unsigned long long*)seed_at, site};
+    hipError_t e = launch_dropout(a, s);
+    return e == hipSuccess ? 0 : hip_fail(e, "dropout launch");
 }
 
 int muon_hip_device_shape(int* compute_units, int* xcds) {

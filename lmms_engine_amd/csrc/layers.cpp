@@ -4,50 +4,10 @@
 //
 // Each function takes calls in which nothing needs a decision: plain tensors of one type on one GPU, of shapes that fit.  For anything else
 // it returns None before it has done anything, and the caller says what is wrong.  What a thread does is looked at here: refuse_recording.
-#define PY_SSIZE_T_CLEAN
-#include <ATen/DeviceGuard.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include "../../include/muon_hip.h"
+#define FUNCTIONS_ARE "linear and gated_linear"
+#include "functions.h"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-PyObject* error_type = nullptr;  // MuonHipError
-
-[[noreturn]] void raise(const char* what, long code) {
-    const std::string text = std::string(what) + " failed (code " + std::to_string(code) + "): " + muon_hip_last_error();
-    python_error e;
-    {
-        pybind11::gil_scoped_acquire gil;
-        PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, text.c_str());
-        e.persist();
-    }
-    throw e;
-}
-
-// Tools that record the torch operations of a function, to run them again on other tensors, or that run it on tensors without values, see the
-// allocation of a result and none of the launches that fill it: what they made would return memory that nothing has written.
-void refuse_recording() {
-    using c10::impl::TorchDispatchModeKey;
-    bool on = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
-    for (const auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-        on = on || c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
-    TORCH_CHECK_NOT_IMPLEMENTED(!on, "linear and gated_linear cannot be recorded or run on tensors without values: their launches are no torch operations");
-}
-
-int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? MUON_HIP_F32 : MUON_HIP_BF16; }
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream(); }
 
 // ---- products -----------------------------------------------------------------------------------
 
@@ -79,30 +39,11 @@ struct Product : muon_hip_product {
     }
 };
 
-// t without its history, its values where its pointer says
-Tensor bare(const Tensor& t) {
-    if (!t.defined()) return t;
-    const Tensor d = t.detach();
-    return d.is_neg() ? d.resolve_neg() : d;
-}
-Tensor dense(const Tensor& t) { return t.defined() ? bare(t).contiguous() : t; }
-int64_t rows_of(const Tensor& t) {
-    int64_t m = 1;
-    for (int64_t d = 0; d + 1 < t.dim(); ++d) m *= t.size(d);
-    return m;
-}
 // t as a matrix of the rows of its last dimension: a view where there is one
 Tensor matrix(const Tensor& t) {
     const Tensor b = bare(t);
     return b.dim() == 2 ? b : b.reshape({rows_of(b), b.size(-1)});
 }
-Tensor result(const Tensor& x, int64_t n) {
-    auto shape = x.sizes().vec();
-    shape.back() = n;
-    return at::empty(shape, x.options());
-}
-const void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
 // Memory for a factor that the backward pass multiplies by, in the form that the library keeps it in.
 Tensor factor(const Tensor& like, int64_t m, int64_t n) {
     return at::empty({muon_hip_product_aux_bytes(dtype_of(like), (int)m, (int)n)}, like.options().dtype(at::kByte));
@@ -181,33 +122,9 @@ Incoming act_grad(const Tensor& dy_, int factors, const Tensor& d0, const Tensor
     return g;
 }
 
-// Stands for the second derivatives that there are none of: whoever comes through here on the way to an input is told so.
-struct Once : torch::autograd::Node {
-    variable_list apply(variable_list&&) override {
-        TORCH_CHECK(false, "linear and gated_linear can be differentiated once: their backward pass has none of its own");
-    }
-};
-// Gradient `g` depends on the inputs whose bits are set in `on` (positions of `edges`; those that need no gradient have no edge) and on
-// the incoming gradient.  Where one of them is differentiated, so would g be: its history leads to all of them, so that a loss that g is a
-// part of raises for each of them and loses no term, and to no other.
-void close_history(Tensor& g, unsigned on, const torch::autograd::edge_list& edges, const Tensor& dy) {
-    if (!g.defined()) return;
-    torch::autograd::edge_list next;
-    for (size_t i = 0; i < edges.size(); ++i)
-        if ((on >> i & 1) && edges[i].is_valid()) next.push_back(edges[i]);
-    if (dy.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(dy));
-    if (next.empty()) return;
-    const auto node = std::shared_ptr<Once>(new Once(), torch::autograd::deleteNode);
-    node->set_next_edges(std::move(next));
-    torch::autograd::impl::set_gradient_edge(g, {node, node->add_input_metadata(g)});
-}
 // The second derivative of an activation without a curve is zero.
 bool curved(int act) { return act != MUON_HIP_ACT_NONE && act != MUON_HIP_ACT_RELU; }
 
-// Tensors that a call may lack travel as optionals, and a context numbers the tensors that there are: `has` holds a bit for each of the two.
-typedef std::optional<Tensor> Maybe;
-Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
-Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
 void note(AutogradContext* ctx, const Maybe& a, const Maybe& b, int64_t act) {
     ctx->saved_data["has"] = (int64_t)(a.has_value() + 2 * b.has_value());
     ctx->saved_data["act"] = act;
@@ -281,9 +198,9 @@ struct Linear : torch::autograd::Function<Linear> {
             enum { X = 1, W = 2, B = 4 };
             const auto edges = more.edges(2);
             const unsigned dz = curved((int)ctx->saved_data["act"].toInt()) ? X | W | B : 0;
-            close_history(grads[0], dz | W, edges, dy);
-            close_history(grads[1], dz | X, edges, dy);
-            close_history(grads[2], dz, edges, dy);
+            close_history(grads[0], dz | W, edges, {dy});
+            close_history(grads[1], dz | X, edges, {dy});
+            close_history(grads[2], dz, edges, {dy});
         }
         return grads;
     }
@@ -345,11 +262,11 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
             const auto edges = more.edges(3);
             const unsigned of_g = X | WG | BG, of_u = X | WU | BU;
             const unsigned dg = of_u | (curved((int)ctx->saved_data["act"].toInt()) ? of_g : 0), du = of_g;
-            close_history(grads[0], dg | du | WG | WU, edges, dh);
-            close_history(grads[1], dg | X, edges, dh);
-            close_history(grads[2], du | X, edges, dh);
-            close_history(grads[3], dg, edges, dh);
-            close_history(grads[4], du, edges, dh);
+            close_history(grads[0], dg | du | WG | WU, edges, {dh});
+            close_history(grads[1], dg | X, edges, {dh});
+            close_history(grads[2], du | X, edges, {dh});
+            close_history(grads[3], dg, edges, {dh});
+            close_history(grads[4], du, edges, {dh});
         }
         return grads;
     }
@@ -357,15 +274,6 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 
 // ---- calls ------------------------------------------------------------------------------------
 
-// A plain tensor on a GPU, of x's type and device, whose memory is there.
-bool plain(PyObject* o, const Tensor* x) {
-    if (!THPVariable_CheckExact(o)) return false;
-    const Tensor& t = THPVariable_Unpack(o);
-    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->is_python_dispatch()) return false;
-    if (t.has_storage() && t.numel() > 0 && !t.storage().data()) return false;
-    if (x) return t.scalar_type() == x->scalar_type() && t.device() == x->device();
-    return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
-}
 // The tensors of a call, None as an undefined one; false where something has to be decided.
 bool unpack(PyObject* const* args, int count, int needed, Tensor* out) {
     if (!plain(args[0], nullptr)) return false;
@@ -383,14 +291,6 @@ bool fits(const Tensor& x, const Tensor& w, const Tensor& b) {
     return x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) <= most && w.size(1) <= most && rows_of(x) <= most &&
            (!b.defined() || (b.dim() == 1 && b.size(0) == w.size(0)));
 }
-// Whether the call has a history; a tangent of forward mode counts too, so that autograd refuses it.
-bool differentiated(const Tensor* t, int count) {
-    const bool backward = at::GradMode::is_enabled();
-    for (int i = 0; i < count; ++i)
-        if (t[i].defined() && ((backward && t[i].requires_grad()) || t[i]._fw_grad(0).defined())) return true;
-    return false;
-}
-
 // linear(x, weight, bias or None, residual or None, activation code)
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
@@ -430,14 +330,6 @@ PyObject* gated_linear(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
 }
-// set_error(type): what a refusal of the library is raised as
-PyObject* set_error(PyObject*, PyObject* type) {
-    Py_INCREF(type);
-    Py_XDECREF(error_type);
-    error_type = type;
-    Py_RETURN_NONE;
-}
-
 PyMethodDef methods[] = {{"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
                          {"gated_linear", (PyCFunction)(void (*)(void))gated_linear, METH_FASTCALL, nullptr},
                          {"set_error", set_error, METH_O, nullptr},

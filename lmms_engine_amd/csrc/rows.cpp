@@ -1,0 +1,324 @@
+// embedding, layer_norm, rms_norm and dropout as differentiable functions of torch tensors, in native code for the reason that layers.cpp gives.
+//
+// Each function takes calls in which nothing needs a decision and returns None for anything else before it has done anything; the caller says
+// what is wrong.
+#define FUNCTIONS_ARE "embedding, layer_norm, rms_norm and dropout"
+#include "functions.h"
+
+namespace {
+
+constexpr int64_t MOST = 0x7fffffff;
+
+// The rows of t's last dimension, back to back within themselves: where they lie, if that is so, else a copy.
+Tensor lines(const Tensor& t) {
+    if (!t.defined()) return t;
+    Tensor b = bare(t);
+    if (b.dim() != 2) b = b.reshape({rows_of(b), b.size(-1)});
+    return (b.size(1) > 1 && b.stride(1) != 1) || (b.size(0) > 1 && b.stride(0) < b.size(1)) ? b.contiguous() : b;
+}
+// The places of the tensors of a context: `always` of them, then those of `count` optional ones that there are.
+struct Places {
+    AutogradContext* ctx;
+    int at[4];
+    Places(AutogradContext* c, int always, int count) : ctx(c) {
+        const int64_t has = ctx->saved_data["has"].toInt();
+        for (int i = 0, next = always; i < count; ++i) at[i] = has >> i & 1 ? next++ : -1;
+    }
+    bool wanted(int i) const { return at[i] >= 0 && ctx->needs_input_grad(at[i]); }
+    torch::autograd::Edge edge(int i) const { return at[i] >= 0 ? torch::autograd::get_current_node()->next_edge(at[i]) : torch::autograd::Edge(); }
+};
+bool trained(const Maybe& t) { return t && t->requires_grad(); }
+
+// ---- norms --------------------------------------------------------------------------------------
+
+struct Normed {
+    Tensor y, sum, stats;
+};
+Normed norm_forward(int kind, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, double eps, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x2 = lines(x), r2 = lines(r), w1 = dense(w), b1 = dense(b);
+    Normed f;
+    f.y = result(x, x.size(-1));
+    if (r.defined()) f.sum = result(x, x.size(-1));
+    if (keep) f.stats = at::empty({kind == MUON_HIP_NORM_LAYER ? 2 : 1, x2.size(0)}, x.options().dtype(at::kFloat));
+    muon_hip_norm p{};
+    p.kind = kind;
+    p.dtype = dtype_of(x);
+    p.rows = (int)x2.size(0);
+    p.n = (int)x2.size(1);
+    p.x = x2.data_ptr();
+    p.x_row = x2.stride(0);
+    if (r.defined()) {
+        p.residual = r2.data_ptr();
+        p.res_row = r2.stride(0);
+        p.sum = f.sum.data_ptr();
+    }
+    p.weight = pointer(w1);
+    p.bias = pointer(b1);
+    p.eps = eps;
+    p.y = f.y.data_ptr();
+    p.stats = (float*)pointer(f.stats);
+    if (const int rc = muon_hip_norm_run(&p, stream_of(x))) raise("norm", rc);
+    return f;
+}
+
+// Kept is what the gradients that can be asked for read: the normalised rows' input for all but the bias', the weight for the input's.
+struct Norm : torch::autograd::Function<Norm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& w, const Maybe& b, const Maybe& r, int64_t kind, double eps) {
+        const bool for_x = x.requires_grad() || trained(r), for_w = trained(w);
+        const Normed f = norm_forward((int)kind, x, given(w), given(b), given(r), eps, for_x || for_w);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({for_x || for_w ? (r ? f.sum : x) : Tensor(), for_x ? given(w) : Tensor(), f.stats});
+        ctx->saved_data["has"] = (int64_t)(w.has_value() + 2 * b.has_value() + 4 * r.has_value());
+        ctx->saved_data["kind"] = kind;
+        if (!r) return {f.y};
+        if (!for_x) ctx->mark_non_differentiable({f.sum});
+        return {f.y, f.sum};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        refuse_recording();
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &s = saved[0], &w = saved[1], &stats = saved[2], &dy = incoming[0], ds = incoming.size() > 1 ? incoming[1] : Tensor();
+        const Places more(ctx, 1, 3);
+        const bool want_x = ctx->needs_input_grad(0), want_r = more.wanted(2), want_w = more.wanted(0), want_b = more.wanted(1);
+        variable_list grads(6);
+        Tensor dx;
+        if (!dy.defined() && !ds.defined()) return grads;
+        const Tensor& like = dy.defined() ? dy : ds;
+        {
+            const at::AutoGradMode off(false);
+            const c10::DeviceGuard guard(like.device());
+            const int64_t n = like.size(-1);
+            if (!dy.defined()) {  // of the sum alone
+                if (want_w) grads[1] = at::zeros({n}, like.options());
+                if (want_b) grads[2] = at::zeros({n}, like.options());
+            } else if (want_x || want_r || want_w || want_b) {
+                const Tensor dy2 = lines(dy), s2 = lines(s), ds2 = lines(ds), w1 = dense(w);
+                muon_hip_norm_grad p{};
+                p.kind = (int)ctx->saved_data["kind"].toInt();
+                p.dtype = dtype_of(like);
+                p.rows = (int)dy2.size(0);
+                p.n = (int)n;
+                p.dy = dy2.data_ptr();
+                p.dy_row = dy2.stride(0);
+                if (s.defined()) {  // (not where the bias alone is trained)
+                    p.s = s2.data_ptr();
+                    p.s_row = s2.stride(0);
+                    p.stats = (const float*)stats.data_ptr();
+                }
+                if (ds.defined()) {
+                    p.ds = ds2.data_ptr();
+                    p.ds_row = ds2.stride(0);
+                }
+                p.weight = pointer(w1);
+                if (want_x || want_r) p.dx = (dx = result(like, n)).data_ptr();
+                if (want_w) p.dweight = (grads[1] = at::empty({n}, like.options())).data_ptr();
+                if (want_b) p.dbias = (grads[2] = at::empty({n}, like.options())).data_ptr();
+                const long need = muon_hip_norm_grad_workspace(&p);
+                if (need < 0) raise("norm_grad", need);
+                Tensor ws;
+                if (need > 0) ws = at::empty({need}, like.options().dtype(at::kByte));
+                if (const int rc = muon_hip_norm_grad_run(&p, need > 0 ? ws.data_ptr() : nullptr, (size_t)need, stream_of(like))) raise("norm_grad", rc);
+            }
+        }
+        if (at::GradMode::is_enabled()) {
+            enum { X = 1, W = 2, R = 4 };
+            const torch::autograd::edge_list edges{torch::autograd::get_current_node()->next_edge(0), more.edge(0), more.edge(2)};
+            close_history(dx, X | W | R, edges, {dy, ds});
+            close_history(grads[1], dy.defined() ? X | R : 0, edges, {dy});
+            close_history(grads[2], 0, edges, {dy});
+        }
+        if (!dy.defined()) dx = ds;  // history and all
+        if (want_x) grads[0] = dx;
+        if (want_r) grads[3] = dx;
+        return grads;
+    }
+};
+
+// ---- embedding ------------------------------------------------------------------------------------
+
+Tensor embedding_forward(const Tensor& weight, const Tensor& ids, double scale) {
+    const c10::DeviceGuard guard(weight.device());
+    const Tensor w2 = lines(weight), i1 = ids.contiguous();
+    auto shape = ids.sizes().vec();
+    shape.push_back(weight.size(1));
+    const Tensor y = at::empty(shape, weight.options());
+    if (const int rc = muon_hip_embedding(i1.data_ptr(), ids.scalar_type() == at::kLong, (int)ids.numel(), w2.data_ptr(), w2.stride(0), (int)w2.size(0),
+                                          (int)w2.size(1), dtype_of(weight), scale, y.data_ptr(), stream_of(weight)))
+        raise("embedding", rc);
+    return y;
+}
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t skip) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["vocab"] = weight.size(0);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["skip"] = skip;
+        return embedding_forward(weight, ids, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        refuse_recording();
+        const Tensor ids = ctx->get_saved_variables()[0], &dy = incoming[0];
+        variable_list grads(4);
+        if (!ctx->needs_input_grad(0)) return grads;
+        {
+            const at::AutoGradMode off(false);
+            const c10::DeviceGuard guard(dy.device());
+            const int64_t vocab = ctx->saved_data["vocab"].toInt(), n = dy.size(-1);
+            const Tensor dy2 = lines(dy), i1 = ids.contiguous();
+            grads[0] = at::empty({vocab, n}, dy.options());
+            const int tokens = (int)ids.numel(), dtype = dtype_of(dy);
+            const long need = muon_hip_embedding_grad_workspace(tokens, (int)vocab, (int)n, dtype);
+            if (need < 0) raise("embedding_grad", need);
+            Tensor ws;
+            if (need > 0) ws = at::empty({need}, dy.options().dtype(at::kByte));
+            if (const int rc = muon_hip_embedding_grad(i1.data_ptr(), ids.scalar_type() == at::kLong, tokens, dy2.data_ptr(), dy2.stride(0), (int)vocab, (int)n,
+                                                       dtype, ctx->saved_data["scale"].toDouble(), (int)ctx->saved_data["skip"].toInt(),
+                                                       grads[0].data_ptr(), need > 0 ? ws.data_ptr() : nullptr, (size_t)need, stream_of(dy)))
+                raise("embedding_grad", rc);
+        }
+        if (at::GradMode::is_enabled()) close_history(grads[0], 0, {}, {dy});
+        return grads;
+    }
+};
+
+// ---- dropout --------------------------------------------------------------------------------------
+
+Tensor dropout_forward(const Tensor& x, const Tensor& r, const Tensor& seed_at, double p, int64_t seed, int64_t site) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor x1 = dense(x), r1 = dense(r);
+    const Tensor y = at::empty(x.sizes(), x.options());
+    if (const int rc = muon_hip_dropout(x1.data_ptr(), pointer(r1), y.data_ptr(), x.numel(), dtype_of(x), p, (unsigned long long)seed, pointer(seed_at),
+                                        (unsigned)site, stream_of(x)))
+        raise("dropout", rc);
+    return y;
+}
+struct Dropout : torch::autograd::Function<Dropout> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& r, const Maybe& seed_at, double p, int64_t seed, int64_t site) {
+        if (x.requires_grad()) ctx->save_for_backward({given(seed_at)});
+        ctx->saved_data["has"] = (int64_t)(r.has_value() + 2 * seed_at.has_value());
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["site"] = site;
+        return dropout_forward(x, given(r), given(seed_at), p, seed, site);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list incoming) {
+        refuse_recording();
+        const Tensor& dy = incoming[0];
+        variable_list grads(6);
+        if (ctx->needs_input_grad(0)) {
+            {
+                const at::AutoGradMode off(false);
+                grads[0] = dropout_forward(dy, Tensor(), ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                                           ctx->saved_data["site"].toInt());
+            }
+            if (at::GradMode::is_enabled()) close_history(grads[0], 0, {}, {dy});
+        }
+        if (Places(ctx, 1, 2).wanted(0)) grads[1] = dy;
+        return grads;
+    }
+};
+
+// ---- calls ----------------------------------------------------------------------------------------
+
+// args[i] as an optional tensor of x's type and device; false where something has to be decided.
+bool optional(PyObject* o, const Tensor& x, Tensor& out) {
+    if (o == Py_None) return true;
+    if (!plain(o, &x)) return false;
+    out = THPVariable_Unpack(o);
+    return true;
+}
+
+// norm(kind, x, weight or None, bias or None, residual or None, eps): y, or (y, sum) with a residual
+PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    refuse_recording();
+    if (count != 6 || !plain(args[1], nullptr)) Py_RETURN_NONE;
+    Tensor t[4] = {THPVariable_Unpack(args[1])};
+    for (int i = 1; i < 4; ++i)
+        if (!optional(args[1 + i], t[0], t[i])) Py_RETURN_NONE;
+    const Tensor& x = t[0];
+    if (x.dim() < 1 || x.size(-1) > MOST || rows_of(x) > MOST || (t[3].defined() && t[3].sizes() != x.sizes())) Py_RETURN_NONE;
+    for (int i = 1; i < 3; ++i)
+        if (t[i].defined() && (t[i].dim() != 1 || t[i].size(0) != x.size(-1))) Py_RETURN_NONE;
+    const long kind = PyLong_AsLong(args[0]);
+    const double eps = PyFloat_AsDouble(args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!(eps >= 0)) Py_RETURN_NONE;
+    variable_list out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (differentiated(t, 4)) out = Norm::apply(x, maybe(t[1]), maybe(t[2]), maybe(t[3]), (int64_t)kind, eps);
+        else {
+            const Normed f = norm_forward((int)kind, x, t[1], t[2], t[3], eps, false);
+            out = {f.y, f.sum};
+        }
+    }
+    if (!t[3].defined()) return THPVariable_Wrap(out[0]);
+    PyObject *y = THPVariable_Wrap(out[0]), *sum = y ? THPVariable_Wrap(out[1]) : nullptr, *pair = sum ? PyTuple_Pack(2, y, sum) : nullptr;
+    Py_XDECREF(y);
+    Py_XDECREF(sum);
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+// embedding(ids, weight, scale, id without a gradient or -1)
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    refuse_recording();
+    if (count != 4 || !present(args[0]) || !plain(args[1], nullptr)) Py_RETURN_NONE;
+    const Tensor ids = THPVariable_Unpack(args[0]), weight = THPVariable_Unpack(args[1]);
+    if ((ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || ids.device() != weight.device() || ids.numel() > MOST || weight.dim() != 2 ||
+        weight.size(0) >= MOST || weight.size(1) > MOST)
+        Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[2]);
+    const long skip = PyLong_AsLong(args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        out = differentiated(&weight, 1) ? Embedding::apply(weight, ids, scale, (int64_t)skip) : embedding_forward(weight, ids, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+// dropout(x, residual or None, p, seed: a whole number or a tensor of one, site)
+PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    refuse_recording();
+    if (count != 5 || !plain(args[0], nullptr)) Py_RETURN_NONE;
+    Tensor t[2] = {THPVariable_Unpack(args[0])}, seed_at;
+    if (!optional(args[1], t[0], t[1]) || (t[1].defined() && t[1].sizes() != t[0].sizes())) Py_RETURN_NONE;
+    if (!PyLong_Check(args[3])) {
+        if (!present(args[3])) Py_RETURN_NONE;
+        seed_at = THPVariable_Unpack(args[3]);
+        if (seed_at.scalar_type() != at::kLong || seed_at.numel() != 1 || seed_at.device() != t[0].device()) Py_RETURN_NONE;
+    }
+    const double p = PyFloat_AsDouble(args[2]);
+    const int64_t seed = seed_at.defined() ? 0 : (int64_t)PyLong_AsUnsignedLongLongMask(args[3]);
+    const unsigned long site = PyLong_AsUnsignedLongMask(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!(p >= 0 && p <= 1)) Py_RETURN_NONE;
+    Tensor out;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (differentiated(t, 2)) out = Dropout::apply(t[0], maybe(t[1]), maybe(seed_at), p, seed, (int64_t)site);
+        else out = dropout_forward(t[0], t[1], seed_at, p, seed, (int64_t)site);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {{"norm", (PyCFunction)(void (*)(void))norm, METH_FASTCALL, nullptr},
+                         {"embedding", (PyCFunction)(void (*)(void))embedding, METH_FASTCALL, nullptr},
+                         {"dropout", (PyCFunction)(void (*)(void))dropout, METH_FASTCALL, nullptr},
+                         {"set_error", set_error, METH_O, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_rows", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__rows() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", ROWS_TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
+}
