@@ -1173,7 +1173,7 @@ int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d
 
 // ---- rows of layers ---------------------------------------------------------------------------
 namespace {
-constexpr int kMostColumns = 0x7fffffff - (1 << 20);  // indexes step beyond a row by less than that
+constexpr int kMostColumns = 0x7fffffff - (1 << 20);  // indexes step beyond a row, or a list of ids, by less than that
 
 int check_sizes(int dtype, int rows, int n) {
     if (!dtype_ok(dtype) || rows < 0 || n < 0) return fail(MUON_HIP_EINVAL, "bad dtype or size");
@@ -1196,9 +1196,14 @@ long norm_grad_bytes(const muon_hip_norm_grad* p, int cus) {
     return (p->dweight != nullptr) + (p->dbias != nullptr) == 0 ? 0 : ((p->dweight != nullptr) + (p->dbias != nullptr)) * norm_grad_groups(*p, cus) * p->n * 4;
 }
 
-int check_embedding(const void* ids, int tokens, const void* rows, long pitch, int count, int vocab, int n, int dtype, double scale) {
+int check_table(int tokens, int vocab, int n, int dtype) {
     if (int rc = check_sizes(dtype, tokens, n)) return rc;
+    if (tokens > kMostColumns) return fail(MUON_HIP_ESHAPE, "%d ids: %d are the most", tokens, kMostColumns);
     if (vocab < 0 || vocab == 0x7fffffff) return fail(MUON_HIP_EINVAL, "a table of %d rows", vocab);
+    return 0;
+}
+int check_embedding(const void* ids, int tokens, const void* rows, long pitch, int count, int vocab, int n, int dtype) {
+    if (int rc = check_table(tokens, vocab, n, dtype)) return rc;
     if (tokens > 0 && n > 0 && (!ids || (!rows && count > 0))) return fail(MUON_HIP_EINVAL, "null ids or rows");
     if (rows_overlap(rows, pitch, count, n)) return fail(MUON_HIP_EINVAL, "rows of %d values that overlap", n);
     return 0;
@@ -1247,7 +1252,7 @@ int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t 
 
 int muon_hip_embedding(const void* ids, int wide_ids, int tokens, const void* table, long table_row, int vocab, int n, int dtype, double scale,
                        void* out, void* stream) {
-    if (int rc = check_embedding(ids, tokens, table, table_row, vocab, vocab, n, dtype, scale)) return rc;
+    if (int rc = check_embedding(ids, tokens, table, table_row, vocab, vocab, n, dtype)) return rc;
     if (tokens == 0 || n == 0) return 0;
     if (!out) return fail(MUON_HIP_EINVAL, "null result");
     hipStream_t s = (hipStream_t)stream;
@@ -1257,14 +1262,13 @@ int muon_hip_embedding(const void* ids, int wide_ids, int tokens, const void* ta
 }
 
 long muon_hip_embedding_grad_workspace(int tokens, int vocab, int n, int dtype) {
-    if (int rc = check_sizes(dtype, tokens, n)) return rc;
-    if (vocab < 0 || vocab == 0x7fffffff) return fail(MUON_HIP_EINVAL, "a table of %d rows", vocab);
+    if (int rc = check_table(tokens, vocab, n, dtype)) return rc;
     return embedding_grad_workspace(tokens, vocab, n, dtype);
 }
 
 int muon_hip_embedding_grad(const void* ids, int wide_ids, int tokens, const void* dy, long dy_row, int vocab, int n, int dtype, double scale, int skip,
                             void* dtable, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int rc = check_embedding(ids, tokens, dy, dy_row, tokens, vocab, n, dtype, scale)) return rc;
+    if (int rc = check_embedding(ids, tokens, dy, dy_row, tokens, vocab, n, dtype)) return rc;
     if (skip < -1 || skip >= vocab) return fail(MUON_HIP_EINVAL, "row %d of a table of %d is to be left out", skip, vocab);
     if (vocab == 0 || n == 0) return 0;
     if (!dtable) return fail(MUON_HIP_EINVAL, "null result");

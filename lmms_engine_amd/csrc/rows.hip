@@ -203,34 +203,269 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a) {
         }
     }
 }
-// A workgroup per row of the table, which looks for its tokens among all of them.
-template <typename T>
-__global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingArgs a) {
-    __shared__ int found[256];
-    for (long row = blockIdx.x; row < a.vocab; row += gridDim.x) {
-        for (int j0 = 0; j0 < a.n; j0 += 2048) {
-            const int j = j0 + threadIdx.x * 8;
-            float sum[8] = {};
-            for (long t0 = 0; t0 < a.tokens && row != a.skip; t0 += 256) {
-                const long t = t0 + threadIdx.x;
-                __syncthreads();
-                found[threadIdx.x] = t < a.tokens && id_at(a.ids, a.wide, t) == row;
-                if (!__syncthreads_or(found[threadIdx.x])) continue;
-                for (int i = 0; i < 256; ++i) {
-                    if (!found[i] || j >= a.n) continue;
-                    float v[8];
-                    load8((const T*)a.rows + (t0 + i) * a.pitch + j, left(a.n, j), v);
+// The table's gradient.  The tokens are sorted by id, keeping their order among equal ones, and the sorted tokens cut into chunks of equal length,
+// whatever ids are in them: one id may have most of the tokens, as the placeholders of an image do.
+//   sort_and_clear  one launch: a workgroup sorts up to 8192 tokens in LDS, the others clear the table meanwhile (151936 x 4096 in bf16 is 1.2 GB, which
+//                   takes longer than any of the rest)
+//   merge           joins up to 16 sorted lists, where there are more tokens than that: a token's place is its place in its own list and
+//                   what binary searches in the other ones say
+//   add             a chunk's lanes walk over its tokens: the sum of a run of equal ids is the table's row, or, where the run goes on in a neighbouring
+//                   chunk, one of two rows of fp32 that a chunk has for that
+//   join            adds those up, in their order.
+constexpr int SORT_TOKENS = 8192, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ROUNDS = SORT_TOKENS / SORT_THREADS;
+constexpr int DIGIT_BITS = 7;  // at most; histograms of 128 digits for each of 16 waves
+constexpr int MERGE_LISTS = 16;
+constexpr int CLEAR_BYTES = SORT_THREADS * 64;  // of a workgroup
+
+struct Sorted {
+    int *key, *at;  // ids (vocab: none that counts) in order, and the tokens they are of
+};
+
+// A number for each token, among those with its digit, in the order of tokens; LDS arrays of the workgroup.
+struct SortSpace {
+    uint32_t key[SORT_TOKENS];
+    uint16_t at[SORT_TOKENS];
+    uint32_t count[(1 << DIGIT_BITS) * SORT_WAVES];  // by digit, then by wave
+    uint32_t total[SORT_WAVES];
+};
+static_assert(sizeof(SortSpace) <= 64 * 1024, "two workgroups to a compute unit");
+
+__device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpace& s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int first = blockIdx.x * SORT_TOKENS, count = a.tokens - first < SORT_TOKENS ? a.tokens - first : SORT_TOKENS;
+    const int rounds = (count + SORT_THREADS - 1) / SORT_THREADS;  // of each wave, whose tokens are back to back
+    const int passes = (bits + DIGIT_BITS - 1) / DIGIT_BITS, digit_bits = (bits + passes - 1) / passes;
+    uint32_t key[SORT_ROUNDS], rank[SORT_ROUNDS];
+    uint16_t at[SORT_ROUNDS];
+    for (int r = 0; r < rounds; ++r) {
+        const int i = (wave * rounds + r) * 64 + lane;
+        if (i < count) {
+            const long id = id_at(a.ids, a.wide, (long)first + i);
+            s.key[i] = id >= 0 && id < a.vocab && id != a.skip ? (uint32_t)id : (uint32_t)a.vocab;
+            s.at[i] = (uint16_t)i;
+        }
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * digit_bits, digits = 1 << digit_bits;
+        for (int i = threadIdx.x; i < digits * SORT_WAVES; i += SORT_THREADS) s.count[i] = 0;
+        __syncthreads();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum[e] += v[e];
-                }
+        for (int r = 0; r < SORT_ROUNDS; ++r) {
+            const int i = (wave * rounds + r) * 64 + lane;
+            const bool in = r < rounds && i < count;
+            const uint64_t here = __ballot(in);
+            if (here == 0) continue;
+            key[r] = in ? s.key[i] : 0;
+            at[r] = in ? s.at[i] : (uint16_t)0;
+            const uint32_t d = key[r] >> shift & (digits - 1);
+            uint64_t same = here;
+            for (int b = 0; b < digit_bits; ++b) {
+                const uint64_t set = __ballot(d >> b & 1);
+                same &= d >> b & 1 ? set : ~set;
             }
-            if (j < a.n) {
+            const uint64_t before = same & ((1ull << lane) - 1);
+            uint32_t base = 0;
+            if (in && before == 0) base = atomicAdd(&s.count[d * SORT_WAVES + wave], (uint32_t)__popcll(same));  // the first of them, for all
+            base = __shfl(base, in ? __ffsll((unsigned long long)same) - 1 : lane, 64);
+            rank[r] = base + __popcll(before);
+        }
+        __syncthreads();
+        // places of digits and, within a digit, of waves: sums of what stands before, of as many counts in a row by each thread as there are
+        const int each = (digits * SORT_WAVES + SORT_THREADS - 1) / SORT_THREADS;
+        uint32_t mine = 0;
+        for (int e = 0; e < each; ++e) {
+            const int i = threadIdx.x * each + e;
+            if (i < digits * SORT_WAVES) mine += s.count[i];
+        }
+        uint32_t upto = mine;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
-                store8((T*)a.out + row * a.n + j, left(a.n, j), sum);
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += o;
+        }
+        if (lane == 63) s.total[wave] = upto;
+        __syncthreads();
+        uint32_t place = upto - mine;
+        for (int w = 0; w < wave; ++w) place += s.total[w];
+        for (int e = 0; e < each; ++e) {
+            const int i = threadIdx.x * each + e;
+            if (i < digits * SORT_WAVES) {
+                const uint32_t c = s.count[i];
+                s.count[i] = place;
+                place += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < SORT_ROUNDS; ++r) {
+            const int i = (wave * rounds + r) * 64 + lane;
+            if (r < rounds && i < count) {
+                const uint32_t to = s.count[(key[r] >> shift & (digits - 1)) * SORT_WAVES + wave] + rank[r];
+                s.key[to] = key[r];
+                s.at[to] = at[r];
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < count; i += SORT_THREADS) {
+        out.key[first + i] = (int)s.key[i];
+        out.at[first + i] = first + s.at[i];
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const EmbeddingArgs a, int sorters, int bits, Sorted out) {
+    __shared__ SortSpace space;
+    if ((int)blockIdx.x < sorters) {
+        sort_block(a, bits, out, space);
+        return;
+    }
+    constexpr int PIECE = 16 / sizeof(T);
+    const long values = (long)a.vocab * a.n;
+    for (long b = blockIdx.x - sorters; b * (long)(CLEAR_BYTES / sizeof(T)) < values; b += gridDim.x - sorters) {
+#pragma unroll
+        for (int e = 0; e < CLEAR_BYTES / (SORT_THREADS * 16); ++e) {
+            const long i = b * (long)(CLEAR_BYTES / sizeof(T)) + ((long)e * SORT_THREADS + threadIdx.x) * PIECE;
+            T* p = (T*)a.out + i;
+            if (i + PIECE <= values) *(f32x4_any __attribute__((aligned(2)))*)p = f32x4{0.f, 0.f, 0.f, 0.f};
+            else
+                for (long k = i; k < values; ++k) ((T*)a.out)[k] = (T)0.f;
+        }
+    }
+}
+
+// Lists of `length` sorted tokens, the last one shorter: every 16 of them become one.
+__global__ void __launch_bounds__(256) embedding_merge_kernel(Sorted in, Sorted out, int tokens, int length) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= tokens) return;
+    const int key = in.key[i], own = (int)(i / length);
+    const int group = own / MERGE_LISTS * MERGE_LISTS;
+    const long start = (long)group * length;
+    int lo[MERGE_LISTS], size[MERGE_LISTS];
+#pragma unroll
+    for (int l = 0; l < MERGE_LISTS; ++l) {
+        const long rest = tokens - (start + (long)l * length);
+        lo[l] = 0;
+        size[l] = group + l == own || rest <= 0 ? 0 : rest < length ? (int)rest : length;
+    }
+    // how many of a list stand before: those with a smaller id, and with the same one where the list stands before the own one
+    for (int left = length; left > 0; left >>= 1) {  // more halvings than any list needs
+#pragma unroll
+        for (int l = 0; l < MERGE_LISTS; ++l) {
+            if (size[l] > 0) {
+                const int half = size[l] >> 1;
+                const int probe = in.key[start + (long)l * length + lo[l] + half];
+                const bool below = group + l < own ? probe <= key : probe < key;
+                lo[l] = below ? lo[l] + half + 1 : lo[l];
+                size[l] = below ? size[l] - half - 1 : half;
             }
         }
     }
+    long to = start + (i - (long)own * length);
+#pragma unroll
+    for (int l = 0; l < MERGE_LISTS; ++l) to += lo[l];
+    out.key[to] = key;
+    out.at[to] = in.at[i];
+}
+
+// How the sorted tokens are cut: `chunk` of them to a group of `lanes` lanes, which takes lanes * 8 columns; `slabs` such pieces make a row.
+struct Cut {
+    int chunk, chunks, lanes, slabs;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) embedding_add_kernel(const EmbeddingArgs a, Sorted s, Cut c, float* parts) {
+    constexpr int AHEAD = 8;
+    const int lane = threadIdx.x & (c.lanes - 1);
+    const long g = ((long)blockIdx.x * 256 + threadIdx.x) / c.lanes;
+    const int slab = (int)(g % c.slabs);
+    const long chunk = g / c.slabs;
+    const int j = (slab * c.lanes + lane) * 8;
+    if (chunk >= c.chunks || j >= a.n) return;
+    const int count = left(a.n, j);
+    const int first = (int)(chunk * c.chunk), last = a.tokens - first < c.chunk ? a.tokens : first + c.chunk;
+    int key = s.key[first];
+    const bool goes_on = first > 0 && s.key[first - 1] == key;  // from the chunk before
+    bool head = goes_on;
+    float sum[8] = {};
+    const T* rows = (const T*)a.rows + j;
+    for (int t0 = first; t0 < last && key < a.vocab; t0 += AHEAD) {
+        float v[AHEAD][8];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (t0 + u < last) load8(rows + s.at[t0 + u] * a.pitch, count, v[u]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (t0 + u >= last) break;
+            const int k = s.key[t0 + u];
+            if (k != key) {
+                if (key < a.vocab) {
+                    if (head) {
+                        float* p = parts + (chunk * 2) * a.n + j;
+                        store8(p, count, sum);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
+                        store8((T*)a.out + (long)key * a.n + j, count, sum);
+                    }
+                }
+                head = false;
+                key = k;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += v[u][e];
+        }
+    }
+    if (key >= a.vocab) return;
+    const bool tail = last < a.tokens && s.key[last] == key;
+    if (head || tail) {
+        store8(parts + (chunk * 2 + (head ? 0 : 1)) * a.n + j, count, sum);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
+        store8((T*)a.out + (long)key * a.n + j, count, sum);
+    }
+}
+// A workgroup for each chunk and slab: where a run begins in the chunk and goes on behind it, its waves take the parts in turn.
+constexpr int JOIN_WAVES = 8;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WAVES * 64) embedding_join_kernel(const EmbeddingArgs a, Sorted s, Cut c, const float* parts) {
+    __shared__ float sums[JOIN_WAVES][64][9];
+    const int slabs = (a.n + 511) / 512;
+    const int chunk = blockIdx.x / slabs, slab = blockIdx.x % slabs;
+    const int first = chunk * c.chunk, next = first + c.chunk;  // (the last chunk has no workgroup)
+    const int key = s.key[next - 1];
+    if (key >= a.vocab || s.key[next] != key || (s.key[first] == key && first > 0 && s.key[first - 1] == key)) return;
+    int lo = next, size = a.tokens - next;  // the end of the run
+    while (size > 0) {
+        const int half = size >> 1;
+        if (s.key[lo + half] <= key) lo += half + 1, size -= half + 1;
+        else size = half;
+    }
+    const int end = (lo - 1) / c.chunk;  // the chunk that it ends in
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = slab * 512 + lane * 8;
+    const int count = left(a.n, j);
+    float sum[8] = {};
+    if (j < a.n) {
+        if (wave == 0) load8(parts + (chunk * 2L + 1) * a.n + j, count, sum);
+#pragma unroll 4
+        for (int p = chunk + 1 + wave; p <= end; p += JOIN_WAVES) {
+            float v[8];
+            load8(parts + p * 2L * a.n + j, count, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[wave][lane][e] = sum[e];
+    __syncthreads();
+    if (wave > 0 || j >= a.n) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        for (int w = 1; w < JOIN_WAVES; ++w) sum[e] += sums[w][lane][e];
+        sum[e] *= a.scale;
+    }
+    store8((T*)a.out + (long)key * a.n + j, count, sum);
 }
 
 // ---- dropout ----------------------------------------------------------------------------------------
@@ -328,14 +563,65 @@ hipError_t launch_embedding(const EmbeddingArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-long embedding_grad_workspace(int, int, int, int) { return 0; }
+namespace {
+// Chunks are as many as fill the machine four waves deep on each of its 1024 SIMDs, and at most 2048, so that the parts of a run over all
+// of them are few; at least 8 tokens, which are loaded at once.
+Cut cut(int tokens, int n) {
+    Cut c;
+    for (c.lanes = 8; c.lanes < 64 && c.lanes * 8 < n; c.lanes *= 2) {}
+    c.slabs = (int)(up(n, c.lanes * 8) / (c.lanes * 8));
+    const long chunks = std::max(1L, std::min(2048L, 4096L * 64 / ((long)c.lanes * c.slabs)));
+    c.chunk = (int)std::max(8L, (tokens + chunks - 1) / chunks);
+    c.chunks = (tokens + c.chunk - 1) / c.chunk;
+    return c;
+}
+struct Lists {
+    Sorted sorted, other;
+    float* parts;
+    long bytes;
+};
+Lists lay_out(void* workspace, int tokens, int n) {
+    const long list = up(tokens, 64);
+    int* p = (int*)workspace;
+    Lists l{{p, p + list}, {}, nullptr, 0};
+    p += 2 * list;
+    if (tokens > SORT_TOKENS) {
+        l.other = Sorted{p, p + list};
+        p += 2 * list;
+    }
+    l.parts = (float*)p;
+    l.bytes = ((char*)p - (char*)workspace) + 2L * cut(tokens, n).chunks * n * 4;
+    return l;
+}
+}  // namespace
 
-hipError_t launch_embedding_grad(const EmbeddingArgs& a, void*, hipStream_t stream) {
-    if (a.vocab == 0 || a.n == 0) return hipSuccess;
-    const unsigned grid = grid_of(a.vocab);
-    if (a.dtype == MUON_HIP_BF16) hipLaunchKernelGGL(embedding_grad_kernel<bf16_t>, dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(embedding_grad_kernel<float>, dim3(grid), dim3(256), 0, stream, a);
+long embedding_grad_workspace(int tokens, int vocab, int n, int) { return tokens == 0 || vocab == 0 || n == 0 ? 0 : lay_out(nullptr, tokens, n).bytes; }
+
+template <typename T>
+static hipError_t run_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStream_t stream) {
+    const long bytes = (long)a.vocab * a.n * (long)sizeof(T);
+    const int sorters = (int)(up(a.tokens, SORT_TOKENS) / SORT_TOKENS);
+    int bits = 1;
+    while (a.vocab >> bits) ++bits;  // ids and `vocab` itself
+    Lists l = lay_out(workspace, a.tokens, a.n);
+    const long clear = std::min(up(bytes, CLEAR_BYTES) / CLEAR_BYTES, MOST_THREADS / SORT_THREADS - sorters);
+    hipLaunchKernelGGL(embedding_sort_kernel<T>, dim3((unsigned)(sorters + clear)), dim3(SORT_THREADS), 0, stream, a, sorters, bits, l.sorted);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || a.tokens == 0) return e;
+    for (long length = SORT_TOKENS; length < a.tokens; length *= MERGE_LISTS) {
+        hipLaunchKernelGGL(embedding_merge_kernel, dim3((unsigned)(up(a.tokens, 256) / 256)), dim3(256), 0, stream, l.sorted, l.other, a.tokens, (int)length);
+        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        std::swap(l.sorted, l.other);
+    }
+    const Cut c = cut(a.tokens, a.n);
+    const long lanes = (long)c.chunks * c.slabs * c.lanes;
+    hipLaunchKernelGGL(embedding_add_kernel<T>, dim3((unsigned)(up(lanes, 256) / 256)), dim3(256), 0, stream, a, l.sorted, c, l.parts);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || c.chunks == 1) return e;
+    hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)((c.chunks - 1) * (up(a.n, 512) / 512))), dim3(JOIN_WAVES * 64), 0, stream, a, l.sorted, c, l.parts);
     return hipGetLastError();
+}
+hipError_t launch_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStream_t stream) {
+    if (a.vocab == 0 || a.n == 0) return hipSuccess;
+    return a.dtype == MUON_HIP_BF16 ? run_embedding_grad<bf16_t>(a, workspace, stream) : run_embedding_grad<float>(a, workspace, stream);
 }
 
 hipError_t launch_dropout(const DropoutArgs& a, hipStream_t stream) {
