@@ -57,11 +57,279 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 }
 
 // ---- norms ------------------------------------------------------------------------------------------
-// A workgroup per row, which reads it once for each sum and once more for the result.
-template <typename T, bool CENTRED>
-__global__ void __launch_bounds__(256) norm_kernel(const muon_hip_norm p) {
-    __shared__ float part[2][4];
+// A row is held in the registers of its lanes, 8 to 512 of them: it is read once, its mean is taken before the squares of what is left are
+// summed, and no sum of squares cancels.  A lane has CH pieces of 16 bytes, neighbouring lanes neighbouring pieces.  Where a row is no whole number of
+// pieces (RAGGED), its last one begins a piece before the row's end: it overlaps the one before, and what it has twice counts once.  Rows at any address.
+constexpr int MOST_LANES = 512;  // of a row, and threads of a workgroup: 256 registers each
+template <typename T> struct Piece;
+template <> struct Piece<bf16_t> {
+    static constexpr int V = 8;
+    u32x4 raw;
+    __device__ __forceinline__ void load(const bf16_t* p) { raw = __builtin_bit_cast(u32x4, (bf16x8) * (const bf16x8_any*)p); }
+    __device__ __forceinline__ void store(bf16_t* p) const { *(bf16x8_any*)p = __builtin_bit_cast(bf16x8, raw); }
+    __device__ __forceinline__ float operator[](int e) const { return e & 1 ? high_bf16(raw[e / 2]) : low_bf16(raw[e / 2]); }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+    }
+};
+template <> struct Piece<float> {
+    static constexpr int V = 4;
+    f32x4 raw;
+    __device__ __forceinline__ void load(const float* p) { raw = *(const f32x4_any*)p; }
+    __device__ __forceinline__ void store(float* p) const { *(f32x4_any*)p = raw; }
+    __device__ __forceinline__ float operator[](int e) const { return raw[e]; }
+    __device__ __forceinline__ void set(const float (&v)[4]) { raw = f32x4{v[0], v[1], v[2], v[3]}; }
+};
+
+template <int CTRL> __device__ __forceinline__ float moved(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// v and what lies in the other of two rows (S = 16) or halves (32) of lanes, added.
+template <int S> __device__ __forceinline__ float across(float v) {
+    const unsigned own = __builtin_bit_cast(unsigned, v);
+    const auto r = S == 16 ? __builtin_amdgcn_permlane16_swap(own, own, false, false) : __builtin_amdgcn_permlane32_swap(own, own, false, false);
+    const unsigned a = r[0], b = r[1];  // (a cast of a vector's element is one of its first element)
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+// The sum over `lanes` neighbouring lanes (8, 16, 32 or 64), in each of them: exchanges within rows of 16 lanes, then of rows and halves.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    v += moved<0xb1>(v);   // lane ^ 1
+    v += moved<0x4e>(v);   // lane ^ 2
+    v += moved<0x141>(v);  // the other four of eight
+    if (lanes > 8) v += moved<0x140>(v);  // the other eight of sixteen
+    if (lanes > 16) v = across<16>(v);
+    if (lanes > 32) v = across<32>(v);
+    return v;
+}
+// The same where a row has several waves, of K values at once: waves 0 to lanes / 64 - 1 of each row in `part`.  Calls alternate between two arrays.
+template <int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], int lanes, float (*part)[8]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lanes_sum(v[k], lanes);
+    if (lanes <= 64) return;
+    const int wave = threadIdx.x >> 6, waves = lanes >> 6, first = wave & ~(waves - 1);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) part[k][wave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        float t = part[k][first];
+        for (int w = 1; w < waves; ++w) t += part[k][first + w];
+        v[k] = t;
+    }
+}
+
+// Where the pieces of a lane are.
+template <typename T, int CH, bool RAGGED>
+struct Place {
+    static constexpr int V = Piece<T>::V;
+    int lane, lanes, n;
+    __device__ __forceinline__ int begin(int c) const { return (c * lanes + lane) * V; }
+    __device__ __forceinline__ bool in(int c) const { return begin(c) < n; }
+    __device__ __forceinline__ int at(int c) const { return RAGGED && begin(c) > n - V ? n - V : begin(c); }
+    __device__ __forceinline__ bool counts(int c, int e) const { return in(c) && (!RAGGED || at(c) + e >= begin(c)); }
+};
+
+template <typename T, bool CENTRED, int CH, bool RAGGED>
+__global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p, int lanes) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float part[2][1][8];
+    const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
+    const int each = blockDim.x / lanes;
+    for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
+        const long r = r0 + threadIdx.x / lanes;
+        const bool row = r < p.rows;  // (only where a wave has several rows can there be none)
+        Piece<T> x[CH], res[CH];
+        float s[CH][V];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            x[c].raw = {};
+            if (row && at.in(c)) x[c].load((const T*)p.x + r * p.x_row + at.at(c));
+        }
+        if (p.residual) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                res[c].raw = {};
+                if (row && at.in(c)) res[c].load((const T*)p.residual + r * p.res_row + at.at(c));
+            }
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                float v[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = x[c][e] + res[c][e];
+                x[c].set(v);
+                if (row && at.in(c)) x[c].store((T*)p.sum + r * p.n + at.at(c));
+            }
+        }
+        float mean = 0.f, total[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s[c][e] = x[c][e];
+                if (CENTRED) total[0] += !RAGGED || at.counts(c, e) ? s[c][e] : 0.f;
+            }
+        }
+        if (CENTRED) {
+            row_sum(total, lanes, part[0]);
+            mean = total[0] / (float)p.n;  // (a quotient: a row of one value has that one for its mean)
+        }
+        total[0] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s[c][e] -= mean;
+                if (CENTRED) total[0] += at.counts(c, e) ? s[c][e] * s[c][e] : 0.f;
+                else total[0] += !RAGGED || at.counts(c, e) ? s[c][e] * s[c][e] : 0.f;  // (what is not there is zero)
+            }
+        }
+        row_sum(total, lanes, part[1]);
+        const float rstd = 1.f / sqrtf(total[0] / (float)p.n + (float)p.eps);
+        if (!CENTRED && lanes > 64) __syncthreads();  // (one sum a row: the next one writes where this one is read)
+        if (p.stats && row && at.lane == 0) {
+            p.stats[r] = rstd;
+            if (CENTRED) p.stats[p.rows + r] = mean;
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (!row || !at.in(c)) continue;
+            Piece<T> w, b, y;
+            float v[V];
+            if (p.weight) w.load((const T*)p.weight + at.at(c));
+            if (p.bias) b.load((const T*)p.bias + at.at(c));
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[e] = s[c][e] * rstd;
+                if (p.weight) v[e] *= w[e];
+                if (p.bias) v[e] += b[e];
+            }
+            y.set(v);
+            y.store((T*)p.y + r * p.n + at.at(c));
+        }
+    }
+}
+
+// The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
+// once, and written as one row of `partials`.
+template <typename T, bool CENTRED, int CH, bool RAGGED>
+__global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int lanes) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float part[2][2][8];
+    extern __shared__ float columns[];
+    const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
+    const int each = blockDim.x / lanes;
     const float over = 1.f / p.n;
+    Piece<T> w[CH];
+    float dw[CH][V], db[CH][V];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        float one[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = 0.f, one[e] = 1.f;
+        w[c].set(one);
+        if (p.weight && at.in(c)) w[c].load((const T*)p.weight + at.at(c));
+    }
+    int turn = 0;
+    for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
+        const long r = r0 + threadIdx.x / lanes;
+        const bool row = r < p.rows;
+        Piece<T> dy[CH], s[CH], ds[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            dy[c].raw = {};
+            s[c].raw = {};
+            if (row && at.in(c)) {
+                dy[c].load((const T*)p.dy + r * p.dy_row + at.at(c));
+                if (p.s) s[c].load((const T*)p.s + r * p.s_row + at.at(c));
+            }
+        }
+        if (p.ds) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (row && at.in(c)) ds[c].load((const T*)p.ds + r * p.ds_row + at.at(c));
+        }
+        const float rstd = p.s && row ? p.stats[r] : 0.f, mean = CENTRED && p.s && row ? p.stats[p.rows + r] : 0.f;
+        float sums[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float g = !RAGGED || at.counts(c, e) ? dy[c][e] : 0.f, hat = (s[c][e] - mean) * rstd, gw = g * w[c][e];
+                const float product = !RAGGED || at.counts(c, e) ? g * hat : 0.f;
+                dw[c][e] += product;
+                if (CENTRED) db[c][e] += g;
+                if (CENTRED) sums[0] += gw;
+                sums[1] += product * w[c][e];
+            }
+        }
+        if (!p.dx) continue;
+        if constexpr (CENTRED) row_sum(sums, lanes, part[turn]);
+        else {
+            float one[1] = {sums[1]};
+            row_sum(one, lanes, part[turn]);
+            sums[1] = one[0];
+        }
+        turn ^= 1;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {  // unpacked again below, not kept as twice the registers
+            asm volatile("" : "+v"(dy[c].raw));
+            asm volatile("" : "+v"(s[c].raw));
+            asm volatile("" : "+v"(w[c].raw));
+        }
+        const float c1 = sums[0] * over, c2 = sums[1] * over;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (!row || !at.in(c)) continue;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float hat = (s[c][e] - mean) * rstd;
+                v[e] = rstd * ((CENTRED ? dy[c][e] * w[c][e] - c1 : dy[c][e] * w[c][e]) - hat * c2);
+                if (p.ds) v[e] += ds[c][e];
+            }
+            dy[c].set(v);
+            dy[c].store((T*)p.dx + r * p.n + at.at(c));
+        }
+    }
+    // what this workgroup has summed: columns of dweight, then those of dbias
+    const int waves = lanes < 64 ? 1 : lanes / 64, turns = (blockDim.x >> 6) / waves, mine = (threadIdx.x >> 6) / waves;
+    for (int f = 0; f < 2; ++f) {
+        float (&sum)[CH][V] = f ? db : dw;
+        if (f ? !CENTRED || !p.dbias : !p.dweight) continue;
+        float* out = partials + ((f && p.dweight ? (long)gridDim.x : 0L) + blockIdx.x) * p.n;
+        for (int off = lanes; off < 64; off <<= 1) {  // rows of one wave
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[c][e] += __shfl_xor(sum[c][e], off, 64);
+        }
+        float* to = turns > 1 ? columns : out;
+        for (int t = 0; t < turns; ++t) {
+            if (t == mine && (int)(threadIdx.x & 63) < lanes) {
+#pragma unroll
+                for (int c = 0; c < CH; ++c)
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (at.counts(c, e)) to[at.at(c) + e] = t ? to[at.at(c) + e] + sum[c][e] : sum[c][e];
+            }
+            if (turns > 1) __syncthreads();
+        }
+        if (turns > 1) {
+            for (int j = threadIdx.x; j < p.n; j += blockDim.x) out[j] = columns[j];
+            __syncthreads();
+        }
+    }
+}
+
+// Rows of less than a piece, or longer than the registers of 512 lanes: a workgroup per row, which reads it once for each sum and once more
+// for the result.
+template <typename T, bool CENTRED>
+__global__ void __launch_bounds__(256) norm_streamed_kernel(const muon_hip_norm p) {
+    __shared__ float part[2][4];
     for (long r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T *x = (const T*)p.x + r * p.x_row, *res = p.residual ? (const T*)p.residual + r * p.res_row : nullptr;
         T *y = (T*)p.y + r * p.n, *sum = res ? (T*)p.sum + r * p.n : nullptr;
@@ -79,7 +347,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const muon_hip_norm p) {
             for (int e = 0; e < 8; ++e) total += (float)(T)v[e];
         }
         const T* s = res ? sum : x;  // (a thread reads what it has written itself)
-        const float mean = CENTRED ? group_sum(total, part[0]) * over : 0.f;
+        const float mean = CENTRED ? group_sum(total, part[0]) / (float)p.n : 0.f;
         float square = 0.f;
         for (int j = threadIdx.x * 8; j < p.n; j += 2048) {
             float v[8];
@@ -87,7 +355,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const muon_hip_norm p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) square += e < p.n - j ? (v[e] - mean) * (v[e] - mean) : 0.f;
         }
-        const float rstd = 1.f / sqrtf(group_sum(square, part[1]) * over + (float)p.eps);
+        const float rstd = 1.f / sqrtf(group_sum(square, part[1]) / (float)p.n + (float)p.eps);
         if (!CENTRED) __syncthreads();  // (one sum a row: the next one writes where this one is read)
         if (p.stats && threadIdx.x == 0) {
             p.stats[r] = rstd;
@@ -111,7 +379,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const muon_hip_norm p) {
 
 // A workgroup takes every gridDim-th row and adds to sums of its own, whose columns belong to one thread each.
 template <typename T, bool CENTRED>
-__global__ void __launch_bounds__(256) norm_grad_kernel(const muon_hip_norm_grad p, float* partials) {
+__global__ void __launch_bounds__(256) norm_grad_streamed_kernel(const muon_hip_norm_grad p, float* partials) {
     __shared__ float part[2][4];
     const float over = 1.f / p.n;
     float* dw = p.dweight ? partials + (long)blockIdx.x * p.n : nullptr;
@@ -524,27 +792,95 @@ inline unsigned grid_of(long groups) { return (unsigned)std::min(groups, MOST_TH
 
 }  // namespace
 
+namespace {
+// How rows are laid over lanes: `lanes` of a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
+struct Layout {
+    int lanes, pieces, threads;
+    bool ragged;
+};
+Layout lay_rows(int dtype, long rows, int n, int most) {
+    const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
+    const long count = up(n, v) / v;
+    if (n < v || count > (long)MOST_LANES * most) return {256, 0, 256, false};
+    Layout l{8, 1, 256, n % v != 0};
+    // As many lanes as leave each of them up to `most` pieces, and fewer pieces where the rows alone do not fill the machine with waves.
+    while (l.lanes < MOST_LANES && l.lanes * (long)most < count) l.lanes *= 2;
+    while (l.lanes < MOST_LANES && l.lanes < count && rows * l.lanes < 256 * 1024) l.lanes *= 2;
+    while (l.pieces * (long)l.lanes < count) l.pieces *= 2;
+    l.threads = std::max(256, l.lanes);
+    return l;
+}
+template <typename T, bool CENTRED, int CH>
+auto norm_of(bool ragged) { return ragged ? norm_kernel<T, CENTRED, CH, true> : norm_kernel<T, CENTRED, CH, false>; }
+template <typename T, bool CENTRED>
+auto norm_of(const Layout& l) {
+    return l.pieces == 1 ? norm_of<T, CENTRED, 1>(l.ragged) : l.pieces == 2 ? norm_of<T, CENTRED, 2>(l.ragged)
+         : l.pieces == 4 ? norm_of<T, CENTRED, 4>(l.ragged) : norm_of<T, CENTRED, 8>(l.ragged);
+}
+template <typename T, bool CENTRED, int CH>
+auto norm_grad_of(bool ragged) { return ragged ? norm_grad_kernel<T, CENTRED, CH, true> : norm_grad_kernel<T, CENTRED, CH, false>; }
+template <typename T, bool CENTRED>
+auto norm_grad_of(const Layout& l) {
+    if constexpr (Piece<T>::V * 8 <= 32)
+        if (l.pieces == 8) return norm_grad_of<T, CENTRED, 8>(l.ragged);
+    return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1>(l.ragged) : l.pieces == 2 ? norm_grad_of<T, CENTRED, 2>(l.ragged) : norm_grad_of<T, CENTRED, 4>(l.ragged);
+}
+#ifndef FWD_MOST
+#define FWD_MOST 8
+#endif
+#ifndef BWD_MOST
+#define BWD_MOST (32 / (p.dtype == MUON_HIP_BF16 ? 8 : 4))
+#endif
+#ifndef BWD_PER_CU
+#define BWD_PER_CU 2
+#endif
+Layout lay_grad(const muon_hip_norm_grad& p) {
+    Layout l = lay_rows(p.dtype, p.rows, p.n, BWD_MOST);
+    if (l.pieces > 0 && l.lanes < 512) l.threads = 512;
+    return l;
+}
+}  // namespace
+
 hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
     if (p.rows == 0 || p.n == 0) return hipSuccess;
     const bool bf = p.dtype == MUON_HIP_BF16, centred = p.kind == MUON_HIP_NORM_LAYER;
-    void (*kern)(const muon_hip_norm);
-    if (bf) kern = centred ? norm_kernel<bf16_t, true> : norm_kernel<bf16_t, false>;
-    else kern = centred ? norm_kernel<float, true> : norm_kernel<float, false>;
-    hipLaunchKernelGGL(kern, dim3(grid_of(p.rows)), dim3(256), 0, stream, p);
+    const Layout l = lay_rows(p.dtype, p.rows, p.n, FWD_MOST);
+    if (l.pieces == 0) {
+        void (*kern)(const muon_hip_norm);
+        if (bf) kern = centred ? norm_streamed_kernel<bf16_t, true> : norm_streamed_kernel<bf16_t, false>;
+        else kern = centred ? norm_streamed_kernel<float, true> : norm_streamed_kernel<float, false>;
+        hipLaunchKernelGGL(kern, dim3(grid_of(p.rows)), dim3(256), 0, stream, p);
+        return hipGetLastError();
+    }
+    const int each = l.threads / l.lanes;
+    const auto kern = bf ? (centred ? norm_of<bf16_t, true>(l) : norm_of<bf16_t, false>(l)) : centred ? norm_of<float, true>(l) : norm_of<float, false>(l);
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, each) / each, MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.lanes);
     return hipGetLastError();
 }
 
-long norm_grad_groups(const muon_hip_norm_grad& p, int cus) { return std::min((long)p.rows, 2L * cus); }
+long norm_grad_groups(const muon_hip_norm_grad& p, int cus) {
+    const Layout l = lay_grad(p);
+    const int each = l.pieces ? l.threads / l.lanes : 1;
+    return std::min(up(p.rows, each) / each, (long)BWD_PER_CU * cus);
+}
 
 hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cus, hipStream_t stream) {
     if (p.n == 0) return hipSuccess;
     const bool bf = p.dtype == MUON_HIP_BF16, centred = p.kind == MUON_HIP_NORM_LAYER;
     const long groups = norm_grad_groups(p, cus);
+    const Layout l = lay_grad(p);
     if (groups > 0) {
-        void (*kern)(const muon_hip_norm_grad, float*);
-        if (bf) kern = centred ? norm_grad_kernel<bf16_t, true> : norm_grad_kernel<bf16_t, false>;
-        else kern = centred ? norm_grad_kernel<float, true> : norm_grad_kernel<float, false>;
-        hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, stream, p, partials);
+        if (l.pieces == 0) {
+            void (*kern)(const muon_hip_norm_grad, float*);
+            if (bf) kern = centred ? norm_grad_streamed_kernel<bf16_t, true> : norm_grad_streamed_kernel<bf16_t, false>;
+            else kern = centred ? norm_grad_streamed_kernel<float, true> : norm_grad_streamed_kernel<float, false>;
+            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, stream, p, partials);
+        } else {
+            const auto kern = bf ? (centred ? norm_grad_of<bf16_t, true>(l) : norm_grad_of<bf16_t, false>(l))
+                                 : centred ? norm_grad_of<float, true>(l) : norm_grad_of<float, false>(l);
+            const size_t lds = l.threads > std::max(l.lanes, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
+            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.lanes);
+        }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     void* out[2] = {p.dweight ? p.dweight : p.dbias, p.dweight ? p.dbias : nullptr};
