@@ -65,8 +65,8 @@ template <typename T> struct Piece;
 template <> struct Piece<bf16_t> {
     static constexpr int V = 8;
     u32x4 raw;
-    __device__ __forceinline__ void load(const bf16_t* p) { raw = __builtin_bit_cast(u32x4, (bf16x8) * (const bf16x8_any*)p); }
-    __device__ __forceinline__ void store(bf16_t* p) const { *(bf16x8_any*)p = __builtin_bit_cast(bf16x8, raw); }
+    __device__ __forceinline__ void load(const void* p, unsigned bytes) { raw = __builtin_bit_cast(u32x4, (bf16x8) * (const bf16x8_any*)((const char*)p + bytes)); }
+    __device__ __forceinline__ void store(void* p, unsigned bytes) const { *(bf16x8_any*)((char*)p + bytes) = __builtin_bit_cast(bf16x8, raw); }
     __device__ __forceinline__ float operator[](int e) const { return e & 1 ? high_bf16(raw[e / 2]) : low_bf16(raw[e / 2]); }
     __device__ __forceinline__ void set(const float (&v)[8]) {
 #pragma unroll
@@ -76,8 +76,8 @@ template <> struct Piece<bf16_t> {
 template <> struct Piece<float> {
     static constexpr int V = 4;
     f32x4 raw;
-    __device__ __forceinline__ void load(const float* p) { raw = *(const f32x4_any*)p; }
-    __device__ __forceinline__ void store(float* p) const { *(f32x4_any*)p = raw; }
+    __device__ __forceinline__ void load(const void* p, unsigned bytes) { raw = *(const f32x4_any*)((const char*)p + bytes); }
+    __device__ __forceinline__ void store(void* p, unsigned bytes) const { *(f32x4_any*)((char*)p + bytes) = raw; }
     __device__ __forceinline__ float operator[](int e) const { return raw[e]; }
     __device__ __forceinline__ void set(const float (&v)[4]) { raw = f32x4{v[0], v[1], v[2], v[3]}; }
 };
@@ -130,30 +130,43 @@ struct Place {
     __device__ __forceinline__ int begin(int c) const { return (c * lanes + lane) * V; }
     __device__ __forceinline__ bool in(int c) const { return begin(c) < n; }
     __device__ __forceinline__ int at(int c) const { return RAGGED && begin(c) > n - V ? n - V : begin(c); }
+    __device__ __forceinline__ unsigned bytes(int c) const { return (unsigned)at(c) * (unsigned)sizeof(T); }
     __device__ __forceinline__ bool counts(int c, int e) const { return in(c) && (!RAGGED || at(c) + e >= begin(c)); }
 };
 
-template <typename T, bool CENTRED, int CH, bool RAGGED>
-__global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p, int lanes) {
+// Which of a workgroup's rows a thread works on.  WIDE rows have whole waves: their addresses are in scalar registers, of which all streams share
+// the offsets of the pieces.
+template <bool WIDE>
+__device__ __forceinline__ int row_of(int shift) {
+    const int r = (int)threadIdx.x >> shift;
+    return WIDE ? __builtin_amdgcn_readfirstlane(r) : r;
+}
+
+template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p, int shift) {
     constexpr int V = Piece<T>::V;
     __shared__ float part[2][1][8];
+    const int lanes = 1 << shift;
     const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
-    const int each = blockDim.x / lanes;
+    const int each = blockDim.x >> shift;
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
-        const long r = r0 + threadIdx.x / lanes;
-        const bool row = r < p.rows;  // (only where a wave has several rows can there be none)
+        const long r = r0 + row_of<WIDE>(shift);
+        const bool row = r < p.rows;
         Piece<T> x[CH], res[CH];
         float s[CH][V];
+        const T* const px = (const T*)p.x + r * p.x_row;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             x[c].raw = {};
-            if (row && at.in(c)) x[c].load((const T*)p.x + r * p.x_row + at.at(c));
+            if (row && at.in(c)) x[c].load(px, at.bytes(c));
         }
         if (p.residual) {
+            const T* const pr = (const T*)p.residual + r * p.res_row;
+            T* const ps = (T*)p.sum + r * p.n;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 res[c].raw = {};
-                if (row && at.in(c)) res[c].load((const T*)p.residual + r * p.res_row + at.at(c));
+                if (row && at.in(c)) res[c].load(pr, at.bytes(c));
             }
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
@@ -161,7 +174,7 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[e] = x[c][e] + res[c][e];
                 x[c].set(v);
-                if (row && at.in(c)) x[c].store((T*)p.sum + r * p.n + at.at(c));
+                if (row && at.in(c)) x[c].store(ps, at.bytes(c));
             }
         }
         float mean = 0.f, total[1] = {0.f};
@@ -190,17 +203,19 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
         row_sum(total, lanes, part[1]);
         const float rstd = 1.f / sqrtf(total[0] / (float)p.n + (float)p.eps);
         if (!CENTRED && lanes > 64) __syncthreads();  // (one sum a row: the next one writes where this one is read)
-        if (p.stats && row && at.lane == 0) {
+        if (!row) continue;
+        if (p.stats && at.lane == 0) {
             p.stats[r] = rstd;
             if (CENTRED) p.stats[p.rows + r] = mean;
         }
+        T* const py = (T*)p.y + r * p.n;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (!row || !at.in(c)) continue;
+            if (!at.in(c)) continue;
             Piece<T> w, b, y;
             float v[V];
-            if (p.weight) w.load((const T*)p.weight + at.at(c));
-            if (p.bias) b.load((const T*)p.bias + at.at(c));
+            if (p.weight) w.load(p.weight, at.bytes(c));
+            if (p.bias) b.load(p.bias, at.bytes(c));
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[e] = s[c][e] * rstd;
@@ -208,20 +223,21 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
                 if (p.bias) v[e] += b[e];
             }
             y.set(v);
-            y.store((T*)p.y + r * p.n + at.at(c));
+            y.store(py, at.bytes(c));
         }
     }
 }
 
 // The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
 // once, and written as one row of `partials`.
-template <typename T, bool CENTRED, int CH, bool RAGGED>
-__global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int lanes) {
+template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(MOST_LANES, CH * Piece<T>::V <= (CENTRED ? 8 : 16) ? 4 : CH * Piece<T>::V <= 16 ? 3 : 2) norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int shift) {
     constexpr int V = Piece<T>::V;
     __shared__ float part[2][2][8];
     extern __shared__ float columns[];
+    const int lanes = 1 << shift;
     const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
-    const int each = blockDim.x / lanes;
+    const int each = blockDim.x >> shift;
     const float over = 1.f / p.n;
     Piece<T> w[CH];
     float dw[CH][V], db[CH][V];
@@ -231,26 +247,23 @@ __global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_no
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[c][e] = db[c][e] = 0.f, one[e] = 1.f;
         w[c].set(one);
-        if (p.weight && at.in(c)) w[c].load((const T*)p.weight + at.at(c));
+        if (p.weight && at.in(c)) w[c].load(p.weight, at.bytes(c));
     }
     int turn = 0;
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
-        const long r = r0 + threadIdx.x / lanes;
+        const long r = r0 + row_of<WIDE>(shift);
         const bool row = r < p.rows;
         Piece<T> dy[CH], s[CH], ds[CH];
+        const T *const pdy = (const T*)p.dy + r * p.dy_row, *const ps = (const T*)p.s + r * p.s_row, *const pds = (const T*)p.ds + r * p.ds_row;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             dy[c].raw = {};
             s[c].raw = {};
             if (row && at.in(c)) {
-                dy[c].load((const T*)p.dy + r * p.dy_row + at.at(c));
-                if (p.s) s[c].load((const T*)p.s + r * p.s_row + at.at(c));
+                dy[c].load(pdy, at.bytes(c));
+                if (p.s) s[c].load(ps, at.bytes(c));
+                if (p.ds) ds[c].load(pds, at.bytes(c));
             }
-        }
-        if (p.ds) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-                if (row && at.in(c)) ds[c].load((const T*)p.ds + r * p.ds_row + at.at(c));
         }
         const float rstd = p.s && row ? p.stats[r] : 0.f, mean = CENTRED && p.s && row ? p.stats[p.rows + r] : 0.f;
         float sums[2] = {0.f, 0.f};
@@ -258,11 +271,13 @@ __global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_no
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float g = !RAGGED || at.counts(c, e) ? dy[c][e] : 0.f, hat = (s[c][e] - mean) * rstd, gw = g * w[c][e];
+                const float g = !RAGGED || at.counts(c, e) ? dy[c][e] : 0.f, hat = (s[c][e] - mean) * rstd;
                 const float product = !RAGGED || at.counts(c, e) ? g * hat : 0.f;
                 dw[c][e] += product;
-                if (CENTRED) db[c][e] += g;
-                if (CENTRED) sums[0] += gw;
+                if (CENTRED) {
+                    db[c][e] += g;
+                    sums[0] += g * w[c][e];
+                }
                 sums[1] += product * w[c][e];
             }
         }
@@ -274,16 +289,18 @@ __global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_no
             sums[1] = one[0];
         }
         turn ^= 1;
+        if (!row) continue;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {  // unpacked again below, not kept as twice the registers
+        for (int c = 0; c < CH && sizeof(T) == 2; ++c) {  // unpacked again below, not kept as twice the registers
             asm volatile("" : "+v"(dy[c].raw));
             asm volatile("" : "+v"(s[c].raw));
             asm volatile("" : "+v"(w[c].raw));
         }
         const float c1 = sums[0] * over, c2 = sums[1] * over;
+        T* const pdx = (T*)p.dx + r * p.n;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (!row || !at.in(c)) continue;
+            if (!at.in(c)) continue;
             float v[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -292,15 +309,12 @@ __global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_no
                 if (p.ds) v[e] += ds[c][e];
             }
             dy[c].set(v);
-            dy[c].store((T*)p.dx + r * p.n + at.at(c));
+            dy[c].store(pdx, at.bytes(c));
         }
     }
     // what this workgroup has summed: columns of dweight, then those of dbias
     const int waves = lanes < 64 ? 1 : lanes / 64, turns = (blockDim.x >> 6) / waves, mine = (threadIdx.x >> 6) / waves;
-    for (int f = 0; f < 2; ++f) {
-        float (&sum)[CH][V] = f ? db : dw;
-        if (f ? !CENTRED || !p.dbias : !p.dweight) continue;
-        float* out = partials + ((f && p.dweight ? (long)gridDim.x : 0L) + blockIdx.x) * p.n;
+    const auto finish = [&](float (&sum)[CH][V], float* out) {
         for (int off = lanes; off < 64; off <<= 1) {  // rows of one wave
 #pragma unroll
             for (int c = 0; c < CH; ++c)
@@ -322,7 +336,9 @@ __global__ void __launch_bounds__(MOST_LANES) norm_grad_kernel(const muon_hip_no
             for (int j = threadIdx.x; j < p.n; j += blockDim.x) out[j] = columns[j];
             __syncthreads();
         }
-    }
+    };
+    if (p.dweight) finish(dw, partials + (long)blockIdx.x * p.n);
+    if (CENTRED && p.dbias) finish(db, partials + ((p.dweight ? (long)gridDim.x : 0L) + blockIdx.x) * p.n);
 }
 
 // Rows of less than a piece, or longer than the registers of 512 lanes: a workgroup per row, which reads it once for each sum and once more
@@ -429,25 +445,28 @@ __global__ void __launch_bounds__(256) norm_grad_streamed_kernel(const muon_hip_
         }
     }
 }
-// Sixteen rows of threads take the rows of sixteen columns in turn; their sums are added in a fixed order.
+// Sixty-four rows of threads take the rows of sixteen columns in turn, all of a thread's loads at once where there are 512 rows; their sums are
+// added in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* partials, int groups, int n, T* out0, T* out1) {
-    __shared__ float part[16][16];
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* partials, int groups, int n, T* out0, T* out1) {
+    __shared__ float part[64][17];
     const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
     T* out = blockIdx.y ? out1 : out0;
     for (long j0 = blockIdx.x * 16L; j0 < n; j0 += gridDim.x * 16L) {
         const long j = j0 + x;
         float v = 0.f;
         if (j < n) {
-#pragma unroll 4
-            for (int c = y; c < groups; c += 16) v += partials[((long)blockIdx.y * groups + c) * n + j];
+#pragma unroll 8
+            for (int c = y; c < groups; c += 64) v += partials[((long)blockIdx.y * groups + c) * n + j];
         }
         part[y][x] = v;
         __syncthreads();
-        if (y == 0 && j < n) {
+        if (y < 4) {
 #pragma unroll
-            for (int r = 1; r < 16; ++r) v += part[r][x];
-            out[j] = (T)v;
+            for (int r = 1; r < 16; ++r) v += part[y + 4 * r][x];
+            v += __shfl_xor(v, 16, 64);
+            v += __shfl_xor(v, 32, 64);
+            if (y == 0 && j < n) out[j] = (T)v;
         }
         __syncthreads();
     }
@@ -793,58 +812,86 @@ inline unsigned grid_of(long groups) { return (unsigned)std::min(groups, MOST_TH
 }  // namespace
 
 namespace {
-// How rows are laid over lanes: `lanes` of a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
+// How rows are laid over lanes: 2^shift of them to a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
 struct Layout {
-    int lanes, pieces, threads;
+    int shift, pieces, threads;
     bool ragged;
+    int rows() const { return pieces ? threads >> shift : 1; }  // that a workgroup works on at once
 };
-Layout lay_rows(int dtype, long rows, int n, int most) {
+// `best` pieces to a lane at most, unless there are no lanes left, and then `most`.
+Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most) {
     const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
     const long count = up(n, v) / v;
-    if (n < v || count > (long)MOST_LANES * most) return {256, 0, 256, false};
-    Layout l{8, 1, 256, n % v != 0};
-    // As many lanes as leave each of them up to `most` pieces, and fewer pieces where the rows alone do not fill the machine with waves.
-    while (l.lanes < MOST_LANES && l.lanes * (long)most < count) l.lanes *= 2;
-    while (l.lanes < MOST_LANES && l.lanes < count && rows * l.lanes < 256 * 1024) l.lanes *= 2;
-    while (l.pieces * (long)l.lanes < count) l.pieces *= 2;
-    l.threads = std::max(256, l.lanes);
+    if (n < v || count > (long)MOST_LANES * most) return {8, 0, 256, false};
+    Layout l{3, 1, threads, n % v != 0};
+    auto lanes = [&] { return 1L << l.shift; };
+    // A wave's lanes have one piece each before any has two; more lanes than that where the pieces are too many, or the rows alone too few to
+    // fill the machine with waves.
+    while (lanes() < count && (lanes() < 64 || (lanes() < MOST_LANES && (lanes() * best < count || rows * lanes() < 256 * 1024)))) ++l.shift;
+    while (l.pieces * lanes() < count) l.pieces *= 2;
+    l.threads = std::max(threads, (int)lanes());
     return l;
 }
-template <typename T, bool CENTRED, int CH>
-auto norm_of(bool ragged) { return ragged ? norm_kernel<T, CENTRED, CH, true> : norm_kernel<T, CENTRED, CH, false>; }
-template <typename T, bool CENTRED>
+template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_of(const Layout& l) {
-    return l.pieces == 1 ? norm_of<T, CENTRED, 1>(l.ragged) : l.pieces == 2 ? norm_of<T, CENTRED, 2>(l.ragged)
-         : l.pieces == 4 ? norm_of<T, CENTRED, 4>(l.ragged) : norm_of<T, CENTRED, 8>(l.ragged);
+    if constexpr (CH == 1)
+        if (l.shift < 6) return norm_kernel<T, CENTRED, CH, RAGGED, false>;
+    return norm_kernel<T, CENTRED, CH, RAGGED, true>;
 }
-template <typename T, bool CENTRED, int CH>
-auto norm_grad_of(bool ragged) { return ragged ? norm_grad_kernel<T, CENTRED, CH, true> : norm_grad_kernel<T, CENTRED, CH, false>; }
-template <typename T, bool CENTRED>
+template <typename T, bool CENTRED, bool RAGGED>
+auto norm_of(const Layout& l) {
+    return l.pieces == 1 ? norm_of<T, CENTRED, 1, RAGGED>(l) : l.pieces == 2 ? norm_of<T, CENTRED, 2, RAGGED>(l)
+         : l.pieces == 4 ? norm_of<T, CENTRED, 4, RAGGED>(l) : norm_of<T, CENTRED, 8, RAGGED>(l);
+}
+template <typename T>
+auto norm_of(const Layout& l, bool centred) {
+    if (centred) return l.ragged ? norm_of<T, true, true>(l) : norm_of<T, true, false>(l);
+    return l.ragged ? norm_of<T, false, true>(l) : norm_of<T, false, false>(l);
+}
+template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_grad_of(const Layout& l) {
-    if constexpr (Piece<T>::V * 8 <= 32)
-        if (l.pieces == 8) return norm_grad_of<T, CENTRED, 8>(l.ragged);
-    return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1>(l.ragged) : l.pieces == 2 ? norm_grad_of<T, CENTRED, 2>(l.ragged) : norm_grad_of<T, CENTRED, 4>(l.ragged);
+    if constexpr (CH == 1)
+        if (l.shift < 6) return norm_grad_kernel<T, CENTRED, CH, RAGGED, false>;
+    return norm_grad_kernel<T, CENTRED, CH, RAGGED, true>;
 }
-#ifndef FWD_MOST
-#define FWD_MOST 8
+template <typename T, bool CENTRED, bool RAGGED>
+auto norm_grad_of(const Layout& l) {
+    if constexpr (sizeof(T) == 4 && !CENTRED)
+        if (l.pieces == 8) return norm_grad_of<T, CENTRED, 8, RAGGED>(l);
+    return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1, RAGGED>(l) : l.pieces == 2 ? norm_grad_of<T, CENTRED, 2, RAGGED>(l) : norm_grad_of<T, CENTRED, 4, RAGGED>(l);
+}
+template <typename T>
+auto norm_grad_of(const Layout& l, bool centred) {
+    if (centred) return l.ragged ? norm_grad_of<T, true, true>(l) : norm_grad_of<T, true, false>(l);
+    return l.ragged ? norm_grad_of<T, false, true>(l) : norm_grad_of<T, false, false>(l);
+}
+#ifndef FWD_BEST
+#define FWD_BEST 4
 #endif
-#ifndef BWD_MOST
-#define BWD_MOST (32 / (p.dtype == MUON_HIP_BF16 ? 8 : 4))
+#ifndef BWD_BEST
+#define BWD_BEST (p.kind == MUON_HIP_NORM_LAYER ? 8 : 16)
+#endif
+#ifndef BWD_THREADS
+#define BWD_THREADS 512
 #endif
 #ifndef BWD_PER_CU
 #define BWD_PER_CU 2
 #endif
 Layout lay_grad(const muon_hip_norm_grad& p) {
-    Layout l = lay_rows(p.dtype, p.rows, p.n, BWD_MOST);
-    if (l.pieces > 0 && l.lanes < 512) l.threads = 512;
-    return l;
+    const int v = p.dtype == MUON_HIP_BF16 ? 8 : 4;
+    return lay_rows(p.dtype, p.rows, p.n, BWD_THREADS, BWD_BEST / v, (p.dtype == MUON_HIP_F32 && p.kind == MUON_HIP_NORM_LAYER ? 16 : 32) / v);
+}
+long grad_groups_per_cu(const muon_hip_norm_grad& p, const Layout& l) {
+    const int values = l.pieces * (p.dtype == MUON_HIP_BF16 ? 8 : 4);
+    const int waves = values <= (p.kind == MUON_HIP_NORM_LAYER ? 8 : 16) ? 16 : values <= 16 ? 12 : 8;
+    return std::max(1, std::min(BWD_PER_CU * 8, waves) * 64 / l.threads);
 }
 }  // namespace
 
 hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
     if (p.rows == 0 || p.n == 0) return hipSuccess;
     const bool bf = p.dtype == MUON_HIP_BF16, centred = p.kind == MUON_HIP_NORM_LAYER;
-    const Layout l = lay_rows(p.dtype, p.rows, p.n, FWD_MOST);
+    const Layout l = lay_rows(p.dtype, p.rows, p.n, 256, FWD_BEST, 8);
     if (l.pieces == 0) {
         void (*kern)(const muon_hip_norm);
         if (bf) kern = centred ? norm_streamed_kernel<bf16_t, true> : norm_streamed_kernel<bf16_t, false>;
@@ -852,16 +899,14 @@ hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
         hipLaunchKernelGGL(kern, dim3(grid_of(p.rows)), dim3(256), 0, stream, p);
         return hipGetLastError();
     }
-    const int each = l.threads / l.lanes;
-    const auto kern = bf ? (centred ? norm_of<bf16_t, true>(l) : norm_of<bf16_t, false>(l)) : centred ? norm_of<float, true>(l) : norm_of<float, false>(l);
-    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, each) / each, MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.lanes);
+    const auto kern = bf ? norm_of<bf16_t>(l, centred) : norm_of<float>(l, centred);
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, l.rows()) / l.rows(), MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.shift);
     return hipGetLastError();
 }
 
 long norm_grad_groups(const muon_hip_norm_grad& p, int cus) {
     const Layout l = lay_grad(p);
-    const int each = l.pieces ? l.threads / l.lanes : 1;
-    return std::min(up(p.rows, each) / each, (long)BWD_PER_CU * cus);
+    return std::min(up(p.rows, l.rows()) / l.rows(), grad_groups_per_cu(p, l) * cus);
 }
 
 hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cus, hipStream_t stream) {
@@ -876,18 +921,17 @@ hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cu
             else kern = centred ? norm_grad_streamed_kernel<float, true> : norm_grad_streamed_kernel<float, false>;
             hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, stream, p, partials);
         } else {
-            const auto kern = bf ? (centred ? norm_grad_of<bf16_t, true>(l) : norm_grad_of<bf16_t, false>(l))
-                                 : centred ? norm_grad_of<float, true>(l) : norm_grad_of<float, false>(l);
-            const size_t lds = l.threads > std::max(l.lanes, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
-            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.lanes);
+            const auto kern = bf ? norm_grad_of<bf16_t>(l, centred) : norm_grad_of<float>(l, centred);
+            const size_t lds = l.threads > std::max(1 << l.shift, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
+            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.shift);
         }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     void* out[2] = {p.dweight ? p.dweight : p.dbias, p.dweight ? p.dbias : nullptr};
     if (!out[0]) return hipSuccess;
     const dim3 grid((unsigned)std::min(up(p.n, 16) / 16, 65536L), out[1] ? 2 : 1);
-    if (bf) hipLaunchKernelGGL(column_sum_kernel<bf16_t>, grid, dim3(256), 0, stream, partials, (int)groups, p.n, (bf16_t*)out[0], (bf16_t*)out[1]);
-    else hipLaunchKernelGGL(column_sum_kernel<float>, grid, dim3(256), 0, stream, partials, (int)groups, p.n, (float*)out[0], (float*)out[1]);
+    if (bf) hipLaunchKernelGGL(column_sum_kernel<bf16_t>, grid, dim3(1024), 0, stream, partials, (int)groups, p.n, (bf16_t*)out[0], (bf16_t*)out[1]);
+    else hipLaunchKernelGGL(column_sum_kernel<float>, grid, dim3(1024), 0, stream, partials, (int)groups, p.n, (float*)out[0], (float*)out[1]);
     return hipGetLastError();
 }
 
