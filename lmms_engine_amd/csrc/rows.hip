@@ -82,6 +82,16 @@ template <> struct Piece<float> {
     __device__ __forceinline__ void set(const float (&v)[4]) { raw = f32x4{v[0], v[1], v[2], v[3]}; }
 };
 
+// One value of a row that is shorter than a piece.
+template <typename T> struct Single {
+    static constexpr int V = 1;
+    T raw;
+    __device__ __forceinline__ void load(const void* p, unsigned bytes) { raw = *(const T*)((const char*)p + bytes); }
+    __device__ __forceinline__ void store(void* p, unsigned bytes) const { *(T*)((char*)p + bytes) = raw; }
+    __device__ __forceinline__ float operator[](int) const { return (float)raw; }
+    __device__ __forceinline__ void set(const float (&v)[1]) { raw = (T)v[0]; }
+};
+
 template <int CTRL> __device__ __forceinline__ float moved(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
@@ -475,18 +485,41 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* partials,
 // ---- embedding --------------------------------------------------------------------------------------
 __device__ __forceinline__ long id_at(const void* ids, int wide, long t) { return wide ? ((const long*)ids)[t] : ((const int*)ids)[t]; }
 
-// A workgroup per token.  An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
-template <typename T>
-__global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a) {
-    for (long t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+// How rows of n values, in pieces of V, are cut: groups of 2^shift lanes with CH pieces each take a segment; `segments` of them make a row.
+struct Cut {
+    int shift, segments;
+};
+// A group of lanes for each segment of each token, all of whose loads are under way before the first store.  The last piece of a ragged row overlaps the one
+// before it: what it has twice is written twice.  An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
+template <typename T, typename P, int CH>
+__global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, Cut cut) {
+    constexpr int V = P::V;
+    const int lanes = 1 << cut.shift, lane = threadIdx.x & (lanes - 1);
+    const long all = (long)a.tokens * cut.segments, step = (long)gridDim.x * (256 >> cut.shift);
+    for (long g = (long)blockIdx.x * (256 >> cut.shift) + (threadIdx.x >> cut.shift); g < all; g += step) {
+        const long t = cut.segments == 1 ? g : g / cut.segments;
+        const int first = (int)(g - t * cut.segments) * (lanes * CH * V) + lane * V;
         const long id = id_at(a.ids, a.wide, t);
         const bool known = id >= 0 && id < a.vocab;
-        for (int j = threadIdx.x * 8; j < a.n; j += 2048) {
-            float v[8];
-            if (known) load8((const T*)a.rows + id * a.pitch + j, left(a.n, j), v);
+        const T* const from = (const T*)a.rows + (known ? id : 0L) * a.pitch;
+        T* const to = (T*)a.out + t * a.n;
+        P v[CH];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = known ? v[e] * a.scale : __builtin_nanf("");
-            store8((T*)a.out + t * a.n + j, left(a.n, j), v);
+        for (int c = 0; c < CH; ++c) {
+            const int j = first + c * lanes * V, at = j > a.n - V ? a.n - V : j;
+            if (j < a.n && known) v[c].load(from + at, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int j = first + c * lanes * V, at = j > a.n - V ? a.n - V : j;
+            if (j >= a.n) continue;
+            if (a.scale != 1.f || !known) {
+                float f[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] = known ? v[c][e] * a.scale : __builtin_nanf("");
+                v[c].set(f);
+            }
+            v[c].store(to + at, 0);
         }
     }
 }
@@ -502,7 +535,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a) {
 constexpr int SORT_TOKENS = 8192, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ROUNDS = SORT_TOKENS / SORT_THREADS;
 constexpr int DIGIT_BITS = 7;  // at most; histograms of 128 digits for each of 16 waves
 constexpr int MERGE_LISTS = 16;
-constexpr int CLEAR_BYTES = SORT_THREADS * 64;  // of a workgroup
+constexpr int CLEAR_BYTES = SORT_THREADS * 128;  // of a workgroup
 
 struct Sorted {
     int *key, *at;  // ids (vocab: none that counts) in order, and the tokens they are of
@@ -522,15 +555,19 @@ __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpa
     const int first = blockIdx.x * SORT_TOKENS, count = a.tokens - first < SORT_TOKENS ? a.tokens - first : SORT_TOKENS;
     const int rounds = (count + SORT_THREADS - 1) / SORT_THREADS;  // of each wave, whose tokens are back to back
     const int passes = (bits + DIGIT_BITS - 1) / DIGIT_BITS, digit_bits = (bits + passes - 1) / passes;
-    uint32_t key[SORT_ROUNDS], rank[SORT_ROUNDS];
-    uint16_t at[SORT_ROUNDS];
-    for (int r = 0; r < rounds; ++r) {
+    uint32_t key[SORT_ROUNDS], moved[SORT_ROUNDS];  // the token in the upper half, its place among those of its digit and wave in the lower one
+    long id[SORT_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r) {  // all asked for at once
         const int i = (wave * rounds + r) * 64 + lane;
-        if (i < count) {
-            const long id = id_at(a.ids, a.wide, (long)first + i);
-            s.key[i] = id >= 0 && id < a.vocab && id != a.skip ? (uint32_t)id : (uint32_t)a.vocab;
-            s.at[i] = (uint16_t)i;
-        }
+        id[r] = r < rounds && i < count ? id_at(a.ids, a.wide, (long)first + i) : -1;
+    }
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r) {
+        const int i = (wave * rounds + r) * 64 + lane;
+        if (r >= rounds || i >= count) continue;
+        s.key[i] = id[r] >= 0 && id[r] < a.vocab && id[r] != a.skip ? (uint32_t)id[r] : (uint32_t)a.vocab;
+        s.at[i] = (uint16_t)i;
     }
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = pass * digit_bits, digits = 1 << digit_bits;
@@ -543,18 +580,23 @@ __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpa
             const uint64_t here = __ballot(in);
             if (here == 0) continue;
             key[r] = in ? s.key[i] : 0;
-            at[r] = in ? s.at[i] : (uint16_t)0;
+            const uint32_t token = in ? s.at[i] : 0;
             const uint32_t d = key[r] >> shift & (digits - 1);
-            uint64_t same = here;
-            for (int b = 0; b < digit_bits; ++b) {
-                const uint64_t set = __ballot(d >> b & 1);
-                same &= d >> b & 1 ? set : ~set;
+            uint32_t low = (uint32_t)here, high = (uint32_t)(here >> 32);  // the lanes with this digit
+#pragma unroll
+            for (int b = 0; b < DIGIT_BITS; ++b) {
+                if (b >= digit_bits) break;
+                const uint32_t bit = (uint32_t)((int32_t)(d << (31 - b)) >> 31);  // of all lanes, where this one's is set
+                const uint64_t set = __ballot(bit != 0);
+                low &= ~((uint32_t)set ^ bit);
+                high &= ~((uint32_t)(set >> 32) ^ bit);
             }
+            const uint64_t same = (uint64_t)high << 32 | low;
             const uint64_t before = same & ((1ull << lane) - 1);
             uint32_t base = 0;
             if (in && before == 0) base = atomicAdd(&s.count[d * SORT_WAVES + wave], (uint32_t)__popcll(same));  // the first of them, for all
             base = __shfl(base, in ? __ffsll((unsigned long long)same) - 1 : lane, 64);
-            rank[r] = base + __popcll(before);
+            moved[r] = token << 16 | (base + __popcll(before));
         }
         __syncthreads();
         // places of digits and, within a digit, of waves: sums of what stands before, of as many counts in a row by each thread as there are
@@ -573,7 +615,8 @@ __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpa
         if (lane == 63) s.total[wave] = upto;
         __syncthreads();
         uint32_t place = upto - mine;
-        for (int w = 0; w < wave; ++w) place += s.total[w];
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) place += w < wave ? s.total[w] : 0;
         for (int e = 0; e < each; ++e) {
             const int i = threadIdx.x * each + e;
             if (i < digits * SORT_WAVES) {
@@ -587,9 +630,9 @@ __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpa
         for (int r = 0; r < SORT_ROUNDS; ++r) {
             const int i = (wave * rounds + r) * 64 + lane;
             if (r < rounds && i < count) {
-                const uint32_t to = s.count[(key[r] >> shift & (digits - 1)) * SORT_WAVES + wave] + rank[r];
+                const uint32_t to = s.count[(key[r] >> shift & (digits - 1)) * SORT_WAVES + wave] + (moved[r] & 0xffff);
                 s.key[to] = key[r];
-                s.at[to] = at[r];
+                s.at[to] = (uint16_t)(moved[r] >> 16);
             }
         }
         __syncthreads();
@@ -600,7 +643,7 @@ __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpa
     }
 }
 template <typename T>
-__global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const EmbeddingArgs a, int sorters, int bits, Sorted out) {
+__global__ void __launch_bounds__(SORT_THREADS, 8) embedding_sort_kernel(const EmbeddingArgs a, int sorters, int bits, Sorted out) {
     __shared__ SortSpace space;
     if ((int)blockIdx.x < sorters) {
         sort_block(a, bits, out, space);
@@ -620,30 +663,49 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const Embe
     }
 }
 
-// Lists of `length` sorted tokens, the last one shorter: every 16 of them become one.
-__global__ void __launch_bounds__(256) embedding_merge_kernel(Sorted in, Sorted out, int tokens, int length) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= tokens) return;
-    const int key = in.key[i], own = (int)(i / length);
-    const int group = own / MERGE_LISTS * MERGE_LISTS;
+// Lists of `length` sorted tokens, the last one shorter: every 16 of them become one.  A search begins among samples of a list in LDS, so that a
+// few of its steps only go to memory, those of all lists at once.
+constexpr int MERGE_THREADS = 512, SAMPLES = 256;
+static_assert(SORT_TOKENS % SAMPLES == 0, "samples at equal distances");
+__global__ void __launch_bounds__(MERGE_THREADS) embedding_merge_kernel(Sorted in, Sorted out, int tokens, int length) {
+    __shared__ int sample[MERGE_LISTS][SAMPLES];
+    const int first = blockIdx.x * MERGE_THREADS, own = first / length;  // (lists are whole numbers of workgroups long)
+    const int group = own / MERGE_LISTS * MERGE_LISTS, step = length / SAMPLES;
     const long start = (long)group * length;
-    int lo[MERGE_LISTS], size[MERGE_LISTS];
+    int size[MERGE_LISTS];
 #pragma unroll
     for (int l = 0; l < MERGE_LISTS; ++l) {
         const long rest = tokens - (start + (long)l * length);
-        lo[l] = 0;
         size[l] = group + l == own || rest <= 0 ? 0 : rest < length ? (int)rest : length;
+        for (int i = threadIdx.x; i * (long)step < size[l]; i += MERGE_THREADS) sample[l][i] = in.key[start + (long)l * length + i * (long)step];
     }
+    __syncthreads();
+    const long i = (long)first + threadIdx.x;
+    if (i >= tokens) return;
+    const int key = in.key[i];
     // how many of a list stand before: those with a smaller id, and with the same one where the list stands before the own one
-    for (int left = length; left > 0; left >>= 1) {  // more halvings than any list needs
+    const auto below = [&](int l, int other) { return group + l < own ? other <= key : other < key; };
+    int lo[MERGE_LISTS];
+#pragma unroll
+    for (int l = 0; l < MERGE_LISTS; ++l) {
+        int at = 0, left = (size[l] + step - 1) / step;
+        while (left > 0) {
+            const int half = left >> 1;
+            if (below(l, sample[l][at + half])) at += half + 1, left -= half + 1;
+            else left = half;
+        }
+        // sample at - 1 stands before, sample `at` does not
+        lo[l] = at == 0 ? 0 : (at - 1) * step + 1;
+        size[l] = at == 0 ? 0 : (size[l] < at * step ? size[l] : at * step) - lo[l];
+    }
+    for (int left = step - 1; left > 0; left >>= 1) {
 #pragma unroll
         for (int l = 0; l < MERGE_LISTS; ++l) {
             if (size[l] > 0) {
                 const int half = size[l] >> 1;
-                const int probe = in.key[start + (long)l * length + lo[l] + half];
-                const bool below = group + l < own ? probe <= key : probe < key;
-                lo[l] = below ? lo[l] + half + 1 : lo[l];
-                size[l] = below ? size[l] - half - 1 : half;
+                const bool b = below(l, in.key[start + (long)l * length + lo[l] + half]);
+                lo[l] = b ? lo[l] + half + 1 : lo[l];
+                size[l] = b ? size[l] - half - 1 : half;
             }
         }
     }
@@ -654,105 +716,152 @@ __global__ void __launch_bounds__(256) embedding_merge_kernel(Sorted in, Sorted 
     out.at[to] = in.at[i];
 }
 
-// How the sorted tokens are cut: `chunk` of them to a group of `lanes` lanes, which takes lanes * 8 columns; `slabs` such pieces make a row.
-struct Cut {
-    int chunk, chunks, lanes, slabs;
+// The sorted tokens in `count` chunks of `length`, the last one shorter.
+struct Chunks {
+    int length, count;
 };
-template <typename T>
-__global__ void __launch_bounds__(256) embedding_add_kernel(const EmbeddingArgs a, Sorted s, Cut c, float* parts) {
-    constexpr int AHEAD = 8;
-    const int lane = threadIdx.x & (c.lanes - 1);
-    const long g = ((long)blockIdx.x * 256 + threadIdx.x) / c.lanes;
-    const int slab = (int)(g % c.slabs);
-    const long chunk = g / c.slabs;
-    const int j = (slab * c.lanes + lane) * 8;
-    if (chunk >= c.chunks || j >= a.n) return;
-    const int count = left(a.n, j);
-    const int first = (int)(chunk * c.chunk), last = a.tokens - first < c.chunk ? a.tokens : first + c.chunk;
+// A value of another lane of the group, whose lanes are a whole wave's where it is WIDE.
+template <bool WIDE> __device__ __forceinline__ int from_lane(int v, int i) { return WIDE ? __builtin_amdgcn_readlane(v, i) : __shfl(v, i, 64); }
+// A group of lanes takes a segment of a chunk's rows.  Ids and places of its next tokens are in the lanes, a token each; AHEAD rows are asked for at once.
+template <typename T, typename P, bool WIDE>
+__global__ void __launch_bounds__(256) embedding_add_kernel(const EmbeddingArgs a, Sorted s, Chunks c, Cut cut, float* parts) {
+    constexpr int V = P::V, AHEAD = 8;
+    const int shift = WIDE ? 6 : cut.shift, lanes = 1 << shift, lane = threadIdx.x & (lanes - 1), base = (threadIdx.x & 63) - lane;
+    long g = ((long)blockIdx.x * 256 + threadIdx.x) >> shift;
+    if (WIDE) g = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long chunk = g / cut.segments;
+    if (chunk >= c.count) return;
+    const int j = ((int)(g - chunk * cut.segments) * lanes + lane) * V, at = j > a.n - V ? a.n - V : j;
+    const bool in = j < a.n;
+    const int first = (int)(chunk * c.length), last = a.tokens - first < c.length ? a.tokens : first + c.length;
+    const int before = first > 0 ? s.key[first - 1] : -1, behind = last < a.tokens ? s.key[last] : -1;
     int key = s.key[first];
-    const bool goes_on = first > 0 && s.key[first - 1] == key;  // from the chunk before
-    bool head = goes_on;
-    float sum[8] = {};
-    const T* rows = (const T*)a.rows + j;
-    for (int t0 = first; t0 < last && key < a.vocab; t0 += AHEAD) {
-        float v[AHEAD][8];
+    bool head = before == key;  // the run goes on from the chunk before
+    float sum[V];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (t0 + u < last) load8(rows + s.at[t0 + u] * a.pitch, count, v[u]);
+    for (int e = 0; e < V; ++e) sum[e] = 0.f;
+    const auto leave = [&](bool part, int which) {
+        if (!in) return;
+        if (part) {
+            float* const p = parts + (chunk * 2 + which) * a.n + at;
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            if (t0 + u >= last) break;
-            const int k = s.key[t0 + u];
-            if (k != key) {
-                if (key < a.vocab) {
-                    if (head) {
-                        float* p = parts + (chunk * 2) * a.n + j;
-                        store8(p, count, sum);
-                    } else {
+            for (int e = 0; e < V; ++e) p[e] = sum[e];
+        } else {
+            P out;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
-                        store8((T*)a.out + (long)key * a.n + j, count, sum);
-                    }
-                }
-                head = false;
-                key = k;
+            for (int e = 0; e < V; ++e) sum[e] *= a.scale;
+            out.set(sum);
+            out.store((T*)a.out + (long)key * a.n + at, 0);
+        }
+    };
+    for (int t0 = first; t0 < last && key < a.vocab; t0 += lanes) {
+        const int here = last - t0 < lanes ? last - t0 : lanes;  // tokens that the lanes hold
+        const int my_key = lane < here ? s.key[t0 + lane] : -1, my_place = lane < here ? s.at[t0 + lane] : 0;
+        for (int u0 = 0; u0 < here && key < a.vocab; u0 += AHEAD) {  // (there are 8 lanes at least)
+            P row[AHEAD];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+            for (int u = 0; u < AHEAD; ++u) {
+                const long place = from_lane<WIDE>(my_place, base + u0 + u);
+                if (u0 + u < here && in) row[u].load((const T*)a.rows + place * a.pitch, (unsigned)at * (unsigned)sizeof(T));
             }
+            // all of them are here before the first sum leaves: waits count loads and stores alike, and one behind a store would wait for that too
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += v[u][e];
+            for (int u = 0; u < AHEAD; ++u) asm volatile("" : "+v"(row[u].raw));
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int k = from_lane<WIDE>(my_key, base + u0 + u);
+                if (u0 + u >= here) continue;
+                if (k != key) {
+                    if (key < a.vocab) leave(head, 0);
+                    head = false;
+                    key = k;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sum[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] += row[u][e];
+            }
         }
     }
-    if (key >= a.vocab) return;
-    const bool tail = last < a.tokens && s.key[last] == key;
-    if (head || tail) {
-        store8(parts + (chunk * 2 + (head ? 0 : 1)) * a.n + j, count, sum);
-    } else {
+    if (key < a.vocab) leave(head || behind == key, head ? 0 : 1);
+}
+// A wave for each of eight chunks and 512 columns: where a run begins in the chunk and goes on behind it, its parts are added up, by the wave alone where
+// they are few, and by all eight, in turn, where they are many.
+constexpr int JOIN_WAVES = 8, JOIN_FEW = 16;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WAVES * 64) embedding_join_kernel(const EmbeddingArgs a, Sorted s, Chunks c, const float* parts) {
+    __shared__ float sums[JOIN_WAVES][64][9];
+    __shared__ int ends[JOIN_WAVES], keys[JOIN_WAVES];
+    const int slabs = (a.n + 511) / 512, slab = blockIdx.x % slabs, chunk0 = blockIdx.x / slabs * JOIN_WAVES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = slab * 512 + lane * 8;
+    const int count = left(a.n, j), chunk = chunk0 + wave;
+    int end = 0, key = 0;  // the chunk that the run ends in, 0: none
+    if (chunk + 1 < c.count) {
+        const int first = chunk * c.length, next = first + c.length;
+        key = s.key[next - 1];
+        const int behind = s.key[next], begin = s.key[first], before = first > 0 ? s.key[first - 1] : -1;
+        if (key < a.vocab && behind == key && !(begin == key && before == key)) {
+            // the last chunk that begins with the id: 64 of them are looked at in one go
+            int lo = chunk + 1, size = c.count - lo;
+            while (size > 1) {
+                const int step = (size + 63) / 64, at = lane * step;
+                const uint64_t with = __ballot(at < size && s.key[(long)(lo + at < c.count ? lo + at : lo) * c.length] == key);
+                const int most = 63 - __clzll((long long)with);  // (lane 0 looks at one that does)
+                lo += most * step;
+                size = size - most * step < step ? size - most * step : step;
+            }
+            end = lo;
+        }
+    }
+    const bool few = end > 0 && end - chunk < JOIN_FEW;
+    if (lane == 0) {
+        ends[wave] = few ? 0 : end;
+        keys[wave] = key;
+    }
+    float sum[8] = {};
+    const auto leave = [&](int id) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] *= a.scale;
-        store8((T*)a.out + (long)key * a.n + j, count, sum);
-    }
-}
-// A workgroup for each chunk and slab: where a run begins in the chunk and goes on behind it, its waves take the parts in turn.
-constexpr int JOIN_WAVES = 8;
-template <typename T>
-__global__ void __launch_bounds__(JOIN_WAVES * 64) embedding_join_kernel(const EmbeddingArgs a, Sorted s, Cut c, const float* parts) {
-    __shared__ float sums[JOIN_WAVES][64][9];
-    const int slabs = (a.n + 511) / 512;
-    const int chunk = blockIdx.x / slabs, slab = blockIdx.x % slabs;
-    const int first = chunk * c.chunk, next = first + c.chunk;  // (the last chunk has no workgroup)
-    const int key = s.key[next - 1];
-    if (key >= a.vocab || s.key[next] != key || (s.key[first] == key && first > 0 && s.key[first - 1] == key)) return;
-    int lo = next, size = a.tokens - next;  // the end of the run
-    while (size > 0) {
-        const int half = size >> 1;
-        if (s.key[lo + half] <= key) lo += half + 1, size -= half + 1;
-        else size = half;
-    }
-    const int end = (lo - 1) / c.chunk;  // the chunk that it ends in
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = slab * 512 + lane * 8;
-    const int count = left(a.n, j);
-    float sum[8] = {};
-    if (j < a.n) {
-        if (wave == 0) load8(parts + (chunk * 2L + 1) * a.n + j, count, sum);
+        store8((T*)a.out + (long)id * a.n + j, count, sum);
+    };
+    if (few && j < a.n) {
+        load8(parts + (chunk * 2L + 1) * a.n + j, count, sum);
 #pragma unroll 4
-        for (int p = chunk + 1 + wave; p <= end; p += JOIN_WAVES) {
+        for (int p = chunk + 1; p <= end; ++p) {
             float v[8];
             load8(parts + p * 2L * a.n + j, count, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] += v[e];
         }
+        leave(key);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sums[wave][lane][e] = sum[e];
     __syncthreads();
-    if (wave > 0 || j >= a.n) return;
+    for (int w = 0; w < JOIN_WAVES; ++w) {
+        const int upto = ends[w];
+        if (upto == 0) continue;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        for (int w = 1; w < JOIN_WAVES; ++w) sum[e] += sums[w][lane][e];
-        sum[e] *= a.scale;
+        for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+        if (j < a.n) {
+            if (wave == 0) load8(parts + ((chunk0 + w) * 2L + 1) * a.n + j, count, sum);
+#pragma unroll 8
+            for (int p = chunk0 + w + 1 + wave; p <= upto; p += JOIN_WAVES) {
+                float v[8];
+                load8(parts + p * 2L * a.n + j, count, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += v[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[wave][lane][e] = sum[e];
+        __syncthreads();
+        if (wave == 0 && j < a.n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                for (int i = 1; i < JOIN_WAVES; ++i) sum[e] += sums[i][lane][e];
+            leave(keys[w]);
+        }
+        __syncthreads();
     }
-    store8((T*)a.out + (long)key * a.n + j, count, sum);
 }
 
 // ---- dropout ----------------------------------------------------------------------------------------
@@ -935,24 +1044,49 @@ hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cu
     return hipGetLastError();
 }
 
+namespace {
+// Lanes for a row of n values in pieces of v, at least 8 and at most `most`, with `pieces` each.
+Cut cut_row(int n, int v, int pieces, int most) {
+    Cut c{3, 1};
+    while ((1 << c.shift) < most && (1L << c.shift) * v * pieces < n) ++c.shift;
+    const long each = (1L << c.shift) * v * pieces;
+    c.segments = (int)(up(n, each) / each);
+    return c;
+}
+template <typename T, typename P, int CH>
+hipError_t run_embedding(const EmbeddingArgs& a, hipStream_t stream) {
+    const Cut c = cut_row(a.n, P::V, CH, 64);
+    const long groups = (long)a.tokens * c.segments, each = 256 >> c.shift;
+    hipLaunchKernelGGL((embedding_kernel<T, P, CH>), dim3(grid_of(up(groups, each) / each)), dim3(256), 0, stream, a, c);
+    return hipGetLastError();
+}
+template <typename T>
+hipError_t run_embedding(const EmbeddingArgs& a, hipStream_t stream) {
+    if (a.n < Piece<T>::V) return run_embedding<T, Single<T>, 1>(a, stream);
+    // few tokens are spread over more lanes
+    if ((long)a.tokens * a.n < 1 << 20) return run_embedding<T, Piece<T>, 1>(a, stream);
+    return run_embedding<T, Piece<T>, 4>(a, stream);
+}
+}  // namespace
+
 hipError_t launch_embedding(const EmbeddingArgs& a, hipStream_t stream) {
     if (a.tokens == 0 || a.n == 0) return hipSuccess;
-    const unsigned grid = grid_of(a.tokens);
-    if (a.dtype == MUON_HIP_BF16) hipLaunchKernelGGL(embedding_kernel<bf16_t>, dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(embedding_kernel<float>, dim3(grid), dim3(256), 0, stream, a);
-    return hipGetLastError();
+    return a.dtype == MUON_HIP_BF16 ? run_embedding<bf16_t>(a, stream) : run_embedding<float>(a, stream);
 }
 
 namespace {
-// Chunks are as many as fill the machine four waves deep on each of its 1024 SIMDs, and at most 2048, so that the parts of a run over all
-// of them are few; at least 8 tokens, which are loaded at once.
-Cut cut(int tokens, int n) {
-    Cut c;
-    for (c.lanes = 8; c.lanes < 64 && c.lanes * 8 < n; c.lanes *= 2) {}
-    c.slabs = (int)(up(n, c.lanes * 8) / (c.lanes * 8));
-    const long chunks = std::max(1L, std::min(2048L, 4096L * 64 / ((long)c.lanes * c.slabs)));
-    c.chunk = (int)std::max(8L, (tokens + chunks - 1) / chunks);
-    c.chunks = (tokens + c.chunk - 1) / c.chunk;
+// Chunks are as many as fill the machine four waves deep on each of its 1024 SIMDs, and at most 1024, so that the parts of a run over all of them
+// are few; at least 8 tokens, whose rows are asked for at once.
+Cut cut_sums(int n, int dtype) {
+    const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
+    return cut_row(n, n < v ? 1 : v, 1, 64);
+}
+Chunks chunks_of(int tokens, int n, int dtype) {
+    const Cut cut = cut_sums(n, dtype);
+    const long chunks = std::max(1L, std::min(1024L, 4096L * 64 / ((long)cut.segments << cut.shift)));
+    Chunks c;
+    c.length = (int)std::max(8L, (tokens + chunks - 1) / chunks);
+    c.count = (tokens + c.length - 1) / c.length;
     return c;
 }
 struct Lists {
@@ -960,7 +1094,7 @@ struct Lists {
     float* parts;
     long bytes;
 };
-Lists lay_out(void* workspace, int tokens, int n) {
+Lists lay_out(void* workspace, int tokens, int n, int dtype) {
     const long list = up(tokens, 64);
     int* p = (int*)workspace;
     Lists l{{p, p + list}, {}, nullptr, 0};
@@ -970,12 +1104,14 @@ Lists lay_out(void* workspace, int tokens, int n) {
         p += 2 * list;
     }
     l.parts = (float*)p;
-    l.bytes = ((char*)p - (char*)workspace) + 2L * cut(tokens, n).chunks * n * 4;
+    l.bytes = ((char*)p - (char*)workspace) + 2L * chunks_of(tokens, n, dtype).count * n * 4;
     return l;
 }
 }  // namespace
 
-long embedding_grad_workspace(int tokens, int vocab, int n, int) { return tokens == 0 || vocab == 0 || n == 0 ? 0 : lay_out(nullptr, tokens, n).bytes; }
+long embedding_grad_workspace(int tokens, int vocab, int n, int dtype) {
+    return tokens == 0 || vocab == 0 || n == 0 ? 0 : lay_out(nullptr, tokens, n, dtype).bytes;
+}
 
 template <typename T>
 static hipError_t run_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStream_t stream) {
@@ -983,20 +1119,25 @@ static hipError_t run_embedding_grad(const EmbeddingArgs& a, void* workspace, hi
     const int sorters = (int)(up(a.tokens, SORT_TOKENS) / SORT_TOKENS);
     int bits = 1;
     while (a.vocab >> bits) ++bits;  // ids and `vocab` itself
-    Lists l = lay_out(workspace, a.tokens, a.n);
+    Lists l = lay_out(workspace, a.tokens, a.n, a.dtype);
     const long clear = std::min(up(bytes, CLEAR_BYTES) / CLEAR_BYTES, MOST_THREADS / SORT_THREADS - sorters);
     hipLaunchKernelGGL(embedding_sort_kernel<T>, dim3((unsigned)(sorters + clear)), dim3(SORT_THREADS), 0, stream, a, sorters, bits, l.sorted);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || a.tokens == 0) return e;
     for (long length = SORT_TOKENS; length < a.tokens; length *= MERGE_LISTS) {
-        hipLaunchKernelGGL(embedding_merge_kernel, dim3((unsigned)(up(a.tokens, 256) / 256)), dim3(256), 0, stream, l.sorted, l.other, a.tokens, (int)length);
+        hipLaunchKernelGGL(embedding_merge_kernel, dim3((unsigned)(up(a.tokens, MERGE_THREADS) / MERGE_THREADS)), dim3(MERGE_THREADS), 0, stream, l.sorted, l.other, a.tokens, (int)length);
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         std::swap(l.sorted, l.other);
     }
-    const Cut c = cut(a.tokens, a.n);
-    const long lanes = (long)c.chunks * c.slabs * c.lanes;
-    hipLaunchKernelGGL(embedding_add_kernel<T>, dim3((unsigned)(up(lanes, 256) / 256)), dim3(256), 0, stream, a, l.sorted, c, l.parts);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess || c.chunks == 1) return e;
-    hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)((c.chunks - 1) * (up(a.n, 512) / 512))), dim3(JOIN_WAVES * 64), 0, stream, a, l.sorted, c, l.parts);
+    const Chunks c = chunks_of(a.tokens, a.n, a.dtype);
+    const Cut cut = cut_sums(a.n, a.dtype);
+    const long lanes = ((long)c.count * cut.segments) << cut.shift;
+    const auto kern = a.n < Piece<T>::V ? embedding_add_kernel<T, Single<T>, false>
+                    : cut.shift < 6     ? embedding_add_kernel<T, Piece<T>, false>
+                                        : embedding_add_kernel<T, Piece<T>, true>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(up(lanes, 256) / 256)), dim3(256), 0, stream, a, l.sorted, c, cut, l.parts);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || c.count == 1) return e;
+    hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((unsigned)(up(c.count - 1, JOIN_WAVES) / JOIN_WAVES * (up(a.n, 512) / 512))), dim3(JOIN_WAVES * 64), 0, stream, a,
+                       l.sorted, c, l.parts);
     return hipGetLastError();
 }
 hipError_t launch_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStream_t stream) {
@@ -1006,8 +1147,10 @@ hipError_t launch_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStr
 
 hipError_t launch_dropout(const DropoutArgs& a, hipStream_t stream) {
     if (a.count == 0) return hipSuccess;
-    const unsigned grid = grid_of(up(a.count, 2048) / 2048);
-    if (a.dtype == MUON_HIP_BF16) hipLaunchKernelGGL(dropout_kernel<bf16_t>, dim3(grid), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(dropout_kernel<float>, dim3(grid), dim3(256), 0, stream, a);
+    // A block of eight values to a thread, and two of them, half of the tensor apart, where bf16 values fill the machine many times over: 8192 x 12288 71.9 us
+    // where it took 77.5, with a residual 107 and 109.5; fp32 values, of which a thread has twice the bytes, lose 3 %, four blocks 2 %.
+    const long each = a.dtype == MUON_HIP_BF16 && a.count >= 1L << 24 ? 4096 : 2048;
+    const auto kern = a.dtype == MUON_HIP_BF16 ? dropout_kernel<bf16_t> : dropout_kernel<float>;
+    hipLaunchKernelGGL(kern, dim3(grid_of(up(a.count, each) / each)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
