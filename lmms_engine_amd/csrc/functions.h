@@ -58,12 +58,6 @@ int64_t rows_of(const Tensor& t) {
     for (int64_t d = 0; d + 1 < t.dim(); ++d) m *= t.size(d);
     return m;
 }
-// Memory for a result of the shape of x but for its last dimension.
-Tensor result(const Tensor& x, int64_t n) {
-    auto shape = x.sizes().vec();
-    shape.back() = n;
-    return at::empty(shape, x.options());
-}
 const void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Stands for the second derivatives that there are none of: whoever comes through here on the way to an input is told so.

@@ -44,6 +44,13 @@ Tensor matrix(const Tensor& t) {
     const Tensor b = bare(t);
     return b.dim() == 2 ? b : b.reshape({rows_of(b), b.size(-1)});
 }
+// Memory for a result of the shape of x but for its last dimension.
+Tensor result(const Tensor& x, int64_t n) {
+    auto shape = x.sizes().vec();
+    shape.back() = n;
+    return at::empty(shape, x.options());
+}
+
 // Memory for a factor that the backward pass multiplies by, in the form that the library keeps it in.
 Tensor factor(const Tensor& like, int64_t m, int64_t n) {
     return at::empty({muon_hip_product_aux_bytes(dtype_of(like), (int)m, (int)n)}, like.options().dtype(at::kByte));

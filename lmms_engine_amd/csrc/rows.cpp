@@ -9,13 +9,36 @@ namespace {
 
 constexpr int64_t MOST = 0x7fffffff;
 
-// The rows of t's last dimension, back to back within themselves: where they lie, if that is so, else a copy.
-Tensor lines(const Tensor& t) {
-    if (!t.defined()) return t;
-    Tensor b = bare(t);
-    if (b.dim() != 2) b = b.reshape({rows_of(b), b.size(-1)});
-    return (b.size(1) > 1 && b.stride(1) != 1) || (b.size(0) > 1 && b.stride(0) < b.size(1)) ? b.contiguous() : b;
-}
+// The rows of a tensor's last dimension, back to back within themselves: where they lie, if that is so, else in a copy that is kept here.  (A view for
+// the same costs a call half a microsecond each.)
+struct Lines {
+    Tensor copy;
+    const void* at = nullptr;
+    int64_t apart = 0;
+    explicit Lines(const Tensor& t) {
+        if (!t.defined()) return;
+        const int64_t n = t.dim() > 0 ? t.size(-1) : 1;
+        if (!t.is_neg() && t.is_contiguous()) {
+            at = t.data_ptr();
+            apart = n;
+            return;
+        }
+        Tensor b = bare(t);
+        if (b.dim() != 2) b = b.reshape({rows_of(b), n});
+        copy = (n > 1 && b.stride(1) != 1) || (b.size(0) > 1 && b.stride(0) < n) ? b.contiguous() : b;
+        at = copy.data_ptr();
+        apart = copy.stride(0);
+    }
+};
+// The values of a tensor in the row-major order of its shape.
+struct Values {
+    Tensor copy;
+    const void* at = nullptr;
+    explicit Values(const Tensor& t) {
+        if (t.defined() && (t.is_neg() || !t.is_contiguous())) copy = dense(t);
+        at = pointer(copy.defined() ? copy : t);
+    }
+};
 // The places of the tensors of a context: `always` of them, then those of `count` optional ones that there are.
 struct Places {
     AutogradContext* ctx;
@@ -36,25 +59,27 @@ struct Normed {
 };
 Normed norm_forward(int kind, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, double eps, bool keep) {
     const c10::DeviceGuard guard(x.device());
-    const Tensor x2 = lines(x), r2 = lines(r), w1 = dense(w), b1 = dense(b);
+    const Lines x2(x), r2(r);
+    const Values w1(w), b1(b);
+    const int64_t rows = rows_of(x);
     Normed f;
-    f.y = result(x, x.size(-1));
-    if (r.defined()) f.sum = result(x, x.size(-1));
-    if (keep) f.stats = at::empty({kind == MUON_HIP_NORM_LAYER ? 2 : 1, x2.size(0)}, x.options().dtype(at::kFloat));
+    f.y = at::empty(x.sizes(), x.options());
+    if (r.defined()) f.sum = at::empty(x.sizes(), x.options());
+    if (keep) f.stats = at::empty({kind == MUON_HIP_NORM_LAYER ? 2 : 1, rows}, x.options().dtype(at::kFloat));
     muon_hip_norm p{};
     p.kind = kind;
     p.dtype = dtype_of(x);
-    p.rows = (int)x2.size(0);
-    p.n = (int)x2.size(1);
-    p.x = x2.data_ptr();
-    p.x_row = x2.stride(0);
+    p.rows = (int)rows;
+    p.n = (int)x.size(-1);
+    p.x = x2.at;
+    p.x_row = x2.apart;
     if (r.defined()) {
-        p.residual = r2.data_ptr();
-        p.res_row = r2.stride(0);
+        p.residual = r2.at;
+        p.res_row = r2.apart;
         p.sum = f.sum.data_ptr();
     }
-    p.weight = pointer(w1);
-    p.bias = pointer(b1);
+    p.weight = w1.at;
+    p.bias = b1.at;
     p.eps = eps;
     p.y = f.y.data_ptr();
     p.stats = (float*)pointer(f.stats);
@@ -93,25 +118,22 @@ struct Norm : torch::autograd::Function<Norm> {
                 if (want_w) grads[1] = at::zeros({n}, like.options());
                 if (want_b) grads[2] = at::zeros({n}, like.options());
             } else if (want_x || want_r || want_w || want_b) {
-                const Tensor dy2 = lines(dy), s2 = lines(s), ds2 = lines(ds), w1 = dense(w);
+                const Lines dy2(dy), s2(s), ds2(ds);
+                const Values w1(w);
                 muon_hip_norm_grad p{};
                 p.kind = (int)ctx->saved_data["kind"].toInt();
                 p.dtype = dtype_of(like);
-                p.rows = (int)dy2.size(0);
+                p.rows = (int)rows_of(dy);
                 p.n = (int)n;
-                p.dy = dy2.data_ptr();
-                p.dy_row = dy2.stride(0);
-                if (s.defined()) {  // (not where the bias alone is trained)
-                    p.s = s2.data_ptr();
-                    p.s_row = s2.stride(0);
-                    p.stats = (const float*)stats.data_ptr();
-                }
-                if (ds.defined()) {
-                    p.ds = ds2.data_ptr();
-                    p.ds_row = ds2.stride(0);
-                }
-                p.weight = pointer(w1);
-                if (want_x || want_r) p.dx = (dx = result(like, n)).data_ptr();
+                p.dy = dy2.at;
+                p.dy_row = dy2.apart;
+                p.s = s2.at;  // (nothing where the bias alone is trained)
+                p.s_row = s2.apart;
+                p.stats = (const float*)pointer(stats);
+                p.ds = ds2.at;
+                p.ds_row = ds2.apart;
+                p.weight = w1.at;
+                if (want_x || want_r) p.dx = (dx = at::empty(like.sizes(), like.options())).data_ptr();
                 if (want_w) p.dweight = (grads[1] = at::empty({n}, like.options())).data_ptr();
                 if (want_b) p.dbias = (grads[2] = at::empty({n}, like.options())).data_ptr();
                 const long need = muon_hip_norm_grad_workspace(&p);
@@ -139,12 +161,13 @@ struct Norm : torch::autograd::Function<Norm> {
 
 Tensor embedding_forward(const Tensor& weight, const Tensor& ids, double scale) {
     const c10::DeviceGuard guard(weight.device());
-    const Tensor w2 = lines(weight), i1 = ids.contiguous();
+    const Lines w2(weight);
+    const Tensor i1 = ids.contiguous();
     auto shape = ids.sizes().vec();
     shape.push_back(weight.size(1));
     const Tensor y = at::empty(shape, weight.options());
-    if (const int rc = muon_hip_embedding(i1.data_ptr(), ids.scalar_type() == at::kLong, (int)ids.numel(), w2.data_ptr(), w2.stride(0), (int)w2.size(0),
-                                          (int)w2.size(1), dtype_of(weight), scale, y.data_ptr(), stream_of(weight)))
+    if (const int rc = muon_hip_embedding(i1.data_ptr(), ids.scalar_type() == at::kLong, (int)ids.numel(), w2.at, w2.apart, (int)weight.size(0),
+                                          (int)weight.size(1), dtype_of(weight), scale, y.data_ptr(), stream_of(weight)))
         raise("embedding", rc);
     return y;
 }
@@ -165,14 +188,15 @@ struct Embedding : torch::autograd::Function<Embedding> {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy.device());
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), n = dy.size(-1);
-            const Tensor dy2 = lines(dy), i1 = ids.contiguous();
+            const Lines dy2(dy);
+            const Tensor i1 = ids.contiguous();
             grads[0] = at::empty({vocab, n}, dy.options());
             const int tokens = (int)ids.numel(), dtype = dtype_of(dy);
             const long need = muon_hip_embedding_grad_workspace(tokens, (int)vocab, (int)n, dtype);
             if (need < 0) raise("embedding_grad", need);
             Tensor ws;
             if (need > 0) ws = at::empty({need}, dy.options().dtype(at::kByte));
-            if (const int rc = muon_hip_embedding_grad(i1.data_ptr(), ids.scalar_type() == at::kLong, tokens, dy2.data_ptr(), dy2.stride(0), (int)vocab, (int)n,
+            if (const int rc = muon_hip_embedding_grad(i1.data_ptr(), ids.scalar_type() == at::kLong, tokens, dy2.at, dy2.apart, (int)vocab, (int)n,
                                                        dtype, ctx->saved_data["scale"].toDouble(), (int)ctx->saved_data["skip"].toInt(),
                                                        grads[0].data_ptr(), need > 0 ? ws.data_ptr() : nullptr, (size_t)need, stream_of(dy)))
                 raise("embedding_grad", rc);
@@ -186,9 +210,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
 
 Tensor dropout_forward(const Tensor& x, const Tensor& r, const Tensor& seed_at, double p, int64_t seed, int64_t site) {
     const c10::DeviceGuard guard(x.device());
-    const Tensor x1 = dense(x), r1 = dense(r);
+    const Values x1(x), r1(r);
     const Tensor y = at::empty(x.sizes(), x.options());
-    if (const int rc = muon_hip_dropout(x1.data_ptr(), pointer(r1), y.data_ptr(), x.numel(), dtype_of(x), p, (unsigned long long)seed, pointer(seed_at),
+    if (const int rc = muon_hip_dropout(x1.at, r1.at, y.data_ptr(), x.numel(), dtype_of(x), p, (unsigned long long)seed, pointer(seed_at),
                                         (unsigned)site, stream_of(x)))
         raise("dropout", rc);
     return y;
