@@ -460,6 +460,16 @@ typedef struct {
 long muon_hip_norm_grad_workspace(const muon_hip_norm_grad* p);
 int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* How such a call is computed on a device of `cus` compute units.  For tests and measurements. */
+typedef struct {
+    int lanes;   /* of a row */
+    int pieces;  /* of 16 bytes that each of them holds; 0: rows of less than a piece or too long for registers, a workgroup each */
+    int ragged;  /* whether rows are no whole number of pieces */
+    int threads; /* of a workgroup */
+    long groups; /* workgroups of the launch */
+} muon_hip_norm_route;
+int muon_hip_route_norm(int kind, int dtype, int rows, int n, int backward, int cus, muon_hip_norm_route* out);
+
 /* out[t] = table[ids[t]] * scale for `tokens` ids, 64-bit integers (wide_ids) or 32-bit ones, into a table of `vocab` rows.  An id outside
  * of it reads nothing: its row of `out` is NaN.
  * Its gradient: dtable[v] = scale * the sum of dy[t] over the tokens whose id is v, in their order; rows without tokens are zero, and so is row `skip` (-1:

@@ -93,6 +93,12 @@ class NormGrad(ctypes.Structure):
                 ("dweight", c_void_p), ("dbias", c_void_p)]
 
 
+class NormRoute(ctypes.Structure):
+    """muon_hip_norm_route"""
+
+    _fields_ = [("lanes", c_int), ("pieces", c_int), ("ragged", c_int), ("threads", c_int), ("groups", c_long)]
+
+
 # name -> (restype, argtypes); mirrors include/muon_hip.h one to one
 SIGNATURES = {
     "muon_hip_version": (c_int, []),
@@ -148,6 +154,7 @@ SIGNATURES = {
     "muon_hip_norm_run": (c_int, [c_void_p] * 2),
     "muon_hip_norm_grad_workspace": (c_long, [c_void_p]),
     "muon_hip_norm_grad_run": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "muon_hip_route_norm": (c_int, [c_int] * 6 + [c_void_p]),
     "muon_hip_embedding": (c_int, [c_void_p, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_double, c_void_p, c_void_p]),
     "muon_hip_embedding_grad_workspace": (c_long, [c_int] * 4),
     "muon_hip_embedding_grad": (c_int, [c_void_p, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_double, c_int, c_void_p, c_void_p, c_size_t,
@@ -297,6 +304,13 @@ def product_route(p: Product, cus: int = 256) -> ProductRoute:
     """How a product is computed on a device of `cus` compute units."""
     out = ProductRoute()
     check(lib().muon_hip_route_product(ctypes.addressof(p), cus, ctypes.addressof(out)), "route_product")
+    return out
+
+
+def norm_route(kind: int, dtype: int, rows: int, n: int, backward: bool, cus: int = 256) -> NormRoute:
+    """How a norm, or its gradient, is computed on a device of `cus` compute units."""
+    out = NormRoute()
+    check(lib().muon_hip_route_norm(kind, dtype, rows, n, int(backward), cus, ctypes.addressof(out)), "route_norm")
     return out
 
 

@@ -1193,7 +1193,7 @@ int check_norm_grad(const muon_hip_norm_grad* p) {
     return 0;
 }
 long norm_grad_bytes(const muon_hip_norm_grad* p, int cus) {
-    return (p->dweight != nullptr) + (p->dbias != nullptr) == 0 ? 0 : ((p->dweight != nullptr) + (p->dbias != nullptr)) * norm_grad_groups(*p, cus) * p->n * 4;
+    return (p->dweight != nullptr) + (p->dbias != nullptr) == 0 ? 0 : ((p->dweight != nullptr) + (p->dbias != nullptr)) * norm_route(p->kind, p->dtype, p->rows, p->n, true, cus).groups * p->n * 4;
 }
 
 int check_table(int tokens, int vocab, int n, int dtype) {
@@ -1248,6 +1248,14 @@ int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t 
     Timed t(MUON_HIP_K_NORM_GRAD, s);
     hipError_t e = launch_norm_grad(*p, (float*)workspace, ms.cus, s);
     return e == hipSuccess ? 0 : hip_fail(e, "norm_grad launch");
+}
+
+int muon_hip_route_norm(int kind, int dtype, int rows, int n, int backward, int cus, muon_hip_norm_route* out) {
+    if (!out || cus < 1) return fail(MUON_HIP_EINVAL, "bad device or output");
+    if (kind != MUON_HIP_NORM_LAYER && kind != MUON_HIP_NORM_RMS) return fail(MUON_HIP_EINVAL, "kind %d of norm", kind);
+    if (int rc = check_sizes(dtype, rows, n)) return rc;
+    *out = norm_route(kind, dtype, rows, n, backward != 0, cus);
+    return 0;
 }
 
 int muon_hip_embedding(const void* ids, int wide_ids, int tokens, const void* table, long table_row, int vocab, int n, int dtype, double scale,

@@ -4,8 +4,8 @@
 #include "../../include/muon_hip.h"
 #include "common.h"
 
-// Workgroups of the first pass of a norm's gradients on a device of `cus` compute units, each of which leaves a row of sums behind.
-long norm_grad_groups(const muon_hip_norm_grad& p, int cus);
+// How a norm or its gradient is computed on a device of `cus` compute units; each workgroup of a gradient leaves a row behind for each sum over the rows.
+muon_hip_norm_route norm_route(int kind, int dtype, int rows, int n, bool backward, int cus);
 hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream);
 hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cus, hipStream_t stream);
 

@@ -941,6 +941,22 @@ Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most) {
     l.threads = std::max(threads, (int)lanes());
     return l;
 }
+// Up to four pieces of each row are under way in a lane: 8192 x 4096 bf16 with a residual 48.1 us, with up to eight 51.5, two 48.6 to 49, one 51.
+Layout lay_norm(int dtype, long rows, int n) { return lay_rows(dtype, rows, n, 256, 4, 8); }
+// A lane of a gradient holds the sums of its columns besides: 16 values of a row at most, of a layer norm, which has two sums, 8, or there are too few waves
+// (8192 x 4096 bf16 with a residual: RMS 52 us, with 32 values 62; layer norm 60, with 16 or 32 73).
+Layout lay_grad(int kind, int dtype, long rows, int n) {
+    const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
+    const bool layer = kind == MUON_HIP_NORM_LAYER;
+    return lay_rows(dtype, rows, n, 512, (layer ? 8 : 16) / v, (layer && dtype == MUON_HIP_F32 ? 16 : 32) / v);
+}
+// As many workgroups as are at work at once, each of which takes rows until there are none left: their registers allow 16, 12 or 8 waves to a compute unit.
+// (Half as many 60 us in place of 52, twice as many 59.)
+long grad_groups(int kind, int dtype, long rows, const Layout& l, int cus) {
+    const int values = l.pieces * (dtype == MUON_HIP_BF16 ? 8 : 4);
+    const int waves = l.pieces == 0 ? 8 : values <= (kind == MUON_HIP_NORM_LAYER ? 8 : 16) ? 16 : values <= 16 ? 12 : 8;
+    return std::min(up(rows, l.rows()) / l.rows(), (long)std::max(1, waves * 64 / l.threads) * cus);
+}
 template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_of(const Layout& l) {
     if constexpr (CH == 1)
@@ -974,33 +990,18 @@ auto norm_grad_of(const Layout& l, bool centred) {
     if (centred) return l.ragged ? norm_grad_of<T, true, true>(l) : norm_grad_of<T, true, false>(l);
     return l.ragged ? norm_grad_of<T, false, true>(l) : norm_grad_of<T, false, false>(l);
 }
-#ifndef FWD_BEST
-#define FWD_BEST 4
-#endif
-#ifndef BWD_BEST
-#define BWD_BEST (p.kind == MUON_HIP_NORM_LAYER ? 8 : 16)
-#endif
-#ifndef BWD_THREADS
-#define BWD_THREADS 512
-#endif
-#ifndef BWD_PER_CU
-#define BWD_PER_CU 2
-#endif
-Layout lay_grad(const muon_hip_norm_grad& p) {
-    const int v = p.dtype == MUON_HIP_BF16 ? 8 : 4;
-    return lay_rows(p.dtype, p.rows, p.n, BWD_THREADS, BWD_BEST / v, (p.dtype == MUON_HIP_F32 && p.kind == MUON_HIP_NORM_LAYER ? 16 : 32) / v);
-}
-long grad_groups_per_cu(const muon_hip_norm_grad& p, const Layout& l) {
-    const int values = l.pieces * (p.dtype == MUON_HIP_BF16 ? 8 : 4);
-    const int waves = values <= (p.kind == MUON_HIP_NORM_LAYER ? 8 : 16) ? 16 : values <= 16 ? 12 : 8;
-    return std::max(1, std::min(BWD_PER_CU * 8, waves) * 64 / l.threads);
-}
 }  // namespace
+
+muon_hip_norm_route norm_route(int kind, int dtype, int rows, int n, bool backward, int cus) {
+    const Layout l = backward ? lay_grad(kind, dtype, rows, n) : lay_norm(dtype, rows, n);
+    const long groups = backward ? grad_groups(kind, dtype, rows, l, cus) : std::min(up(rows, l.rows()) / l.rows(), MOST_THREADS / l.threads);
+    return muon_hip_norm_route{1 << l.shift, l.pieces, l.ragged, l.threads, groups};
+}
 
 hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
     if (p.rows == 0 || p.n == 0) return hipSuccess;
     const bool bf = p.dtype == MUON_HIP_BF16, centred = p.kind == MUON_HIP_NORM_LAYER;
-    const Layout l = lay_rows(p.dtype, p.rows, p.n, 256, FWD_BEST, 8);
+    const Layout l = lay_norm(p.dtype, p.rows, p.n);
     if (l.pieces == 0) {
         void (*kern)(const muon_hip_norm);
         if (bf) kern = centred ? norm_streamed_kernel<bf16_t, true> : norm_streamed_kernel<bf16_t, false>;
@@ -1013,16 +1014,11 @@ hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-long norm_grad_groups(const muon_hip_norm_grad& p, int cus) {
-    const Layout l = lay_grad(p);
-    return std::min(up(p.rows, l.rows()) / l.rows(), grad_groups_per_cu(p, l) * cus);
-}
-
 hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cus, hipStream_t stream) {
     if (p.n == 0) return hipSuccess;
     const bool bf = p.dtype == MUON_HIP_BF16, centred = p.kind == MUON_HIP_NORM_LAYER;
-    const long groups = norm_grad_groups(p, cus);
-    const Layout l = lay_grad(p);
+    const Layout l = lay_grad(p.kind, p.dtype, p.rows, p.n);
+    const long groups = grad_groups(p.kind, p.dtype, p.rows, l, cus);
     if (groups > 0) {
         if (l.pieces == 0) {
             void (*kern)(const muon_hip_norm_grad, float*);

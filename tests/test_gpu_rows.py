@@ -1,4 +1,6 @@
 """embedding, layer_norm, rms_norm and dropout against their formulas in 64 bits (rows_reference.py)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -54,15 +56,20 @@ def compare_norm(kind, x, w, b, r, eps, dy, ds, got):
             R.check(name, got[name], *want["dx" if name == "dr" else name], dtype)
 
 
-# columns: one, less than a vector, whole ones and odd ones, every number of threads to a row, more than fits into registers
-COLUMNS = [1, 5, 8, 12, 64, 100, 128, 251, 256, 500, 896, 1024, 1028, 2047, 2048, 4096, 4100, 6144, 8192, 12288, 16381, 16384, 33000, 70001]
+# columns: one, less than a piece, whole pieces and odd ones, every number of lanes to a row, more than fits into registers; test_rows_host.py holds these
+# lists to running every kernel
+COLUMNS = [1, 5, 8, 12, 64, 100, 128, 251, 256, 500, 896, 1024, 1028, 2047, 2048, 4096, 4100, 6144, 8192, 12288, 10001, 2502, 5005, 16381, 16384, 20000, 24577, 33000, 70001]
+
+
+def ROWS_OF(n):
+    return (1, 3, 70 if n < 20000 else 5)
 
 
 @pytest.mark.parametrize("n", COLUMNS)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_norms_of_all_widths(kind, dtype, n):
-    for rows in (1, 3, 70 if n < 20000 else 5):
+    for rows in ROWS_OF(n):
         g = gen_of(kind, dtype, n, rows)
         print(kind, dtype, rows, n, flush=True)
         x, r, dy, ds = (rnd(g, rows, n, dtype=dtype) for _ in range(4))
@@ -74,7 +81,10 @@ def test_norms_of_all_widths(kind, dtype, n):
             compare_norm(kind, x, weight, bias, residual, 1e-5, dy, ds, got)
 
 
-@pytest.mark.parametrize("rows,n", [(777, 251), (2100, 128), (5000, 80), (1030, 1024), (1500, 4096), (600, 2056), (300, 8192)])
+MANY_ROWS = [(777, 251), (2100, 128), (5000, 80), (1030, 1024), (1500, 4096), (600, 2056), (300, 8192), (4200, 2048), (2100, 4090), (4200, 1000)]
+
+
+@pytest.mark.parametrize("rows,n", MANY_ROWS)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_norms_of_many_rows(kind, dtype, rows, n):
@@ -346,7 +356,7 @@ def compare_dropout(x, p, seed, site, r, dy, got):
     return kept
 
 
-@pytest.mark.parametrize("shape", [(1,), (7,), (8,), (9,), (3, 5, 11), (64, 896), (1237, 333), (1500, 1001)])
+@pytest.mark.parametrize("shape", [(1,), (7,), (8,), (9,), (3, 5, 11), (64, 896), (1237, 333), (1500, 1001), (4100, 4099)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_dropouts(dtype, shape):
     g = gen_of(dtype, shape)
@@ -424,6 +434,68 @@ def test_shares_that_are_kept():
             assert abs(m.float().mean().item() - p) < far + 2 ** -20
         both, next_to = (masks[0] & masks[1]).float().mean().item(), (masks[0][1:] & masks[0][:-1]).float().mean().item()
         assert abs(both - p * p) < 5 * p / n ** 0.5 and abs(next_to - p * p) < 5 * p / n ** 0.5
+
+
+# ---- entry points -----------------------------------------------------------------------------------
+
+
+def test_nothing_is_written_beside_the_results():
+    """Results in the middle of larger buffers, at addresses of any element: what lies around them stays as it was."""
+    lib, stream = _abi.lib(), torch.cuda.current_stream().cuda_stream
+    g = gen_of("beside")
+    for dtype in DTYPES:
+        code, size = _abi.dtype_code(dtype), dtype.itemsize
+        for rows, n in ((5, 77), (33, 264), (3, 5), (2, 4099)):
+            count = rows * n
+
+            def around(values):
+                return torch.full((values + 14,), 7.0, dtype=dtype, device=DEV)
+
+            def beside(t, values):
+                assert bool((t[:7] == 7).all()) and bool((t[7 + values:] == 7).all())
+
+            x, r, dy, ds = (rnd(g, count + 3, dtype=dtype)[3:] for _ in range(4))
+            w = rnd(g, n + 1, dtype=dtype)[1:]
+            y, s, dx, dw, db = (around(v) for v in (count, count, count, n, n))
+            stats = torch.full((2 * rows + 2,), 7.0, device=DEV)
+            p = _abi.Norm(kind=_abi.NORM_LAYER, dtype=code, rows=rows, n=n, x=x.data_ptr(), x_row=n, residual=r.data_ptr(), res_row=n, weight=w.data_ptr(), eps=1e-5,
+                          y=y.data_ptr() + 7 * size, sum=s.data_ptr() + 7 * size, stats=stats.data_ptr() + 4)
+            _abi.check(lib.muon_hip_norm_run(ctypes.addressof(p), stream))
+            q = _abi.NormGrad(kind=_abi.NORM_LAYER, dtype=code, rows=rows, n=n, dy=dy.data_ptr(), dy_row=n, s=s.data_ptr() + 7 * size, s_row=n, ds=ds.data_ptr(), ds_row=n,
+                              weight=w.data_ptr(), stats=stats.data_ptr() + 4, dx=dx.data_ptr() + 7 * size, dweight=dw.data_ptr() + 7 * size, dbias=db.data_ptr() + 7 * size)
+            need = lib.muon_hip_norm_grad_workspace(ctypes.addressof(q))
+            ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=DEV)
+            assert lib.muon_hip_norm_grad_run(ctypes.addressof(q), ws.data_ptr(), need - 1, stream) == -1
+            _abi.check(lib.muon_hip_norm_grad_run(ctypes.addressof(q), ws.data_ptr(), need, stream))
+            for t, values in ((y, count), (s, count), (dx, count), (dw, n), (db, n)):
+                beside(t, values)
+            assert stats[0] == 7 and stats[-1] == 7 and bool((ws[need:] == 9).all())
+            got = {"y": y[7:7 + count].view(rows, n), "s": s[7:7 + count].view(rows, n), "dx": dx[7:7 + count].view(rows, n), "dw": dw[7:7 + n], "db": db[7:7 + n]}
+            compare_norm("layer", x.view(rows, n), w, None, r.view(rows, n), 1e-5, dy.view(rows, n), ds.view(rows, n), got)
+
+            vocab = 19
+            table, out, grad = rnd(g, vocab * n + 1, dtype=dtype)[1:], around(count), around(vocab * n)
+            ids = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+            _abi.check(lib.muon_hip_embedding(ids.data_ptr(), 1, rows, table.data_ptr(), n, vocab, n, code, 1.0, out.data_ptr() + 7 * size, stream))
+            beside(out, count)
+            assert torch.equal(out[7:7 + count].view(rows, n), table.view(vocab, n)[ids])
+            need = lib.muon_hip_embedding_grad_workspace(rows, vocab, n, code)
+            ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=DEV)
+            args = (ids.data_ptr(), 1, rows, dy.data_ptr(), n, vocab, n, code, 1.0, -1, grad.data_ptr() + 7 * size, ws.data_ptr())
+            assert lib.muon_hip_embedding_grad(*args, need - 1, stream) == -1
+            _abi.check(lib.muon_hip_embedding_grad(*args, need, stream))
+            beside(grad, vocab * n)
+            assert bool((ws[need:] == 9).all())
+            R.check("dw", grad[7:7 + vocab * n].view(vocab, n), *R.embedding_grad(ids, dy.double().view(rows, n), vocab, 1.0), dtype)
+
+            out = around(count)
+            _abi.check(lib.muon_hip_dropout(x.data_ptr(), None, out.data_ptr() + 7 * size, count, code, 0.5, 3, None, 1, stream))
+            beside(out, count)
+            want = E.dropout(x, 0.5, seed=3, site=1)
+            assert torch.equal(out[7:7 + count], want)
+            own = x.clone()
+            _abi.check(lib.muon_hip_dropout(own.data_ptr(), None, own.data_ptr(), count, code, 0.5, 3, None, 1, stream))  # in place
+            assert torch.equal(own, want)
 
 
 # ---- all of them --------------------------------------------------------------------------------------

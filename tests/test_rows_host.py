@@ -97,6 +97,49 @@ def test_norms_are_checked_before_any_launch(change, code, match):
     assert match in lib.muon_hip_last_error().decode()
 
 
+def kernel(kind, dtype, rows, n, backward):
+    r = _abi.norm_route(kind, dtype, rows, n, backward)
+    # lanes below a wave's are a kernel of their own, which has one piece
+    return (kind, dtype, backward, r.pieces) + ((bool(r.ragged), r.lanes < 64) if r.pieces else ())
+
+
+def test_the_gpu_tests_run_every_kernel_of_the_norms():
+    from tests.test_gpu_rows import COLUMNS, MANY_ROWS, ROWS_OF
+
+    cases = [(m, n) for n in COLUMNS for m in ROWS_OF(n)] + MANY_ROWS
+    sizes = [(m, n) for m in (1, 70, 2000, 5000, 300000) for n in list(range(1, 200)) + list(range(200, 40000, 37)) + [2 ** i for i in range(17)]]
+    for kind in (_abi.NORM_LAYER, _abi.NORM_RMS):
+        for dtype in (_abi.F32, _abi.BF16):
+            for backward in (False, True):
+                ran, there_are = ({kernel(kind, dtype, m, n, backward) for m, n in some} for some in (cases, sizes))
+                assert there_are <= ran, there_are - ran
+                assert len(there_are) >= 9
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("dtype", [_abi.F32, _abi.BF16])
+def test_norms_are_laid_over_whole_rows_and_launches(dtype, backward):
+    piece = 4 if dtype == _abi.F32 else 8
+    for kind in (_abi.NORM_LAYER, _abi.NORM_RMS):
+        for n in list(range(1, 300)) + [1000, 4096, 8200, 16384, 16385, 32769, 70001, 0x7fffffff - (1 << 20)]:
+            for rows in (1, 9, 4097, 0x7fffffff):
+                r = _abi.norm_route(kind, dtype, rows, n, backward)
+                assert 0 < r.groups * r.threads < 2 ** 32 and r.threads % 64 == 0 and r.threads <= 512
+                if r.pieces:
+                    assert r.lanes * r.pieces * piece >= n >= piece and r.lanes <= r.threads and bool(r.ragged) == (n % piece != 0)
+                    assert r.pieces == 1 or r.lanes >= 64
+                    if backward:  # the columns' sums of several rows at once meet in LDS
+                        assert r.threads <= max(r.lanes, 64) or 4 * n <= 64 * 1024
+                if backward:
+                    assert r.groups <= 1024
+    lib = _abi.lib()
+    out = _abi.NormRoute()
+    assert lib.muon_hip_route_norm(3, dtype, 4, 8, 0, 256, ctypes.addressof(out)) == -1
+    assert lib.muon_hip_route_norm(0, 5, 4, 8, 0, 256, ctypes.addressof(out)) == -1
+    assert lib.muon_hip_route_norm(0, dtype, 4, 8, 0, 0, ctypes.addressof(out)) == -1
+    assert lib.muon_hip_route_norm(0, dtype, 4, 8, 0, 256, None) == -1
+
+
 def norm_grad(**change):
     p = _abi.NormGrad(kind=_abi.NORM_LAYER, dtype=_abi.BF16, rows=4, n=8, dy=ONE, dy_row=8, s=ONE, s_row=8, weight=ONE, stats=ONE, dx=ONE, dweight=ONE, dbias=ONE)
     for name, v in change.items():
