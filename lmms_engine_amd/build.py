@@ -10,6 +10,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -101,8 +102,11 @@ def build_library(verbose: bool = False) -> str:
     _build_scan(verbose)
     _compile_and_link(PROBE_SOURCES, PROBE_LIB, hipcc, verbose)
     lib = _compile_and_link(SOURCES, LIB, hipcc, verbose)
-    _build_functions("layers.cpp", LAYERS_LIB, "LAYERS_TORCH_VERSION", hipcc, verbose)
-    _build_functions("rows.cpp", ROWS_LIB, "ROWS_TORCH_VERSION", hipcc, verbose)
+    with ThreadPoolExecutor(2) as pool:  # torch's headers take half a minute each
+        modules = [pool.submit(_build_functions, "layers.cpp", LAYERS_LIB, "LAYERS_TORCH_VERSION", hipcc, verbose),
+                   pool.submit(_build_functions, "rows.cpp", ROWS_LIB, "ROWS_TORCH_VERSION", hipcc, verbose)]
+        for m in modules:
+            m.result()
     return lib
 
 

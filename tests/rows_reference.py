@@ -77,14 +77,15 @@ def norm_grad(kind, s, w, eps, dy, ds):
 
 
 def embedding_grad(ids, dy, vocab, scale, skip=-1):
-    dw, mag = (torch.zeros(vocab, dy.size(-1), dtype=torch.float64, device=dy.device) for _ in range(2))
-    count = torch.zeros(vocab, dtype=torch.float64, device=dy.device)
+    device, ids, dy = dy.device, ids.cpu(), dy.cpu()  # (a GPU adds to one row in turn)
+    dw, mag = (torch.zeros(vocab, dy.size(-1), dtype=torch.float64) for _ in range(2))
+    count = torch.zeros(vocab, dtype=torch.float64)
     fine = (ids >= 0) & (ids < vocab) & (ids != skip)
     at = ids[fine].long()
     dw.index_add_(0, at, dy[fine] * scale)
     mag.index_add_(0, at, dy[fine].abs() * abs(scale))
     count.index_add_(0, at, torch.ones_like(at, dtype=torch.float64))
-    return dw, (count[:, None] + 3) * F * mag
+    return dw.to(device), ((count[:, None] + 3) * F * mag).to(device)
 
 
 def philox(c, key):
