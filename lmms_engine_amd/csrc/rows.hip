@@ -60,6 +60,11 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 // A row is held in the registers of its lanes, 8 to 512 of them: it is read once, its mean is taken before the squares of what is left are
 // summed, and no sum of squares cancels.  A lane has CH pieces of 16 bytes, neighbouring lanes neighbouring pieces.  Where a row is no whole number of
 // pieces (RAGGED), its last one begins a piece before the row's end: it overlaps the one before, and what it has twice counts once.  Rows at any address.
+//
+// Bound by memory.  8192 x 4096 bf16 values: the RMS norm of x + residual, four streams of them, takes 45 us (5.9 TB/s), its gradient, four streams
+// too, 46 (5.8 TB/s) and 4 for the last sums of the weight's; a layer norm's gradient 55.  262144 rows of 128 (16 lanes each): 26 us (5.1) and 34 (5.9).
+// One row of 4096: 2.5 us.  A large copy reaches 4.9 on the same card.  Asking for the next row before the present one is through changed none of
+// these by more than 2 %: there are waves enough to take turns.
 constexpr int MOST_LANES = 512;  // of a row, and threads of a workgroup: 256 registers each
 template <typename T> struct Piece;
 template <> struct Piece<bf16_t> {
@@ -162,7 +167,8 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
         const long r = r0 + row_of<WIDE>(shift);
         const bool row = r < p.rows;
-        Piece<T> x[CH], res[CH];
+        constexpr int EARLY = CH <= 2 ? CH : 0;
+        Piece<T> x[CH], res[CH], w[EARLY + 1], b[EARLY + 1];
         float s[CH][V];
         const T* const px = (const T*)p.x + r * p.x_row;
 #pragma unroll
@@ -170,6 +176,14 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
             x[c].raw = {};
             if (row && at.in(c)) x[c].load(px, at.bytes(c));
         }
+        // weights are asked for with the row where there is room for them (262144 rows of 128: 26.3 us in place of 29, 4096 x 1024 9.1 in place of 9.4)
+        const auto weights = [&](int c, Piece<T>& wc, Piece<T>& bc) {
+            if (!row || !at.in(c)) return;
+            if (p.weight) wc.load(p.weight, at.bytes(c));
+            if (p.bias) bc.load(p.bias, at.bytes(c));
+        };
+#pragma unroll
+        for (int c = 0; c < EARLY; ++c) weights(c, w[c], b[c]);
         if (p.residual) {
             const T* const pr = (const T*)p.residual + r * p.res_row;
             T* const ps = (T*)p.sum + r * p.n;
@@ -222,15 +236,15 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             if (!at.in(c)) continue;
-            Piece<T> w, b, y;
+            constexpr bool LATE = EARLY == 0;
+            Piece<T> y, &wc = w[LATE ? 0 : c], &bc = b[LATE ? 0 : c];
             float v[V];
-            if (p.weight) w.load(p.weight, at.bytes(c));
-            if (p.bias) b.load(p.bias, at.bytes(c));
+            if (LATE) weights(c, wc, bc);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[e] = s[c][e] * rstd;
-                if (p.weight) v[e] *= w[e];
-                if (p.bias) v[e] += b[e];
+                if (p.weight) v[e] *= wc[e];
+                if (p.bias) v[e] += bc[e];
             }
             y.set(v);
             y.store(py, at.bytes(c));
@@ -489,7 +503,8 @@ __device__ __forceinline__ long id_at(const void* ids, int wide, long t) { retur
 struct Cut {
     int shift, segments;
 };
-// A group of lanes for each segment of each token, all of whose loads are under way before the first store.  The last piece of a ragged row overlaps the one
+// A group of lanes for each segment of each token, all of whose loads are under way before the first store: 8192 rows of 4096 bf16 values from a table of
+// 151936 take 25 us (5.2 TB/s of results and rows).  The last piece of a ragged row overlaps the one
 // before it: what it has twice is written twice.  An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
 template <typename T, typename P, int CH>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, Cut cut) {
@@ -525,13 +540,16 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, C
 }
 // The table's gradient.  The tokens are sorted by id, keeping their order among equal ones, and the sorted tokens cut into chunks of equal length,
 // whatever ids are in them: one id may have most of the tokens, as the placeholders of an image do.
-//   sort_and_clear  one launch: a workgroup sorts up to 8192 tokens in LDS, the others clear the table meanwhile (151936 x 4096 in bf16 is 1.2 GB, which
-//                   takes longer than any of the rest)
-//   merge           joins up to 16 sorted lists, where there are more tokens than that: a token's place is its place in its own list and
-//                   what binary searches in the other ones say
-//   add             a chunk's lanes walk over its tokens: the sum of a run of equal ids is the table's row, or, where the run goes on in a neighbouring
-//                   chunk, one of two rows of fp32 that a chunk has for that
-//   join            adds those up, in their order.
+//   sort    one launch: a workgroup sorts up to 8192 tokens in LDS (24 us: a digit of up to 7 bits at a time, bound by the vector instructions of 16 waves
+//           on one compute unit), the others clear the table meanwhile, which for large tables takes longer than any of the rest
+//   merge   joins up to 16 sorted lists, where there are more tokens than that: a token's place is its place in its own list and what binary
+//           searches in the other ones say (16384 tokens 10 us, 131072 29)
+//   add     a chunk's lanes walk over its tokens: the sum of a run of equal ids is the table's row, or, where the run goes on in a neighbouring
+//           chunk, one of two rows of fp32 that a chunk has for that
+//   join    adds those up, in their order.
+// Bound by memory: 8192 tokens into 151936 x 4096 bf16 values take 195 us to clear 1.24 GB (6.4 TB/s; a fill alone 6.9), 35 to add up 67 MB, while the
+// memory-side cache still writes back what was cleared (268 MB of gradients after as many of cleared table: 85, in whatever order and by
+// however many waves), and 8 to join.
 constexpr int SORT_TOKENS = 8192, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ROUNDS = SORT_TOKENS / SORT_THREADS;
 constexpr int DIGIT_BITS = 7;  // at most; histograms of 128 digits for each of 16 waves
 constexpr int MERGE_LISTS = 16;
@@ -865,6 +883,10 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) embedding_join_kernel(const E
 }
 
 // ---- dropout ----------------------------------------------------------------------------------------
+// Bound by memory: 8192 x 12288 bf16 values take 72 us (5.6 TB/s), with a residual 107 (5.6); with three rounds of the generator in place of ten
+// the first took 70.6 where it took 77.8 with one block to a thread.  Sixteen random bits a value instead of 32 are what makes it so: a thread draws one block
+// for its eight values.
+//
 // Philox4x32-10: Salmon, Moraes, Dror and Shaw, Parallel random numbers: as easy as 1, 2, 3 (2011).
 __device__ __forceinline__ u32x4 philox(u32x4 c, uint32_t k0, uint32_t k1) {
 #pragma unroll
