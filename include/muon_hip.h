@@ -420,7 +420,7 @@ int muon_hip_act_grad(const void* dy, int factors, const void* d0, const void* d
  * muon_hip_norm_grad_run: with g = dy * weight and hat = (s - mean) * rstd (s * rstd),
  *   LAYER  dx = rstd * (g - mean(g) - hat * mean(g * hat)) + ds
  *   RMS    dx = rstd * (g - hat * mean(g * hat)) + ds
- *   dweight = the sum of dy * hat over the rows, dbias that of dy.
+ *   dweight = the sum of dy * hat over the rows, dbias that of dy (of LAYER; null with RMS).
  * ds, the gradient of `sum`, may be null; dx, dweight and dbias where they are not wanted; dbias alone
  * needs no s and no stats.  dx is the gradient of x and of the residual. */
 #define MUON_HIP_NORM_LAYER 0

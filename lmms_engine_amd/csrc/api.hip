@@ -1186,6 +1186,7 @@ int check_norm_grad(const muon_hip_norm_grad* p) {
     if (!p) return fail(MUON_HIP_EINVAL, "null norm");
     if (p->kind != MUON_HIP_NORM_LAYER && p->kind != MUON_HIP_NORM_RMS) return fail(MUON_HIP_EINVAL, "kind %d of norm", p->kind);
     if (int rc = check_sizes(p->dtype, p->rows, p->n)) return rc;
+    if (p->kind == MUON_HIP_NORM_RMS && p->dbias) return fail(MUON_HIP_EINVAL, "an RMS norm has no bias");
     if (p->rows == 0 || p->n == 0) return 0;
     if (!p->dy || ((p->dx || p->dweight) && (!p->s || !p->stats))) return fail(MUON_HIP_EINVAL, "null gradient, input or statistics");
     if (rows_overlap(p->dy, p->dy_row, p->rows, p->n) || rows_overlap(p->s, p->s_row, p->rows, p->n) || rows_overlap(p->ds, p->ds_row, p->rows, p->n))

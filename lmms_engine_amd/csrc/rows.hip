@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(256) embedding_add_kernel(const EmbeddingArgs 
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const long place = from_lane<WIDE>(my_place, base + u0 + u);
-                if (u0 + u < here && in) row[u].load((const T*)a.rows + place * a.pitch, (unsigned)at * (unsigned)sizeof(T));
+                if (u0 + u < here && in) row[u].load((const T*)a.rows + place * a.pitch + at, 0);
             }
             // all of them are here before the first sum leaves: waits count loads and stores alike, and one behind a store would wait for that too
 #pragma unroll

@@ -21,6 +21,7 @@ second derivatives, tensor subclasses and recording (torch.jit.trace, make_fx, f
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -73,8 +74,10 @@ def dropout(x: Tensor, p: float = 0.5, *, seed: Union[int, Tensor], site: int = 
     bits, or an int64 tensor of one element on x's device that is read when the kernels run (for a recorded HIP graph, whose replays would
     otherwise repeat one mask); it has to hold the same value in the backward pass.  `site` is a whole number below 2^32.  p is taken to 32 bits,
     and 1 / (1 - p) of what is taken."""
-    if not isinstance(seed, Tensor) and not -2 ** 63 <= seed < 2 ** 64:
-        raise ValueError(f"seed {seed} is no number of 64 bits")
+    if not isinstance(seed, Tensor):
+        seed = operator.index(seed)
+        if not -2 ** 63 <= seed < 2 ** 64:
+            raise ValueError(f"seed {seed} is no number of 64 bits")
     if not 0 <= site < 2 ** 32:
         raise ValueError(f"site {site} is no number of 32 bits")
     out = _abi.rows().dropout(x, residual, p, seed, site)

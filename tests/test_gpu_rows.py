@@ -1,12 +1,16 @@
 """embedding, layer_norm, rms_norm and dropout against their formulas in 64 bits (rows_reference.py)."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
+
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import lmms_engine_amd as E
 from lmms_engine_amd import _abi
 from tests import rows_reference as R
+from tests.test_layers_recording import RECORDERS
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -412,6 +416,7 @@ def test_numbers_go_by_the_place_in_a_shape(dtype):
 def test_a_seed_in_device_memory():
     g = gen_of("seed")
     x, dy = rnd(g, 70, 33), rnd(g, 70, 33)
+    assert torch.equal(E.dropout(x, 0.2, seed=np.int64(5), site=np.int32(1)), E.dropout(x, 0.2, seed=5, site=1))
     for seed in (5, -5, 2 ** 40 + 3):
         at = torch.tensor([seed], device=DEV)
         assert all(torch.equal(a, e) for a, e in zip(run_dropout(x, 0.2, at, 1, x, dy), run_dropout(x, 0.2, seed, 1, x, dy)))
@@ -517,7 +522,6 @@ def test_values_beyond_32_bit_offsets():
     y = E.dropout(x, 0.3, seed=8)[-24:].clone()
     first = (rows - 24) * n
     assert first % 8 == 0 and first > 2 ** 31
-    import numpy as np
     kept = torch.from_numpy(R.numbers(24 * n, 8, 0, first) >= int(np.rint(0.3 * 2 ** 32))).to(DEV).view(24, n)
     assert torch.equal(y != 0, kept & (tail != 0))
 
@@ -627,6 +631,74 @@ def test_inputs_that_gradients_read_may_not_change():
     ids.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(y.sum(), x)
+
+
+CALLS = {"embedding": lambda x, w: E.embedding(torch.arange(3, device=DEV), x), "layer_norm": lambda x, w: E.layer_norm(x, w, residual=x)[0],
+         "rms_norm": lambda x, w: E.rms_norm(x, w), "dropout": lambda x, w: E.dropout(x, 0.5, seed=1, residual=x)}
+
+
+def both_ways(f, x, w):
+    y = f(x, w)
+    leaves = [t for t in (x, w) if t.requires_grad]
+    return [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y), allow_unused=True)]
+
+
+@pytest.mark.parametrize("record", RECORDERS)
+@pytest.mark.parametrize("name", list(CALLS))
+def test_recording_is_refused(name, record):
+    x, w = torch.ones(4, 16, device=DEV), torch.ones(16, device=DEV)
+    with pytest.raises(NotImplementedError, match="recorded"):
+        record(CALLS[name], x, w)
+    y = CALLS[name](x.requires_grad_(True), w)
+    with pytest.raises(NotImplementedError, match="recorded"):
+        make_fx(lambda dy: torch.autograd.grad(y, x, dy, retain_graph=True)[0])(torch.ones_like(y))
+    assert torch.isfinite(torch.autograd.grad(y, x, torch.ones_like(y))[0]).all()  # and afterwards calls are taken again
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_recomputed_and_compiled_passes_give_the_same(name):
+    from torch.utils.checkpoint import checkpoint
+    from torch.utils.flop_counter import FlopCounterMode
+
+    g = gen_of(name, "again")
+    x, w = rnd(g, 6, 16).requires_grad_(True), rnd(g, 16).requires_grad_(True)
+
+    def f(a, b):
+        return CALLS[name](a * 2, b).relu() + 1
+
+    def same(got):
+        for a, e in zip(got, both_ways(f, x, w)):
+            assert a is e is None or torch.equal(a, e)
+
+    same(both_ways(lambda a, b: checkpoint(f, a, b, use_reentrant=False), x, w))
+    same(both_ways(torch.compile(f, backend="eager"), x, w))
+    with FlopCounterMode(display=False):
+        got = both_ways(f, x, w)
+    same(got)
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_the_same_tensor_twice_and_parameters(name):
+    """A tensor that is input and residual at once gets both gradients; parameters are tensors like others."""
+    g = gen_of(name, "twice")
+    x, r, w = rnd(g, 5, 40), rnd(g, 5, 40), rnd(g, 40)
+    if name == "embedding":
+        p = torch.nn.Parameter(x)
+        ids = torch.tensor([1, 1, 4], device=DEV)
+        (E.embedding(ids, p).sum() + E.embedding(ids, p, scale=2.0).sum()).backward()
+        assert torch.equal(p.grad.sum(1), torch.tensor([0.0, 240.0, 0.0, 0.0, 120.0], device=DEV))
+        return
+    call = {"layer_norm": lambda a, b: E.layer_norm(a, w, residual=b), "rms_norm": lambda a, b: E.rms_norm(a, w, residual=b),
+            "dropout": lambda a, b: (E.dropout(a, 0.5, seed=1, residual=b),)}[name]
+    p = torch.nn.Parameter(x)
+    outs = call(p, p)
+    torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+    a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    outs = call(a, b)
+    torch.autograd.backward(outs, [torch.ones_like(o) for o in outs])
+    assert torch.equal(p.grad, a.grad + b.grad)
+    a.grad.zero_()  # each leaf has a gradient of its own
+    assert b.grad.any()
 
 
 def test_kernels_are_timed_by_name():

@@ -70,6 +70,8 @@ def ids(*values, dtype=torch.int64):
     (lambda: E.dropout(gpu(2, 8), 0.1, seed=ids(1, dtype=torch.int32)), TypeError, "seed: "),
     (lambda: E.dropout(gpu(2, 8), 0.1, seed=torch.tensor([1])), _abi.MuonHipError, "seed must live on a GPU"),
     (lambda: E.dropout(gpu(2, 8), 0.1), TypeError, "seed"),
+    (lambda: E.dropout(gpu(2, 8), 0.1, seed=1.5), TypeError, "integer"),
+    (lambda: E.dropout(gpu(2, 8), 0.1, seed="1"), TypeError, "integer"),
     (lambda: E.dropout(gpu(2, 8), 0.1, seed=1, residual=gpu(2, 1)), ValueError, "residual has shape"),
     (lambda: E.dropout(gpu(2, 8), 0.1, seed=1), NotImplementedError, "OnGpu"),
 ])
@@ -150,7 +152,7 @@ def norm_grad(**change):
 @pytest.mark.parametrize("change,code,match", [
     (dict(kind=-1), -1, "kind"), (dict(dtype=2), -1, "dtype"), (dict(rows=-1), -1, "size"), (dict(n=0x7fffffff), -2, "the most"), (dict(dy=None), -1, "null"),
     (dict(s=None), -1, "null"), (dict(stats=None, dx=None), -1, "null"), (dict(dy_row=7), -1, "overlap"), (dict(s_row=-8), -1, "overlap"),
-    (dict(ds=ONE, ds_row=1), -1, "overlap"),
+    (dict(ds=ONE, ds_row=1), -1, "overlap"), (dict(kind=_abi.NORM_RMS), -1, "no bias"),
 ])
 def test_gradients_of_norms_are_checked_before_any_launch(change, code, match):
     lib, p = _abi.lib(), norm_grad(**change)
