@@ -574,6 +574,30 @@ def test_passes_are_recorded_and_replayed(dtype):
             everything(x.detach(), ids, table.detach(), w.detach(), b.detach(), 5)  # eager work of the program's own in between
 
 
+def test_two_graphs_take_turns():
+    """Each has workspaces of its own, whichever is replayed between two replays of the other."""
+    g = gen_of("two graphs")
+    sets = [leaves_of(g, BF16, t=t, n=264, v=77) for t in (50, 700)]
+
+    def grads(i):
+        x, ids, table, w, b = sets[i]
+        return torch.autograd.grad(everything(x, ids, table, w, b, 3 + i), (x, table, w, b))
+
+    want = [grads(i) for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            got.append(grads(i))
+    for i in (0, 1, 1, 0, 1, 0):
+        for t in got[i]:
+            t.zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(got[i], want[i])), i
+
+
 def test_two_streams_at_once():
     g = gen_of("streams")
     sets = [leaves_of(g, BF16, t=600, n=1000, v=200) for _ in range(2)]
