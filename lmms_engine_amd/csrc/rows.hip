@@ -57,7 +57,7 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 }
 
 // ---- norms ------------------------------------------------------------------------------------------
-// A row is held in the registers of its lanes, 8 to 512 of them: it is read once, its mean is taken before the squares of what is left are
+// A row is held in the registers of its lanes, 8 to 1024 of them: it is read once, its mean is taken before the squares of what is left are
 // summed, and no sum of squares cancels.  A lane has CH pieces of 16 bytes, neighbouring lanes neighbouring pieces.  Where a row is no whole number of
 // pieces (RAGGED), its last one begins a piece before the row's end: it overlaps the one before, and what it has twice counts once.  Rows at any address.
 //
@@ -65,7 +65,7 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 // too, 46 (5.8 TB/s) and 4 for the last sums of the weight's; a layer norm's gradient 55.  262144 rows of 128 (16 lanes each): 26 us (5.1) and 34 (5.9).
 // One row of 4096: 2.5 us.  A large copy reaches 4.9 on the same card.  Asking for the next row before the present one is through changed none of
 // these by more than 2 %: there are waves enough to take turns.
-constexpr int MOST_LANES = 512;  // of a row, and threads of a workgroup: 256 registers each
+constexpr int MOST_LANES = 1024, MOST_WAVES = MOST_LANES / 64;  // of a row; half as many where they need more than 128 registers each
 template <typename T> struct Piece;
 template <> struct Piece<bf16_t> {
     static constexpr int V = 8;
@@ -117,16 +117,27 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
     if (lanes > 32) v = across<32>(v);
     return v;
 }
-// The same where a row has several waves, of K values at once: waves 0 to lanes / 64 - 1 of each row in `part`.  Calls alternate between two arrays.
+// Which of a workgroup's rows a thread works on, and as which of the row's lanes.  WIDE rows have whole waves: their addresses are in scalar registers, of
+// which all streams share the offsets of the pieces.  Other rows have 8, 16 or 32 lanes.
+struct Spot {
+    int row, lane;
+};
+template <bool WIDE> __device__ __forceinline__ Spot spot_of(int lanes) {
+    const int t = threadIdx.x;
+    if (!WIDE) return {t >> __builtin_ctz(lanes), t & (lanes - 1)};
+    const int row = __builtin_amdgcn_readfirstlane(t >> 6) / (lanes >> 6);
+    return {row, t - row * lanes};
+}
+// The same where a row has several waves, of K values at once, by way of LDS.  Calls alternate between two arrays.
 template <int K>
-__device__ __forceinline__ void row_sum(float (&v)[K], int lanes, float (*part)[8]) {
+__device__ __forceinline__ void row_sum(float (&v)[K], int lanes, int row, float (*part)[MOST_WAVES]) {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = lanes_sum(v[k], lanes);
     if (lanes <= 64) return;
-    const int wave = threadIdx.x >> 6, waves = lanes >> 6, first = wave & ~(waves - 1);
+    const int waves = lanes >> 6, first = row * waves;
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) part[k][wave] = v[k];
+        for (int k = 0; k < K; ++k) part[k][threadIdx.x >> 6] = v[k];
     }
     __syncthreads();
 #pragma unroll
@@ -149,23 +160,15 @@ struct Place {
     __device__ __forceinline__ bool counts(int c, int e) const { return in(c) && (!RAGGED || at(c) + e >= begin(c)); }
 };
 
-// Which of a workgroup's rows a thread works on.  WIDE rows have whole waves: their addresses are in scalar registers, of which all streams share
-// the offsets of the pieces.
-template <bool WIDE>
-__device__ __forceinline__ int row_of(int shift) {
-    const int r = (int)threadIdx.x >> shift;
-    return WIDE ? __builtin_amdgcn_readfirstlane(r) : r;
-}
-
 template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
-__global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p, int shift) {
+__global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_norm p, int lanes) {
     constexpr int V = Piece<T>::V;
-    __shared__ float part[2][1][8];
-    const int lanes = 1 << shift;
-    const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
-    const int each = blockDim.x >> shift;
+    __shared__ float part[2][1][MOST_WAVES];
+    const Spot spot = spot_of<WIDE>(lanes);
+    const Place<T, CH, RAGGED> at{spot.lane, lanes, p.n};
+    const int each = blockDim.x / lanes;
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
-        const long r = r0 + row_of<WIDE>(shift);
+        const long r = r0 + spot.row;
         const bool row = r < p.rows;
         constexpr int EARLY = CH <= 2 ? CH : 0;
         Piece<T> x[CH], res[CH], w[EARLY + 1], b[EARLY + 1];
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
             }
         }
         if (CENTRED) {
-            row_sum(total, lanes, part[0]);
+            row_sum(total, lanes, spot.row, part[0]);
             mean = total[0] / (float)p.n;  // (a quotient: a row of one value has that one for its mean)
         }
         total[0] = 0.f;
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
                 else total[0] += !RAGGED || at.counts(c, e) ? s[c][e] * s[c][e] : 0.f;  // (what is not there is zero)
             }
         }
-        row_sum(total, lanes, part[1]);
+        row_sum(total, lanes, spot.row, part[1]);
         const float rstd = 1.f / sqrtf(total[0] / (float)p.n + (float)p.eps);
         if (!CENTRED && lanes > 64) __syncthreads();  // (one sum a row: the next one writes where this one is read)
         if (!row) continue;
@@ -254,14 +257,19 @@ __global__ void __launch_bounds__(MOST_LANES) norm_kernel(const muon_hip_norm p,
 
 // The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
 // once, and written as one row of `partials`.
+// Waves that a SIMD holds of a gradient with so many values of a row in a lane, by the registers that their sums, one of each value or two, leave; and the
+// lanes that a row can have with all of a compute unit's.
+constexpr int grad_waves(int values, bool centred) { return values <= 8 && centred ? 5 : values <= 16 && !centred ? 4 : values <= 16 ? 3 : 2; }
+constexpr int grad_lanes(int values, bool centred) { return grad_waves(values, centred) >= 4 ? MOST_LANES : 256 * grad_waves(values, centred); }
 template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
-__global__ void __launch_bounds__(MOST_LANES, CH * Piece<T>::V <= (CENTRED ? 8 : 16) ? 4 : CH * Piece<T>::V <= 16 ? 3 : 2) norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int shift) {
+__global__ void __launch_bounds__(grad_lanes(CH * Piece<T>::V, CENTRED), grad_waves(CH * Piece<T>::V, CENTRED))
+    norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int lanes) {
     constexpr int V = Piece<T>::V;
-    __shared__ float part[2][2][8];
+    __shared__ float part[2][2][MOST_WAVES];
     extern __shared__ float columns[];
-    const int lanes = 1 << shift;
-    const Place<T, CH, RAGGED> at{(int)threadIdx.x & (lanes - 1), lanes, p.n};
-    const int each = blockDim.x >> shift;
+    const Spot spot = spot_of<WIDE>(lanes);
+    const Place<T, CH, RAGGED> at{spot.lane, lanes, p.n};
+    const int each = blockDim.x / lanes;
     const float over = 1.f / p.n;
     Piece<T> w[CH];
     float dw[CH][V], db[CH][V];
@@ -275,7 +283,7 @@ __global__ void __launch_bounds__(MOST_LANES, CH * Piece<T>::V <= (CENTRED ? 8 :
     }
     int turn = 0;
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
-        const long r = r0 + row_of<WIDE>(shift);
+        const long r = r0 + spot.row;
         const bool row = r < p.rows;
         Piece<T> dy[CH], s[CH], ds[CH];
         const T *const pdy = (const T*)p.dy + r * p.dy_row, *const ps = (const T*)p.s + r * p.s_row, *const pds = (const T*)p.ds + r * p.ds_row;
@@ -306,10 +314,10 @@ __global__ void __launch_bounds__(MOST_LANES, CH * Piece<T>::V <= (CENTRED ? 8 :
             }
         }
         if (!p.dx) continue;
-        if constexpr (CENTRED) row_sum(sums, lanes, part[turn]);
+        if constexpr (CENTRED) row_sum(sums, lanes, spot.row, part[turn]);
         else {
             float one[1] = {sums[1]};
-            row_sum(one, lanes, part[turn]);
+            row_sum(one, lanes, spot.row, part[turn]);
             sums[1] = one[0];
         }
         turn ^= 1;
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(MOST_LANES, CH * Piece<T>::V <= (CENTRED ? 8 :
     if (CENTRED && p.dbias) finish(db, partials + ((p.dweight ? (long)gridDim.x : 0L) + blockIdx.x) * p.n);
 }
 
-// Rows of less than a piece, or longer than the registers of 512 lanes: a workgroup per row, which reads it once for each sum and once more
+// Rows of less than a piece, or longer than the registers of its lanes hold: a workgroup per row, which reads it once for each sum and once more
 // for the result, and, for the sums over rows, a workgroup per block of columns.  Most of what is read again comes from the caches: 2048 x 20000 bf16 values
 // with a residual take 80 us (4.1 TB/s) and 118.
 template <typename T, bool CENTRED>
@@ -972,48 +980,61 @@ inline unsigned grid_of(long groups) { return (unsigned)std::min(groups, MOST_TH
 }  // namespace
 
 namespace {
-// How rows are laid over lanes: 2^shift of them to a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
+// How rows are laid over lanes: `lanes` of them to a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
 struct Layout {
-    int shift, pieces, threads;
+    int lanes, pieces, threads;
     bool ragged;
-    int rows() const { return pieces ? threads >> shift : 1; }  // that a workgroup works on at once
+    int rows() const { return pieces ? threads / lanes : 1; }  // that a workgroup works on at once
 };
-// `best` pieces to a lane at most, unless there are no lanes left, and then `most`.
-Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most) {
+// Up to `best` pieces to a lane, fewer where the rows alone are too few to fill the machine with waves, more, up to `most`, where there are no lanes left
+// of the `limit` for so many pieces.  A row has 8, 16 or 32 lanes, or whole waves, whose number is a power of two where `doubled`.
+template <typename Limit>
+Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most, bool doubled, const Limit& limit) {
     const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
     const long count = up(n, v) / v;
-    if (n < v || count > (long)MOST_LANES * most) return {8, 0, 256, false};
-    Layout l{3, 1, threads, n % v != 0};
-    auto lanes = [&] { return 1L << l.shift; };
-    // A wave's lanes have one piece each before any has two; more lanes than that where the pieces are too many, or the rows alone too few to
-    // fill the machine with waves.
-    while (lanes() < count && (lanes() < 64 || (lanes() < MOST_LANES && (lanes() * best < count || rows * lanes() < 256 * 1024)))) ++l.shift;
-    while (l.pieces * lanes() < count) l.pieces *= 2;
-    l.threads = std::max(threads, (int)lanes());
+    const auto lanes_for = [&](int pieces) {
+        const long need = up((count + pieces - 1) / pieces, 64);
+        long lanes = 64;
+        while (doubled && lanes < need) lanes *= 2;
+        return std::max(need, lanes);
+    };
+    const auto fits = [&](int pieces) { return lanes_for(pieces) <= limit(pieces); };
+    if (n < v || !fits(most)) return {256, 0, 256, false};
+    Layout l{8, 1, threads, n % v != 0};
+    if (count <= 32) {
+        while (l.lanes < count) l.lanes *= 2;
+        return l;
+    }
+    while (l.pieces < best && count > 64L * l.pieces) l.pieces *= 2;
+    while (l.pieces > 1 && rows * lanes_for(l.pieces) < 256 * 1024 && fits(l.pieces / 2)) l.pieces /= 2;
+    while (!fits(l.pieces)) l.pieces *= 2;
+    l.lanes = (int)lanes_for(l.pieces);
+    l.threads = l.lanes * std::max(1, threads / l.lanes);
     return l;
 }
 // Up to four pieces of each row are under way in a lane: 8192 x 4096 bf16 with a residual 48.1 us, with up to eight 51.5, two 48.6 to 49, one 51.
-Layout lay_norm(int dtype, long rows, int n) { return lay_rows(dtype, rows, n, 256, 4, 8); }
+// Numbers of waves that are no powers of two, by which gradients gain, lose here: 8192 x 12288 143 us in place of 137, 8192 x 6144 71 and 69.
+Layout lay_norm(int dtype, long rows, int n) { return lay_rows(dtype, rows, n, 256, 4, 8, true, [](int) { return MOST_LANES / 2; }); }
 // A lane of a gradient holds the sums of its columns besides: 16 values of a row at most, of a layer norm, which has two sums, 8, or there are too few waves
-// (8192 x 4096 bf16 with a residual: RMS 52 us, with 32 values 62; layer norm 60, with 16 or 32 73).
+// (8192 x 4096 bf16 with a residual: RMS 52 us, with 32 values 62; layer norm 60, with 16 or 32 73).  Rows have as many waves as they need and up to all of
+// a compute unit's: layer norms of 8192 x 5120 63 us where 512 lanes of two pieces took 94, 8192 x 6144 105 and 116, 8192 x 12288 176 and 186.
 Layout lay_grad(int kind, int dtype, long rows, int n) {
     const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
     const bool layer = kind == MUON_HIP_NORM_LAYER;
-    return lay_rows(dtype, rows, n, 512, (layer ? 8 : 16) / v, (layer && dtype == MUON_HIP_F32 ? 16 : 32) / v);
+    return lay_rows(dtype, rows, n, 512, (layer ? 8 : 16) / v, (layer && dtype == MUON_HIP_BF16 ? 32 : 16) / v, false, [&](int pieces) { return grad_lanes(pieces * v, layer); });
 }
-// As many workgroups as are at work at once, each of which takes rows until there are none left: their registers allow 16, 12 or 8 waves to a compute unit.
-// (Half as many 60 us in place of 52, twice as many 59.)
+// As many workgroups as are at work at once, each of which takes rows until there are none left.  (8192 x 4096 RMS: half as many 60 us in place of 52, twice as
+// many 59.)
 long grad_groups(int kind, int dtype, long rows, int n, const Layout& l, int cus) {
     // (streamed rows: parts of the sums over columns, of 32 rows at least, and as many as make 2048 workgroups)
     if (l.pieces == 0) return std::min(up(rows, 32) / 32, std::max(1L, std::min(1024L, 2048 / (up(n, 256) / 256))));
-    const int values = l.pieces * (dtype == MUON_HIP_BF16 ? 8 : 4);
-    const int waves = values <= (kind == MUON_HIP_NORM_LAYER ? 8 : 16) ? 16 : values <= 16 ? 12 : 8;
+    const int waves = 4 * grad_waves(l.pieces * (dtype == MUON_HIP_BF16 ? 8 : 4), kind == MUON_HIP_NORM_LAYER);
     return std::min(up(rows, l.rows()) / l.rows(), (long)std::max(1, waves * 64 / l.threads) * cus);
 }
 template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_of(const Layout& l) {
     if constexpr (CH == 1)
-        if (l.shift < 6) return norm_kernel<T, CENTRED, CH, RAGGED, false>;
+        if (l.lanes < 64) return norm_kernel<T, CENTRED, CH, RAGGED, false>;
     return norm_kernel<T, CENTRED, CH, RAGGED, true>;
 }
 template <typename T, bool CENTRED, bool RAGGED>
@@ -1029,14 +1050,14 @@ auto norm_of(const Layout& l, bool centred) {
 template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_grad_of(const Layout& l) {
     if constexpr (CH == 1)
-        if (l.shift < 6) return norm_grad_kernel<T, CENTRED, CH, RAGGED, false>;
+        if (l.lanes < 64) return norm_grad_kernel<T, CENTRED, CH, RAGGED, false>;
     return norm_grad_kernel<T, CENTRED, CH, RAGGED, true>;
 }
 template <typename T, bool CENTRED, bool RAGGED>
 auto norm_grad_of(const Layout& l) {
-    if constexpr (sizeof(T) == 4 && !CENTRED)
-        if (l.pieces == 8) return norm_grad_of<T, CENTRED, 8, RAGGED>(l);
-    return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1, RAGGED>(l) : l.pieces == 2 ? norm_grad_of<T, CENTRED, 2, RAGGED>(l) : norm_grad_of<T, CENTRED, 4, RAGGED>(l);
+    if constexpr (sizeof(T) == 4 || CENTRED)
+        if (l.pieces == 4) return norm_grad_of<T, CENTRED, 4, RAGGED>(l);
+    return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1, RAGGED>(l) : norm_grad_of<T, CENTRED, 2, RAGGED>(l);
 }
 template <typename T>
 auto norm_grad_of(const Layout& l, bool centred) {
@@ -1048,7 +1069,7 @@ auto norm_grad_of(const Layout& l, bool centred) {
 muon_hip_norm_route norm_route(int kind, int dtype, int rows, int n, bool backward, int cus) {
     const Layout l = backward ? lay_grad(kind, dtype, rows, n) : lay_norm(dtype, rows, n);
     const long groups = backward ? grad_groups(kind, dtype, rows, n, l, cus) : std::min(up(rows, l.rows()) / l.rows(), MOST_THREADS / l.threads);
-    return muon_hip_norm_route{1 << l.shift, l.pieces, l.ragged, l.threads, groups};
+    return muon_hip_norm_route{l.lanes, l.pieces, l.ragged, l.threads, groups};
 }
 
 hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
@@ -1063,7 +1084,7 @@ hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
         return hipGetLastError();
     }
     const auto kern = bf ? norm_of<bf16_t>(l, centred) : norm_of<float>(l, centred);
-    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, l.rows()) / l.rows(), MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.shift);
+    hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, l.rows()) / l.rows(), MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.lanes);
     return hipGetLastError();
 }
 
@@ -1086,8 +1107,8 @@ hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cu
                 hipLaunchKernelGGL(column_kern, dim3((unsigned)(groups * (up(p.n, 256) / 256))), dim3(256), 0, stream, p, partials, (int)groups);
         } else {
             const auto kern = bf ? norm_grad_of<bf16_t>(l, centred) : norm_grad_of<float>(l, centred);
-            const size_t lds = l.threads > std::max(1 << l.shift, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
-            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.shift);
+            const size_t lds = l.threads > std::max(l.lanes, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
+            hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.lanes);
         }
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }

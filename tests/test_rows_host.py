@@ -115,7 +115,7 @@ def test_the_gpu_tests_run_every_kernel_of_the_norms():
             for backward in (False, True):
                 ran, there_are = ({kernel(kind, dtype, m, n, backward) for m, n in some} for some in (cases, sizes))
                 assert there_are <= ran, there_are - ran
-                assert len(there_are) >= 9
+                assert len(there_are) >= 7
 
 
 @pytest.mark.parametrize("backward", [False, True])
@@ -126,10 +126,10 @@ def test_norms_are_laid_over_whole_rows_and_launches(dtype, backward):
         for n in list(range(1, 300)) + [1000, 4096, 8200, 16384, 16385, 32769, 70001, 0x7fffffff - (1 << 20)]:
             for rows in (1, 9, 4097, 0x7fffffff):
                 r = _abi.norm_route(kind, dtype, rows, n, backward)
-                assert 0 < r.groups * r.threads < 2 ** 32 and r.threads % 64 == 0 and r.threads <= 512
+                assert 0 < r.groups * r.threads < 2 ** 32 and r.threads % 64 == 0 and r.threads <= 1024
                 if r.pieces:
                     assert r.lanes * r.pieces * piece >= n >= piece and r.lanes <= r.threads and bool(r.ragged) == (n % piece != 0)
-                    assert r.pieces == 1 or r.lanes >= 64
+                    assert r.lanes % 64 == 0 or (r.lanes in (8, 16, 32) and r.pieces == 1)
                     if backward:  # the columns' sums of several rows at once meet in LDS
                         assert r.threads <= max(r.lanes, 64) or 4 * n <= 64 * 1024
                 if backward:
