@@ -65,7 +65,7 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 // too, 46 (5.8 TB/s) and 4 for the last sums of the weight's; a layer norm's gradient 55.  262144 rows of 128 (16 lanes each): 26 us (5.1) and 34 (5.9).
 // One row of 4096: 2.5 us.  A large copy reaches 4.9 on the same card.  Asking for the next row before the present one is through changed none of
 // these by more than 2 %: there are waves enough to take turns.
-constexpr int MOST_LANES = 1024, MOST_WAVES = MOST_LANES / 64;  // of a row; half as many where they need more than 128 registers each
+constexpr int MOST_LANES = 1024, MOST_WAVES = MOST_LANES / 64;  // of a row
 template <typename T> struct Piece;
 template <> struct Piece<bf16_t> {
     static constexpr int V = 8;
@@ -255,12 +255,12 @@ __global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_nor
     }
 }
 
-// The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
-// once, and written as one row of `partials`.
 // Waves that a SIMD holds of a gradient with so many values of a row in a lane, by the registers that their sums, one of each value or two, leave; and the
 // lanes that a row can have with all of a compute unit's.
 constexpr int grad_waves(int values, bool centred) { return values <= 8 && centred ? 5 : values <= 16 && !centred ? 4 : values <= 16 ? 3 : 2; }
 constexpr int grad_lanes(int values, bool centred) { return grad_waves(values, centred) >= 4 ? MOST_LANES : 256 * grad_waves(values, centred); }
+// The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
+// once, and written as one row of `partials`.
 template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
 __global__ void __launch_bounds__(grad_lanes(CH * Piece<T>::V, CENTRED), grad_waves(CH * Piece<T>::V, CENTRED))
     norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int lanes) {
@@ -541,8 +541,8 @@ struct Cut {
     int shift, segments;
 };
 // A group of lanes for each segment of each token, all of whose loads are under way before the first store: 8192 rows of 4096 bf16 values from a table of
-// 151936 take 25 us (5.2 TB/s of results and rows).  The last piece of a ragged row overlaps the one
-// before it: what it has twice is written twice.  An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
+// 151936 take 25 us (5.2 TB/s of results and rows).  The last piece of a ragged row overlaps the one before it: what it has twice is written twice.
+// An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
 template <typename T, typename P, int CH>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, Cut cut) {
     constexpr int V = P::V;
@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, C
         }
     }
 }
+
 // The table's gradient.  The tokens are sorted by id, keeping their order among equal ones, and the sorted tokens cut into chunks of equal length,
 // whatever ids are in them: one id may have most of the tokens, as the placeholders of an image do.
 //   sort    one launch: a workgroup sorts up to 8192 tokens in LDS (24 us: a digit of up to 7 bits at a time, bound by the vector instructions of 16 waves
@@ -596,7 +597,6 @@ struct Sorted {
     int *key, *at;  // ids (vocab: none that counts) in order, and the tokens they are of
 };
 
-// A number for each token, among those with its digit, in the order of tokens; LDS arrays of the workgroup.
 struct SortSpace {
     uint32_t key[SORT_TOKENS];
     uint16_t at[SORT_TOKENS];
@@ -605,6 +605,8 @@ struct SortSpace {
 };
 static_assert(sizeof(SortSpace) <= 64 * 1024, "two workgroups to a compute unit");
 
+// A digit at a time, from the lowest: a wave's tokens are back to back, each counts the ones before it that have its digit, by ballots, and the sums of
+// all counts say where each digit's tokens of each wave go.
 __device__ void sort_block(const EmbeddingArgs& a, int bits, Sorted out, SortSpace& s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int first = blockIdx.x * SORT_TOKENS, count = a.tokens - first < SORT_TOKENS ? a.tokens - first : SORT_TOKENS;
@@ -975,11 +977,9 @@ __global__ void __launch_bounds__(256) dropout_kernel(const DropoutArgs a) {
     }
 }
 
+// ---- host side ----------------------------------------------------------------------------------------
 inline unsigned grid_of(long groups) { return (unsigned)std::min(groups, MOST_THREADS / 256); }
 
-}  // namespace
-
-namespace {
 // How rows are laid over lanes: `lanes` of them to a row, `pieces` of 16 bytes to a lane (0: the streamed kernels), `threads` of a workgroup.
 struct Layout {
     int lanes, pieces, threads;
