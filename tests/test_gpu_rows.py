@@ -725,6 +725,19 @@ def test_the_same_tensor_twice_and_parameters(name):
     assert b.grad.any()
 
 
+def test_results_under_inference_mode():
+    g = gen_of("inference")
+    x, w = rnd(g, 6, 48, dtype=BF16), rnd(g, 48, dtype=BF16)
+    ids = torch.tensor([5, 0], device=DEV)
+    want = [E.layer_norm(x, w, w), *E.rms_norm(x, w, residual=x), E.dropout(x, 0.5, seed=1), E.embedding(ids, x)]
+    with torch.inference_mode():
+        got = [E.layer_norm(x, w, w), *E.rms_norm(x, w, residual=x), E.dropout(x, 0.5, seed=1), E.embedding(ids, x)]
+        assert all(t.is_inference() for t in got)
+        again = E.rms_norm(got[0], w)
+    assert all(torch.equal(a, e) for a, e in zip(got, want)) and torch.equal(again, E.rms_norm(want[0], w))
+    assert not any(t.is_inference() for t in want)
+
+
 def test_kernels_are_timed_by_name():
     x = torch.ones(4, 64, device=DEV)
     _abi.timing_enable(True)
