@@ -1151,15 +1151,15 @@ hipError_t launch_embedding(const EmbeddingArgs& a, hipStream_t stream) {
 }
 
 namespace {
-// Chunks are as many as fill the machine four waves deep on each of its 1024 SIMDs, and at most 1024, so that the parts of a run over all of them
-// are few; at least 8 tokens, whose rows are asked for at once.
+// Chunks are as many as fill the machine two waves deep on each of its 1024 SIMDs, and at most 1024, so that the parts of a run over all of them
+// are few (four waves deep 1 % slower at 8192 tokens of 4096 values, the same elsewhere); at least 8 tokens, whose rows are asked for at once.
 Cut cut_sums(int n, int dtype) {
     const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
     return cut_row(n, n < v ? 1 : v, 1, 64);
 }
 Chunks chunks_of(int tokens, int n, int dtype) {
     const Cut cut = cut_sums(n, dtype);
-    const long chunks = std::max(1L, std::min(1024L, 4096L * 64 / ((long)cut.segments << cut.shift)));
+    const long chunks = std::max(1L, std::min(1024L, 2048L * 64 / ((long)cut.segments << cut.shift)));
     Chunks c;
     c.length = (int)std::max(8L, (tokens + chunks - 1) / chunks);
     c.count = (tokens + c.length - 1) / c.length;

@@ -58,12 +58,18 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [..., n]; weight and bias [n].
 
     With a residual, of the shape of x, the sum s = x + residual is normalised, as it is rounded to the tensors' type, and (y, s) is returned."""
-    return _norm(_abi.NORM_LAYER, x, weight, bias, eps, residual)
+    out = _abi.rows().norm(_abi.NORM_LAYER, x, weight, bias, residual, eps)
+    if out is None:
+        _refuse_norm(x, weight, bias, eps, residual)
+    return out
 
 
 def rms_norm(x: Tensor, weight: Optional[Tensor] = None, *, eps: float = 1e-6, residual: Optional[Tensor] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension of x [..., n]; weight [n].  A residual is taken as in `layer_norm`."""
-    return _norm(_abi.NORM_RMS, x, weight, None, eps, residual)
+    out = _abi.rows().norm(_abi.NORM_RMS, x, weight, None, residual, eps)
+    if out is None:
+        _refuse_norm(x, weight, None, eps, residual)
+    return out
 
 
 def dropout(x: Tensor, p: float = 0.5, *, seed: Union[int, Tensor], site: int = 0, residual: Optional[Tensor] = None) -> Tensor:
@@ -93,23 +99,6 @@ def dropout(x: Tensor, p: float = 0.5, *, seed: Union[int, Tensor], site: int = 
     return out
 
 
-def _norm(kind: int, x, weight, bias, eps, residual):
-    out = _abi.rows().norm(kind, x, weight, bias, residual, eps)
-    if out is None:
-        if not eps >= 0:
-            raise ValueError(f"eps is {eps}: a number that is not negative is wanted")
-        _check_like(x, residual)
-        if x.ndim < 1:
-            raise ValueError("x needs at least one dimension")
-        for t, name in ((weight, "weight"), (bias, "bias")):
-            if t is not None:
-                _check_one(t, x, name)
-                if t.shape != (x.size(-1),):
-                    raise ValueError(f"{name} has shape {tuple(t.shape)}, ({x.size(-1)},) is wanted")
-        _refuse(x, weight, bias, residual)
-    return out
-
-
 # ---- what the native calls leave to be refused ------------------------------------------------------
 
 
@@ -120,6 +109,20 @@ def _check_like(x: Tensor, residual: Optional[Tensor]) -> None:
         _check_one(residual, x, "residual")
         if residual.shape != x.shape:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+
+
+def _refuse_norm(x, weight, bias, eps, residual) -> None:
+    if not eps >= 0:
+        raise ValueError(f"eps is {eps}: a number that is not negative is wanted")
+    _check_like(x, residual)
+    if x.ndim < 1:
+        raise ValueError("x needs at least one dimension")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_one(t, x, name)
+            if t.shape != (x.size(-1),):
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, ({x.size(-1)},) is wanted")
+    _refuse(x, weight, bias, residual)
 
 
 def _check_whole(t: Tensor, like: Tensor, name: str, dtypes) -> None:
