@@ -463,7 +463,7 @@ int muon_hip_norm_grad_run(const muon_hip_norm_grad* p, void* workspace, size_t 
 /* How such a call is computed on a device of `cus` compute units.  For tests and measurements. */
 typedef struct {
     int lanes;   /* of a row */
-    int pieces;  /* of 16 bytes that each of them holds; 0: rows of less than a piece or too long for registers, a workgroup each */
+    int pieces;  /* of 16 bytes (of one value, in rows of less) that each of them holds; 0: rows too long for registers, a workgroup each */
     int ragged;  /* whether rows are no whole number of pieces */
     int threads; /* of a workgroup */
     long groups; /* workgroups of the launch */

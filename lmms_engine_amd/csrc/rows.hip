@@ -87,7 +87,7 @@ template <> struct Piece<float> {
     __device__ __forceinline__ void set(const float (&v)[4]) { raw = f32x4{v[0], v[1], v[2], v[3]}; }
 };
 
-// One value of a row that is shorter than a piece.
+// One value, of rows that are shorter than a piece.
 template <typename T> struct Single {
     static constexpr int V = 1;
     T raw;
@@ -149,9 +149,9 @@ __device__ __forceinline__ void row_sum(float (&v)[K], int lanes, int row, float
 }
 
 // Where the pieces of a lane are.
-template <typename T, int CH, bool RAGGED>
+template <typename T, typename P, bool RAGGED>
 struct Place {
-    static constexpr int V = Piece<T>::V;
+    static constexpr int V = P::V;
     int lane, lanes, n;
     __device__ __forceinline__ int begin(int c) const { return (c * lanes + lane) * V; }
     __device__ __forceinline__ bool in(int c) const { return begin(c) < n; }
@@ -160,18 +160,18 @@ struct Place {
     __device__ __forceinline__ bool counts(int c, int e) const { return in(c) && (!RAGGED || at(c) + e >= begin(c)); }
 };
 
-template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
+template <typename T, typename P, bool CENTRED, int CH, bool RAGGED, bool WIDE>
 __global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_norm p, int lanes) {
-    constexpr int V = Piece<T>::V;
+    constexpr int V = P::V;
     __shared__ float part[2][1][MOST_WAVES];
     const Spot spot = spot_of<WIDE>(lanes);
-    const Place<T, CH, RAGGED> at{spot.lane, lanes, p.n};
+    const Place<T, P, RAGGED> at{spot.lane, lanes, p.n};
     const int each = blockDim.x / lanes;
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
         const long r = r0 + spot.row;
         const bool row = r < p.rows;
         constexpr int EARLY = CH <= 2 ? CH : 0;
-        Piece<T> x[CH], res[CH], w[EARLY + 1], b[EARLY + 1];
+        P x[CH], res[CH], w[EARLY + 1], b[EARLY + 1];
         float s[CH][V];
         const T* const px = (const T*)p.x + r * p.x_row;
 #pragma unroll
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_nor
             if (row && at.in(c)) x[c].load(px, at.bytes(c));
         }
         // weights are asked for with the row where there is room for them (262144 rows of 128: 26.3 us in place of 29, 4096 x 1024 9.1 in place of 9.4)
-        const auto weights = [&](int c, Piece<T>& wc, Piece<T>& bc) {
+        const auto weights = [&](int c, P& wc, P& bc) {
             if (!row || !at.in(c)) return;
             if (p.weight) wc.load(p.weight, at.bytes(c));
             if (p.bias) bc.load(p.bias, at.bytes(c));
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_nor
         for (int c = 0; c < CH; ++c) {
             if (!at.in(c)) continue;
             constexpr bool LATE = EARLY == 0;
-            Piece<T> y, &wc = w[LATE ? 0 : c], &bc = b[LATE ? 0 : c];
+            P y, &wc = w[LATE ? 0 : c], &bc = b[LATE ? 0 : c];
             float v[V];
             if (LATE) weights(c, wc, bc);
 #pragma unroll
@@ -261,17 +261,17 @@ constexpr int grad_waves(int values, bool centred) { return values <= 8 && centr
 constexpr int grad_lanes(int values, bool centred) { return grad_waves(values, centred) >= 4 ? MOST_LANES : 256 * grad_waves(values, centred); }
 // The sums over the rows stay in the registers of a workgroup's lanes until its rows are through, are added up in LDS where several rows were worked on at
 // once, and written as one row of `partials`.
-template <typename T, bool CENTRED, int CH, bool RAGGED, bool WIDE>
-__global__ void __launch_bounds__(grad_lanes(CH * Piece<T>::V, CENTRED), grad_waves(CH * Piece<T>::V, CENTRED))
+template <typename T, typename P, bool CENTRED, int CH, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(grad_lanes(CH * P::V, CENTRED), grad_waves(CH * P::V, CENTRED))
     norm_grad_kernel(const muon_hip_norm_grad p, float* partials, int lanes) {
-    constexpr int V = Piece<T>::V;
+    constexpr int V = P::V;
     __shared__ float part[2][2][MOST_WAVES];
     extern __shared__ float columns[];
     const Spot spot = spot_of<WIDE>(lanes);
-    const Place<T, CH, RAGGED> at{spot.lane, lanes, p.n};
+    const Place<T, P, RAGGED> at{spot.lane, lanes, p.n};
     const int each = blockDim.x / lanes;
     const float over = 1.f / p.n;
-    Piece<T> w[CH];
+    P w[CH];
     float dw[CH][V], db[CH][V];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(grad_lanes(CH * Piece<T>::V, CENTRED), grad_wa
     for (long r0 = (long)blockIdx.x * each; r0 < p.rows; r0 += (long)gridDim.x * each) {
         const long r = r0 + spot.row;
         const bool row = r < p.rows;
-        Piece<T> dy[CH], s[CH], ds[CH];
+        P dy[CH], s[CH], ds[CH];
         const T *const pdy = (const T*)p.dy + r * p.dy_row, *const ps = (const T*)p.s + r * p.s_row, *const pds = (const T*)p.ds + r * p.ds_row;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(grad_lanes(CH * Piece<T>::V, CENTRED), grad_wa
     if (CENTRED && p.dbias) finish(db, partials + ((p.dweight ? (long)gridDim.x : 0L) + blockIdx.x) * p.n);
 }
 
-// Rows of less than a piece, or longer than the registers of its lanes hold: a workgroup per row, which reads it once for each sum and once more
+// Rows longer than the registers of their lanes hold: a workgroup per row, which reads it once for each sum and once more
 // for the result, and, for the sums over rows, a workgroup per block of columns.  Most of what is read again comes from the caches: 2048 x 20000 bf16 values
 // with a residual take 80 us (4.1 TB/s) and 118.
 template <typename T, bool CENTRED>
@@ -999,8 +999,9 @@ Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most, bo
         return std::max(need, lanes);
     };
     const auto fits = [&](int pieces) { return lanes_for(pieces) <= limit(pieces); };
-    if (n < v || !fits(most)) return {256, 0, 256, false};
-    Layout l{8, 1, threads, n % v != 0};
+    if (!fits(most)) return {256, 0, 256, false};
+    Layout l{8, 1, threads, n > v && n % v != 0};
+    if (n < v) return l;  // a value to a lane: 262144 rows of 4 bf16 values take 11.3 us and their gradient 13.6, a workgroup per row 400 and 475
     if (count <= 32) {
         while (l.lanes < count) l.lanes *= 2;
         return l;
@@ -1034,8 +1035,8 @@ long grad_groups(int kind, int dtype, long rows, int n, const Layout& l, int cus
 template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_of(const Layout& l) {
     if constexpr (CH == 1)
-        if (l.lanes < 64) return norm_kernel<T, CENTRED, CH, RAGGED, false>;
-    return norm_kernel<T, CENTRED, CH, RAGGED, true>;
+        if (l.lanes < 64) return norm_kernel<T, Piece<T>, CENTRED, CH, RAGGED, false>;
+    return norm_kernel<T, Piece<T>, CENTRED, CH, RAGGED, true>;
 }
 template <typename T, bool CENTRED, bool RAGGED>
 auto norm_of(const Layout& l) {
@@ -1043,15 +1044,16 @@ auto norm_of(const Layout& l) {
          : l.pieces == 4 ? norm_of<T, CENTRED, 4, RAGGED>(l) : norm_of<T, CENTRED, 8, RAGGED>(l);
 }
 template <typename T>
-auto norm_of(const Layout& l, bool centred) {
+auto norm_of(const Layout& l, int n, bool centred) {
+    if (n < Piece<T>::V) return centred ? norm_kernel<T, Single<T>, true, 1, false, false> : norm_kernel<T, Single<T>, false, 1, false, false>;
     if (centred) return l.ragged ? norm_of<T, true, true>(l) : norm_of<T, true, false>(l);
     return l.ragged ? norm_of<T, false, true>(l) : norm_of<T, false, false>(l);
 }
 template <typename T, bool CENTRED, int CH, bool RAGGED>
 auto norm_grad_of(const Layout& l) {
     if constexpr (CH == 1)
-        if (l.lanes < 64) return norm_grad_kernel<T, CENTRED, CH, RAGGED, false>;
-    return norm_grad_kernel<T, CENTRED, CH, RAGGED, true>;
+        if (l.lanes < 64) return norm_grad_kernel<T, Piece<T>, CENTRED, CH, RAGGED, false>;
+    return norm_grad_kernel<T, Piece<T>, CENTRED, CH, RAGGED, true>;
 }
 template <typename T, bool CENTRED, bool RAGGED>
 auto norm_grad_of(const Layout& l) {
@@ -1060,7 +1062,8 @@ auto norm_grad_of(const Layout& l) {
     return l.pieces == 1 ? norm_grad_of<T, CENTRED, 1, RAGGED>(l) : norm_grad_of<T, CENTRED, 2, RAGGED>(l);
 }
 template <typename T>
-auto norm_grad_of(const Layout& l, bool centred) {
+auto norm_grad_of(const Layout& l, int n, bool centred) {
+    if (n < Piece<T>::V) return centred ? norm_grad_kernel<T, Single<T>, true, 1, false, false> : norm_grad_kernel<T, Single<T>, false, 1, false, false>;
     if (centred) return l.ragged ? norm_grad_of<T, true, true>(l) : norm_grad_of<T, true, false>(l);
     return l.ragged ? norm_grad_of<T, false, true>(l) : norm_grad_of<T, false, false>(l);
 }
@@ -1083,7 +1086,7 @@ hipError_t launch_norm(const muon_hip_norm& p, hipStream_t stream) {
         hipLaunchKernelGGL(kern, dim3(grid_of(p.rows)), dim3(256), 0, stream, p);
         return hipGetLastError();
     }
-    const auto kern = bf ? norm_of<bf16_t>(l, centred) : norm_of<float>(l, centred);
+    const auto kern = bf ? norm_of<bf16_t>(l, p.n, centred) : norm_of<float>(l, p.n, centred);
     hipLaunchKernelGGL(kern, dim3((unsigned)std::min(up(p.rows, l.rows()) / l.rows(), MOST_THREADS / l.threads)), dim3(l.threads), 0, stream, p, l.lanes);
     return hipGetLastError();
 }
@@ -1106,7 +1109,7 @@ hipError_t launch_norm_grad(const muon_hip_norm_grad& p, float* partials, int cu
             if (p.dweight || p.dbias)
                 hipLaunchKernelGGL(column_kern, dim3((unsigned)(groups * (up(p.n, 256) / 256))), dim3(256), 0, stream, p, partials, (int)groups);
         } else {
-            const auto kern = bf ? norm_grad_of<bf16_t>(l, centred) : norm_grad_of<float>(l, centred);
+            const auto kern = bf ? norm_grad_of<bf16_t>(l, p.n, centred) : norm_grad_of<float>(l, p.n, centred);
             const size_t lds = l.threads > std::max(l.lanes, 64) && (p.dweight || p.dbias) ? (size_t)p.n * 4 : 0;
             hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(l.threads), lds, stream, p, partials, l.lanes);
         }

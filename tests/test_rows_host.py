@@ -102,7 +102,8 @@ def test_norms_are_checked_before_any_launch(change, code, match):
 def kernel(kind, dtype, rows, n, backward):
     r = _abi.norm_route(kind, dtype, rows, n, backward)
     # lanes below a wave's are a kernel of their own, which has one piece
-    return (kind, dtype, backward, r.pieces) + ((bool(r.ragged), r.lanes < 64) if r.pieces else ())
+    single = n < (4 if dtype == _abi.F32 else 8)  # rows of less than a piece
+    return (kind, dtype, backward, r.pieces) + ((bool(r.ragged), r.lanes < 64, single) if r.pieces else ())
 
 
 def test_the_gpu_tests_run_every_kernel_of_the_norms():
@@ -128,7 +129,7 @@ def test_norms_are_laid_over_whole_rows_and_launches(dtype, backward):
                 r = _abi.norm_route(kind, dtype, rows, n, backward)
                 assert 0 < r.groups * r.threads < 2 ** 32 and r.threads % 64 == 0 and r.threads <= 1024
                 if r.pieces:
-                    assert r.lanes * r.pieces * piece >= n >= piece and r.lanes <= r.threads and bool(r.ragged) == (n % piece != 0)
+                    assert r.lanes * r.pieces * (piece if n >= piece else 1) >= n and r.lanes <= r.threads and bool(r.ragged) == (n > piece and n % piece != 0)
                     assert r.lanes % 64 == 0 or (r.lanes in (8, 16, 32) and r.pieces == 1)
                     if backward:  # the columns' sums of several rows at once meet in LDS
                         assert r.threads <= max(r.lanes, 64) or 4 * n <= 64 * 1024
