@@ -87,12 +87,21 @@ typedef std::optional<Tensor> Maybe;
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
 
+// Whether the program has freed the memory of a tensor and kept the tensor, as sharded training does: no version counter tells, and the address of what was
+// freed is null, or a small number in a view, not that of nothing.
+bool freed(const Tensor& t) { return t.defined() && t.has_storage() && t.numel() > 0 && !t.storage().data(); }
+// Of what a backward pass reads, where it may have happened since the forward pass.
+template <typename... Tensors>
+void refuse_freed(const Tensors&... all) {
+    const auto one = [](const Tensor& t) { TORCH_CHECK_VALUE(!freed(t), "the memory of a tensor of shape ", t.sizes(), " was freed before its backward pass"); };
+    (one(all), ...);
+}
 // A plain tensor on a GPU whose memory is there.
 bool present(PyObject* o) {
     if (!THPVariable_CheckExact(o)) return false;
     const Tensor& t = THPVariable_Unpack(o);
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->is_python_dispatch()) return false;
-    return !(t.has_storage() && t.numel() > 0 && !t.storage().data());
+    return !freed(t);
 }
 // The same of x's type and device.
 bool plain(PyObject* o, const Tensor* x) {

@@ -126,8 +126,12 @@ struct Norm : torch::autograd::Function<Norm> {
                 if (want_w) grads[1] = at::zeros({n}, like.options());
                 if (want_b) grads[2] = at::zeros({n}, like.options());
             } else if (want_x || want_r || want_w || want_b) {
-                const Lines dy2(dy), s2(s), ds2(ds);
-                const Values w1(w);
+                const bool for_x = want_x || want_r;
+                const Tensor none, &s_read = for_x || want_w ? s : none, &stats_read = for_x || want_w ? stats : none;
+                const Tensor &w_read = for_x ? w : none, &ds_read = for_x ? ds : none;
+                refuse_freed(dy, s_read, stats_read, w_read, ds_read);
+                const Lines dy2(dy), s2(s_read), ds2(ds_read);
+                const Values w1(w_read);
                 muon_hip_norm_grad p{};
                 p.kind = (int)ctx->saved_data["kind"].toInt();
                 p.dtype = dtype_of(like);
@@ -135,13 +139,13 @@ struct Norm : torch::autograd::Function<Norm> {
                 p.n = (int)n;
                 p.dy = dy2.at;
                 p.dy_row = dy2.apart;
-                p.s = s2.at;  // (nothing where the bias alone is trained)
+                p.s = s2.at;  // (nothing where the bias' gradient alone is asked for)
                 p.s_row = s2.apart;
-                p.stats = (const float*)pointer(stats);
+                p.stats = (const float*)pointer(stats_read);
                 p.ds = ds2.at;
                 p.ds_row = ds2.apart;
                 p.weight = w1.at;
-                if (want_x || want_r) p.dx = (dx = fresh(like.sizes(), like.scalar_type())).data_ptr();
+                if (for_x) p.dx = (dx = fresh(like.sizes(), like.scalar_type())).data_ptr();
                 if (want_w) p.dweight = (grads[1] = fresh({n}, like.scalar_type())).data_ptr();
                 if (want_b) p.dbias = (grads[2] = fresh({n}, like.scalar_type())).data_ptr();
                 const long need = muon_hip_norm_grad_workspace(&p);
@@ -196,6 +200,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy.device());
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), n = dy.size(-1);
+            refuse_freed(dy, ids);
             const Lines dy2(dy);
             const Tensor i1 = ids.contiguous();
             grads[0] = fresh({vocab, n}, dy.scalar_type());
@@ -241,8 +246,9 @@ struct Dropout : torch::autograd::Function<Dropout> {
         if (ctx->needs_input_grad(0)) {
             {
                 const at::AutoGradMode off(false);
-                grads[0] = dropout_forward(dy, Tensor(), ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                                           ctx->saved_data["site"].toInt());
+                const Tensor seed_at = ctx->get_saved_variables()[0];
+                refuse_freed(dy, seed_at);
+                grads[0] = dropout_forward(dy, Tensor(), seed_at, ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), ctx->saved_data["site"].toInt());
             }
             if (at::GradMode::is_enabled()) close_history(grads[0], 0, {}, {dy});
         }
