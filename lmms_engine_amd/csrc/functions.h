@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
+
 #include "../../include/muon_hip.h"
 
 namespace {
@@ -95,6 +97,16 @@ template <typename... Tensors>
 void refuse_freed(const Tensors&... all) {
     const auto one = [](const Tensor& t) { TORCH_CHECK_VALUE(!freed(t), "the memory of a tensor of shape ", t.sizes(), " was freed before its backward pass"); };
     (one(all), ...);
+}
+// What was kept for a backward pass comes back through the program's hooks, if it has any: it has to be of the type and shape that it had, and where the incoming
+// gradient is, before its address goes to a kernel.
+void check_kept(const Tensor& t, std::initializer_list<at::ScalarType> types, at::IntArrayRef sizes, const Tensor& like) {
+    if (!t.defined()) return;
+    TORCH_CHECK_NOT_IMPLEMENTED(t.layout() == at::kStrided && !t.unsafeGetTensorImpl()->is_python_dispatch(), "what was kept for a backward pass is no plain tensor");
+    TORCH_CHECK_TYPE(std::find(types.begin(), types.end(), t.scalar_type()) != types.end(), "what was kept for a backward pass is ", t.scalar_type(), ", it was ",
+                     *types.begin());
+    TORCH_CHECK_VALUE(t.sizes() == sizes, "what was kept for a backward pass has shape ", t.sizes(), ", it had ", sizes);
+    TORCH_CHECK_VALUE(t.device() == like.device(), "what was kept for a backward pass is on ", t.device(), ", the incoming gradient on ", like.device());
 }
 // A plain tensor on a GPU whose memory is there.
 bool present(PyObject* o) {

@@ -129,19 +129,22 @@ struct Norm : torch::autograd::Function<Norm> {
                 const bool for_x = want_x || want_r;
                 const Tensor none, &s_read = for_x || want_w ? s : none, &stats_read = for_x || want_w ? stats : none;
                 const Tensor &w_read = for_x ? w : none, &ds_read = for_x ? ds : none;
-                refuse_freed(dy, s_read, stats_read, w_read, ds_read);
-                const Lines dy2(dy), s2(s_read), ds2(ds_read);
-                const Values w1(w_read);
                 muon_hip_norm_grad p{};
                 p.kind = (int)ctx->saved_data["kind"].toInt();
                 p.dtype = dtype_of(like);
                 p.rows = (int)rows_of(dy);
+                check_kept(s_read, {like.scalar_type()}, like.sizes(), like);
+                check_kept(stats_read, {at::kFloat}, {p.kind == MUON_HIP_NORM_LAYER ? 2 : 1, (int64_t)p.rows}, like);
+                check_kept(w_read, {like.scalar_type()}, {n}, like);
+                refuse_freed(dy, s_read, stats_read, w_read, ds_read);
+                const Lines dy2(dy), s2(s_read), ds2(ds_read);
+                const Values w1(w_read), stats1(stats_read);
                 p.n = (int)n;
                 p.dy = dy2.at;
                 p.dy_row = dy2.apart;
                 p.s = s2.at;  // (nothing where the bias' gradient alone is asked for)
                 p.s_row = s2.apart;
-                p.stats = (const float*)pointer(stats_read);
+                p.stats = (const float*)stats1.at;
                 p.ds = ds2.at;
                 p.ds_row = ds2.apart;
                 p.weight = w1.at;
@@ -200,6 +203,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy.device());
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), n = dy.size(-1);
+            check_kept(ids, {at::kLong, at::kInt}, dy.sizes().slice(0, dy.dim() - 1), dy);
             refuse_freed(dy, ids);
             const Lines dy2(dy);
             const Tensor i1 = ids.contiguous();
@@ -247,6 +251,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
             {
                 const at::AutoGradMode off(false);
                 const Tensor seed_at = ctx->get_saved_variables()[0];
+                if (seed_at.defined()) check_kept(seed_at, {at::kLong}, seed_at.numel() == 1 ? seed_at.sizes() : at::IntArrayRef({1}), dy);
                 refuse_freed(dy, seed_at);
                 grads[0] = dropout_forward(dy, Tensor(), seed_at, ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), ctx->saved_data["site"].toInt());
             }

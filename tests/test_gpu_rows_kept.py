@@ -1,6 +1,7 @@
-"""What embedding, layer_norm, rms_norm and dropout keep for their backward pass, when it is not there any more."""
+"""What embedding, layer_norm, rms_norm and dropout keep for their backward pass, when it is not there any more, or not what it was."""
 import pytest
 import torch
+from torch.autograd.graph import saved_tensors_hooks
 
 import lmms_engine_amd as E
 
@@ -91,3 +92,58 @@ def test_what_a_gradient_does_not_read_may_be_gone():
     y = E.dropout(x, 0.5, seed=3, residual=r)
     free(x)
     assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+
+
+def kept_by(call, dtype):
+    """The tensors that a call keeps, as hooks see them."""
+    kept = []
+    with saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        call(leaf(6, 40, dtype=dtype), leaf(6, 40, dtype=dtype), leaf(40, dtype=dtype))
+    return len(kept)
+
+
+CALLS = [weight, weight_beside_a_residual, input_for_the_weight, ids, seed]
+OTHERS = {
+    "a type": (lambda t: t.to(torch.float16 if t.is_floating_point() else torch.int16), TypeError),
+    "a wider type": (lambda t: t.double(), TypeError),
+    "a device": (lambda t: t.cpu(), ValueError),
+    "fewer values": (lambda t: t.flatten()[:0], ValueError),
+    "a shape": (lambda t: torch.stack([t, t]), ValueError),
+    "a layout": (lambda t: t.to_sparse(), NotImplementedError),
+}
+
+
+@pytest.mark.parametrize("other", list(OTHERS))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("call", CALLS)
+def test_what_hooks_give_back_is_what_was_kept(call, dtype, other):
+    change, error = OTHERS[other]
+    count = kept_by(call, dtype)
+    assert count == {"ids": 1, "seed": 1, "input_for_the_weight": 2}.get(call.__name__, 3)
+    for i in range(count):
+        seen = []
+        with saved_tensors_hooks(lambda t: seen.append(t) or (len(seen) - 1, t), lambda p: change(p[1]) if p[0] == i else p[1]):
+            y, of, _ = call(leaf(6, 40, dtype=dtype), leaf(6, 40, dtype=dtype), leaf(40, dtype=dtype))
+        with pytest.raises(error, match="kept for a backward pass"):
+            torch.autograd.grad(y, of, torch.ones_like(y))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("call", CALLS)
+def test_hooks_may_give_back_other_strides_and_addresses(call, dtype):
+    def gradient(unpack):
+        with saved_tensors_hooks(lambda t: t.cpu(), lambda t: unpack(t.cuda())):
+            y, of, _ = call(leaf(6, 40, dtype=dtype), leaf(6, 40, dtype=dtype), leaf(40, dtype=dtype))
+        return torch.autograd.grad(y, of, torch.ones_like(y))[0]
+
+    want = gradient(lambda t: t)
+    for lay in (lambda t: torch.stack([t, t], -1)[..., 0], lambda t: t.t().contiguous().t() if t.dim() == 2 else t, part):
+        assert torch.equal(gradient(lay), want)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_incoming_gradients_that_are_no_plain_tensors_raise(call):
+    y, of, _ = call(leaf(6, 40), leaf(6, 40), leaf(40))
+    for dy, batched in ((torch.ones_like(y).to_sparse(), False), (torch.ones(3, *y.shape, device=DEV), True)):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, of, dy, is_grads_batched=batched, retain_graph=True)
