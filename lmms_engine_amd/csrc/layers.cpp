@@ -173,11 +173,13 @@ struct Linear : torch::autograd::Function<Linear> {
         const Wanted more(ctx, 2);
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = more.a;
         variable_list grads(5);
+        const Tensor none;
         {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy.device());
             if (want_x || want_w || want_b) {
                 const int64_t m = rows_of(dy), n = dy.size(-1);
+                refuse_freed(dy, want_w ? x : none, want_x ? w : none, d);
                 Incoming g = act_grad(dy, d.defined() ? 1 : 0, d, Tensor(), want_x || want_w, want_b, false, m, n);
                 grads[2] = g.db[0];
                 if (want_x) {
@@ -236,6 +238,8 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dh.device());
             const int64_t m = rows_of(dh), n = dh.size(-1);
+            const Tensor none;
+            refuse_freed(dh, want_wg || want_wu ? x : none, want_x ? wg : none, want_x ? wu : none, want_u ? s : none, want_g ? t : none);
             Incoming g = act_grad(dh, two ? 2 : 1, want_g ? t : s, two ? s : Tensor(), want_x || want_wg || want_wu, want_g ? more.a : more.b,
                                   two && more.b, m, n);
             const int u = two ? 1 : 0;  // which of them is the other projection's, where it is wanted
