@@ -56,6 +56,21 @@ Tensor factor(const Tensor& like, int64_t m, int64_t n) {
     return at::empty({muon_hip_product_aux_bytes(dtype_of(like), (int)m, (int)n)}, like.options().dtype(at::kByte));
 }
 
+// What a factor kept for m x n values has to be, and a form of it that the library takes: hooks may have laid it elsewhere.
+Tensor factor_back(const Tensor& d, const Tensor& like, int64_t m, int64_t n) {
+    if (!d.defined()) return d;
+    check_kept(d, {at::kByte}, {muon_hip_product_aux_bytes(dtype_of(like), (int)m, (int)n)}, like);
+    refuse_freed(d);
+    return d.is_contiguous() && ((uintptr_t)d.data_ptr() & 15) == 0 ? d : d.clone(at::MemoryFormat::Contiguous);
+}
+// What an input, of k columns and the leading shape of the incoming gradient, and a weight have to be.
+void check_input(const Tensor& x, const Tensor& dy, int64_t k) {
+    auto shape = dy.sizes().vec();
+    shape.back() = k;
+    check_kept(x, {dy.scalar_type()}, shape, dy);
+}
+void check_weight(const Tensor& w, const Tensor& dy, int64_t k) { check_kept(w, {dy.scalar_type()}, {dy.size(-1), k}, dy); }
+
 // Results of a forward pass, and the factors of the backward pass where they are kept.
 struct Forward {
     Tensor out, aux[2];
@@ -132,7 +147,8 @@ Incoming act_grad(const Tensor& dy_, int factors, const Tensor& d0, const Tensor
 // The second derivative of an activation without a curve is zero.
 bool curved(int act) { return act != MUON_HIP_ACT_NONE && act != MUON_HIP_ACT_RELU; }
 
-void note(AutogradContext* ctx, const Maybe& a, const Maybe& b, int64_t act) {
+void note(AutogradContext* ctx, const Tensor& x, const Maybe& a, const Maybe& b, int64_t act) {
+    ctx->saved_data["k"] = x.size(-1);
     ctx->saved_data["has"] = (int64_t)(a.has_value() + 2 * b.has_value());
     ctx->saved_data["act"] = act;
 }
@@ -163,23 +179,26 @@ struct Linear : torch::autograd::Function<Linear> {
         const bool for_x = x.requires_grad(), for_w = w.requires_grad(), for_b = b && b->requires_grad();
         Forward f = linear_forward(x, w, given(b), given(r), (int)act, for_x || for_w || for_b);
         ctx->save_for_backward({for_w ? x : Tensor(), for_x ? w : Tensor(), f.aux[0]});
-        note(ctx, b, r, act);
+        note(ctx, x, b, r, act);
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         refuse_recording();
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1], &d = saved[2], &dy = incoming[0];
+        const Tensor none, &dy = incoming[0];
         const Wanted more(ctx, 2);
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = more.a;
+        const Tensor &x = want_w ? saved[0] : none, &w = want_x ? saved[1] : none;
         variable_list grads(5);
-        const Tensor none;
         {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy.device());
             if (want_x || want_w || want_b) {
-                const int64_t m = rows_of(dy), n = dy.size(-1);
-                refuse_freed(dy, want_w ? x : none, want_x ? w : none, d);
+                const int64_t m = rows_of(dy), n = dy.size(-1), k = ctx->saved_data["k"].toInt();
+                check_input(x, dy, k);
+                check_weight(w, dy, k);
+                refuse_freed(dy, x, w);
+                const Tensor d = factor_back(saved[2], dy, m, n);
                 Incoming g = act_grad(dy, d.defined() ? 1 : 0, d, Tensor(), want_x || want_w, want_b, false, m, n);
                 grads[2] = g.db[0];
                 if (want_x) {
@@ -223,23 +242,27 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
         Forward f = gated_forward(x, wg, wu, given(bg), given(bu), (int)act, true);
         const Tensor none;
         ctx->save_for_backward({for_wg || for_wu ? x : none, for_x ? wg : none, for_x ? wu : none, for_u ? f.aux[0] : none, for_g ? f.aux[1] : none});
-        note(ctx, bg, bu, act);
+        note(ctx, x, bg, bu, act);
         return f.out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         refuse_recording();
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &s = saved[3], &t = saved[4], &dh = incoming[0];
+        const Tensor none, &dh = incoming[0];
         const bool want_x = ctx->needs_input_grad(0), want_wg = ctx->needs_input_grad(1), want_wu = ctx->needs_input_grad(2);
         const Wanted more(ctx, 3);
         const bool want_g = want_x || want_wg || more.a, want_u = want_x || want_wu || more.b, two = want_g && want_u;
+        const Tensor &x = want_wg || want_wu ? saved[0] : none, &wg = want_x ? saved[1] : none, &wu = want_x ? saved[2] : none;
         variable_list grads(6);
         if (want_g || want_u) {
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dh.device());
-            const int64_t m = rows_of(dh), n = dh.size(-1);
-            const Tensor none;
-            refuse_freed(dh, want_wg || want_wu ? x : none, want_x ? wg : none, want_x ? wu : none, want_u ? s : none, want_g ? t : none);
+            const int64_t m = rows_of(dh), n = dh.size(-1), k = ctx->saved_data["k"].toInt();
+            check_input(x, dh, k);
+            check_weight(wg, dh, k);
+            check_weight(wu, dh, k);
+            refuse_freed(dh, x, wg, wu);
+            const Tensor s = factor_back(want_u ? saved[3] : none, dh, m, n), t = factor_back(want_g ? saved[4] : none, dh, m, n);
             Incoming g = act_grad(dh, two ? 2 : 1, want_g ? t : s, two ? s : Tensor(), want_x || want_wg || want_wu, want_g ? more.a : more.b,
                                   two && more.b, m, n);
             const int u = two ? 1 : 0;  // which of them is the other projection's, where it is wanted

@@ -1,6 +1,7 @@
-"""What linear and gated_linear keep for their backward pass, when it is not there any more."""
+"""What linear and gated_linear keep for their backward pass, when it is not there any more, or not what it was."""
 import pytest
 import torch
+from torch.autograd.graph import saved_tensors_hooks
 
 import lmms_engine_amd as E
 
@@ -59,3 +60,45 @@ def test_an_incoming_gradient_that_was_freed(kind):
     free(dy)
     with pytest.raises(ValueError, match="freed"):
         torch.autograd.grad(y, list(v.values()), dy)
+
+
+OTHERS = {
+    "a type": (lambda t: t.to(torch.float16 if t.is_floating_point() else torch.int8), TypeError),
+    "a wider type": (lambda t: t.double(), TypeError),
+    "a device": (lambda t: t.cpu(), ValueError),
+    "fewer values": (lambda t: t.flatten()[:0], ValueError),
+    "fewer columns": (lambda t: t[..., :-1], ValueError),
+    "a shape": (lambda t: torch.stack([t, t]), ValueError),
+    "a layout": (lambda t: t.to_sparse(), NotImplementedError),
+}
+
+
+@pytest.mark.parametrize("other", list(OTHERS))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", list(SHAPES))
+def test_what_hooks_give_back_is_what_was_kept(kind, dtype, other):
+    change, error = OTHERS[other]
+    count = {"linear": 3, "gated": 5}[kind]
+    for i in range(count):
+        seen, v = [], inputs(kind, dtype)
+        with saved_tensors_hooks(lambda t: seen.append(t) or (len(seen) - 1, t), lambda p: change(p[1]) if p[0] == i else p[1]):
+            y = call(kind, v)
+        assert len(seen) == count
+        with pytest.raises(error, match="kept for a backward pass"):
+            torch.autograd.grad(y, list(v.values()), torch.ones_like(y))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", list(SHAPES))
+def test_hooks_may_give_back_other_strides_and_addresses(kind, dtype):
+    """Which operands are copied, not what is added up, goes by them."""
+    def gradients(unpack):
+        v = inputs(kind, dtype)
+        with saved_tensors_hooks(lambda t: t.cpu(), lambda t: unpack(t.cuda())):
+            y = call(kind, v)
+        return torch.autograd.grad(y, list(v.values()), torch.ones_like(y))
+
+    want = gradients(lambda t: t)
+    for lay in (lambda t: torch.stack([t, t], -1)[..., 0], lambda t: t.t().contiguous().t() if t.dim() == 2 else t, part,
+                lambda t: torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)):
+        assert all(torch.equal(a, e) for a, e in zip(gradients(lay), want))
