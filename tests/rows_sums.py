@@ -17,6 +17,21 @@ def embedding_grad(ids, dy, vocab, scale, skip):
     return torch.zeros(vocab, dy.size(-1), dtype=torch.float64).index_add_(0, ids[fine].long(), dy[fine]) * scale
 
 
+def rows_of_ones(g, rows, n, centred, dtype):
+    """Values of 1 and -1, of a centred row as many of either: mean 0, mean of squares 1, so that with eps = 0 a norm's hat is its input, exactly."""
+    if not centred:
+        return torch.where(torch.rand(rows, n, generator=g, device=g.device) < 0.5, 1.0, -1.0).to(dtype)
+    assert n % 2 == 0
+    first = torch.where(torch.rand(rows, n // 2, generator=g, device=g.device) < 0.5, 1.0, -1.0)
+    x = torch.cat([first, -first], 1)
+    return x[:, torch.randperm(n, generator=g, device=g.device)].to(dtype)
+
+
+# (rows, columns), columns even: test_rows_sums_host.py holds the list to giving a workgroup of every kernel of a norm's gradient several turns, or several parts
+# to a sum over columns, with a rest behind them
+NORMS = [(150001, 2), (90001, 6), (40003, 30), (40003, 128), (20003, 250), (20003, 256), (12003, 506), (12003, 512), (7003, 1002), (7003, 1024), (3001, 4096), (3001, 4098),
+         (2001, 8192), (2001, 8194), (1501, 12288), (1501, 12290), (1301, 16382), (1301, 16384), (300, 20000), (203, 33002)]
+
 HOT = "one", "most of one", "two in turn"
 IDS = {
     "any": lambda g, t, v: torch.randint(0, v, (t,), generator=g, device=g.device),
