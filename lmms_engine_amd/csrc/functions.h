@@ -84,7 +84,8 @@ void close_history(Tensor& g, unsigned on, const torch::autograd::edge_list& edg
     torch::autograd::impl::set_gradient_edge(g, {node, node->add_input_metadata(g)});
 }
 
-// Tensors that a call may lack travel as optionals, and a context numbers the tensors that there are: `has` holds a bit for each of the two.
+// Tensors that a call may lack travel as optionals, and a context numbers the tensors that there are: `has` holds a bit for each that a call
+// may have, the first one's lowest.
 typedef std::optional<Tensor> Maybe;
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }

@@ -47,13 +47,13 @@ struct Values {
         at = pointer(copy.defined() ? copy : t);
     }
 };
-// The places of the tensors of a context: `always` of them, then those of `count` optional ones that there are.
-struct Places {
+// The places of the tensors of a context: `always` of them, then those of COUNT optional ones that there are.
+template <int COUNT> struct Places {
     AutogradContext* ctx;
-    int at[4];
-    Places(AutogradContext* c, int always, int count) : ctx(c) {
+    int at[COUNT];
+    Places(AutogradContext* c, int always) : ctx(c) {
         const int64_t has = ctx->saved_data["has"].toInt();
-        for (int i = 0, next = always; i < count; ++i) at[i] = has >> i & 1 ? next++ : -1;
+        for (int i = 0, next = always; i < COUNT; ++i) at[i] = has >> i & 1 ? next++ : -1;
     }
     bool wanted(int i) const { return at[i] >= 0 && ctx->needs_input_grad(at[i]); }
     torch::autograd::Edge edge(int i) const { return at[i] >= 0 ? torch::autograd::get_current_node()->next_edge(at[i]) : torch::autograd::Edge(); }
@@ -112,7 +112,7 @@ struct Norm : torch::autograd::Function<Norm> {
         refuse_recording();
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &s = saved[0], &w = saved[1], &stats = saved[2], &dy = incoming[0], ds = incoming.size() > 1 ? incoming[1] : Tensor();
-        const Places more(ctx, 1, 3);
+        const Places<3> more(ctx, 1);
         const bool want_x = ctx->needs_input_grad(0), want_r = more.wanted(2), want_w = more.wanted(0), want_b = more.wanted(1);
         variable_list grads(6);
         Tensor dx;
@@ -257,7 +257,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
             }
             if (at::GradMode::is_enabled()) close_history(grads[0], 0, {}, {dy});
         }
-        if (Places(ctx, 1, 2).wanted(0)) grads[1] = dy;
+        if (Places<2>(ctx, 1).wanted(0)) grads[1] = dy;
         return grads;
     }
 };
