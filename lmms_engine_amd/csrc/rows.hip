@@ -61,10 +61,11 @@ __device__ __forceinline__ float group_sum(float v, float* part) {
 // summed, and no sum of squares cancels.  A lane has CH pieces of 16 bytes, neighbouring lanes neighbouring pieces.  Where a row is no whole number of
 // pieces (RAGGED), its last one begins a piece before the row's end: it overlaps the one before, and what it has twice counts once.  Rows at any address.
 //
-// Bound by memory.  8192 x 4096 bf16 values: the RMS norm of x + residual, four streams of them, takes 45 us (5.9 TB/s), its gradient, four streams
-// too, 46 (5.8 TB/s) and 4 for the last sums of the weight's; a layer norm's gradient 55.  262144 rows of 128 (16 lanes each): 26 us (5.1) and 34 (5.9).
-// One row of 4096: 2.5 us.  A large copy reaches 4.9 on the same card.  Asking for the next row before the present one is through changed none of
-// these by more than 2 %: there are waves enough to take turns.
+// Bound by memory.  8192 x 4096 bf16 values: the RMS norm of x + residual, four streams of them, takes 46 us (5.8 TB/s), its gradient, four streams
+// too, 46 (5.8 TB/s) and 4 for the last sums of the weight's; a layer norm's 48, 54 and 7.  The same in fp32: 87 (6.2), 112 (4.8) and 5.  262144 rows of 128 bf16
+// values (16 lanes each): 27 us (4.9) and 34 (5.9).  Rows of 4090, which begin at any address: an RMS norm 50 and 48, a layer norm 54 and 60.  One row of
+// 4096: 3 us.  A large copy reaches 4.9 on the same card.  Asking for the next row before the present one is through changed none of these by more than
+// 2 %: there are waves enough to take turns.
 constexpr int MOST_LANES = 1024, MOST_WAVES = MOST_LANES / 64;  // of a row
 template <typename T> struct Piece;
 template <> struct Piece<bf16_t> {
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(MOST_LANES / 2) norm_kernel(const muon_hip_nor
             x[c].raw = {};
             if (row && at.in(c)) x[c].load(px, at.bytes(c));
         }
-        // weights are asked for with the row where there is room for them (262144 rows of 128: 26.3 us in place of 29, 4096 x 1024 9.1 in place of 9.4)
+        // weights are asked for with the row where there is room for them (262144 rows of 128: 10 % less, 4096 x 1024 3 %)
         const auto weights = [&](int c, P& wc, P& bc) {
             if (!row || !at.in(c)) return;
             if (p.weight) wc.load(p.weight, at.bytes(c));
@@ -374,8 +375,8 @@ __global__ void __launch_bounds__(grad_lanes(CH * P::V, CENTRED), grad_waves(CH 
 }
 
 // Rows longer than the registers of their lanes hold: a workgroup per row, which reads it once for each sum and once more
-// for the result, and, for the sums over rows, a workgroup per block of columns.  Most of what is read again comes from the caches: 2048 x 20000 bf16 values
-// with a residual take 80 us (4.1 TB/s) and 118.
+// for the result, and, for the sums over rows, a workgroup per block of columns.  Most of what is read again comes from the caches: an RMS norm of
+// 1024 x 40000 bf16 values with a residual takes 93 us (3.5 TB/s of four streams), its gradient 101, the sums over rows 25 and 7 more.
 template <typename T, bool CENTRED>
 __global__ void __launch_bounds__(256) norm_streamed_kernel(const muon_hip_norm p) {
     __shared__ float part[2][4];
@@ -541,8 +542,9 @@ struct Cut {
     int shift, segments;
 };
 // A group of lanes for each segment of each token, all of whose loads are under way before the first store: 8192 rows of 4096 bf16 values from a table of
-// 151936 take 25 us (5.2 TB/s of results and rows).  The last piece of a ragged row overlaps the one before it: what it has twice is written twice.
-// An id that is none of the table's has a row of NaN: the host cannot be told without waiting for the device.
+// 151936 take 27 us where a third of them are one id and the others go by rank, 41 where hardly two are alike (3.3 TB/s of results and rows).  The last
+// piece of a ragged row overlaps the one before it: what it has twice is written twice.  An id that is none of the table's has a row of NaN: the host
+// cannot be told without waiting for the device.
 template <typename T, typename P, int CH>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, Cut cut) {
     constexpr int V = P::V;
@@ -578,16 +580,16 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbeddingArgs a, C
 
 // The table's gradient.  The tokens are sorted by id, keeping their order among equal ones, and the sorted tokens cut into chunks of equal length,
 // whatever ids are in them: one id may have most of the tokens, as the placeholders of an image do.
-//   sort    one launch: a workgroup sorts up to 8192 tokens in LDS (24 us: a digit of up to 7 bits at a time, bound by the vector instructions of 16 waves
+//   sort    one launch: a workgroup sorts up to 8192 tokens in LDS (27 us: a digit of up to 7 bits at a time, bound by the vector instructions of 16 waves
 //           on one compute unit), the others clear the table meanwhile, which for large tables takes longer than any of the rest
 //   merge   joins up to 16 sorted lists, where there are more tokens than that: a token's place is its place in its own list and what binary
-//           searches in the other ones say (16384 tokens 10 us, 131072 29)
+//           searches in the other ones say (16384 tokens 10 us, 131072 33)
 //   add     a chunk's lanes walk over its tokens: the sum of a run of equal ids is the table's row, or, where the run goes on in a neighbouring
 //           chunk, one of two rows of fp32 that a chunk has for that
 //   join    adds those up, in their order.
-// Bound by memory: 8192 tokens into 151936 x 4096 bf16 values take 195 us to clear 1.24 GB (6.4 TB/s; a fill alone 6.9), 35 to add up 67 MB, while the
-// memory-side cache still writes back what was cleared (268 MB of gradients after as many of cleared table: 85, in whatever order and by
-// however many waves), and 8 to join.
+// Bound by memory: 8192 tokens into 151936 x 4096 bf16 values take 197 us to clear 1.24 GB (6.3 TB/s; a fill alone 6.9), 35 to add up 67 MB, while the
+// memory-side cache still writes back what was cleared (41 where hardly two ids are alike; 268 MB into 32768 rows of a table as large: 108, in whatever order
+// and by however many waves), and 6 to join.
 constexpr int SORT_TOKENS = 8192, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ROUNDS = SORT_TOKENS / SORT_THREADS;
 constexpr int DIGIT_BITS = 7;  // at most; histograms of 128 digits for each of 16 waves
 constexpr int MERGE_LISTS = 16;
@@ -922,9 +924,9 @@ __global__ void __launch_bounds__(JOIN_WAVES * 64) embedding_join_kernel(const E
 }
 
 // ---- dropout ----------------------------------------------------------------------------------------
-// Bound by memory: 8192 x 12288 bf16 values take 72 us (5.6 TB/s), with a residual 107 (5.6); with three rounds of the generator in place of ten
-// the first took 70.6 where it took 77.8 with one block to a thread.  Sixteen random bits a value instead of 32 are what makes it so: a thread draws one block
-// for its eight values.
+// Bound by memory: 8192 x 12288 bf16 values take 70 us, 75 behind another pass over them (5.7 and 5.4 TB/s), with a residual 106 (5.7), fp32 values 136
+// (5.9).  With one block to a thread three rounds of the generator in place of ten took 9 % less.  Sixteen random bits a value instead of 32 are
+// what keeps it bound by memory: a thread draws one block for its eight values.
 //
 // Philox4x32-10: Salmon, Moraes, Dror and Shaw, Parallel random numbers: as easy as 1, 2, 3 (2011).
 __device__ __forceinline__ u32x4 philox(u32x4 c, uint32_t k0, uint32_t k1) {
@@ -1001,7 +1003,7 @@ Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most, bo
     const auto fits = [&](int pieces) { return lanes_for(pieces) <= limit(pieces); };
     if (!fits(most)) return {256, 0, 256, false};
     Layout l{8, 1, threads, n > v && n % v != 0};
-    if (n < v) return l;  // a value to a lane: 262144 rows of 4 bf16 values take 11.3 us and their gradient 13.6, a workgroup per row 400 and 475
+    if (n < v) return l;  // a value to a lane: 262144 rows of 4 bf16 values take 8.6 us and their gradient 11.3, a workgroup per row 400 and 475
     if (count <= 32) {
         while (l.lanes < count) l.lanes *= 2;
         return l;
@@ -1013,19 +1015,19 @@ Layout lay_rows(int dtype, long rows, int n, int threads, int best, int most, bo
     l.threads = l.lanes * std::max(1, threads / l.lanes);
     return l;
 }
-// Up to four pieces of each row are under way in a lane: 8192 x 4096 bf16 with a residual 48.1 us, with up to eight 51.5, two 48.6 to 49, one 51.
-// Numbers of waves that are no powers of two, by which gradients gain, lose here: 8192 x 12288 143 us in place of 137, 8192 x 6144 71 and 69.
+// Up to four pieces of each row are under way in a lane: 8192 x 4096 bf16 with a residual takes 7 % longer with up to eight, 1 to 2 with two, 6 with one.
+// Numbers of waves that are no powers of two, by which gradients gain, lose here: 8192 x 12288 4 %, 8192 x 6144 3 %.
 Layout lay_norm(int dtype, long rows, int n) { return lay_rows(dtype, rows, n, 256, 4, 8, true, [](int) { return MOST_LANES / 2; }); }
 // A lane of a gradient holds the sums of its columns besides: 16 values of a row at most, of a layer norm, which has two sums, 8, or there are too few waves
-// (8192 x 4096 bf16 with a residual: RMS 52 us, with 32 values 62; layer norm 60, with 16 or 32 73).  Rows have as many waves as they need and up to all of
-// a compute unit's: layer norms of 8192 x 5120 63 us where 512 lanes of two pieces took 94, 8192 x 6144 105 and 116, 8192 x 12288 176 and 186.
+// (8192 x 4096 bf16 with a residual: an RMS norm's with 32 values takes 19 % longer, a layer norm's with 16 or 32 22 %).  Rows have as many waves as they need and
+// up to all of a compute unit's: layer norms of 8192 x 5120 take 33 % less than with 512 lanes of two pieces, 8192 x 6144 9 %, 8192 x 12288 5 %.
 Layout lay_grad(int kind, int dtype, long rows, int n) {
     const int v = dtype == MUON_HIP_BF16 ? 8 : 4;
     const bool layer = kind == MUON_HIP_NORM_LAYER;
     return lay_rows(dtype, rows, n, 512, (layer ? 8 : 16) / v, (layer && dtype == MUON_HIP_BF16 ? 32 : 16) / v, false, [&](int pieces) { return grad_lanes(pieces * v, layer); });
 }
-// As many workgroups as are at work at once, each of which takes rows until there are none left.  (8192 x 4096 RMS: half as many 60 us in place of 52, twice as
-// many 59.)
+// As many workgroups as are at work at once, each of which takes rows until there are none left.  (8192 x 4096 RMS: half as many take 15 % longer,
+// twice as many 13 %.)
 long grad_groups(int kind, int dtype, long rows, int n, const Layout& l, int cus) {
     // (streamed rows: parts of the sums over columns, of 32 rows at least, and as many as make 2048 workgroups)
     if (l.pieces == 0) return std::min(up(rows, 32) / 32, std::max(1L, std::min(1024L, 2048 / (up(n, 256) / 256))));
@@ -1226,8 +1228,8 @@ hipError_t launch_embedding_grad(const EmbeddingArgs& a, void* workspace, hipStr
 
 hipError_t launch_dropout(const DropoutArgs& a, hipStream_t stream) {
     if (a.count == 0) return hipSuccess;
-    // A block of eight values to a thread, and two of them, half of the tensor apart, where bf16 values fill the machine many times over: 8192 x 12288 71.9 us
-    // where it took 77.5, with a residual 107 and 109.5; fp32 values, of which a thread has twice the bytes, lose 3 %, four blocks 2 %.
+    // A block of eight values to a thread, and two of them, half of the tensor apart, where bf16 values fill the machine many times over: 8192 x 12288 take 7 %
+    // less, with a residual 2 %; fp32 values, of which a thread has twice the bytes, lose 3 %, four blocks 2 %.
     const long each = a.dtype == MUON_HIP_BF16 && a.count >= 1L << 24 ? 4096 : 2048;
     const auto kern = a.dtype == MUON_HIP_BF16 ? dropout_kernel<bf16_t> : dropout_kernel<float>;
     hipLaunchKernelGGL(kern, dim3(grid_of(up(a.count, each) / each)), dim3(256), 0, stream, a);
